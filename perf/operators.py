@@ -43,9 +43,9 @@ def listed():
         # the same at the end of a long context, where the cache is most of what a step reads
         {"name": "decode after 32767", **_decode(32, 8, 128, 32767, 1)},
         # six drafted tokens checked at once by a TinyLlama-shaped model whose cache is kept to a budget: weights are tracked
-        {"name": "draft of 6, weights", **_decode(32, 4, 64, 3001, 6, True)},
+        {"name": "draft of 6 with weights", **_decode(32, 4, 64, 3001, 6, True)},
         # a prompt of 2048 tokens attending to itself, with the weights that the eviction after it goes by
-        {"name": "prompt 2048, weights", **_attention(32, 8, 128, 0, 2048, True)},
+        {"name": "prompt 2048 with weights", **_attention(32, 8, 128, 0, 2048, True)},
         # a few tokens, and the keys and values of a prompt, into the cache, and back as the values that it holds
         {"name": "append 7", **_append(4, 64, 3001, 7, 10000.0)},
         {"name": "append 2048", **_append(8, 128, 37, 2048, 1000000.0)},
