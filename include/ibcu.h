@@ -238,6 +238,51 @@ int ibcu_pq_lm_head_topk(ibcu_ctx* ctx, const ibcu_pq_t* t, const float* x, int 
 int ibcu_pqkv_encode(ibcu_ctx* ctx, const float* vec, int dim, int n_vec, int G, int K1,
                      const uint16_t* cb_l, const uint16_t* cb_r, uint8_t* idx, float* scale);
 
+/* ── KV cache in 4 bits ──────────────────────────────────────────────────────────────── */
+/* Beside the FP32 cache of ibcu_attention*: 4.5 bits a value instead of 32. The reference keeps its cache in FP32
+ * (src/forward.c:463-504); its compressed forms live in the session engine (see ibcu_pqkv_encode). A row of a KV head is head_dim
+ * values in groups of 32, each with an fp16 scale s = max|x| * (1 / 7) and codes clamp(rint(x * (1 / s)), -7, 7) + 8 (products and
+ * reciprocals in FP32): the value held is (code - 8) * s. A group that holds NaN or Inf has s = NaN, so that it shows wherever it is seen; one whose s rounds to zero
+ * holds zeros; s is at most 65504. Planes are per KV head, two codes a byte, first code in the low nibble:
+ *   k, v   [n_kv_heads][max_rows][head_dim / 2] bytes, 16-byte aligned
+ *   scale  [n_kv_heads][max_rows][2 * head_dim / 32] fp16: the key's groups, then the value's; 16-byte aligned
+ *   weight [n_kv_heads][max_rows] float, or NULL: the attention that each row has drawn so far
+ * Order of the codes in a row, as the kernels' lanes take them: of a key, four pieces, piece t holding values 8t..8t+7 of every
+ * group of 32 in turn; of a value row, eight pieces, piece g holding values 4g..4g+3 of every group (ibcu_kv4_read gives the
+ * plain order). head_dim 32, 64, 96, 128, 192 or 256; max_rows a multiple of 8; memory behind the last written row is not used,
+ * whatever it holds.
+ * A row of the cache need not be a position: after an eviction, rows and positions go on side by side, which is why the calls
+ * take both row0 (where) and pos0 (the angle). */
+typedef struct {
+    uint8_t*  k;
+    uint8_t*  v;
+    uint16_t* scale;
+    float*    weight;
+    float     decay;                  /* what a call leaves of earlier weights: 1 sums them up, 0 keeps this call's alone; 0..1 */
+    int n_kv_heads, head_dim, max_rows;
+} ibcu_kv4_t;
+/* Rows row0..row0+B-1 from k, v [B][n_kv_heads * head_dim]. Keys are rotated (adjacent pairs, position pos0 + b, as
+ * ibcu_rope_kv_write) before they are coded: angles pos * theta^(-2m / head_dim) in 64 bits, the result rounded once; theta = 0: not rotated.
+ * The rows' weights start at zero. k and v are left as they are. */
+int ibcu_kv4_write(ibcu_ctx* ctx, const ibcu_kv4_t* cache, const float* k, const float* v, int row0, int pos0, int B, float theta);
+/* The values that rows row0..row0+n-1 hold, as [n][n_kv_heads * head_dim]. */
+int ibcu_kv4_read(ibcu_ctx* ctx, const ibcu_kv4_t* cache, float* k, float* v, int row0, int n);
+/* GQA attention as ibcu_attention, over the cache: query position b (q [B][n_heads * head_dim], rotated already) sees rows 0..row0+b,
+ * which includes its own. Any B that the cache has rows for. Products and sums keep FP32's accuracy (FP32 queries and
+ * weights times the held codes; nothing is rounded to fewer bits). With cache->weight, row r of a KV head gets
+ * weight = decay * weight + the softmax weights that it had over all positions of the call and query heads of the group. */
+int ibcu_attention_kv4(ibcu_ctx* ctx, const ibcu_kv4_t* cache, const float* q, float* out, int n_heads, int row0, int B);
+/* The attention step of a decode layer, as ibcu_attention_decode: queries and keys rotated, the new rows row0..row0+B-1 written,
+ * attention over rows 0..row0+b. q, k and v hold the raw projections and are left as they are. */
+int ibcu_attention_decode_kv4(ibcu_ctx* ctx, const ibcu_kv4_t* cache, const float* q, const float* k, const float* v, float* out,
+                              int n_heads, int row0, int pos0, int B, float theta);
+/* Cuts rows 0..rows-1 of a cache down to `keep` of them, for every KV head by its own weights: the first `sink` and the last
+ * `recent` rows stay, and of the others those with the largest weight (equal weights: the lower row; NaN counts as less than any
+ * number). Kept rows go to rows 0..keep-1 of dst in their old order, weights with them. dst may be the same cache (cut in place),
+ * else the two share no memory; a dst without weights gets none. kept (may be NULL): int32 [n_kv_heads][keep], the old rows.
+ * 1 <= keep <= rows, sink + recent <= keep. Needs src->weight. */
+int ibcu_kv4_evict(ibcu_ctx* ctx, const ibcu_kv4_t* src, const ibcu_kv4_t* dst, int rows, int keep, int sink, int recent, int32_t* kept);
+
 /* ── group-scaled INT4 matvec ────────────────────────────────────────────────────────── */
 /* The INT4 tensors of the reference's session engine (struct ib_int4_tensor, src/pq_decode.c:3474-3483; arithmetic of
  * int4_matmul_rows_skip, :3565-3651; skip rule of build_skip_mask, :3854-3882). The reference has these only as static

@@ -16,9 +16,9 @@ import ctypes as C
 import numpy as np
 
 from . import _ffi
-from ._ffi import LinearT, PqT
+from ._ffi import Kv4T, LinearT, PqT
 
-__all__ = ["Backend", "IbcuError", "LinearT", "PqT"]
+__all__ = ["Backend", "IbcuError", "Kv4T", "LinearT", "PqT"]
 
 
 class IbcuError(RuntimeError):
@@ -210,6 +210,17 @@ class Backend:
         self._check(self.lib.ibcu_pq_lm_head_topk(self.ctx, C.byref(t), dx.ptr, k_top, dl.ptr, di.ptr))
         self.sync()
         return self.download(dl, np.float32, k_top), self.download(di, np.int32, k_top)
+
+    def make_kv4(self, n_kv_heads, head_dim, max_rows, weights=False, decay=1.0):
+        """An empty 4-bit KV cache (ibcu_kv4_t); its buffers are in ._keep as k, v, scale and, with weights, weight."""
+        rows = n_kv_heads * max_rows
+        keep = [self.alloc(rows * head_dim // 2), self.alloc(rows * head_dim // 2), self.alloc(rows * head_dim // 8)]
+        if weights:
+            keep.append(self.alloc(rows * 4))
+            self._check(self.lib.ibcu_memset(self.ctx, keep[3].ptr, 0, rows * 4))
+        t = Kv4T(keep[0].ptr, keep[1].ptr, keep[2].ptr, keep[3].ptr if weights else None, decay, n_kv_heads, head_dim, max_rows)
+        t._keep = keep
+        return t
 
     def kmeans_assign(self, X, Cn, want_dist=False, path=0):
         """path: IBCU_KMEANS_AUTO (0), _EXACT (1) or _MMA_SYNC (2)"""

@@ -42,6 +42,12 @@ class Int4gT(C.Structure):
                 ("q", C.c_void_p), ("s", C.c_void_p), ("outl_idx", C.c_void_p), ("outl_val", C.c_void_p)]
 
 
+class Kv4T(C.Structure):
+    """ibcu_kv4_t"""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("scale", C.c_void_p), ("weight", C.c_void_p), ("decay", C.c_float),
+                ("n_kv_heads", C.c_int), ("head_dim", C.c_int), ("max_rows", C.c_int)]
+
+
 # name -> (restype, argtypes); every symbol include/ibcu.h declares
 IBCU_SYMBOLS = {
     "ibcu_ctx_create": (C.c_int, [C.c_int, c_void_pp]),
@@ -91,6 +97,12 @@ IBCU_SYMBOLS = {
     "ibcu_pq_matmul_fp32": (C.c_int, [C.c_void_p, C.POINTER(PqT), C.c_void_p, C.c_void_p, C.c_int]),
     "ibcu_pqkv_encode": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "ibcu_pq_matmul_fp32_strided": (C.c_int, [C.c_void_p, C.POINTER(PqT), C.c_void_p, C.c_void_p, C.c_int, C.c_int]),
+    "ibcu_kv4_write": (C.c_int, [C.c_void_p, C.POINTER(Kv4T), C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_float]),
+    "ibcu_kv4_read": (C.c_int, [C.c_void_p, C.POINTER(Kv4T), C.c_void_p, C.c_void_p, C.c_int, C.c_int]),
+    "ibcu_attention_kv4": (C.c_int, [C.c_void_p, C.POINTER(Kv4T), C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int]),
+    "ibcu_attention_decode_kv4": (C.c_int, [C.c_void_p, C.POINTER(Kv4T), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                            C.c_int, C.c_int, C.c_int, C.c_int, C.c_float]),
+    "ibcu_kv4_evict": (C.c_int, [C.c_void_p, C.POINTER(Kv4T), C.POINTER(Kv4T), C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p]),
     "ibcu_int4g_matmul_fp32": (C.c_int, [C.c_void_p, C.POINTER(Int4gT), C.c_void_p, C.c_void_p, C.c_float]),
     "ibcu_pq_lm_head_topk": (C.c_int, [C.c_void_p, C.POINTER(PqT), C.c_void_p, C.c_int, C.c_void_p, C.c_void_p]),
     "ibcu_pq_matmul_fp32_noalloc": (C.c_int, [C.c_void_p, C.POINTER(PqT), C.c_void_p, C.c_void_p, C.c_int]),

@@ -1,0 +1,242 @@
+"""The 4-bit KV cache: codes and scales bit for bit, attention and the weight of rows against 64 bits, eviction row for row."""
+import numpy as np
+import pytest
+
+from tests import _kv4
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _free(backend):
+    had = list(backend._bufs)
+    yield
+    for b in [b for b in backend._bufs if b not in had]:
+        b.free()
+        backend._bufs.remove(b)
+
+
+def put(be, k, v, s, weight=None, decay=1.0):
+    t = be.make_kv4(k.shape[0], k.shape[2] * 2, k.shape[1], weights=weight is not None, decay=decay)
+    for b, a in zip(t._keep, (k, v, s.view(np.uint16)) + (() if weight is None else (weight.astype(np.float32),))):
+        be.write(b, a)
+    return t
+
+
+def get(be, t):
+    n, hd, rows = t.n_kv_heads, t.head_dim, t.max_rows
+    k, v = (be.download(t._keep[i], np.uint8, n * rows * hd // 2).reshape(n, rows, hd // 2) for i in (0, 1))
+    s = be.download(t._keep[2], np.uint16, n * rows * hd // 16).view(np.float16).reshape(n, rows, hd // 16)
+    return (k, v, s) + ((be.download(t._keep[3], np.float32, n * rows).reshape(n, rows),) if t.weight else ())
+
+
+def same(a, b):
+    return np.array_equal(raw(a), raw(b)) or (np.array_equal(np.isnan(a), np.isnan(b)) and np.array_equal(a[~np.isnan(a)], b[~np.isnan(b)]))
+
+
+def raw(a):
+    return np.ascontiguousarray(a).view(np.uint8)
+
+
+def rows_of(x, n_kv):
+    return np.ascontiguousarray(x.reshape(x.shape[0], n_kv, -1).transpose(1, 0, 2))
+
+
+@pytest.mark.parametrize("n_kv,hd,row0,pos0,B,theta", [(1, 32, 0, 0, 1, 10000.0), (8, 128, 5, 5, 3, 10000.0), (2, 64, 7, 100000, 9, 500000.0), (3, 96, 0, 3, 40, 0.0),
+                                                        (5, 192, 11, 0, 2, 10000.0), (1, 256, 0, 77, 17, 10000.0), (4, 64, 130, 2000000, 65, 1000000.0)])
+def test_rows_are_written_as_the_formula_says(backend, n_kv, hd, row0, pos0, B, theta):
+    """Every code and scale of the new rows, the other rows untouched, and the read-back in the plain order."""
+    be, rng = backend, np.random.default_rng(hd + B)
+    max_rows = (row0 + B + 7) // 8 * 8 + 8
+    k, v = (rng.standard_normal((B, n_kv * hd), dtype=np.float32) * np.float32(3) for _ in range(2))
+    planes = _kv4.random_planes(rng, n_kv, hd, max_rows, row0)
+    t = put(be, *planes, weight=rng.standard_normal((n_kv, max_rows)))
+    before = get(be, t)
+    dk, dv = be.upload(k), be.upload(v)
+    be._check(be.lib.ibcu_kv4_write(be.ctx, t, dk.ptr, dv.ptr, row0, pos0, B, theta)); be.sync()
+    after = get(be, t)
+    kc, ks = _kv4.quantise(rows_of(_kv4.rotate(k, n_kv, pos0, theta).astype(np.float32), n_kv))
+    vc, vs = _kv4.quantise(rows_of(v, n_kv))
+    new = slice(row0, row0 + B)
+    assert np.array_equal(after[0][:, new], _kv4.pack(kc, True)) and np.array_equal(after[1][:, new], _kv4.pack(vc, False))
+    assert same(after[2][:, new], np.concatenate([ks, vs], -1)) and not after[3][:, new].any()
+    for a, b in zip(before, after):
+        old = [i for i in range(max_rows) if not row0 <= i < row0 + B]
+        assert np.array_equal(raw(a[:, old]), raw(b[:, old]))
+    assert np.array_equal(be.download(dk, np.float32, k.size), k.reshape(-1))
+    ok, ov = be.alloc(k.nbytes), be.alloc(v.nbytes)
+    be._check(be.lib.ibcu_kv4_read(be.ctx, t, ok.ptr, ov.ptr, row0, B)); be.sync()
+    for o, c, s in ((ok, kc, ks), (ov, vc, vs)):
+        assert np.array_equal(be.download(o, np.float32, k.size).reshape(B, n_kv, hd), _kv4.values(c, s).transpose(1, 0, 2).astype(np.float32))
+
+
+def test_groups_out_of_the_ordinary(backend):
+    """Zeros, values below the smallest scale, beyond the largest, Inf and NaN: each group by itself."""
+    be, rng = backend, np.random.default_rng(1)
+    x = rng.standard_normal((1, 256), dtype=np.float32).reshape(8, 32)
+    x[0] = 0; x[1] *= 1e-9; x[2] *= 1e-6; x[3] *= 1e38; x[4, 3] = np.inf; x[5, 31] = np.nan; x[6] *= 65504 * 7; x[7, 0] = -np.inf
+    x = x.reshape(1, 256)
+    t = be.make_kv4(1, 256, 8)
+    dx = be.upload(x)
+    be._check(be.lib.ibcu_kv4_write(be.ctx, t, dx.ptr, dx.ptr, 2, 9, 1, 0.0)); be.sync()
+    c, s = _kv4.quantise(x)
+    k, v, sc = get(be, t)
+    assert np.array_equal(k[0, 2], _kv4.pack(c, True)[0]) and np.array_equal(v[0, 2], _kv4.pack(c, False)[0])
+    assert same(sc[0, 2], np.concatenate([s, s], -1)[0])
+    assert np.isnan(s[0, [4, 5, 7]]).all() and s[0, 0] == 0 and s[0, 1] == 0 and s[0, 2] > 0 and s[0, 3] == 65504
+
+
+SHAPES = [(1, 1, 32, 0, 1), (32, 8, 128, 0, 1), (32, 8, 128, 511, 1), (32, 4, 64, 3001, 6), (8, 1, 256, 100, 9), (6, 2, 96, 33, 5), (12, 12, 64, 257, 3), (10, 2, 192, 60, 8),
+          (9, 1, 32, 17, 2), (24, 2, 64, 40, 3), (4, 4, 128, 0, 130), (8, 2, 64, 700, 70), (2, 1, 128, 9000, 1), (16, 16, 64, 1, 33), (40, 1, 128, 70, 1)]
+
+
+@pytest.mark.parametrize("n_heads,n_kv,hd,row0,B", SHAPES)
+def test_attention_and_weights(backend, n_heads, n_kv, hd, row0, B):
+    """Heads in groups of 1 to 40, single positions and several, rows that end anywhere; what lies behind the last row is garbage."""
+    be, rng = backend, np.random.default_rng(n_heads + hd + row0)
+    R = row0 + B
+    max_rows = (R + 7) // 8 * 8 + 16
+    planes = _kv4.random_planes(rng, n_kv, hd, max_rows, R)
+    q = rng.standard_normal((B, n_heads * hd), dtype=np.float32) * np.float32(1.5)
+    old = rng.uniform(0, 2, (n_kv, max_rows)).astype(np.float32)
+    want, weight, tol, wtol = _kv4.attention(q.astype(np.float64), _kv4.plane_values(*(p[:, :R] for p in planes)), n_heads, row0)
+    dq, do = be.upload(q), be.alloc(q.nbytes)
+    for decay, w0 in ((None, None), (1.0, old), (0.5, old), (0.0, np.full_like(old, np.nan))):
+        t = put(be, *planes, weight=w0, decay=decay or 0.0)
+        be._check(be.lib.ibcu_memset(be.ctx, do.ptr, 0xFF, q.nbytes))
+        be._check(be.lib.ibcu_attention_kv4(be.ctx, t, dq.ptr, do.ptr, n_heads, row0, B)); be.sync()
+        got = be.download(do, np.float32, q.size).reshape(q.shape)
+        assert np.all(np.abs(got - want) <= tol), (decay, np.max(np.abs(got - want) / tol))
+        if w0 is not None:
+            after = get(be, t)[3]
+            full = weight + (decay * w0[:, :R].astype(np.float64) if decay else 0.0)
+            assert np.all(np.abs(after[:, :R] - full) <= wtol + 3 * 2.0 ** -24 * full), decay
+            assert np.array_equal(after[:, R:], w0[:, R:], equal_nan=True)
+        assert np.array_equal(be.download(dq, np.float32, q.size), q.reshape(-1))
+
+
+@pytest.mark.parametrize("n_heads,n_kv,hd,row0,pos0,B,theta", [(32, 8, 128, 512, 512, 1, 10000.0), (32, 4, 64, 0, 0, 1, 10000.0), (8, 2, 128, 100, 5000, 4, 500000.0),
+                                                                (6, 6, 96, 31, 31, 33, 10000.0), (4, 1, 256, 15, 70000, 2, 10000.0), (5, 1, 32, 3, 3, 1, 0.0), (32, 8, 128, 0, 0, 150, 10000.0)])
+def test_decode_step(backend, n_heads, n_kv, hd, row0, pos0, B, theta):
+    """One call: queries and keys rotated, the rows written as ibcu_kv4_write writes them, attention over them; inputs left alone."""
+    be, rng = backend, np.random.default_rng(row0 + B)
+    R = row0 + B
+    max_rows = (R + 7) // 8 * 8
+    planes = _kv4.random_planes(rng, n_kv, hd, max_rows, row0)
+    q = rng.standard_normal((B, n_heads * hd), dtype=np.float32)
+    k, v = (rng.standard_normal((B, n_kv * hd), dtype=np.float32) for _ in range(2))
+    dq, dk, dv, do = be.upload(q), be.upload(k), be.upload(v), be.alloc(q.nbytes)
+    t, t2 = put(be, *planes, weight=np.ones((n_kv, max_rows)), decay=0.0), put(be, *planes, weight=np.ones((n_kv, max_rows)))
+    be._check(be.lib.ibcu_attention_decode_kv4(be.ctx, t, dq.ptr, dk.ptr, dv.ptr, do.ptr, n_heads, row0, pos0, B, theta))
+    be._check(be.lib.ibcu_kv4_write(be.ctx, t2, dk.ptr, dv.ptr, row0, pos0, B, theta)); be.sync()
+    a, b = get(be, t), get(be, t2)
+    for x, y in zip(a[:3], b[:3]):
+        assert np.array_equal(raw(x), raw(y))
+    want, weight, tol, wtol = _kv4.attention(_kv4.rotate(q, n_heads, pos0, theta).astype(np.float32).astype(np.float64), _kv4.plane_values(*(p[:, :R] for p in b[:3])), n_heads, row0)
+    got = be.download(do, np.float32, q.size).reshape(q.shape)
+    assert np.all(np.abs(got - want) <= tol), np.max(np.abs(got - want) / tol)
+    assert np.all(np.abs(a[3][:, :R] - weight) <= wtol + 2.0 ** -24 * weight)
+    for d, x in ((dq, q), (dk, k), (dv, v)):
+        assert np.array_equal(be.download(d, np.float32, x.size), x.reshape(-1))
+
+
+@pytest.mark.parametrize("n_heads,n_kv,hd,row0,B,at", [(8, 2, 64, 0, 6, 3), (4, 4, 128, 29, 9, 30), (4, 1, 256, 60, 8, 67), (8, 8, 64, 0, 80, 33), (32, 8, 128, 200, 3, 201)])
+def test_a_later_row_does_not_reach_an_earlier_position(backend, n_heads, n_kv, hd, row0, B, at):
+    """Row `at` holds NaN in key and value: positions that do not see it keep their bits, the others show it."""
+    be, rng = backend, np.random.default_rng(at)
+    R = row0 + B
+    k, v, s = _kv4.random_planes(rng, n_kv, hd, (R + 7) // 8 * 8, R)
+    q = be.upload(rng.standard_normal((B, n_heads * hd), dtype=np.float32))
+    outs = []
+    for poison in (False, True):
+        if poison:
+            s[:, at] = np.nan
+        t, o = put(be, k, v, s, weight=np.zeros(k.shape[:2]), decay=0.0), be.alloc(B * n_heads * hd * 4)
+        be._check(be.lib.ibcu_attention_kv4(be.ctx, t, q.ptr, o.ptr, n_heads, row0, B)); be.sync()
+        outs.append(be.download(o, np.float32, B * n_heads * hd).reshape(B, -1))
+    first = at - row0
+    assert np.isfinite(outs[0]).all() and np.array_equal(outs[0][:first], outs[1][:first])
+    assert np.isnan(outs[1][first:]).all()
+
+
+def test_extreme_queries(backend):
+    """A query of zeros weighs all rows alike, one of 1e30 picks the row of the largest score, Inf or NaN shows in its head alone."""
+    be, rng = backend, np.random.default_rng(5)
+    n_heads, n_kv, hd, row0 = 8, 2, 64, 99
+    planes = _kv4.random_planes(rng, n_kv, hd, 104, 100)
+    K, V = _kv4.plane_values(*(p[:, :100] for p in planes))
+    q = rng.standard_normal((1, n_heads, hd)).astype(np.float32)
+    q[0, 1] = 0; q[0, 2] *= np.float32(1e30); q[0, 3, 5] = np.inf; q[0, 4, 0] = np.nan; q[0, 5] *= np.float32(1e-30); q[0, 6] *= np.float32(1e-41)
+    dq, do = be.upload(q), be.alloc(q.nbytes)
+    be._check(be.lib.ibcu_attention_kv4(be.ctx, put(be, *planes), dq.ptr, do.ptr, n_heads, row0, 1)); be.sync()
+    got = be.download(do, np.float32, q.size).reshape(n_heads, hd)
+    mean = V.mean(1)
+    tol = 700 * 2.0 ** -24 * np.abs(V).mean(1)
+    for h in (1, 5, 6):
+        assert np.all(np.abs(got[h] - mean[h // 4]) <= tol[h // 4] + 1e-28)
+    best = np.argmax(K[0] @ q[0, 2].astype(np.float64))
+    assert np.allclose(got[2], V[0, best], rtol=2.0 ** -20, atol=0)
+    assert np.isnan(got[3]).all() and np.isnan(got[4]).all() and np.isfinite(got[[0, 1, 2, 5, 6, 7]]).all()
+
+
+@pytest.mark.parametrize("n_kv,hd,rows,keep,sink,recent", [(1, 32, 1, 1, 0, 0), (8, 128, 4096, 1024, 4, 256), (2, 64, 1000, 999, 0, 0), (3, 96, 777, 100, 0, 100), (4, 64, 50, 50, 3, 9),
+                                                            (5, 192, 2049, 1025, 1, 0), (1, 256, 5000, 7, 0, 1), (2, 64, 30001, 12345, 10, 500), (2, 32, 70001, 69999, 0, 3), (16, 32, 300, 5, 2, 2)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_eviction(backend, n_kv, hd, rows, keep, sink, recent, in_place):
+    """Which rows stay, head by head, with weights that repeat, zeros of both signs, infinities and NaN; the rows themselves as they were."""
+    be, rng = backend, np.random.default_rng(rows + keep)
+    max_rows, dst_rows = (rows + 7) // 8 * 8 + 8, (keep + 7) // 8 * 8
+    k, v, s = _kv4.random_planes(rng, n_kv, hd, max_rows, rows)
+    w = np.exp(2 * rng.standard_normal((n_kv, max_rows))).astype(np.float16).astype(np.float32)
+    w[rng.random(w.shape) < 0.2] = 1.0
+    w[rng.random(w.shape) < 0.1] = 0.0
+    w[rng.random(w.shape) < 0.05] = -0.0
+    w[rng.random(w.shape) < 0.02] = np.nan
+    w[rng.random(w.shape) < 0.02] = np.inf
+    w[rng.random(w.shape) < 0.02] = -np.inf
+    t = put(be, k, v, s, weight=w)
+    d = t if in_place else put(be, *(np.zeros((n_kv, dst_rows, p.shape[2]), p.dtype) for p in (k, v, s)), weight=np.zeros((n_kv, dst_rows)))
+    kept = be.alloc(n_kv * keep * 4)
+    be._check(be.lib.ibcu_kv4_evict(be.ctx, t, d, rows, keep, sink, recent, None if in_place and keep % 2 else kept.ptr)); be.sync()
+    got = get(be, d)
+    for h in range(n_kv):
+        at = _kv4.choose(w[h, :rows], keep, sink, recent)
+        if not (in_place and keep % 2):
+            assert np.array_equal(be.download(kept, np.int32, keep, 4 * h * keep), at)
+        for a, b in zip((k, v, s, w), got):
+            assert np.array_equal(raw(a[h, at]), raw(b[h, :keep]))
+            if in_place:
+                assert np.array_equal(raw(a[h, rows:]), raw(b[h, rows:]))
+
+
+def test_prompt_then_eviction_then_decode(backend):
+    """As they are used together: a prompt written and attended with weights, the cache cut in place to a budget, and further tokens
+    at their own positions over the rows that stayed; the weights go on."""
+    be, rng = backend, np.random.default_rng(8)
+    n_heads, n_kv, hd, n, keep, sink, recent, theta = 16, 4, 64, 300, 90, 4, 30, 10000.0
+    t = be.make_kv4(n_kv, hd, 304, weights=True)
+    draw = lambda B, heads: rng.standard_normal((B, heads * hd), dtype=np.float32)
+    q, k, v = draw(n, n_heads), draw(n, n_kv), draw(n, n_kv)
+    d, o = [be.upload(x) for x in (q, k, v)], be.alloc(q.nbytes)
+    be._check(be.lib.ibcu_attention_decode_kv4(be.ctx, t, *(b.ptr for b in d), o.ptr, n_heads, 0, 0, n, theta)); be.sync()
+    planes = get(be, t)
+    _, weight, _, wtol = _kv4.attention(_kv4.rotate(q, n_heads, 0, theta), _kv4.plane_values(*(p[:, :n] for p in planes[:3])), n_heads, 0)
+    assert np.all(np.abs(planes[3][:, :n] - weight) <= wtol + 1e-6 * weight)
+    be._check(be.lib.ibcu_kv4_evict(be.ctx, t, t, n, keep, sink, recent, None))
+    held = [np.stack([p[h, _kv4.choose(planes[3][h, :n], keep, sink, recent)] for h in range(n_kv)]) for p in planes]
+    total = held[3].astype(np.float64)
+    for step in range(3):
+        q, k, v = draw(1, n_heads), draw(1, n_kv), draw(1, n_kv)
+        d = [be.upload(x) for x in (q, k, v)]
+        be._check(be.lib.ibcu_attention_decode_kv4(be.ctx, t, *(b.ptr for b in d), o.ptr, n_heads, keep + step, n + step, 1, theta)); be.sync()
+        kc, ks = _kv4.quantise(rows_of(_kv4.rotate(k, n_kv, n + step, theta).astype(np.float32), n_kv))
+        vc, vs = _kv4.quantise(rows_of(v, n_kv))
+        for i, new in enumerate((_kv4.pack(kc, True), _kv4.pack(vc, False), np.concatenate([ks, vs], -1))):
+            held[i] = np.concatenate([held[i], new], 1)
+        want, weight, tol, wtol = _kv4.attention(_kv4.rotate(q, n_heads, n + step, theta).astype(np.float32).astype(np.float64), _kv4.plane_values(*held[:3]), n_heads, keep + step)
+        assert np.all(np.abs(be.download(o, np.float32, n_heads * hd) - want[0]) <= tol[0])
+        total = np.concatenate([total, np.zeros((n_kv, 1))], 1) + weight
+    after = get(be, t)
+    assert np.all(np.abs(after[3][:, :keep + 3] - total) <= 1e-5 * total + 1e-9)
+    for a, b in zip(after[:3], held[:3]):
+        assert np.array_equal(raw(a[:, :keep + 3]), raw(b))
