@@ -160,6 +160,20 @@ int ibcu_linear_w4a8(ibcu_ctx* ctx, const ibcu_linear_t* tensor, const int8_t* x
  * the quantiser and the matvec (one launch for a single activation of up to 4096 columns, else two). Same bits as the two calls. */
 int ibcu_linear_w4a8_fp32(ibcu_ctx* ctx, const ibcu_linear_t* tensor, const float* x, int N, int B);
 
+/* INT8 weights times INT8 activations with one scale per token (x: max|x| over the token's row * (1 / 127)) beside the one per output
+ * row: the integer route for any number of tokens, where ibcu_linear takes up to 32 and W4A8 scales groups of 128 columns. No
+ * counterpart in the reference.
+ * ibcu_quantize_rows_int8: scale[b] = max|x[b]| * (1 / 127), q[b*N+j] = rint(x * (1 / scale)), ties to even, products and reciprocals in
+ * FP32. A row whose maximum is below 2^-100 gives zeros and scale 0; one that holds NaN or Inf zeros and scale NaN. */
+int ibcu_quantize_rows_int8(ibcu_ctx* ctx, const float* x, int8_t* q, float* scale, int N, int B);
+/* out[b*out_stride + m] = (sum_j w[m][j] * xq[b][j]) * (scale_w[m] * sx[b]), or added to out (IBCU_EPI_ADD), for n_tensors (1..4) INT8
+ * tensors that share the activations. The sums are exact (int32): the same bits however the call is cut. The outputs of a
+ * call do not overlap. N up to 131072, B up to 2^20. w and xq at any address; rows that do not start on 16 bytes (w or xq unaligned, or N no multiple
+ * of 16) are first copied so that they do. */
+int ibcu_linear_w8a8(ibcu_ctx* ctx, const ibcu_linear_t* tensors, int n_tensors, const int8_t* xq, const float* sx, int N, int B);
+/* Both steps for FP32 activations x[b*N + j]. Same bits as the two calls. */
+int ibcu_linear_w8a8_fp32(ibcu_ctx* ctx, const ibcu_linear_t* tensors, int n_tensors, const float* x, int N, int B);
+
 /* ── PQ matvec ───────────────────────────────────────────────────────────────────────── */
 /* Stands in for ib_pq_matmul_fp32 / _threaded / _streaming (src/pq_decode.h:189-222; body
  * src/pq_decode.c:1504-1682), including the second residual level with one-byte or 4-bit packed indices
