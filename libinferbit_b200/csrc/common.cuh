@@ -100,6 +100,10 @@ int ibcu_flush_gather_wait(ibcu_ctx* ctx);
 
 int ibcu_fail(ibcu_ctx* ctx, int code, const char* fmt, ...);
 
+// left in kern_err by a kernel that read its place in a cache from the device and found none
+constexpr int IBCU_KV4_PLACE_ERR = 400;
+constexpr int IBCU_KV4_WAIT_ERR = 401;                       // its bulk copies did not arrive in time
+
 // What a kernel's host part returns when the call is not one for it: nothing was launched, reserved or taken and the context's error
 // is untouched, so the caller takes another kernel. Positive, unlike every error, so that no failure can be taken for it.
 constexpr int IBCU_DECLINED = 1;

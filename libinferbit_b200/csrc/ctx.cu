@@ -162,6 +162,7 @@ static int ibcu_collect_kernel_errors(ibcu_ctx* ctx) {
         const int e = *(volatile int*)ctx->kern_err;
         *(volatile int*)ctx->kern_err = 0;
         if (e >= IBCU_PQ_TC_ERR && e < IBCU_PQ_TC_ERR + 100 && ctx->pq_acc) IBCU_CUDA(ctx, cudaMemsetAsync(ctx->pq_acc, 0, ctx->pq_acc_bytes, ctx->stream));
+        if (e == IBCU_KV4_PLACE_ERR) return ibcu_fail(ctx, IBCU_ERR_PARAM, "a row or position read on the device lies outside the cache: nothing was written");
         return ibcu_fail(ctx, IBCU_ERR_CUDA, "a kernel gave up a bounded wait (code %d): its results are not valid", e);
     }
     return ctx->status;

@@ -6,31 +6,15 @@
 // scale [head][max_rows][2 hd / 32] (the key's groups, then the value's). Inside a row the values lie in the order in which
 // the lanes of a matrix instruction take them: a key row is four pieces, piece t with values 8t..8t+7 of group 0, then of group 1, and
 // so on; a value row is eight pieces, piece g with values 4g..4g+3 of every group. Two values a byte, the first in the low nibble.
-#include "common.cuh"
+#include "kv4.cuh"
 #include <algorithm>
 #include <cmath>
 
 namespace {
 
-struct Kv4 {
-    uint8_t* k; uint8_t* v; __half* scale; float* weight;
-    int n_kv, hd, max_rows;
-    __host__ __device__ size_t row(int h, int r) const { return (size_t)h * max_rows + r; }
-};
-
 __device__ __forceinline__ int key_place(int i, int ng) { return ((i & 31) / 8 * ng + i / 32) * 8 + (i & 7); }      // where value i of a row lies
 __device__ __forceinline__ int value_place(int i, int ng) { return ((i & 31) / 4 * ng + i / 32) * 4 + (i & 3); }
 __device__ __forceinline__ float held(const uint8_t* row, int place, float s) { return (float)((row[place >> 1] >> ((place & 1) * 4) & 15) - 8) * s; }
-
-// The adjacent pair (x0, x1) at angle pos * theta^(-2m / hd): in 64 bits, because far positions times a rounded frequency are off by
-// whole steps of a 4-bit code, rounded once at the end.
-__device__ __forceinline__ void turn_pair(float& x0, float& x1, int m, int hd, int pos, double log2_theta) {
-    double s, c;
-    sincos((double)pos * exp2(-2.0 * m / hd * log2_theta), &s, &c);
-    const double a = x0, b = x1;
-    x0 = (float)(a * c - b * s);
-    x1 = (float)(a * s + b * c);
-}
 
 // A group's scale and the factor that turns its values into codes; amax_bits: the largest magnitude's bits (NaN and Inf above all)
 __device__ __forceinline__ __half group_scale(uint32_t amax_bits, float& inv) {
@@ -45,35 +29,118 @@ __device__ __forceinline__ uint32_t code_of(float x, float inv) {
     return (uint32_t)((int)q + 8);
 }
 
-// grid (positions, KV heads, 2): the key (z = 0, rotated) or value row of one position; a thread has four values of a row
-__global__ void __launch_bounds__(64) kv4_write_kernel(Kv4 c, const float* __restrict__ k, const float* __restrict__ v, int row0, int pos0, double log2_theta, int rotate) {
-    pdl_launch_dependents();
-    pdl_wait();
-    const int b = blockIdx.x, h = blockIdx.y, i = threadIdx.x * 4, ng = c.hd / 32;
-    const bool key = blockIdx.z == 0;
-    if (i >= c.hd) return;                                    // whole groups of eight lanes stay
-    const float* src = (key ? k : v) + ((size_t)b * c.n_kv + h) * c.hd + i;
-    float x[4] = { src[0], src[1], src[2], src[3] };
-    if (key && rotate) {
-        turn_pair(x[0], x[1], i / 2, c.hd, pos0 + b, log2_theta);
-        turn_pair(x[2], x[3], i / 2 + 1, c.hd, pos0 + b, log2_theta);
+// One launch ahead of the attention: blocks below qblocks turn a tile of columns into fragments, the others write rows. Angles of a position are
+// shared by all its heads: a block computes their sines once, in 64 bits, which is most of its time (about a microsecond).
+struct PrepParams { Kv4 c; Kv4Columns t; Kv4Place at; Kv4Prep w; int qblocks, wparts; int* err; };
+
+__global__ void __launch_bounds__(128) kv4_prep_kernel(const PrepParams p) {
+    extern __shared__ __align__(16) double2 turn[];           // [positions of the block][hd / 2] cosine and sine; then [8 columns a warp][hd] turned queries
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hd = p.c.hd, half = hd / 2, ng = hd / 32;
+    const bool queries = (int)blockIdx.x < p.qblocks;
+    const int cols = p.t.cols(), kvh = blockIdx.x / p.t.ntiles, c0 = blockIdx.x % p.t.ntiles * cols, wb = blockIdx.x - p.qblocks;
+    const int b0 = queries ? c0 / p.t.group : wb / p.wparts, b1 = queries ? min(p.t.B - 1, (c0 + cols - 1) / p.t.group) : b0;
+    int row0 = p.at.row0, pos0 = p.at.pos0;
+    if (p.at.at) {
+        pdl_wait();
+        if (!kv4_place(p.at, p.t.B, p.c.max_rows, p.err, row0, pos0)) return;
     }
-    uint32_t m = 0;
+    if (p.w.rotate)
+        for (int e = tid; e < (b1 - b0 + 1) * half; e += 128) {
+            double s, c;
+            sincos((double)(pos0 + b0 + e / half) * exp2((double)(e % half) * (-2.0 / hd * p.w.log2_theta)), &s, &c);
+            turn[e] = make_double2(c, s);
+        }
+    if (!p.at.at) pdl_wait();
+    pdl_launch_dependents();                                  // not earlier: the attention reads rows of earlier calls ahead of its own wait
+    __syncthreads();
+    // the pairs m, m + 1, .. of position b, turned and rounded once
+    auto turn_pair = [&](float& x0, float& x1, int b, int m) {
+        const double2 cs = turn[(b - b0) * half + m];
+        const double a = x0, z = x1;
+        x0 = (float)(a * cs.x - z * cs.y);
+        x1 = (float)(a * cs.y + z * cs.x);
+    };
+    if (queries) {
+        if (warp >= cols / 8) return;
+        // a warp prepares eight columns, lane = column * 4 + t: values 8t..8t+7 of every group
+        float* qr = reinterpret_cast<float*>(turn + (p.w.rotate ? (size_t)min(cols, (cols - 1) / p.t.group + 2) * half : 0)) + (size_t)warp * 8 * hd;
+        const int g = lane >> 2, t = lane & 3, col = c0 + warp * 8 + g, b = col / p.t.group;
+        const bool on = b < p.t.B;
+        const float* src = p.w.q + ((size_t)b * p.t.n_heads + (size_t)kvh * p.t.group + col % p.t.group) * hd;
+        uint32_t m = 0;
+        for (int j = 0; j < ng; j++) {
+            const int d = 32 * j + 8 * t;
+            float x[8];
 #pragma unroll
-    for (int u = 0; u < 4; u++) m = max(m, __float_as_uint(x[u]) & 0x7FFFFFFFu);
-    const unsigned lanes = 0xFFu << (threadIdx.x & 24);       // the eight lanes of a group
+            for (int i = 0; i < 8; i++) x[i] = on ? src[d + i] : 0.0f;
+            if (on && p.w.rotate) {
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(lanes, m, o));
-    float inv;
-    const __half s = group_scale(m, inv);
-    uint32_t w = 0;
+                for (int i = 0; i < 8; i += 2) turn_pair(x[i], x[i + 1], b, (d + i) / 2);
+            }
 #pragma unroll
-    for (int u = 0; u < 4; u++) w |= code_of(x[u], inv) << (4 * u);
-    const size_t row = c.row(h, row0 + b);
-    const int place = key ? key_place(i, ng) : value_place(i, ng);       // four values stay together in both orders
-    *reinterpret_cast<uint16_t*>((key ? c.k : c.v) + row * (c.hd / 2) + place / 2) = (uint16_t)w;
-    if ((i & 31) == 0) c.scale[row * 2 * ng + (key ? 0 : ng) + i / 32] = s;
-    if (key && i == 0 && c.weight) c.weight[row] = 0.0f;
+            for (int i = 0; i < 8; i++) { m = max(m, __float_as_uint(x[i]) & 0x7FFFFFFFu); qr[(size_t)g * hd + d + i] = x[i]; }
+        }
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        // The largest magnitude goes to [2^13, 2^14). A power of 2 up to 2^120, in two factors: what that leaves small are queries below 2^-106, whose
+        // scores are zeros beside one another anyway.
+        const int e = min(120, max(-114, 13 - ((int)(m >> 23) - 127)));
+        const float up = __int_as_float(((e >> 1) + 127) << 23), up2 = __int_as_float((e - (e >> 1) + 127) << 23);
+        const size_t unit = blockIdx.x;
+        // takes the sums' 2^e off; log2(e) makes exponents of 2 of them
+        if (t == 0) p.w.qc[unit * 16 + warp * 8 + g] = (float)fmin(exp2((double)-e) * (1.4426950408889634 / sqrt((double)hd)), 3.0e38);
+        uint2* qf = p.w.qf + unit * kv4_frag_uint2(ng, p.t.large);
+        for (int j = 0; j < ng; j++) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = qr[(size_t)g * hd + 32 * j + 8 * t + i] * up * up2;
+#pragma unroll
+            for (int s = 0; s < 2; s++) {                     // codes 0 and 4, 1 and 5 of a word in the first step, 2 and 6, 3 and 7 in the second
+                __half2 h[2], l[2];
+#pragma unroll
+                for (int u = 0; u < 2; u++) {                 // odd codes reach the product as 16 times themselves
+                    const float f = u ? 0.0625f : 1.0f, a = x[2 * s + u] * f, z = x[2 * s + u + 4] * f;
+                    h[u] = __floats2half2_rn(a, z);
+                    l[u] = __floats2half2_rn(a - __low2float(h[u]), z - __high2float(h[u]));
+                }
+                const uint2 hi = make_uint2(*reinterpret_cast<uint32_t*>(&h[0]), *reinterpret_cast<uint32_t*>(&h[1]));
+                const uint2 lo = make_uint2(*reinterpret_cast<uint32_t*>(&l[0]), *reinterpret_cast<uint32_t*>(&l[1]));
+                if (p.t.large) {
+                    qf[((j * 2 + s) * 2 + warp) * 32 + lane] = hi;
+                    qf[(((ng + j) * 2 + s) * 2 + warp) * 32 + lane] = lo;
+                } else {
+                    qf[((j * 2 + s) * 2) * 32 + lane] = hi;
+                    qf[((j * 2 + s) * 2 + 1) * 32 + lane] = lo;
+                }
+            }
+        }
+        return;
+    }
+    // rows of position b: four values a thread, eight neighbouring threads a group; heads wparts apart
+    const int quads = hd / 4, heads = (p.c.n_kv - wb % p.wparts + p.wparts - 1) / p.wparts;
+    for (int e = tid; e < 2 * heads * quads; e += 128) {
+        const bool key = e < heads * quads;
+        const int f = key ? e : e - heads * quads, h = wb % p.wparts + f / quads * p.wparts, i = f % quads * 4;
+        const float* src = (key ? p.w.k : p.w.v) + ((size_t)b0 * p.c.n_kv + h) * hd + i;
+        float x[4] = { src[0], src[1], src[2], src[3] };
+        if (key && p.w.rotate) { turn_pair(x[0], x[1], b0, i / 2); turn_pair(x[2], x[3], b0, i / 2 + 1); }
+        uint32_t m = 0;
+#pragma unroll
+        for (int u = 0; u < 4; u++) m = max(m, __float_as_uint(x[u]) & 0x7FFFFFFFu);
+        const unsigned lanes = 0xFFu << (lane & 24);
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(lanes, m, o));
+        float inv;
+        const __half s = group_scale(m, inv);
+        uint32_t w = 0;
+#pragma unroll
+        for (int u = 0; u < 4; u++) w |= code_of(x[u], inv) << (4 * u);
+        const size_t row = p.c.row(h, row0 + b0);
+        const int place = key ? key_place(i, ng) : value_place(i, ng);       // four values stay together in both orders
+        *reinterpret_cast<uint16_t*>((key ? p.c.k : p.c.v) + row * (hd / 2) + place / 2) = (uint16_t)w;
+        if ((i & 31) == 0) p.c.scale[row * 2 * ng + (key ? 0 : ng) + i / 32] = s;
+        if (key && i == 0 && p.c.weight) p.c.weight[row] = 0.0f;
+    }
 }
 
 // grid (rows, KV heads): the values that the cache holds
@@ -87,75 +154,6 @@ __global__ void __launch_bounds__(128) kv4_read_kernel(Kv4 c, float* __restrict_
         k[o] = held(c.k + row * (c.hd / 2), key_place(i, ng), __half2float(c.scale[row * 2 * ng + i / 32]));
         v[o] = held(c.v + row * (c.hd / 2), value_place(i, ng), __half2float(c.scale[row * 2 * ng + ng + i / 32]));
     }
-}
-
-__global__ void __launch_bounds__(128) turn_queries_kernel(const float* __restrict__ q, float* __restrict__ out, int hd, int n_heads, int pos0, double log2_theta, int rotate) {
-    pdl_launch_dependents();
-    pdl_wait();
-    const size_t base = ((size_t)blockIdx.x * n_heads + blockIdx.y) * hd;
-    for (int m = threadIdx.x; m < hd / 2; m += blockDim.x) {
-        float a = q[base + 2 * m], b = q[base + 2 * m + 1];
-        if (rotate) turn_pair(a, b, m, hd, pos0 + blockIdx.x, log2_theta);
-        out[base + 2 * m] = a; out[base + 2 * m + 1] = b;
-    }
-}
-
-// grid (positions, query heads), 8 warps: a warp takes every eighth row, a lane one value of each group, with a running maximum and sum
-__global__ void __launch_bounds__(256) kv4_attn_kernel(Kv4 c, const float* __restrict__ q, float* __restrict__ out, float2* __restrict__ stat, int n_heads, int row0) {
-    __shared__ float sm[8], sl[8], sa[8][256];
-    pdl_launch_dependents();
-    pdl_wait();
-    const int b = blockIdx.x, h = blockIdx.y, kvh = h / (n_heads / c.n_kv), lane = threadIdx.x & 31, warp = threadIdx.x >> 5, ng = c.hd / 32;
-    const size_t at = ((size_t)b * n_heads + h) * c.hd;
-    const float scale = 1.0f / sqrtf((float)c.hd);
-    float qv[8], acc[8], m = -INFINITY, l = 0.0f;
-    for (int j = 0; j < 8; j++) { qv[j] = j < ng ? q[at + 32 * j + lane] : 0.0f; acc[j] = 0.0f; }
-    for (int r = warp; r <= row0 + b; r += 8) {
-        const size_t row = c.row(kvh, r);
-        float s = 0.0f;
-        for (int j = 0; j < 8; j++)
-            if (j < ng) s = fmaf(qv[j], held(c.k + row * (c.hd / 2), key_place(32 * j + lane, ng), __half2float(c.scale[row * 2 * ng + j])), s);
-        s = warp_sum(s) * scale;
-        const float mn = fmaxf(m, s), corr = m == -INFINITY ? 0.0f : expf(m - mn), p = expf(s - mn);
-        l = l * corr + p;
-        for (int j = 0; j < 8; j++)
-            if (j < ng) acc[j] = acc[j] * corr + p * held(c.v + row * (c.hd / 2), value_place(32 * j + lane, ng), __half2float(c.scale[row * 2 * ng + ng + j]));
-        m = mn;
-    }
-    if (lane == 0) { sm[warp] = m; sl[warp] = l; }
-    for (int j = 0; j < 8; j++) sa[warp][32 * j + lane] = acc[j];
-    __syncthreads();
-    float M = -INFINITY, L = 0.0f;
-    for (int w = 0; w < 8; w++) M = fmaxf(M, sm[w]);
-    for (int w = 0; w < 8; w++) L += sl[w] == 0.0f ? 0.0f : sl[w] * expf(sm[w] - M);
-    for (int d = threadIdx.x; d < c.hd; d += 256) {
-        float a = 0.0f;
-        for (int w = 0; w < 8; w++) a += sl[w] == 0.0f ? 0.0f : sa[w][d] * expf(sm[w] - M);
-        out[at + d] = a / L;
-    }
-    if (threadIdx.x == 0 && stat) stat[(size_t)b * n_heads + h] = make_float2(M, L);
-}
-
-// grid (rows, KV heads), a warp: weight of a row = decay * weight + its share of every query's attention
-__global__ void __launch_bounds__(32) kv4_weight_kernel(Kv4 c, const float* __restrict__ q, const float2* __restrict__ stat, int n_heads, int row0, int B, float decay) {
-    pdl_launch_dependents();
-    pdl_wait();
-    const int r = blockIdx.x, kvh = blockIdx.y, group = n_heads / c.n_kv, lane = threadIdx.x, ng = c.hd / 32;
-    const size_t row = c.row(kvh, r);
-    const float scale = 1.0f / sqrtf((float)c.hd);
-    float kv[8], w = 0.0f;
-    for (int j = 0; j < 8; j++) kv[j] = j < ng ? held(c.k + row * (c.hd / 2), key_place(32 * j + lane, ng), __half2float(c.scale[row * 2 * ng + j])) : 0.0f;
-    for (int b = max(0, r - row0); b < B; b++)
-        for (int g = 0; g < group; g++) {
-            const int h = kvh * group + g;
-            const float* qh = q + ((size_t)b * n_heads + h) * c.hd;
-            float s = 0.0f;
-            for (int j = 0; j < 8; j++) if (j < ng) s = fmaf(kv[j], qh[32 * j + lane], s);
-            s = warp_sum(s) * scale;
-            const float2 st = stat[(size_t)b * n_heads + h];
-            w += expf(s - st.x) / st.y;
-        }
-    if (lane == 0) c.weight[row] = (decay == 0.0f ? 0.0f : decay * c.weight[row]) + w;
 }
 
 // weights as whole numbers in the order of the choice: larger weight first, NaN last, the two zeros equal
@@ -272,13 +270,14 @@ int check_rotation(ibcu_ctx* ctx, int pos0, int B, float theta, const char* call
 }
 double log2_of(float theta) { return theta > 0.0f ? log2((double)theta) : 0.0; }
 
-int attend(ibcu_ctx* ctx, const Kv4& c, float decay, const float* q, float* out, int n_heads, int row0, int B, float2* stat) {
-    int rc = ibcu_launch(ctx, kv4_attn_kernel, dim3(B, n_heads), dim3(256), 0, 1, true, c, q, out, stat, n_heads, row0);
-    if (!rc && c.weight) rc = ibcu_launch(ctx, kv4_weight_kernel, dim3(row0 + B, c.n_kv), dim3(32), 0, 1, true, c, q, (const float2*)stat, n_heads, row0, B, decay);
-    return rc;
-}
-
 }  // namespace
+
+int kv4_prepare(ibcu_ctx* ctx, const Kv4& c, const Kv4Columns& t, const Kv4Place& at, const Kv4Prep& w) {
+    PrepParams p = { c, t, at, w, w.q ? c.n_kv * t.ntiles : 0, t.B <= 8 ? c.n_kv : 1, ctx->kern_err };
+    const int cols = t.cols(), nb = w.q ? std::min(cols, (cols - 1) / t.group + 2) : 1;          // positions that a block may have to do with
+    const size_t smem = (w.rotate ? (size_t)nb * c.hd / 2 * sizeof(double2) : 0) + (w.q ? (size_t)cols * c.hd * sizeof(float) : 0);
+    return ibcu_launch(ctx, kv4_prep_kernel, dim3(p.qblocks + (w.k ? t.B * p.wparts : 0)), dim3(128), smem, 1, true, p);
+}
 
 extern "C" int ibcu_kv4_write(ibcu_ctx* ctx, const ibcu_kv4_t* cache, const float* k, const float* v, int row0, int pos0, int B, float theta) {
     IBCU_CHECK_CTX(ctx);
@@ -286,7 +285,7 @@ extern "C" int ibcu_kv4_write(ibcu_ctx* ctx, const ibcu_kv4_t* cache, const floa
     IBCU_REQUIRE(ctx, k && v, "ibcu_kv4_write: null pointer");
     if (int rc = check_rows(ctx, cache, row0, B, "ibcu_kv4_write")) return rc;
     if (int rc = check_rotation(ctx, pos0, B, theta, "ibcu_kv4_write")) return rc;
-    return ibcu_launch(ctx, kv4_write_kernel, dim3(B, cache->n_kv_heads, 2), dim3(64), 0, 1, true, planes(cache), k, v, row0, pos0, log2_of(theta), theta > 0.0f ? 1 : 0);
+    return kv4_prepare(ctx, planes(cache), Kv4Columns{ cache->n_kv_heads, 1, B, 0, 1 }, Kv4Place{ row0, pos0, nullptr }, Kv4Prep{ nullptr, k, v, nullptr, nullptr, log2_of(theta), theta > 0.0f });
 }
 
 extern "C" int ibcu_kv4_read(ibcu_ctx* ctx, const ibcu_kv4_t* cache, float* k, float* v, int row0, int n) {
@@ -308,9 +307,7 @@ extern "C" int ibcu_attention_kv4(ibcu_ctx* ctx, const ibcu_kv4_t* cache, const 
     IBCU_REQUIRE(ctx, q && out, "ibcu_attention_kv4: null pointer");
     if (int rc = check_rows(ctx, cache, row0, B, "ibcu_attention_kv4")) return rc;
     if (int rc = check_heads(ctx, cache, n_heads, B, "ibcu_attention_kv4")) return rc;
-    int rc = ibcu_reserve(ctx, &ctx->scratch, &ctx->scratch_bytes, (size_t)B * n_heads * sizeof(float2));
-    if (rc) return rc;
-    return attend(ctx, planes(cache), cache->decay, q, out, n_heads, row0, B, (float2*)ctx->scratch);
+    return kv4_attend(ctx, planes(cache), cache->decay, Kv4Place{ row0, 0, nullptr }, q, nullptr, nullptr, out, n_heads, B, 0.0, 0);
 }
 
 extern "C" int ibcu_attention_decode_kv4(ibcu_ctx* ctx, const ibcu_kv4_t* cache, const float* q, const float* k, const float* v, float* out,
@@ -321,14 +318,7 @@ extern "C" int ibcu_attention_decode_kv4(ibcu_ctx* ctx, const ibcu_kv4_t* cache,
     if (int rc = check_rows(ctx, cache, row0, B, "ibcu_attention_decode_kv4")) return rc;
     if (int rc = check_heads(ctx, cache, n_heads, B, "ibcu_attention_decode_kv4")) return rc;
     if (int rc = check_rotation(ctx, pos0, B, theta, "ibcu_attention_decode_kv4")) return rc;
-    const size_t st = ((size_t)B * n_heads * sizeof(float2) + 255) & ~(size_t)255;
-    int rc = ibcu_reserve(ctx, &ctx->scratch, &ctx->scratch_bytes, st + (size_t)B * n_heads * cache->head_dim * sizeof(float));
-    if (rc) return rc;
-    float* qr = (float*)((char*)ctx->scratch + st);
-    rc = ibcu_kv4_write(ctx, cache, k, v, row0, pos0, B, theta);
-    if (!rc) rc = ibcu_launch(ctx, turn_queries_kernel, dim3(B, n_heads), dim3(128), 0, 1, true, q, qr, cache->head_dim, n_heads, pos0, log2_of(theta), theta > 0.0f ? 1 : 0);
-    if (!rc) rc = attend(ctx, planes(cache), cache->decay, qr, out, n_heads, row0, B, (float2*)ctx->scratch);
-    return rc;
+    return kv4_attend(ctx, planes(cache), cache->decay, Kv4Place{ row0, pos0, nullptr }, q, k, v, out, n_heads, B, log2_of(theta), theta > 0.0f);
 }
 
 extern "C" int ibcu_kv4_evict(ibcu_ctx* ctx, const ibcu_kv4_t* src, const ibcu_kv4_t* dst, int rows, int keep, int sink, int recent, int32_t* kept) {
