@@ -26,7 +26,7 @@
 #include "common.cuh"
 #include "tc_common.cuh"
 #include "xconvert.cuh"
-#include <cudaTypedefs.h>
+#include "tc_maps.cuh"
 
 bool ibcu_push_match(ibcu_ctx* ctx, float* const* outs, int n);      // comm.cu
 void ibcu_push_fill(ibcu_ctx* ctx, GatherPush* gp, size_t bytes);
@@ -66,23 +66,12 @@ struct TqShared {
     long long bias[TQ_MAX_B];
 };
 
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-                 :: "r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
-}
-__device__ __forceinline__ void mma_i8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
-                 :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
-}
 __device__ __forceinline__ void mma_i8_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
                  "tcgen05.mma.cta_group::1.kind::i8 [%0], [%1], %2, %3, p;\n\t}"
                  :: "r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
 }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // the four digit sums of one (row, activation) as one integer
 __device__ __forceinline__ long long join_limbs(const uint32_t* a) {
@@ -512,17 +501,6 @@ __global__ void __launch_bounds__(Tq<T, Q>::THREADS, T * Q == 2 ? 2 : 1) linear_
 }
 
 // ── host ──
-using EncodeFn = PFN_cuTensorMapEncodeTiled_v12000;
-EncodeFn encode_fn() {
-    static EncodeFn fn = [] {
-        void* f = nullptr;
-        cudaDriverEntryPointQueryResult r;
-        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &r) != cudaSuccess || r != cudaDriverEntryPointSuccess) { cudaGetLastError(); f = nullptr; }
-        return (EncodeFn)f;
-    }();
-    return fn;
-}
-
 // How a call's digits are prepared: parts blocks of part_kb blocks of columns each per activation, as a cluster or not.
 struct TqPrep { bool clustered; int parts, part_kb; };
 TqPrep tq_prep(const TqCut& cut, int bits, int B, int op) {
@@ -620,7 +598,7 @@ TqCut ibcu_linear_tc_cut(int sm_count, const ibcu_linear_t* tensors, int n_tenso
 // The call as the preparation kernel and the tcgen05 kernel. Returns IBCU_DECLINED without touching the context's error when
 // the call is not its own (the caller takes the other kernels).
 int ibcu_linear_tc(ibcu_ctx* ctx, const ibcu_linear_t* tensors, int n_tensors, const float* x, int N, int B, int bits, const ibcu_prologue_t* pro, int op) {
-    EncodeFn encode = encode_fn();
+    TensorMapEncodeFn encode = tensor_map_encoder();
     const int rowbytes = bits == 8 ? N : N / 2;
     if (!encode || rowbytes % 16 || B > TQ_MAX_B) return IBCU_DECLINED;
     long total_rows = 0;

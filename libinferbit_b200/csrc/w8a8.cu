@@ -1,6 +1,10 @@
 // INT8 weights x INT8 activations with one scale per output row and one per token: a prompt's projections as integer products, any
 // number of tokens. Sums are exact 32-bit integers, so a result does not depend on how the work is cut.
 #include "common.cuh"
+#include "tc_common.cuh"
+#include "tc_maps.cuh"
+#include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -24,22 +28,239 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const float* __restr
     if (threadIdx.x == 0) scale[b] = s;
 }
 
-// a warp per output row and token
-__global__ void __launch_bounds__(256) w8a8_kernel(ibcu_linear_t t, const int8_t* __restrict__ xq, const float* __restrict__ sx, int N, int ldq) {
+// ── the product on the fifth-generation tensor cores ──
+// tcgen05.mma kind::i8: weights are the A operand, 128 output rows, tokens the B operand, up to 256; a lane of tensor memory is an output row,
+// so that a warp's store of one token's results is 128 bytes in a row. Per block of 128 columns TMA brings both operands; 32-bit
+// accumulators are two buffers of tensor memory, one being read out while the other is filled. Blocks walk the tiles, the tiles of
+// tokens of the same rows next to one another, so that weights are read from memory once.
+// Few tiles are cut along the columns, over a cluster of S blocks: block r takes the r-th part, and token t's sums meet in the
+// shared memory of block t mod S. They are whole numbers: S changes nothing in the result.
+constexpr int W8_MAX_STAGES = 12, W8_THREADS = 192, W8_TMA_WARP = 4, W8_MMA_WARP = 5;
+
+struct alignas(64) W8Maps { CUtensorMap w[4], x; };
+struct W8Params {
+    ibcu_linear_t t[4];
+    int n_tensors, tile_start[5];                    // tiles of 128 rows of tensor i: [tile_start[i], tile_start[i + 1])
+    int B, NT, token_tiles, nkb, S, stages, tmem_cols, early_weights;   // NT: tokens a tile; nkb: blocks of 128 columns; early_weights: no launch of this call writes them
+    const float* sx;
+    int* err;
+};
+struct W8Shared {
+    unsigned long long full[W8_MAX_STAGES], empty[W8_MAX_STAGES], acc_full[2], acc_empty[2], drained;
+    uint32_t tmem_base;
+    int abort_flag;
+    float sx[2][256];
+};
+
+__global__ void __launch_bounds__(W8_THREADS, 1) w8a8_tc_kernel(const __grid_constant__ W8Maps maps, const W8Params p) {
+    extern __shared__ __align__(1024) unsigned char w8_smem[];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int S = p.S, rank = (int)blockIdx.x % S, first = (int)blockIdx.x / S, step = (int)gridDim.x / S;
+    const int tiles = p.tile_start[p.n_tensors] * p.token_tiles;
+    const int k0 = (int)((long)p.nkb * rank / S), nk = (int)((long)p.nkb * (rank + 1) / S) - k0;
+    const int stage_bytes = 16384 + p.NT * 128;
+    W8Shared* sh = reinterpret_cast<W8Shared*>(w8_smem + (size_t)p.stages * stage_bytes);
+    volatile int* abort_flag = &sh->abort_flag;
+    if (tid == 0) {
+        for (int s = 0; s < W8_MAX_STAGES; s++) { mbar_init(smem_u32(&sh->full[s]), 1); mbar_init(smem_u32(&sh->empty[s]), 1); }
+        for (int s = 0; s < 2; s++) { mbar_init(smem_u32(&sh->acc_full[s]), 1); mbar_init(smem_u32(&sh->acc_empty[s]), 4); }
+        mbar_init(smem_u32(&sh->drained), 1);
+        sh->abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    auto place = [&](int tile, int& ti, int& row0, int& tok0) {
+        const int rt = tile / p.token_tiles;
+        tok0 = tile % p.token_tiles * p.NT;
+        ti = 0;
+#pragma unroll
+        for (int i = 1; i < 4; i++) if (i < p.n_tensors && rt >= p.tile_start[i]) ti = i;
+        row0 = (rt - p.tile_start[ti]) * 128;
+    };
+
+    if (warp == W8_MMA_WARP) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&sh->tmem_base)), "r"((uint32_t)p.tmem_cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        pdl_launch_dependents();                     // not before this block holds its tensor memory: see linear_tc.cu
+    }
+    if (warp == W8_TMA_WARP) {
+        // the first stages' weights are on their way before the tokens' codes are there
+        const bool one = elect_one();
+        int ti, row0, tok0;
+        const int ahead = p.early_weights && first < tiles ? min(p.stages, nk) : 0;
+        if (one && ahead) {
+            place(first, ti, row0, tok0);
+            for (int s = 0; s < ahead; s++) {
+                mbar_expect_tx(smem_u32(&sh->full[s]), (uint32_t)stage_bytes);
+                tma_load_2d(smem_u32(w8_smem + (size_t)s * stage_bytes), &maps.w[ti], (k0 + s) * 128, row0, smem_u32(&sh->full[s]));
+            }
+        }
+        __syncwarp();
+        pdl_wait();
+        if (one) {
+            asm volatile("fence.proxy.async.global;" ::: "memory");
+            int s = 0; uint32_t ph = 1;
+            bool ok = true;
+            long n = 0;
+            for (int tile = first; tile < tiles && ok; tile += step) {
+                place(tile, ti, row0, tok0);
+                for (int i = 0; i < nk; i++, n++) {
+                    const uint32_t at = smem_u32(w8_smem + (size_t)s * stage_bytes), bar = smem_u32(&sh->full[s]);
+                    if (n >= ahead) {
+                        ok = mbar_wait(smem_u32(&sh->empty[s]), ph, abort_flag, 1);
+                        if (!ok) break;
+                        mbar_expect_tx(bar, (uint32_t)stage_bytes);
+                        tma_load_2d(at, &maps.w[ti], (k0 + i) * 128, row0, bar);
+                    }
+                    tma_load_2d(at + 16384, &maps.x, (k0 + i) * 128, tok0, bar);
+                    if (++s == p.stages) { s = 0; ph ^= 1; }
+                }
+            }
+        }
+        __syncwarp();
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    if (warp != W8_TMA_WARP) asm volatile("bar.sync 1, %0;" :: "n"(W8_THREADS - 32) : "memory");
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = warp == W8_TMA_WARP ? 0u : sh->tmem_base;
+
+    if (warp == W8_MMA_WARP) {
+        pdl_wait();
+        if (elect_one()) {
+            // s32 accumulators, both operands signed bytes, 128 rows
+            const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(p.NT >> 3) << 17) | (8u << 24);
+            int s = 0, j = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int tile = first; tile < tiles && ok; tile += step, j++) {
+                ok = mbar_wait(smem_u32(&sh->acc_empty[j & 1]), (uint32_t)((j >> 1) & 1) ^ 1u, abort_flag, 2);
+                const uint32_t d = tmem + (uint32_t)((j & 1) * p.NT);
+                for (int i = 0; i < nk && ok; i++) {
+                    ok = mbar_wait(smem_u32(&sh->full[s]), ph, abort_flag, 3);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t at = smem_u32(w8_smem + (size_t)s * stage_bytes);
+                    const uint64_t ad = smem_desc_sw128(at), bd = smem_desc_sw128(at + 16384);
+#pragma unroll
+                    for (int m = 0; m < 4; m++) mma_i8_ss(d, ad + m * 2, bd + m * 2, idesc, (i | m) ? 1u : 0u);
+                    mma_commit(smem_u32(&sh->empty[s]));
+                    if (++s == p.stages) { s = 0; ph ^= 1; }
+                }
+                if (ok) mma_commit(smem_u32(&sh->acc_full[j & 1]));
+            }
+            mma_commit(smem_u32(&sh->drained));
+            mbar_wait(smem_u32(&sh->drained), 0u, abort_flag, 4);              // nothing of this block is left in the tensor pipe
+        }
+        __syncwarp();
+    } else if (warp < 4) {
+        pdl_wait();
+        int j = 0;
+        for (int tile = first; tile < tiles; tile += step, j++) {
+            int ti, row0, tok0;
+            place(tile, ti, row0, tok0);
+            const ibcu_linear_t& W = p.t[ti];
+            const int row = row0 + tid, tokens = min(p.NT, p.B - tok0);
+            const bool have = row < W.M;
+            const float sw = !have ? 0.0f : W.scales_fp32 ? reinterpret_cast<const float*>(W.scales)[row] : __half2float(reinterpret_cast<const __half*>(W.scales)[row]);
+            for (int i = tid; i < tokens; i += 128) sh->sx[j & 1][i] = __ldcg(p.sx + tok0 + i);
+            asm volatile("bar.sync 2, 128;" ::: "memory");
+            const bool there = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->acc_full[j & 1]), (uint32_t)((j >> 1) & 1), abort_flag, 5));
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (S > 1) break;                        // one tile a cluster; its parts meet below
+            if (!there) continue;                    // gave up: the barrier above is still everyone's
+            float* o = W.out + (size_t)tok0 * W.out_stride + row;
+            const uint32_t from = tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)((j & 1) * p.NT);
+            const float* sx = sh->sx[j & 1];
+            auto finish = [&](const uint32_t* acc, int c, auto count) {
+                if (!have) return;
+#pragma unroll
+                for (int u = 0; u < decltype(count)::value; u++)
+                    if (c + u < tokens) {
+                        float* to = o + (size_t)(c + u) * W.out_stride;
+                        const float y = (float)(int)acc[u] * (sw * sx[c + u]);
+                        *to = W.epilogue == IBCU_EPI_ADD ? *to + y : y;
+                    }
+            };
+            for (int c = 0; c < p.NT; c += 32) {
+                uint32_t acc[32];
+                if (p.NT - c >= 32) { tmem_ld32(from + c, acc); tmem_wait_ld(acc); finish(acc, c, std::integral_constant<int, 32>()); }
+                else { tmem_ld16(from + c, acc); finish(acc, c, std::integral_constant<int, 16>()); }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sh->acc_empty[j & 1]));
+        }
+    }
+    if (S > 1) {
+        __syncwarp();
+        cluster_arrive(); cluster_wait();            // every block of the cluster has done its products: the rings are free
+        const int TL = (p.NT + S - 1) / S;           // tokens a block
+        const uint32_t meet = smem_u32(w8_smem);     // [source block][token][row]
+        if (warp < 4 && !*abort_flag) {
+            const uint32_t from = tmem + ((uint32_t)(warp * 32) << 16);
+            for (int c = 0; c < p.NT; c += 16) {
+                uint32_t acc[16];
+                tmem_ld16(from + c, acc);
+#pragma unroll
+                for (int u = 0; u < 16; u++) peer_store_u32(meet + (uint32_t)(((rank * TL + (c + u) / S) * 128 + tid) * 4), (uint32_t)((c + u) % S), acc[u]);
+            }
+        }
+        __syncwarp();
+        cluster_arrive(); cluster_wait();
+        if (warp < 4 && !*abort_flag) {
+            int ti, row0, tok0;
+            place(first, ti, row0, tok0);
+            const ibcu_linear_t& W = p.t[ti];
+            const int row = row0 + tid, tokens = min(p.NT, p.B - tok0);
+            const int* got = reinterpret_cast<const int*>(w8_smem);
+            if (row < W.M) {
+                const float sw = W.scales_fp32 ? reinterpret_cast<const float*>(W.scales)[row] : __half2float(reinterpret_cast<const __half*>(W.scales)[row]);
+                for (int t = rank; t < tokens; t += S) {
+                    int sum = 0;
+                    for (int k = 0; k < S; k++) sum += got[(k * TL + t / S) * 128 + tid];
+                    float* to = W.out + (size_t)(tok0 + t) * W.out_stride + row;
+                    const float y = (float)sum * (sw * sh->sx[0][t]);
+                    *to = W.epilogue == IBCU_EPI_ADD ? *to + y : y;
+                }
+            }
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == W8_MMA_WARP) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"((uint32_t)p.tmem_cols) : "memory");
+    }
+    if (tid == 0 && sh->abort_flag) {
+        *p.err = 420 + sh->abort_flag;
+        for (int i = 0; i < 1000; i++) __nanosleep(1000);      // copies still on their way into this block's shared memory land before it goes
+    }
+}
+
+// Rows of `n` bytes that begin anywhere, `from` apart, into rows `to` apart (a multiple of 16): TMA wants rows that start on 16 bytes.
+__global__ void __launch_bounds__(256) align_rows_kernel(const uint8_t* __restrict__ src, long from, uint8_t* __restrict__ dst, long to, int n, long rows) {
     pdl_launch_dependents();
     pdl_wait();
-    const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    const size_t b = blockIdx.y;
-    if (row >= t.M) return;
-    const int8_t* w = (const int8_t*)t.w + (size_t)row * N;
-    int sum = 0;
-    for (int i = lane; i < N; i += 32) sum += (int)w[i] * (int)xq[b * ldq + i];
-    sum = __reduce_add_sync(0xffffffffu, sum);
-    if (lane == 0) {
-        const float sw = t.scales_fp32 ? ((const float*)t.scales)[row] : __half2float(((const __half*)t.scales)[row]);
-        float* o = t.out + b * t.out_stride + row;
-        const float y = (float)sum * (sw * sx[b]);
-        *o = t.epilogue == IBCU_EPI_ADD ? *o + y : y;
+    const int per = (int)(to / 16);
+    for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < rows * per; e += (long)gridDim.x * 256) {
+        const long r = e / per;
+        const int c = (int)(e % per) * 16;
+        const uint8_t* a = src + r * from + c;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (c + 16 < n) {                                     // aligned words and a shift; the last word is not past the row's end
+            const uint32_t* w = reinterpret_cast<const uint32_t*>((uintptr_t)a & ~(uintptr_t)3);
+            const uint32_t sh = (uint32_t)((uintptr_t)a & 3) * 8;
+            uint32_t x[5];
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = w[i];
+            x[4] = sh ? w[4] : 0u;
+            v = make_uint4(__funnelshift_r(x[0], x[1], sh), __funnelshift_r(x[1], x[2], sh), __funnelshift_r(x[2], x[3], sh), __funnelshift_r(x[3], x[4], sh));
+        } else {
+            uint8_t b[16];
+            for (int i = 0; i < 16; i++) b[i] = c + i < n ? a[i] : (uint8_t)0;
+            memcpy(&v, b, 16);
+        }
+        *reinterpret_cast<uint4*>(dst + r * to + c) = v;
     }
 }
 
@@ -54,14 +275,73 @@ int check_call(ibcu_ctx* ctx, const ibcu_linear_t* ts, int n, int N, int B, cons
     return IBCU_OK;
 }
 
-int product(ibcu_ctx* ctx, const ibcu_linear_t* ts, int n, const int8_t* xq, const float* sx, int N, int ldq, int B) {
-    for (int i = 0; i < n; i++)
-        for (int b = 0; b < B; b += 65535) {
-            ibcu_linear_t t = ts[i];
-            t.out += (size_t)b * t.out_stride;
-            if (int rc = ibcu_launch(ctx, w8a8_kernel, dim3((t.M + 7) / 8, B - b < 65535 ? B - b : 65535), dim3(256), 0, 1, true, t, xq + (size_t)b * ldq, sx + b, N, ldq)) return rc;
+// How a call is cut: tokens in tiles of equal size (up to 256), and columns over S blocks where the tiles leave SMs idle.
+struct W8Cut { int NT, token_tiles, S; };
+W8Cut w8_cut(int sm_count, long row_tiles, int nkb, int B) {
+    W8Cut best = { 0, 0, 1 };
+    double least = 1e30;
+    for (int n = (B + 255) / 256; n <= (B + 255) / 256 + 3; n++) {
+        const int NT = ((B + n - 1) / n + 15) / 16 * 16, tt = (B + NT - 1) / NT;
+        for (int S = 1; S <= 8; S *= 2) {
+            if (S > 1 && (row_tiles * tt * S > sm_count || nkb < 4 * S)) break;
+            const double waves = (double)((row_tiles * tt * S + sm_count - 1) / sm_count);
+            // a block of columns takes the tensor core NT / 2 cycles, or as long as its bytes are on their way; sums of S blocks that meet cost their exchange
+            const double t = waves * ((double)((nkb + S - 1) / S) * (NT < 96 ? 72 + NT / 4 : 48 + NT / 2) + (S > 1 ? 1500 + NT * 8 : 600 + NT * 4));
+            if (t < least) { least = t; best = { NT, tt, S }; }
         }
-    return IBCU_OK;
+    }
+    return best;
+}
+
+int product(ibcu_ctx* ctx, const ibcu_linear_t* ts, int n, const int8_t* xq, const float* sx, int N, int ldq, int B, const char* call) {
+    const size_t pitch = (N + 15) & ~15;
+    IBCU_REQUIRE(ctx, tensor_map_encoder(), "%s: the driver has no tensor maps", call);
+    // operands whose rows do not start on 16 bytes: copies whose rows do
+    size_t need = 0, at[5] = {};
+    bool copy[5] = {};
+    for (int i = 0; i < n; i++)
+        if ((copy[i] = N % 16 || ((uintptr_t)ts[i].w & 15))) { at[i] = need; need += ((size_t)ts[i].M * pitch + 255) & ~(size_t)255; }
+    if ((copy[4] = ldq % 16 || ((uintptr_t)xq & 15))) { at[4] = need; need += ((size_t)B * pitch + 255) & ~(size_t)255; }
+    if (need) {
+        if (int rc = ibcu_reserve(ctx, &ctx->scratch, &ctx->scratch_bytes, need)) return rc;
+        for (int i = 0; i < 5; i++) {
+            if (!copy[i]) continue;
+            const long rows = i < 4 ? ts[i].M : B;
+            const int grid = (int)std::min((rows * (long)(pitch / 16) + 255) / 256, 16L * ctx->sm_count);
+            if (int rc = ibcu_launch(ctx, align_rows_kernel, dim3(grid), dim3(256), 0, 1, true, (const uint8_t*)(i < 4 ? ts[i].w : xq), (long)(i < 4 ? N : ldq),
+                                     (uint8_t*)ctx->scratch + at[i], (long)pitch, N, rows)) return rc;
+        }
+    }
+    W8Maps maps;
+    W8Params p;
+    memset(&p, 0, sizeof p);
+    bool ok = true;
+    p.early_weights = 1;
+    for (int i = 0; i < n; i++) {
+        p.t[i] = ts[i];
+        p.tile_start[i + 1] = p.tile_start[i] + (ts[i].M + 127) / 128;
+        if (copy[i]) p.early_weights = 0;
+        ok = ok && tensor_map_bytes(&maps.w[i], copy[i] ? (uint8_t*)ctx->scratch + at[i] : (const uint8_t*)ts[i].w, ts[i].M, N, copy[i] ? (long)pitch : N, 128);
+    }
+    for (int i = n; i < 4; i++) maps.w[i] = maps.w[0];
+    p.n_tensors = n; p.B = B; p.nkb = (N + 127) / 128; p.sx = sx; p.err = ctx->kern_err;
+    const long row_tiles = p.tile_start[n];
+    const W8Cut cut = w8_cut(ctx->sm_count, row_tiles, p.nkb, B);
+    p.NT = cut.NT; p.token_tiles = cut.token_tiles; p.S = cut.S;
+    ok = ok && tensor_map_bytes(&maps.x, copy[4] ? (uint8_t*)ctx->scratch + at[4] : (const uint8_t*)xq, B, N, copy[4] ? (long)pitch : ldq, p.NT);
+    IBCU_REQUIRE(ctx, ok, "%s: no tensor map for N=%d", call, N);
+    const int stage = 16384 + p.NT * 128, room = 227 * 1024 - (int)sizeof(W8Shared) - 1024;
+    p.stages = std::min(std::min(W8_MAX_STAGES, room / stage), std::max(2, (p.nkb + p.S - 1) / p.S * 2));
+    size_t rings = (size_t)p.stages * stage;
+    const size_t meet = p.S > 1 ? (size_t)p.S * ((p.NT + p.S - 1) / p.S) * 512 : 0;
+    if (rings < meet) { p.stages = (int)((meet + stage - 1) / stage); rings = (size_t)p.stages * stage; }
+    for (p.tmem_cols = 32; p.tmem_cols < 2 * p.NT; p.tmem_cols *= 2) {}
+    const long tiles = row_tiles * p.token_tiles;
+    const int grid = p.S > 1 ? (int)tiles * p.S : (int)std::min(tiles, (long)ctx->sm_count);
+    static SmemOptIn opt;
+    const size_t smem = rings + sizeof(W8Shared);
+    if (int rc = ibcu_allow_smem(ctx, opt, w8a8_tc_kernel, smem)) return rc;
+    return ibcu_launch(ctx, w8a8_tc_kernel, dim3(grid), dim3(W8_THREADS), smem, p.S, true, maps, p);
 }
 
 }  // namespace
@@ -77,7 +357,7 @@ extern "C" int ibcu_linear_w8a8(ibcu_ctx* ctx, const ibcu_linear_t* tensors, int
     IBCU_CHECK_CTX(ctx);
     if (int rc = check_call(ctx, tensors, n_tensors, N, B, "ibcu_linear_w8a8")) return rc;
     IBCU_REQUIRE(ctx, xq && sx, "ibcu_linear_w8a8: null pointer");
-    return product(ctx, tensors, n_tensors, xq, sx, N, N, B);
+    return product(ctx, tensors, n_tensors, xq, sx, N, N, B, "ibcu_linear_w8a8");
 }
 
 extern "C" int ibcu_linear_w8a8_fp32(ibcu_ctx* ctx, const ibcu_linear_t* tensors, int n_tensors, const float* x, int N, int B) {
@@ -91,6 +371,6 @@ extern "C" int ibcu_linear_w8a8_fp32(ibcu_ctx* ctx, const ibcu_linear_t* tensors
     int8_t* q = (int8_t*)ctx->xpack;
     float* sx = (float*)((char*)ctx->xpack + qb);
     rc = ibcu_launch(ctx, quantize_rows_kernel, dim3(B), dim3(256), 0, 1, true, x, q, sx, N, ldq);
-    if (!rc) rc = product(ctx, tensors, n_tensors, q, sx, N, ldq, B);
+    if (!rc) rc = product(ctx, tensors, n_tensors, q, sx, N, ldq, B, "ibcu_linear_w8a8_fp32");
     return rc;
 }
