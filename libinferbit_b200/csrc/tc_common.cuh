@@ -115,9 +115,9 @@ __device__ __forceinline__ void mma_i8_ss(uint32_t d_tmem, uint64_t a_desc, uint
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-// a word into the shared memory of block `rank` of the cluster, at the address that `addr` has in this block's (a barrier of the cluster has said that it runs)
-__device__ __forceinline__ void peer_store_u32(uint32_t addr, uint32_t rank, uint32_t v) {
+// four words into the shared memory of block `rank` of the cluster, at the address that `addr` has in this block's (a barrier of the cluster has said that it runs)
+__device__ __forceinline__ void peer_store_u32x4(uint32_t addr, uint32_t rank, const uint32_t* v) {
     uint32_t remote;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-    asm volatile("st.shared::cluster.u32 [%0], %1;" :: "r"(remote), "r"(v) : "memory");
+    asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" :: "r"(remote), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
 }

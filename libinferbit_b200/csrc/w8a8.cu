@@ -8,34 +8,61 @@
 
 namespace {
 
-// one block per token: scale = max|x| * (1 / 127), codes rint(x * (1 / scale)); columns N..ldq-1 of the codes are zero
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const float* __restrict__ x, int8_t* __restrict__ q, float* __restrict__ scale, int N, int ldq) {
-    __shared__ uint32_t red[8];
+// one block per token: scale = max|x| * (1 / 127), codes rint(x * (1 / scale)); columns N..ldq-1 of the codes are zero. VEC: rows of whole
+// float4s, which the thread keeps between the maximum and the codes (up to QR_KEEP of them; further ones are read twice). Bound by memory: 511 rows of 14336
+// took 12 us one value at a time.
+constexpr int QR_KEEP = 8;
+template <bool VEC>
+__global__ void __launch_bounds__(512) quantize_rows_kernel(const float* __restrict__ x, int8_t* __restrict__ q, float* __restrict__ scale, int N, int ldq) {
+    __shared__ uint32_t red[16];
     pdl_launch_dependents();
     pdl_wait();
     const size_t b = blockIdx.x;
     const float* xb = x + b * N;
+    int8_t* qb = q + b * ldq;
+    const int tid = threadIdx.x, nth = blockDim.x, n4 = N / 4;
+    const float4* x4 = reinterpret_cast<const float4*>(xb);
+    auto size4 = [](const float4& v) { return max(max(__float_as_uint(v.x) & 0x7FFFFFFFu, __float_as_uint(v.y) & 0x7FFFFFFFu), max(__float_as_uint(v.z) & 0x7FFFFFFFu, __float_as_uint(v.w) & 0x7FFFFFFFu)); };
+    float4 kept[QR_KEEP];
     uint32_t m = 0;
-    for (int i = threadIdx.x; i < N; i += 256) m = max(m, __float_as_uint(xb[i]) & 0x7FFFFFFFu);
+    if (VEC) {
+#pragma unroll
+        for (int u = 0; u < QR_KEEP; u++) kept[u] = tid + u * nth < n4 ? __ldcg(x4 + tid + u * nth) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int u = 0; u < QR_KEEP; u++) m = max(m, size4(kept[u]));
+        for (int i = tid + QR_KEEP * nth; i < n4; i += nth) m = max(m, size4(__ldcg(x4 + i)));
+    } else {
+        for (int i = tid; i < N; i += nth) m = max(m, __float_as_uint(xb[i]) & 0x7FFFFFFFu);
+    }
     m = __reduce_max_sync(0xffffffffu, m);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+    if ((tid & 31) == 0) red[tid >> 5] = m;
     __syncthreads();
-    for (int w = 0; w < 8; w++) m = max(m, red[w]);
+    for (int w = 0; w < nth / 32; w++) m = max(m, red[w]);
     float s = __fmul_rn(__uint_as_float(m), 1.0f / 127.0f), inv = __fdiv_rn(1.0f, s);
     if (m < 0x0D800000u) { s = 0.0f; inv = 0.0f; }            // below 2^-100: zeros
     if (m >= 0x7F800000u) { s = __uint_as_float(0x7FFFFFFFu); inv = 0.0f; }      // NaN or Inf: all results of the token are NaN
-    for (int i = threadIdx.x; i < ldq; i += 256) q[b * ldq + i] = i < N && inv > 0.0f ? (int8_t)(int)rintf(__fmul_rn(xb[i], inv)) : (int8_t)0;
-    if (threadIdx.x == 0) scale[b] = s;
+    auto code = [&](float v) { return inv > 0.0f ? (int)rintf(__fmul_rn(v, inv)) & 255 : 0; };
+    if (VEC) {
+        auto put = [&](int i, const float4& v) { reinterpret_cast<uint32_t*>(qb)[i] = (uint32_t)(code(v.x) | code(v.y) << 8 | code(v.z) << 16 | code(v.w) << 24); };
+#pragma unroll
+        for (int u = 0; u < QR_KEEP; u++) if (tid + u * nth < n4) put(tid + u * nth, kept[u]);
+        for (int i = tid + QR_KEEP * nth; i < n4; i += nth) put(i, __ldcg(x4 + i));
+        for (int i = N + tid; i < ldq; i += nth) qb[i] = 0;
+    } else {
+        for (int i = tid; i < ldq; i += nth) qb[i] = i < N ? (int8_t)code(xb[i]) : (int8_t)0;
+    }
+    if (tid == 0) scale[b] = s;
 }
 
 // ── the product on the fifth-generation tensor cores ──
 // tcgen05.mma kind::i8: weights are the A operand, 128 output rows, tokens the B operand, up to 256; a lane of tensor memory is an output row,
 // so that a warp's store of one token's results is 128 bytes in a row. Per block of 128 columns TMA brings both operands; 32-bit
 // accumulators are two buffers of tensor memory, one being read out while the other is filled. Blocks walk the tiles, the tiles of
-// tokens of the same rows next to one another, so that weights are read from memory once.
-// Few tiles are cut along the columns, over a cluster of S blocks: block r takes the r-th part, and token t's sums meet in the
-// shared memory of block t mod S. They are whole numbers: S changes nothing in the result.
-constexpr int W8_MAX_STAGES = 12, W8_THREADS = 192, W8_TMA_WARP = 4, W8_MMA_WARP = 5;
+// tokens of the same rows next to one another, so that weights are read from memory once. Eight warps write results out: with four, two tensors of
+// 14336 x 4096 at 2048 tokens took 263 us, 174 of them without the stores.
+// Few tiles are cut along the columns, over a cluster of S blocks: block r takes the r-th part, and the sums of the r-th TL tokens meet in
+// its shared memory. They are whole numbers: S changes nothing in the result.
+constexpr int W8_MAX_STAGES = 12, W8_OUT_WARPS = 8, W8_TMA_WARP = W8_OUT_WARPS, W8_MMA_WARP = W8_OUT_WARPS + 1, W8_THREADS = (W8_OUT_WARPS + 2) * 32;
 
 struct alignas(64) W8Maps { CUtensorMap w[4], x; };
 struct W8Params {
@@ -52,6 +79,9 @@ struct W8Shared {
     float sx[2][256];
 };
 
+// tokens of a tile whose sums meet in one block of S, in fours
+__host__ __device__ __forceinline__ int w8_share(int NT, int S) { return (NT / 4 + S - 1) / S * 4; }
+
 __global__ void __launch_bounds__(W8_THREADS, 1) w8a8_tc_kernel(const __grid_constant__ W8Maps maps, const W8Params p) {
     extern __shared__ __align__(1024) unsigned char w8_smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -63,7 +93,7 @@ __global__ void __launch_bounds__(W8_THREADS, 1) w8a8_tc_kernel(const __grid_con
     volatile int* abort_flag = &sh->abort_flag;
     if (tid == 0) {
         for (int s = 0; s < W8_MAX_STAGES; s++) { mbar_init(smem_u32(&sh->full[s]), 1); mbar_init(smem_u32(&sh->empty[s]), 1); }
-        for (int s = 0; s < 2; s++) { mbar_init(smem_u32(&sh->acc_full[s]), 1); mbar_init(smem_u32(&sh->acc_empty[s]), 4); }
+        for (int s = 0; s < 2; s++) { mbar_init(smem_u32(&sh->acc_full[s]), 1); mbar_init(smem_u32(&sh->acc_empty[s]), W8_OUT_WARPS); }
         mbar_init(smem_u32(&sh->drained), 1);
         sh->abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -76,6 +106,13 @@ __global__ void __launch_bounds__(W8_THREADS, 1) w8a8_tc_kernel(const __grid_con
 #pragma unroll
         for (int i = 1; i < 4; i++) if (i < p.n_tensors && rt >= p.tile_start[i]) ti = i;
         row0 = (rt - p.tile_start[ti]) * 128;
+    };
+
+    // Blocks at work at the same time start at different blocks of columns: those that share rows or tokens would otherwise read the same
+    // lines at the same moment and queue for them. (Integer sums: the order is free.)
+    auto column = [&](int tile, int i) {
+        const int k = i + (tile / p.token_tiles + tile % p.token_tiles * 4) % nk;
+        return (k0 + (k < nk ? k : k - nk)) * 128;
     };
 
     if (warp == W8_MMA_WARP) {
@@ -92,7 +129,7 @@ __global__ void __launch_bounds__(W8_THREADS, 1) w8a8_tc_kernel(const __grid_con
             place(first, ti, row0, tok0);
             for (int s = 0; s < ahead; s++) {
                 mbar_expect_tx(smem_u32(&sh->full[s]), (uint32_t)stage_bytes);
-                tma_load_2d(smem_u32(w8_smem + (size_t)s * stage_bytes), &maps.w[ti], (k0 + s) * 128, row0, smem_u32(&sh->full[s]));
+                tma_load_2d(smem_u32(w8_smem + (size_t)s * stage_bytes), &maps.w[ti], column(first, s), row0, smem_u32(&sh->full[s]));
             }
         }
         __syncwarp();
@@ -110,9 +147,9 @@ __global__ void __launch_bounds__(W8_THREADS, 1) w8a8_tc_kernel(const __grid_con
                         ok = mbar_wait(smem_u32(&sh->empty[s]), ph, abort_flag, 1);
                         if (!ok) break;
                         mbar_expect_tx(bar, (uint32_t)stage_bytes);
-                        tma_load_2d(at, &maps.w[ti], (k0 + i) * 128, row0, bar);
+                        tma_load_2d(at, &maps.w[ti], column(tile, i), row0, bar);
                     }
-                    tma_load_2d(at + 16384, &maps.x, (k0 + i) * 128, tok0, bar);
+                    tma_load_2d(at + 16384, &maps.x, column(tile, i), tok0, bar);
                     if (++s == p.stages) { s = 0; ph ^= 1; }
                 }
             }
@@ -152,39 +189,52 @@ __global__ void __launch_bounds__(W8_THREADS, 1) w8a8_tc_kernel(const __grid_con
             mbar_wait(smem_u32(&sh->drained), 0u, abort_flag, 4);              // nothing of this block is left in the tensor pipe
         }
         __syncwarp();
-    } else if (warp < 4) {
+    } else if (warp < W8_OUT_WARPS) {
         pdl_wait();
         int j = 0;
         for (int tile = first; tile < tiles; tile += step, j++) {
             int ti, row0, tok0;
             place(tile, ti, row0, tok0);
             const ibcu_linear_t& W = p.t[ti];
-            const int row = row0 + tid, tokens = min(p.NT, p.B - tok0);
+            const int row = row0 + (tid & 127), tokens = min(p.NT, p.B - tok0);
             const bool have = row < W.M;
             const float sw = !have ? 0.0f : W.scales_fp32 ? reinterpret_cast<const float*>(W.scales)[row] : __half2float(reinterpret_cast<const __half*>(W.scales)[row]);
-            for (int i = tid; i < tokens; i += 128) sh->sx[j & 1][i] = __ldcg(p.sx + tok0 + i);
-            asm volatile("bar.sync 2, 128;" ::: "memory");
+            float* sx = sh->sx[j & 1];
+            if (tid < p.NT) sx[tid] = tid < tokens ? __ldcg(p.sx + tok0 + tid) : 0.0f;
+            asm volatile("bar.sync 2, %0;" :: "n"(W8_OUT_WARPS * 32) : "memory");
             const bool there = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->acc_full[j & 1]), (uint32_t)((j >> 1) & 1), abort_flag, 5));
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (S > 1) break;                        // one tile a cluster; its parts meet below
             if (!there) continue;                    // gave up: the barrier above is still everyone's
-            float* o = W.out + (size_t)tok0 * W.out_stride + row;
-            const uint32_t from = tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)((j & 1) * p.NT);
-            const float* sx = sh->sx[j & 1];
-            auto finish = [&](const uint32_t* acc, int c, auto count) {
-                if (!have) return;
-#pragma unroll
-                for (int u = 0; u < decltype(count)::value; u++)
-                    if (c + u < tokens) {
-                        float* to = o + (size_t)(c + u) * W.out_stride;
-                        const float y = (float)(int)acc[u] * (sw * sx[c + u]);
-                        *to = W.epilogue == IBCU_EPI_ADD ? *to + y : y;
-                    }
-            };
-            for (int c = 0; c < p.NT; c += 32) {
+            const size_t ld = (size_t)W.out_stride;
+            const uint32_t from = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)((j & 1) * p.NT);
+            for (int c = (warp >> 2) * 32; c < p.NT; c += W8_OUT_WARPS * 8) {          // 32 tokens at a time, or the last 16
                 uint32_t acc[32];
-                if (p.NT - c >= 32) { tmem_ld32(from + c, acc); tmem_wait_ld(acc); finish(acc, c, std::integral_constant<int, 32>()); }
-                else { tmem_ld16(from + c, acc); finish(acc, c, std::integral_constant<int, 16>()); }
+                if (p.NT - c >= 32) { tmem_ld32(from + c, acc); tmem_wait_ld(acc); }
+                else tmem_ld16(from + c, acc);
+                if (!have) continue;
+                const int n = min(32, tokens - c);
+                float* o = W.out + (size_t)(tok0 + c) * ld + row;
+                auto finish = [&](auto whole, auto add) {
+#pragma unroll
+                    for (int u0 = 0; u0 < 32; u0 += 8) {
+                        float old[8];
+#pragma unroll
+                        for (int u = 0; u < 8; u++) old[u] = decltype(add)::value && (decltype(whole)::value || u0 + u < n) ? o[(size_t)u * ld] : 0.0f;
+                        const float4 s0 = *reinterpret_cast<const float4*>(sx + c + u0), s1 = *reinterpret_cast<const float4*>(sx + c + u0 + 4);
+                        const float f[8] = { s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w };
+#pragma unroll
+                        for (int u = 0; u < 8; u++) {
+                            const float y = (float)(int)acc[u0 + u] * (sw * f[u]);
+                            if (decltype(whole)::value || u0 + u < n) o[(size_t)u * ld] = decltype(add)::value ? old[u] + y : y;
+                        }
+                        o += 8 * ld;
+                        if (!decltype(whole)::value && u0 + 8 >= n) break;
+                    }
+                };
+                if (W.epilogue == IBCU_EPI_ADD) { if (n == 32) finish(std::true_type(), std::true_type()); else finish(std::false_type(), std::true_type()); }
+                else if (n == 32) finish(std::true_type(), std::false_type());
+                else if (n > 0) finish(std::false_type(), std::false_type());
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
@@ -194,33 +244,40 @@ __global__ void __launch_bounds__(W8_THREADS, 1) w8a8_tc_kernel(const __grid_con
     if (S > 1) {
         __syncwarp();
         cluster_arrive(); cluster_wait();            // every block of the cluster has done its products: the rings are free
-        const int TL = (p.NT + S - 1) / S;           // tokens a block
-        const uint32_t meet = smem_u32(w8_smem);     // [source block][token][row]
-        if (warp < 4 && !*abort_flag) {
-            const uint32_t from = tmem + ((uint32_t)(warp * 32) << 16);
-            for (int c = 0; c < p.NT; c += 16) {
+        const int TL = w8_share(p.NT, S);            // tokens a block
+        const uint32_t meet = smem_u32(w8_smem);     // [source block][4 tokens][row][token]
+        const int r = tid & 127;
+        if (warp < W8_OUT_WARPS && !*abort_flag) {
+            const uint32_t from = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+            for (int c = (warp >> 2) * 16; c < p.NT; c += W8_OUT_WARPS * 4) {
                 uint32_t acc[16];
                 tmem_ld16(from + c, acc);
 #pragma unroll
-                for (int u = 0; u < 16; u++) peer_store_u32(meet + (uint32_t)(((rank * TL + (c + u) / S) * 128 + tid) * 4), (uint32_t)((c + u) % S), acc[u]);
+                for (int u = 0; u < 16; u += 4)
+                    peer_store_u32x4(meet + (uint32_t)((((rank * TL + (c + u) % TL) / 4) * 128 + r) * 16), (uint32_t)((c + u) / TL), acc + u);
             }
         }
         __syncwarp();
         cluster_arrive(); cluster_wait();
-        if (warp < 4 && !*abort_flag) {
+        if (warp < W8_OUT_WARPS && !*abort_flag) {
             int ti, row0, tok0;
             place(first, ti, row0, tok0);
             const ibcu_linear_t& W = p.t[ti];
-            const int row = row0 + tid, tokens = min(p.NT, p.B - tok0);
-            const int* got = reinterpret_cast<const int*>(w8_smem);
+            const int row = row0 + r, mine = min(TL, min(p.NT, p.B - tok0) - rank * TL);
+            const int4* got = reinterpret_cast<const int4*>(w8_smem);
             if (row < W.M) {
                 const float sw = W.scales_fp32 ? reinterpret_cast<const float*>(W.scales)[row] : __half2float(reinterpret_cast<const __half*>(W.scales)[row]);
-                for (int t = rank; t < tokens; t += S) {
-                    int sum = 0;
-                    for (int k = 0; k < S; k++) sum += got[(k * TL + t / S) * 128 + tid];
-                    float* to = W.out + (size_t)(tok0 + t) * W.out_stride + row;
-                    const float y = (float)sum * (sw * sh->sx[0][t]);
-                    *to = W.epilogue == IBCU_EPI_ADD ? *to + y : y;
+                for (int t = (tid >> 7) * 4; t < mine; t += 8) {
+                    int4 sum = got[(t / 4) * 128 + r];
+                    for (int k = 1; k < S; k++) { const int4 v = got[((k * TL + t) / 4) * 128 + r]; sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w; }
+                    const int four[4] = { sum.x, sum.y, sum.z, sum.w };
+#pragma unroll
+                    for (int u = 0; u < 4; u++)
+                        if (t + u < mine) {
+                            float* to = W.out + (size_t)(tok0 + rank * TL + t + u) * W.out_stride + row;
+                            const float y = (float)four[u] * (sw * sh->sx[0][rank * TL + t + u]);
+                            *to = W.epilogue == IBCU_EPI_ADD ? *to + y : y;
+                        }
                 }
             }
         }
@@ -273,6 +330,11 @@ int check_call(ibcu_ctx* ctx, const ibcu_linear_t* ts, int n, int N, int B, cons
         IBCU_REQUIRE(ctx, ts[i].epilogue == IBCU_EPI_STORE || ts[i].epilogue == IBCU_EPI_ADD, "%s: epilogue=%d", call, ts[i].epilogue);
     }
     return IBCU_OK;
+}
+
+int quantize(ibcu_ctx* ctx, const float* x, int8_t* q, float* scale, int N, int ldq, int B) {
+    const bool vec = N % 4 == 0 && ldq % 4 == 0 && ((uintptr_t)x & 15) == 0 && ((uintptr_t)q & 3) == 0;
+    return ibcu_launch(ctx, vec ? quantize_rows_kernel<true> : quantize_rows_kernel<false>, dim3(B), dim3(N > 8192 || (B < ctx->sm_count && N >= 2048) ? 512 : 256), 0, 1, true, x, q, scale, N, ldq);
 }
 
 // How a call is cut: tokens in tiles of equal size (up to 256), and columns over S blocks where the tiles leave SMs idle.
@@ -333,7 +395,7 @@ int product(ibcu_ctx* ctx, const ibcu_linear_t* ts, int n, const int8_t* xq, con
     const int stage = 16384 + p.NT * 128, room = 227 * 1024 - (int)sizeof(W8Shared) - 1024;
     p.stages = std::min(std::min(W8_MAX_STAGES, room / stage), std::max(2, (p.nkb + p.S - 1) / p.S * 2));
     size_t rings = (size_t)p.stages * stage;
-    const size_t meet = p.S > 1 ? (size_t)p.S * ((p.NT + p.S - 1) / p.S) * 512 : 0;
+    const size_t meet = p.S > 1 ? (size_t)p.S * w8_share(p.NT, p.S) * 512 : 0;
     if (rings < meet) { p.stages = (int)((meet + stage - 1) / stage); rings = (size_t)p.stages * stage; }
     for (p.tmem_cols = 32; p.tmem_cols < 2 * p.NT; p.tmem_cols *= 2) {}
     const long tiles = row_tiles * p.token_tiles;
@@ -350,7 +412,7 @@ extern "C" int ibcu_quantize_rows_int8(ibcu_ctx* ctx, const float* x, int8_t* q,
     IBCU_CHECK_CTX(ctx);
     IBCU_REQUIRE(ctx, x && q && scale, "ibcu_quantize_rows_int8: null pointer");
     IBCU_REQUIRE(ctx, N >= 1 && B >= 1, "ibcu_quantize_rows_int8: N=%d B=%d", N, B);
-    return ibcu_launch(ctx, quantize_rows_kernel, dim3(B), dim3(256), 0, 1, true, x, q, scale, N, N);
+    return quantize(ctx, x, q, scale, N, N, B);
 }
 
 extern "C" int ibcu_linear_w8a8(ibcu_ctx* ctx, const ibcu_linear_t* tensors, int n_tensors, const int8_t* xq, const float* sx, int N, int B) {
@@ -370,7 +432,7 @@ extern "C" int ibcu_linear_w8a8_fp32(ibcu_ctx* ctx, const ibcu_linear_t* tensors
     if (rc) return rc;
     int8_t* q = (int8_t*)ctx->xpack;
     float* sx = (float*)((char*)ctx->xpack + qb);
-    rc = ibcu_launch(ctx, quantize_rows_kernel, dim3(B), dim3(256), 0, 1, true, x, q, sx, N, ldq);
+    rc = quantize(ctx, x, q, sx, N, ldq, B);
     if (!rc) rc = product(ctx, tensors, n_tensors, q, sx, N, ldq, B, "ibcu_linear_w8a8_fp32");
     return rc;
 }
