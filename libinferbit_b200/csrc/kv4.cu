@@ -7,14 +7,18 @@
 // the lanes of a matrix instruction take them: a key row is four pieces, piece t with values 8t..8t+7 of group 0, then of group 1, and
 // so on; a value row is eight pieces, piece g with values 4g..4g+3 of every group. Two values a byte, the first in the low nibble.
 #include "kv4.cuh"
+#include "tc_common.cuh"
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace {
 
 __device__ __forceinline__ int key_place(int i, int ng) { return ((i & 31) / 8 * ng + i / 32) * 8 + (i & 7); }      // where value i of a row lies
 __device__ __forceinline__ int value_place(int i, int ng) { return ((i & 31) / 4 * ng + i / 32) * 4 + (i & 3); }
-__device__ __forceinline__ float held(const uint8_t* row, int place, float s) { return (float)((row[place >> 1] >> ((place & 1) * 4) & 15) - 8) * s; }
+__device__ __forceinline__ float held(const uint8_t* row, int place, float s) { return (float)((__ldcg(row + (place >> 1)) >> ((place & 1) * 4) & 15) - 8) * s; }
+
+__device__ __forceinline__ float scale_at(const Kv4& c, size_t i) { return __half2float(__ushort_as_half(__ldcg(reinterpret_cast<const unsigned short*>(c.scale) + i))); }
 
 // A group's scale and the factor that turns its values into codes; amax_bits: the largest magnitude's bits (NaN and Inf above all)
 __device__ __forceinline__ __half group_scale(uint32_t amax_bits, float& inv) {
@@ -72,7 +76,7 @@ __global__ void __launch_bounds__(128) kv4_prep_kernel(const PrepParams p) {
             const int d = 32 * j + 8 * t;
             float x[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = on ? src[d + i] : 0.0f;
+            for (int i = 0; i < 8; i++) x[i] = on ? __ldcg(src + d + i) : 0.0f;
             if (on && p.w.rotate) {
 #pragma unroll
                 for (int i = 0; i < 8; i += 2) turn_pair(x[i], x[i + 1], b, (d + i) / 2);
@@ -122,7 +126,7 @@ __global__ void __launch_bounds__(128) kv4_prep_kernel(const PrepParams p) {
         const bool key = e < heads * quads;
         const int f = key ? e : e - heads * quads, h = wb % p.wparts + f / quads * p.wparts, i = f % quads * 4;
         const float* src = (key ? p.w.k : p.w.v) + ((size_t)b0 * p.c.n_kv + h) * hd + i;
-        float x[4] = { src[0], src[1], src[2], src[3] };
+        float x[4] = { __ldcg(src), __ldcg(src + 1), __ldcg(src + 2), __ldcg(src + 3) };
         if (key && p.w.rotate) { turn_pair(x[0], x[1], b0, i / 2); turn_pair(x[2], x[3], b0, i / 2 + 1); }
         uint32_t m = 0;
 #pragma unroll
@@ -151,8 +155,8 @@ __global__ void __launch_bounds__(128) kv4_read_kernel(Kv4 c, float* __restrict_
     const size_t row = c.row(h, row0 + b);
     for (int i = threadIdx.x; i < c.hd; i += blockDim.x) {
         const size_t o = ((size_t)b * c.n_kv + h) * c.hd + i;
-        k[o] = held(c.k + row * (c.hd / 2), key_place(i, ng), __half2float(c.scale[row * 2 * ng + i / 32]));
-        v[o] = held(c.v + row * (c.hd / 2), value_place(i, ng), __half2float(c.scale[row * 2 * ng + ng + i / 32]));
+        k[o] = held(c.k + row * (c.hd / 2), key_place(i, ng), scale_at(c, row * 2 * ng + i / 32));
+        v[o] = held(c.v + row * (c.hd / 2), value_place(i, ng), scale_at(c, row * 2 * ng + ng + i / 32));
     }
 }
 
@@ -164,89 +168,158 @@ __device__ __forceinline__ uint32_t weight_order(float w) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// one block per KV head: the `want` rows of [lo, hi) with the largest weights, equal ones from the lowest row, beside all rows outside it,
-// in ascending order into kept[]. The bound is found bit by bit.
-__global__ void __launch_bounds__(1024) kv4_choose_kernel(Kv4 c, int32_t* __restrict__ kept, int rows, int keep, int lo, int hi, int want) {
-    __shared__ int count, base_gt, base_eq;
-    __shared__ int wsum[32], wsum2[32];
+// The choice: the `want` rows of [lo, hi) with the largest weights, equal ones from the lowest row, beside all rows outside it, in ascending
+// order into kept[]. A cluster of CS blocks per KV head, block r with the r-th part of the rows, a thread with `per` neighbouring ones (in registers up to CH_KEEP).
+// The bound is found eight bits at a time: every block counts its rows by those bits, and adds up the blocks' counts for itself; one barrier of
+// the cluster a round, since each round has counters of its own. MOVE: the block then copies its kept rows into another cache.
+// 32 rounds of one bit by one block a head, every weight read again each time, took 330 us for 65529 rows of 8 heads.
+constexpr int CH_THREADS = 1024, CH_KEEP = 8;
+template <bool IN_REGISTERS, bool MOVE>
+__global__ void __launch_bounds__(CH_THREADS) kv4_choose_kernel(Kv4 src, Kv4 dst, int32_t* __restrict__ kept, int rows, int keep, int lo, int hi, int want, int CS) {
+    __shared__ uint32_t hist[4][256], total[256], totals[2], found[2];
+    __shared__ uint32_t warp_gt[32], warp_eq[32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = blockIdx.x % CS, h = blockIdx.x / CS;
+    for (int i = tid; i < 1024; i += CH_THREADS) (&hist[0][0])[i] = 0;
     pdl_launch_dependents();
     pdl_wait();
-    const int h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const float* w = c.weight + c.row(h, 0);
-    uint32_t bound = 0;                                       // the largest order that at least `want` rows reach
-    for (int bit = 31; bit >= 0 && want > 0; bit--) {
-        const uint32_t t = bound | 1u << bit;
-        __syncthreads();
-        if (tid == 0) count = 0;
-        __syncthreads();
-        int n = 0;
-        for (int r = lo + tid; r < hi; r += 1024) n += weight_order(w[r]) >= t;
-        n = __reduce_add_sync(0xffffffffu, n);
-        if (lane == 0) atomicAdd(&count, n);
-        __syncthreads();
-        if (count >= want) bound = t;
+    auto meet = [&]() { if (CS > 1) { cluster_arrive(); cluster_wait(); } else __syncthreads(); };
+    auto theirs = [&](const uint32_t* mine, int r) { return CS > 1 ? peer_load_u32(smem_u32(mine), (uint32_t)r) : *mine; };
+    const int slice = (rows + CS - 1) / CS, per = (slice + CH_THREADS - 1) / CH_THREADS;
+    const int r0 = rank * slice + tid * per, n = max(0, min(min(per, slice - tid * per), rows - r0));
+    const float* w = src.weight + src.row(h, 0);
+    uint32_t key[CH_KEEP];
+    if (IN_REGISTERS) {
+#pragma unroll
+        for (int i = 0; i < CH_KEEP; i++) key[i] = i < n ? weight_order(__ldcg(w + r0 + i)) : 0u;
     }
+    // f(row, order, whether the row is one of those chosen from) for this thread's rows in order
+    auto each = [&](auto f) {
+        if (IN_REGISTERS) {
+#pragma unroll
+            for (int i = 0; i < CH_KEEP; i++) if (i < n) f(r0 + i, key[i], r0 + i >= lo && r0 + i < hi);
+        } else {
+            for (int i = 0; i < n; i++) f(r0 + i, weight_order(__ldcg(w + r0 + i)), r0 + i >= lo && r0 + i < hi);
+        }
+    };
+    uint32_t bound = 0, left = (uint32_t)want;                // rows still to be found among those that share the bound's bits so far
     __syncthreads();
-    if (tid == 0) count = 0;
-    __syncthreads();
-    int n = 0;
-    for (int r = lo + tid; r < hi; r += 1024) n += weight_order(w[r]) > bound;
-    n = __reduce_add_sync(0xffffffffu, n);
-    if (lane == 0) atomicAdd(&count, n);
-    __syncthreads();
-    const int ties = want - count;                            // rows at the bound that stay, from the lowest
-    if (tid == 0) { base_gt = 0; base_eq = 0; }
-    for (int r0 = 0; r0 < rows; r0 += 1024) {
-        __syncthreads();
-        const int r = r0 + tid;
-        const bool inside = r >= lo && r < hi;
-        const uint32_t o = inside ? weight_order(w[r]) : 0u;
-        const bool eq = inside && o == bound && want > 0, sure = r < rows && (!inside || (want > 0 && o > bound));
-        const unsigned me = __ballot_sync(0xffffffffu, eq);
-        if (lane == 0) wsum[warp] = __popc(me);
-        __syncthreads();
-        int eq_before = base_eq + __popc(me & ((1u << lane) - 1));
-        for (int i = 0; i < warp; i++) eq_before += wsum[i];
-        const bool stay = sure || (eq && eq_before < ties);
-        const unsigned ms = __ballot_sync(0xffffffffu, stay);
-        if (lane == 0) wsum2[warp] = __popc(ms);
-        __syncthreads();
-        int at = base_gt + __popc(ms & ((1u << lane) - 1));
-        for (int i = 0; i < warp; i++) at += wsum2[i];
-        if (stay && at < keep) kept[(size_t)h * keep + at] = r;
-        __syncthreads();
-        if (tid == 0) for (int i = 0; i < 32; i++) { base_eq += wsum[i]; base_gt += wsum2[i]; }
+    if (want > 0) {
+        for (int round = 0; round < 4; round++) {
+            const int shift = 24 - 8 * round;
+            const uint32_t above = round ? 0xFFFFFFFFu << (shift + 8) : 0u;
+            each([&](int, uint32_t k, bool in) { if (in && (k & above) == bound) atomicAdd(&hist[round][(k >> shift) & 255], 1u); });
+            meet();
+            if (tid < 256) {
+                uint32_t t = 0;
+                for (int r = 0; r < CS; r++) t += theirs(&hist[round][tid], r);
+                total[tid] = t;
+            }
+            __syncthreads();
+            if (warp == 0) {                                  // lane l has bins 255 - 8 l .. 248 - 8 l
+                uint32_t c[8], sum = 0;
+#pragma unroll
+                for (int i = 0; i < 8; i++) { c[i] = total[255 - 8 * lane - i]; sum += c[i]; }
+                uint32_t before = sum;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) { const uint32_t v = __shfl_up_sync(0xffffffffu, before, o); if (lane >= o) before += v; }
+                before -= sum;
+                if (before < left && before + sum >= left) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        if (before < left && before + c[i] >= left) { found[0] = 255 - 8 * lane - i; found[1] = before; }
+                        before += c[i];
+                    }
+                }
+            }
+            __syncthreads();
+            bound |= found[0] << shift;
+            left -= found[1];
+        }
     }
+    // left: rows at the bound that stay, from the lowest. Who stays, and where it goes:
+    uint32_t gt = 0, eq = 0;
+    each([&](int, uint32_t k, bool in) { gt += !in || (want > 0 && k > bound); eq += in && want > 0 && k == bound; });
+    uint32_t pgt = gt, peq = eq;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t a = __shfl_up_sync(0xffffffffu, pgt, o), b = __shfl_up_sync(0xffffffffu, peq, o);
+        if (lane >= o) { pgt += a; peq += b; }
+    }
+    if (lane == 31) { warp_gt[warp] = pgt; warp_eq[warp] = peq; }
+    __syncthreads();
+    if (warp == 0) {
+        uint32_t a = warp_gt[lane], b = warp_eq[lane];
+        const uint32_t a0 = a, b0 = b;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o);
+            if (lane >= o) { a += x; b += y; }
+        }
+        warp_gt[lane] = a - a0; warp_eq[lane] = b - b0;
+        if (lane == 31) { totals[0] = a; totals[1] = b; }
+    }
+    meet();
+    __syncthreads();
+    uint32_t base = 0, eq_before = 0;                         // kept rows of the blocks below, and their rows at the bound
+    for (int r = 0; r < rank; r++) {
+        const uint32_t g = theirs(&totals[0], r), e = theirs(&totals[1], r);
+        base += g + min(e, left - min(left, eq_before));
+        eq_before += e;
+    }
+    const uint32_t room = left - min(left, eq_before);        // rows at the bound that stay in this block
+    const uint32_t count = totals[0] + min(totals[1], room);
+    if (CS > 1) cluster_arrive();                             // done with the other blocks' shared memory
+    uint32_t at_gt = warp_gt[warp] + pgt - gt, at_eq = warp_eq[warp] + peq - eq;
+    int32_t* mine = kept + (size_t)h * keep;
+    each([&](int r, uint32_t k, bool in) {
+        const bool sure = !in || (want > 0 && k > bound), tie = in && want > 0 && k == bound;
+        if (sure || (tie && at_eq < room)) mine[base + at_gt + min(at_eq, room)] = r;
+        at_gt += sure;
+        at_eq += tie;
+    });
+    if (MOVE) {
+        __syncthreads();
+        const int ng = src.hd / 32;
+        const int32_t* idx = mine + base;
+        auto copy = [&](auto* to, const auto* from, int pieces) {                      // `pieces` of a row, rows as chosen
+            const long total_pieces = (long)count * pieces;
+            for (long e0 = tid; e0 < total_pieces; e0 += 4 * CH_THREADS) {
+                std::remove_const_t<std::remove_reference_t<decltype(*to)>> v[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++) { const long e = e0 + u * CH_THREADS; if (e < total_pieces) v[u] = __ldcg(from + src.row(h, __ldcg(idx + e / pieces)) * pieces + e % pieces); }
+#pragma unroll
+                for (int u = 0; u < 4; u++) { const long e = e0 + u * CH_THREADS; if (e < total_pieces) to[(dst.row(h, base) + e / pieces) * pieces + e % pieces] = v[u]; }
+            }
+        };
+        copy(reinterpret_cast<uint4*>(dst.k), reinterpret_cast<const uint4*>(src.k), ng);
+        copy(reinterpret_cast<uint4*>(dst.v), reinterpret_cast<const uint4*>(src.v), ng);
+        copy(reinterpret_cast<uint32_t*>(dst.scale), reinterpret_cast<const uint32_t*>(src.scale), ng);
+        if (dst.weight) copy(dst.weight, src.weight, 1);
+    }
+    if (CS > 1) cluster_wait();
 }
 
-// grid (pieces, KV heads): a block moves 16 bytes (4 of the weights) of every kept row. Rows only move towards the front, so a pass that has
-// all its rows in registers before it stores the first may write over the rows it came from.
-__global__ void __launch_bounds__(1024) kv4_move_kernel(Kv4 src, Kv4 dst, const int32_t* __restrict__ kept, int keep) {
+// In place: grid (3, KV heads), a block moves the keys, the values or the scales and weights of all kept rows. Rows only move towards the
+// front, so a pass that has all its pieces in registers before it stores the first may write over the rows they came from.
+__global__ void __launch_bounds__(1024) kv4_move_kernel(Kv4 c, const int32_t* __restrict__ kept, int keep) {
     pdl_launch_dependents();
     pdl_wait();
-    const int h = blockIdx.y, kp = src.hd / 32, sp = src.hd / 32;                     // pieces of 16 bytes in a code row; words of 4 bytes in a row of scales
+    const int h = blockIdx.y, ng = c.hd / 32, tid = threadIdx.x;
     const int32_t* idx = kept + (size_t)h * keep;
-    const int p = blockIdx.x;
-    for (int i0 = 0; i0 < keep; i0 += 1024) {
-        const int i = i0 + threadIdx.x;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        size_t from = 0, to = 0;
-        if (i < keep) {
-            from = src.row(h, idx[i]); to = dst.row(h, i);
-            if (p < kp) x = reinterpret_cast<const uint4*>(src.k)[from * kp + p];
-            else if (p < 2 * kp) x = reinterpret_cast<const uint4*>(src.v)[from * kp + p - kp];
-            else if (p < 2 * kp + sp) x.x = reinterpret_cast<const uint32_t*>(src.scale)[from * sp + p - 2 * kp];
-            else if (src.weight && dst.weight) x.x = __float_as_uint(src.weight[from]);
+    auto shift = [&](auto* plane, int pieces) {
+        for (long e0 = 0; e0 < (long)keep * pieces; e0 += 4096) {
+            std::remove_reference_t<decltype(*plane)> v[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) { const long e = e0 + u * 1024 + tid; if (e < (long)keep * pieces) v[u] = __ldcg(plane + c.row(h, __ldcg(idx + e / pieces)) * pieces + e % pieces); }
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < 4; u++) { const long e = e0 + u * 1024 + tid; if (e < (long)keep * pieces) plane[c.row(h, (int)(e / pieces)) * pieces + e % pieces] = v[u]; }
+            __syncthreads();
         }
-        __syncthreads();
-        if (i < keep) {
-            if (p < kp) reinterpret_cast<uint4*>(dst.k)[to * kp + p] = x;
-            else if (p < 2 * kp) reinterpret_cast<uint4*>(dst.v)[to * kp + p - kp] = x;
-            else if (p < 2 * kp + sp) reinterpret_cast<uint32_t*>(dst.scale)[to * sp + p - 2 * kp] = x.x;
-            else if (src.weight && dst.weight) dst.weight[to] = __uint_as_float(x.x);
-        }
-        __syncthreads();
-    }
+    };
+    if (blockIdx.x == 0) shift(reinterpret_cast<uint4*>(c.k), ng);
+    else if (blockIdx.x == 1) shift(reinterpret_cast<uint4*>(c.v), ng);
+    else { shift(reinterpret_cast<uint32_t*>(c.scale), ng); shift(c.weight, 1); }
 }
 
 Kv4 planes(const ibcu_kv4_t* t) { return Kv4{ t->k, t->v, (__half*)t->scale, t->weight, t->n_kv_heads, t->head_dim, t->max_rows }; }
@@ -330,12 +403,19 @@ extern "C" int ibcu_kv4_evict(ibcu_ctx* ctx, const ibcu_kv4_t* src, const ibcu_k
     IBCU_REQUIRE(ctx, rows >= 1 && rows <= src->max_rows && keep >= 1 && keep <= rows && keep <= dst->max_rows && sink >= 0 && recent >= 0 && (long)sink + recent <= keep,
                  "ibcu_kv4_evict: %d of %d rows (at most %d), first %d and last %d", keep, rows, dst->max_rows, sink, recent);
     const int nkv = src->n_kv_heads;
+    const bool in_place = src->k == dst->k;
+    IBCU_REQUIRE(ctx, in_place ? src->v == dst->v && src->scale == dst->scale && src->weight == dst->weight && src->max_rows == dst->max_rows
+                               : src->v != dst->v && src->scale != dst->scale && src->weight != dst->weight, "ibcu_kv4_evict: two caches that share some planes");
     if (!kept) {
         int rc = ibcu_reserve(ctx, &ctx->scratch, &ctx->scratch_bytes, (size_t)nkv * keep * sizeof(int32_t));
         if (rc) return rc;
         kept = (int32_t*)ctx->scratch;
     }
-    int rc = ibcu_launch(ctx, kv4_choose_kernel, dim3(nkv), dim3(1024), 0, 1, true, planes(src), kept, rows, keep, sink, rows - recent, keep - sink - recent);
-    if (!rc) rc = ibcu_launch(ctx, kv4_move_kernel, dim3(3 * (src->head_dim / 32) + 1, nkv), dim3(1024), 0, 1, true, planes(src), planes(dst), (const int32_t*)kept, keep);
+    int CS = 1;                                               // a block a thousand rows, up to eight
+    while (CS < 8 && rows > 1024 * CS) CS *= 2;
+    const bool regs = (rows + CS - 1) / CS <= CH_THREADS * CH_KEEP;
+    auto choose = regs ? (in_place ? kv4_choose_kernel<true, false> : kv4_choose_kernel<true, true>) : (in_place ? kv4_choose_kernel<false, false> : kv4_choose_kernel<false, true>);
+    int rc = ibcu_launch(ctx, choose, dim3(CS * nkv), dim3(CH_THREADS), 0, CS, true, planes(src), planes(dst), kept, rows, keep, sink, rows - recent, keep - sink - recent, CS);
+    if (!rc && in_place && keep < rows) rc = ibcu_launch(ctx, kv4_move_kernel, dim3(3, nkv), dim3(1024), 0, 1, true, planes(src), (const int32_t*)kept, keep);
     return rc;
 }

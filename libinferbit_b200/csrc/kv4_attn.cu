@@ -515,7 +515,7 @@ __global__ void __launch_bounds__(128) kv4_weight_kernel(const KaParams p, float
             if (g == 0 && r < R) {
                 const size_t at = p.c.row(kvh, r);
                 if (parts) parts[((size_t)blockIdx.z * p.c.n_kv + kvh) * p.c.max_rows + r] = x;
-                else p.c.weight[at] = (decay == 0.0f ? 0.0f : decay * p.c.weight[at]) + x;
+                else p.c.weight[at] = (decay == 0.0f ? 0.0f : decay * __ldcg(p.c.weight + at)) + x;
             }
         }
 }
@@ -529,7 +529,7 @@ __global__ void __launch_bounds__(256) kv4_weight_join_kernel(const KaParams p, 
     const size_t at = p.c.row(blockIdx.y, r);
     float x = 0.0f;
     for (int i = 0; i < n; i++) x += __ldcg(parts + (size_t)i * p.c.n_kv * p.c.max_rows + at);
-    p.c.weight[at] = (decay == 0.0f ? 0.0f : decay * p.c.weight[at]) + x;
+    p.c.weight[at] = (decay == 0.0f ? 0.0f : decay * __ldcg(p.c.weight + at)) + x;
 }
 
 template <int NG, bool LARGE>

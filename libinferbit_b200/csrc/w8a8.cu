@@ -32,7 +32,7 @@ __global__ void __launch_bounds__(512) quantize_rows_kernel(const float* __restr
         for (int u = 0; u < QR_KEEP; u++) m = max(m, size4(kept[u]));
         for (int i = tid + QR_KEEP * nth; i < n4; i += nth) m = max(m, size4(__ldcg(x4 + i)));
     } else {
-        for (int i = tid; i < N; i += nth) m = max(m, __float_as_uint(xb[i]) & 0x7FFFFFFFu);
+        for (int i = tid; i < N; i += nth) m = max(m, __float_as_uint(__ldcg(xb + i)) & 0x7FFFFFFFu);
     }
     m = __reduce_max_sync(0xffffffffu, m);
     if ((tid & 31) == 0) red[tid >> 5] = m;
@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(512) quantize_rows_kernel(const float* __restr
         for (int i = tid + QR_KEEP * nth; i < n4; i += nth) put(i, __ldcg(x4 + i));
         for (int i = N + tid; i < ldq; i += nth) qb[i] = 0;
     } else {
-        for (int i = tid; i < ldq; i += nth) qb[i] = i < N ? (int8_t)code(xb[i]) : (int8_t)0;
+        for (int i = tid; i < ldq; i += nth) qb[i] = i < N ? (int8_t)code(__ldcg(xb + i)) : (int8_t)0;
     }
     if (tid == 0) scale[b] = s;
 }
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(W8_THREADS, 1) w8a8_tc_kernel(const __grid_con
                     for (int u0 = 0; u0 < 32; u0 += 8) {
                         float old[8];
 #pragma unroll
-                        for (int u = 0; u < 8; u++) old[u] = decltype(add)::value && (decltype(whole)::value || u0 + u < n) ? o[(size_t)u * ld] : 0.0f;
+                        for (int u = 0; u < 8; u++) old[u] = decltype(add)::value && (decltype(whole)::value || u0 + u < n) ? __ldcg(o + (size_t)u * ld) : 0.0f;
                         const float4 s0 = *reinterpret_cast<const float4*>(sx + c + u0), s1 = *reinterpret_cast<const float4*>(sx + c + u0 + 4);
                         const float f[8] = { s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w };
 #pragma unroll
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(W8_THREADS, 1) w8a8_tc_kernel(const __grid_con
                         if (t + u < mine) {
                             float* to = W.out + (size_t)(tok0 + rank * TL + t + u) * W.out_stride + row;
                             const float y = (float)four[u] * (sw * sh->sx[0][rank * TL + t + u]);
-                            *to = W.epilogue == IBCU_EPI_ADD ? *to + y : y;
+                            *to = W.epilogue == IBCU_EPI_ADD ? __ldcg(to) + y : y;
                         }
                 }
             }
@@ -309,12 +309,12 @@ __global__ void __launch_bounds__(256) align_rows_kernel(const uint8_t* __restri
             const uint32_t sh = (uint32_t)((uintptr_t)a & 3) * 8;
             uint32_t x[5];
 #pragma unroll
-            for (int i = 0; i < 4; i++) x[i] = w[i];
-            x[4] = sh ? w[4] : 0u;
+            for (int i = 0; i < 4; i++) x[i] = __ldcg(w + i);
+            x[4] = sh ? __ldcg(w + 4) : 0u;
             v = make_uint4(__funnelshift_r(x[0], x[1], sh), __funnelshift_r(x[1], x[2], sh), __funnelshift_r(x[2], x[3], sh), __funnelshift_r(x[3], x[4], sh));
         } else {
             uint8_t b[16];
-            for (int i = 0; i < 16; i++) b[i] = c + i < n ? a[i] : (uint8_t)0;
+            for (int i = 0; i < 16; i++) b[i] = c + i < n ? __ldcg(a + i) : (uint8_t)0;
             memcpy(&v, b, 16);
         }
         *reinterpret_cast<uint4*>(dst + r * to + c) = v;
