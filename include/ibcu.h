@@ -263,7 +263,7 @@ int ibcu_pqkv_encode(ibcu_ctx* ctx, const float* vec, int dim, int n_vec, int G,
  *   weight [n_kv_heads][max_rows] float, or NULL: the attention that each row has drawn so far
  * Order of the codes in a row, as the kernels' lanes take them: of a key, four pieces, piece t holding values 8t..8t+7 of every
  * group of 32 in turn; of a value row, eight pieces, piece g holding values 4g..4g+3 of every group (ibcu_kv4_read gives the
- * plain order). head_dim 32, 64, 96, 128, 192 or 256; max_rows a multiple of 8; memory behind the last written row is not used,
+ * plain order). head_dim 32, 64, 96, 128, 192 or 256; max_rows a multiple of 8 up to 2^30; memory behind the last written row is not used,
  * whatever it holds.
  * A row of the cache need not be a position: after an eviction, rows and positions go on side by side, which is why the calls
  * take both row0 (where) and pos0 (the angle). */

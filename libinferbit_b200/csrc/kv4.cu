@@ -267,8 +267,6 @@ __global__ void __launch_bounds__(CH_THREADS) kv4_choose_kernel(Kv4 src, Kv4 dst
         eq_before += e;
     }
     const uint32_t room = left - min(left, eq_before);        // rows at the bound that stay in this block
-    const uint32_t count = totals[0] + min(totals[1], room);
-    if (CS > 1) cluster_arrive();                             // done with the other blocks' shared memory
     uint32_t at_gt = warp_gt[warp] + pgt - gt, at_eq = warp_eq[warp] + peq - eq;
     int32_t* mine = kept + (size_t)h * keep;
     each([&](int r, uint32_t k, bool in) {
@@ -277,26 +275,38 @@ __global__ void __launch_bounds__(CH_THREADS) kv4_choose_kernel(Kv4 src, Kv4 dst
         at_gt += sure;
         at_eq += tie;
     });
+    if (CS > 1) { cluster_arrive(); cluster_wait(); }         // nobody needs another block's shared memory any more, and the list is whole
+    else __syncthreads();
     if (MOVE) {
-        __syncthreads();
-        const int ng = src.hd / 32;
-        const int32_t* idx = mine + base;
-        auto copy = [&](auto* to, const auto* from, int pieces) {                      // `pieces` of a row, rows as chosen
-            const long total_pieces = (long)count * pieces;
-            for (long e0 = tid; e0 < total_pieces; e0 += 4 * CH_THREADS) {
-                std::remove_const_t<std::remove_reference_t<decltype(*to)>> v[4];
+        // Equal parts of the list (the last rows, which all stay, would otherwise fall to the last block).
+        const int ng = src.hd / 32, piece = tid % ng, at_once = CH_THREADS / ng;
+        const int i1 = (int)((long)keep * (rank + 1) / CS);
+        for (long i0 = (long)keep * rank / CS + tid / ng; tid < at_once * ng && i0 < i1; i0 += 2 * at_once) {
+            uint4 vk[2], vv[2];
+            uint32_t vs[2];
+            float vw[2];
 #pragma unroll
-                for (int u = 0; u < 4; u++) { const long e = e0 + u * CH_THREADS; if (e < total_pieces) v[u] = __ldcg(from + src.row(h, __ldcg(idx + e / pieces)) * pieces + e % pieces); }
-#pragma unroll
-                for (int u = 0; u < 4; u++) { const long e = e0 + u * CH_THREADS; if (e < total_pieces) to[(dst.row(h, base) + e / pieces) * pieces + e % pieces] = v[u]; }
+            for (int u = 0; u < 2; u++) {
+                const long i = i0 + u * at_once;
+                if (i >= i1) break;
+                const size_t from = src.row(h, __ldcg(mine + i));
+                vk[u] = __ldcg(reinterpret_cast<const uint4*>(src.k) + from * ng + piece);
+                vv[u] = __ldcg(reinterpret_cast<const uint4*>(src.v) + from * ng + piece);
+                vs[u] = __ldcg(reinterpret_cast<const uint32_t*>(src.scale) + from * ng + piece);
+                vw[u] = piece == 0 ? __ldcg(src.weight + from) : 0.0f;
             }
-        };
-        copy(reinterpret_cast<uint4*>(dst.k), reinterpret_cast<const uint4*>(src.k), ng);
-        copy(reinterpret_cast<uint4*>(dst.v), reinterpret_cast<const uint4*>(src.v), ng);
-        copy(reinterpret_cast<uint32_t*>(dst.scale), reinterpret_cast<const uint32_t*>(src.scale), ng);
-        if (dst.weight) copy(dst.weight, src.weight, 1);
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const long i = i0 + u * at_once;
+                if (i >= i1) break;
+                const size_t to = dst.row(h, (int)i);
+                reinterpret_cast<uint4*>(dst.k)[to * ng + piece] = vk[u];
+                reinterpret_cast<uint4*>(dst.v)[to * ng + piece] = vv[u];
+                reinterpret_cast<uint32_t*>(dst.scale)[to * ng + piece] = vs[u];
+                if (piece == 0 && dst.weight) dst.weight[to] = vw[u];
+            }
+        }
     }
-    if (CS > 1) cluster_wait();
 }
 
 // In place: grid (3, KV heads), a block moves the keys, the values or the scales and weights of all kept rows. Rows only move towards the
@@ -307,13 +317,14 @@ __global__ void __launch_bounds__(1024) kv4_move_kernel(Kv4 c, const int32_t* __
     const int h = blockIdx.y, ng = c.hd / 32, tid = threadIdx.x;
     const int32_t* idx = kept + (size_t)h * keep;
     auto shift = [&](auto* plane, int pieces) {
-        for (long e0 = 0; e0 < (long)keep * pieces; e0 += 4096) {
+        const int piece = tid % pieces, at_once = 1024 / pieces, mine = tid < at_once * pieces ? tid / pieces : keep;
+        for (int i0 = 0; i0 < keep; i0 += 4 * at_once) {
             std::remove_reference_t<decltype(*plane)> v[4];
 #pragma unroll
-            for (int u = 0; u < 4; u++) { const long e = e0 + u * 1024 + tid; if (e < (long)keep * pieces) v[u] = __ldcg(plane + c.row(h, __ldcg(idx + e / pieces)) * pieces + e % pieces); }
+            for (int u = 0; u < 4; u++) { const long i = (long)mine + i0 + u * at_once; if (i < keep) v[u] = __ldcg(plane + c.row(h, __ldcg(idx + i)) * pieces + piece); }
             __syncthreads();
 #pragma unroll
-            for (int u = 0; u < 4; u++) { const long e = e0 + u * 1024 + tid; if (e < (long)keep * pieces) plane[c.row(h, (int)(e / pieces)) * pieces + e % pieces] = v[u]; }
+            for (int u = 0; u < 4; u++) { const long i = (long)mine + i0 + u * at_once; if (i < keep) plane[c.row(h, (int)i) * pieces + piece] = v[u]; }
             __syncthreads();
         }
     };
@@ -328,7 +339,7 @@ int check_cache(ibcu_ctx* ctx, const ibcu_kv4_t* t, const char* call) {
     IBCU_REQUIRE(ctx, t && t->k && t->v && t->scale, "%s: null pointer", call);
     const int hd = t->head_dim;
     IBCU_REQUIRE(ctx, hd == 32 || hd == 64 || hd == 96 || hd == 128 || hd == 192 || hd == 256, "%s: head_dim=%d (32, 64, 96, 128, 192 or 256)", call, hd);
-    IBCU_REQUIRE(ctx, t->n_kv_heads >= 1 && t->n_kv_heads <= 1024 && t->max_rows >= 8 && t->max_rows % 8 == 0, "%s: n_kv_heads=%d max_rows=%d (rows in multiples of 8)", call, t->n_kv_heads, t->max_rows);
+    IBCU_REQUIRE(ctx, t->n_kv_heads >= 1 && t->n_kv_heads <= 1024 && t->max_rows >= 8 && t->max_rows <= (1 << 30) && t->max_rows % 8 == 0, "%s: n_kv_heads=%d max_rows=%d (rows in multiples of 8, up to 2^30)", call, t->n_kv_heads, t->max_rows);
     IBCU_REQUIRE(ctx, (((uintptr_t)t->k | (uintptr_t)t->v | (uintptr_t)t->scale) & 15) == 0 && ((uintptr_t)t->weight & 3) == 0, "%s: k, v and scale must be 16-byte aligned", call);
     IBCU_REQUIRE(ctx, !t->weight || (t->decay >= 0.0f && t->decay <= 1.0f), "%s: decay=%g outside 0..1", call, (double)t->decay);
     return IBCU_OK;
