@@ -14,136 +14,70 @@
 
 namespace {
 
-__device__ __forceinline__ int key_place(int i, int ng) { return ((i & 31) / 8 * ng + i / 32) * 8 + (i & 7); }      // where value i of a row lies
-__device__ __forceinline__ int value_place(int i, int ng) { return ((i & 31) / 4 * ng + i / 32) * 4 + (i & 3); }
 __device__ __forceinline__ float held(const uint8_t* row, int place, float s) { return (float)((__ldcg(row + (place >> 1)) >> ((place & 1) * 4) & 15) - 8) * s; }
 
 __device__ __forceinline__ float scale_at(const Kv4& c, size_t i) { return __half2float(__ushort_as_half(__ldcg(reinterpret_cast<const unsigned short*>(c.scale) + i))); }
 
-// A group's scale and the factor that turns its values into codes; amax_bits: the largest magnitude's bits (NaN and Inf above all)
-__device__ __forceinline__ __half group_scale(uint32_t amax_bits, float& inv) {
-    if (amax_bits >= 0x7F800000u) { inv = 0.0f; return __ushort_as_half(0x7FFF); }          // NaN: the row says so wherever it is seen
-    const float s = __fmul_rn(__uint_as_float(amax_bits), 1.0f / 7.0f);
-    const __half h = __float2half_rn(fminf(s, 65504.0f));
-    inv = __half2float(h) > 0.0f ? __fdiv_rn(1.0f, __half2float(h)) : 0.0f;
-    return h;
-}
-__device__ __forceinline__ uint32_t code_of(float x, float inv) {
-    const float q = inv > 0.0f ? fminf(fmaxf(rintf(__fmul_rn(x, inv)), -7.0f), 7.0f) : 0.0f;
-    return (uint32_t)((int)q + 8);
-}
-
-// One launch ahead of the attention: blocks below qblocks turn a tile of columns into fragments, the others write rows. Angles of a position are
-// shared by all its heads: a block computes their sines once, in 64 bits, which is most of its time (about a microsecond).
+// One launch ahead of the attention of more than eight columns, and that of ibcu_kv4_write: blocks below qblocks turn a tile of 16 columns into
+// fragments, the others write the rows of a position, whose heads share its angles.
 struct PrepParams { Kv4 c; Kv4Columns t; Kv4Place at; Kv4Prep w; int qblocks, wparts; int* err; };
 
 __global__ void __launch_bounds__(128) kv4_prep_kernel(const PrepParams p) {
-    extern __shared__ __align__(16) double2 turn[];           // [positions of the block][hd / 2] cosine and sine; then [8 columns a warp][hd] turned queries
+    extern __shared__ __align__(16) double2 turn[];           // [positions of the block][hd / 2]; then [8 columns a warp][hd] turned queries
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hd = p.c.hd, half = hd / 2, ng = hd / 32;
     const bool queries = (int)blockIdx.x < p.qblocks;
-    const int cols = p.t.cols(), kvh = blockIdx.x / p.t.ntiles, c0 = blockIdx.x % p.t.ntiles * cols, wb = blockIdx.x - p.qblocks;
-    const int b0 = queries ? c0 / p.t.group : wb / p.wparts, b1 = queries ? min(p.t.B - 1, (c0 + cols - 1) / p.t.group) : b0;
+    const int kvh = blockIdx.x / p.t.ntiles, c0 = blockIdx.x % p.t.ntiles * 16, wb = blockIdx.x - p.qblocks;
+    const int b0 = queries ? c0 / p.t.group : wb / p.wparts, b1 = queries ? min(p.t.B - 1, (c0 + 15) / p.t.group) : b0;
     int row0 = p.at.row0, pos0 = p.at.pos0;
     if (p.at.at) {
         pdl_wait();
         if (!kv4_place(p.at, p.t.B, p.c.max_rows, p.err, row0, pos0)) return;
     }
-    if (p.w.rotate)
-        for (int e = tid; e < (b1 - b0 + 1) * half; e += 128) {
-            double s, c;
-            sincos((double)(pos0 + b0 + e / half) * exp2((double)(e % half) * (-2.0 / hd * p.w.log2_theta)), &s, &c);
-            turn[e] = make_double2(c, s);
-        }
+    if (p.w.rotate) kv4_angles(turn, b1 - b0 + 1, pos0 + b0, hd, p.w.log2_theta);
     if (!p.at.at) pdl_wait();
     pdl_launch_dependents();                                  // not earlier: the attention reads rows of earlier calls ahead of its own wait
     __syncthreads();
-    // the pairs m, m + 1, .. of position b, turned and rounded once
-    auto turn_pair = [&](float& x0, float& x1, int b, int m) {
-        const double2 cs = turn[(b - b0) * half + m];
-        const double a = x0, z = x1;
-        x0 = (float)(a * cs.x - z * cs.y);
-        x1 = (float)(a * cs.y + z * cs.x);
-    };
     if (queries) {
-        if (warp >= cols / 8) return;
+        if (warp >= 2) return;
         // a warp prepares eight columns, lane = column * 4 + t: values 8t..8t+7 of every group
-        float* qr = reinterpret_cast<float*>(turn + (p.w.rotate ? (size_t)min(cols, (cols - 1) / p.t.group + 2) * half : 0)) + (size_t)warp * 8 * hd;
         const int g = lane >> 2, t = lane & 3, col = c0 + warp * 8 + g, b = col / p.t.group;
+        float* qr = reinterpret_cast<float*>(turn + (p.w.rotate ? (size_t)min(16, 15 / p.t.group + 2) * half : 0)) + ((size_t)warp * 8 + g) * hd + 8 * t;
         const bool on = b < p.t.B;
-        const float* src = p.w.q + ((size_t)b * p.t.n_heads + (size_t)kvh * p.t.group + col % p.t.group) * hd;
+        const float* src = p.w.q + ((size_t)b * p.t.n_heads + (size_t)kvh * p.t.group + col % p.t.group) * hd + 8 * t;
+        const double2* angles = on && p.w.rotate ? turn + (b - b0) * half + 4 * t : nullptr;
         uint32_t m = 0;
         for (int j = 0; j < ng; j++) {
-            const int d = 32 * j + 8 * t;
             float x[8];
+            kv4_query(x, src + 32 * j, on, angles ? angles + 16 * j : nullptr);
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = on ? __ldcg(src + d + i) : 0.0f;
-            if (on && p.w.rotate) {
-#pragma unroll
-                for (int i = 0; i < 8; i += 2) turn_pair(x[i], x[i + 1], b, (d + i) / 2);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; i++) { m = max(m, __float_as_uint(x[i]) & 0x7FFFFFFFu); qr[(size_t)g * hd + d + i] = x[i]; }
+            for (int i = 0; i < 8; i++) { m = max(m, __float_as_uint(x[i]) & 0x7FFFFFFFu); qr[32 * j + i] = x[i]; }
         }
         m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
         m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        // The largest magnitude goes to [2^13, 2^14). A power of 2 up to 2^120, in two factors: what that leaves small are queries below 2^-106, whose
-        // scores are zeros beside one another anyway.
-        const int e = min(120, max(-114, 13 - ((int)(m >> 23) - 127)));
-        const float up = __int_as_float(((e >> 1) + 127) << 23), up2 = __int_as_float((e - (e >> 1) + 127) << 23);
-        const size_t unit = blockIdx.x;
-        // takes the sums' 2^e off; log2(e) makes exponents of 2 of them
-        if (t == 0) p.w.qc[unit * 16 + warp * 8 + g] = (float)fmin(exp2((double)-e) * (1.4426950408889634 / sqrt((double)hd)), 3.0e38);
-        uint2* qf = p.w.qf + unit * kv4_frag_uint2(ng, p.t.large);
+        const Kv4Up up = kv4_up(m, hd);
+        if (t == 0) p.w.qc[(size_t)blockIdx.x * 16 + warp * 8 + g] = up.back;
+        uint32_t* qf = reinterpret_cast<uint32_t*>(p.w.qf + blockIdx.x * kv4_frags(ng, true)) + lane * 4 + warp;
         for (int j = 0; j < ng; j++) {
             float x[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = qr[(size_t)g * hd + 32 * j + 8 * t + i] * up * up2;
+            for (int i = 0; i < 8; i++) x[i] = qr[32 * j + i] * up.a * up.b;
 #pragma unroll
-            for (int s = 0; s < 2; s++) {                     // codes 0 and 4, 1 and 5 of a word in the first step, 2 and 6, 3 and 7 in the second
-                __half2 h[2], l[2];
-#pragma unroll
-                for (int u = 0; u < 2; u++) {                 // odd codes reach the product as 16 times themselves
-                    const float f = u ? 0.0625f : 1.0f, a = x[2 * s + u] * f, z = x[2 * s + u + 4] * f;
-                    h[u] = __floats2half2_rn(a, z);
-                    l[u] = __floats2half2_rn(a - __low2float(h[u]), z - __high2float(h[u]));
-                }
-                const uint2 hi = make_uint2(*reinterpret_cast<uint32_t*>(&h[0]), *reinterpret_cast<uint32_t*>(&h[1]));
-                const uint2 lo = make_uint2(*reinterpret_cast<uint32_t*>(&l[0]), *reinterpret_cast<uint32_t*>(&l[1]));
-                if (p.t.large) {
-                    qf[((j * 2 + s) * 2 + warp) * 32 + lane] = hi;
-                    qf[(((ng + j) * 2 + s) * 2 + warp) * 32 + lane] = lo;
-                } else {
-                    qf[((j * 2 + s) * 2) * 32 + lane] = hi;
-                    qf[((j * 2 + s) * 2 + 1) * 32 + lane] = lo;
-                }
+            for (int s = 0; s < 2; s++) {
+                uint32_t hi[2], lo[2];
+                kv4_pieces(x, s, hi, lo);
+                uint32_t* to = qf + (j * 2 + s) * 128;
+                to[0] = hi[0]; to[2] = hi[1];
+                to += ng * 256;
+                to[0] = lo[0]; to[2] = lo[1];
             }
         }
         return;
     }
-    // rows of position b: four values a thread, eight neighbouring threads a group; heads wparts apart
-    const int quads = hd / 4, heads = (p.c.n_kv - wb % p.wparts + p.wparts - 1) / p.wparts;
+    const int quads = hd / 4, heads = (p.c.n_kv - wb % p.wparts + p.wparts - 1) / p.wparts;          // heads wparts apart
     for (int e = tid; e < 2 * heads * quads; e += 128) {
         const bool key = e < heads * quads;
-        const int f = key ? e : e - heads * quads, h = wb % p.wparts + f / quads * p.wparts, i = f % quads * 4;
-        const float* src = (key ? p.w.k : p.w.v) + ((size_t)b0 * p.c.n_kv + h) * hd + i;
-        float x[4] = { __ldcg(src), __ldcg(src + 1), __ldcg(src + 2), __ldcg(src + 3) };
-        if (key && p.w.rotate) { turn_pair(x[0], x[1], b0, i / 2); turn_pair(x[2], x[3], b0, i / 2 + 1); }
-        uint32_t m = 0;
-#pragma unroll
-        for (int u = 0; u < 4; u++) m = max(m, __float_as_uint(x[u]) & 0x7FFFFFFFu);
-        const unsigned lanes = 0xFFu << (lane & 24);
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(lanes, m, o));
-        float inv;
-        const __half s = group_scale(m, inv);
-        uint32_t w = 0;
-#pragma unroll
-        for (int u = 0; u < 4; u++) w |= code_of(x[u], inv) << (4 * u);
-        const size_t row = p.c.row(h, row0 + b0);
-        const int place = key ? key_place(i, ng) : value_place(i, ng);       // four values stay together in both orders
-        *reinterpret_cast<uint16_t*>((key ? p.c.k : p.c.v) + row * (hd / 2) + place / 2) = (uint16_t)w;
-        if ((i & 31) == 0) p.c.scale[row * 2 * ng + (key ? 0 : ng) + i / 32] = s;
-        if (key && i == 0 && p.c.weight) p.c.weight[row] = 0.0f;
+        const int f = key ? e : e - heads * quads, h = wb % p.wparts + f / quads * p.wparts;
+        kv4_write_four(p.c, (key ? p.w.k : p.w.v) + ((size_t)b0 * p.c.n_kv + h) * hd, key, h, row0 + b0, f % quads * 4, p.w.rotate ? turn : nullptr);
     }
 }
 
@@ -155,8 +89,8 @@ __global__ void __launch_bounds__(128) kv4_read_kernel(Kv4 c, float* __restrict_
     const size_t row = c.row(h, row0 + b);
     for (int i = threadIdx.x; i < c.hd; i += blockDim.x) {
         const size_t o = ((size_t)b * c.n_kv + h) * c.hd + i;
-        k[o] = held(c.k + row * (c.hd / 2), key_place(i, ng), scale_at(c, row * 2 * ng + i / 32));
-        v[o] = held(c.v + row * (c.hd / 2), value_place(i, ng), scale_at(c, row * 2 * ng + ng + i / 32));
+        k[o] = held(c.k + row * (c.hd / 2), kv4_key_place(i, ng), scale_at(c, row * 2 * ng + i / 32));
+        v[o] = held(c.v + row * (c.hd / 2), kv4_value_place(i, ng), scale_at(c, row * 2 * ng + ng + i / 32));
     }
 }
 
@@ -358,8 +292,8 @@ double log2_of(float theta) { return theta > 0.0f ? log2((double)theta) : 0.0; }
 
 int kv4_prepare(ibcu_ctx* ctx, const Kv4& c, const Kv4Columns& t, const Kv4Place& at, const Kv4Prep& w) {
     PrepParams p = { c, t, at, w, w.q ? c.n_kv * t.ntiles : 0, t.B <= 8 ? c.n_kv : 1, ctx->kern_err };
-    const int cols = t.cols(), nb = w.q ? std::min(cols, (cols - 1) / t.group + 2) : 1;          // positions that a block may have to do with
-    const size_t smem = (w.rotate ? (size_t)nb * c.hd / 2 * sizeof(double2) : 0) + (w.q ? (size_t)cols * c.hd * sizeof(float) : 0);
+    const int nb = w.q ? std::min(16, 15 / t.group + 2) : 1;  // positions that a block may have to do with
+    const size_t smem = (w.rotate ? (size_t)nb * c.hd / 2 * sizeof(double2) : 0) + (w.q ? (size_t)16 * c.hd * sizeof(float) : 0);
     return ibcu_launch(ctx, kv4_prep_kernel, dim3(p.qblocks + (w.k ? t.B * p.wparts : 0)), dim3(128), smem, 1, true, p);
 }
 

@@ -10,15 +10,15 @@ struct Kv4 {
 };
 
 // The columns of a KV head are its query heads at every position, column = position * group + head of the group. They go through the
-// kernels in tiles of 8 (all columns of a call, if they are no more than that) or of 16. A tile's queries lie in scratch as the A
-// operand's fragments, two fp16 pieces of every value: [unit = KV head * tiles + tile][part][group of 32][step][half][lane] uint2. Tiles of 16 have two parts (high
-// and low pieces), whose halves are columns 0-7 and 8-15; a tile of 8 has one, whose halves are the high and the low pieces.
-// Beside them qc [unit][16]: the factor that turns a column's sums into exponents of 2.
+// kernels in tiles of 8 (all columns of a call, if they are no more than that) or of 16. A tile's queries are the A operand's fragments, two fp16 pieces of every
+// value: [unit = KV head * tiles + tile][part][group of 32][step][lane] uint4. Tiles of 16 have two parts, high and low pieces, with columns 0-7 in the
+// fragments' even registers and 8-15 in the odd ones; a tile of 8 has one, with high and low pieces there. Beside them
+// qc [unit][16]: the factor that turns a column's sums into exponents of 2.
 struct Kv4Columns {
     int n_heads, group, B, large, ntiles;
     __host__ __device__ int cols() const { return large ? 16 : 8; }
 };
-__host__ __device__ constexpr size_t kv4_frag_uint2(int ng, bool large) { return (size_t)(large ? 2 : 1) * ng * 128; }     // of a unit
+__host__ __device__ constexpr size_t kv4_frags(int ng, bool large) { return (size_t)(large ? 2 : 1) * ng * 64; }     // uint4s of a unit
 
 // where rows and positions of a call are: arguments, or {row0, pos0} in device memory
 struct Kv4Place { int row0, pos0; const int* at; };
@@ -32,8 +32,93 @@ __device__ __forceinline__ bool kv4_place(const Kv4Place& p, int B, int max_rows
     return false;
 }
 
+// ── rows ──
+__device__ __forceinline__ int kv4_key_place(int i, int ng) { return ((i & 31) / 8 * ng + i / 32) * 8 + (i & 7); }      // where value i of a row lies
+__device__ __forceinline__ int kv4_value_place(int i, int ng) { return ((i & 31) / 4 * ng + i / 32) * 4 + (i & 3); }
+
+// Angles of positions pos0, pos0 + 1, ..: turn[position][pair] = cosine and sine of position * theta^(-2 pair / hd), in 64 bits, because far positions
+// times a rounded frequency are off by whole steps of a 4-bit code. By all threads of a block; about a microsecond.
+__device__ __forceinline__ void kv4_angles(double2* turn, int positions, int pos0, int hd, double log2_theta) {
+    const int half = hd / 2;
+    for (int e = threadIdx.x; e < positions * half; e += blockDim.x) {
+        double s, c;
+        sincos((double)(pos0 + e / half) * exp2((double)(e % half) * (-2.0 / hd * log2_theta)), &s, &c);
+        turn[e] = make_double2(c, s);
+    }
+}
+// an adjacent pair, turned in 64 bits and rounded once
+__device__ __forceinline__ void kv4_turn(float& x0, float& x1, const double2 cs) {
+    const double a = x0, z = x1;
+    x0 = (float)(a * cs.x - z * cs.y);
+    x1 = (float)(a * cs.y + z * cs.x);
+}
+// A group's scale and the factor that turns its values into codes; amax_bits: the largest magnitude's bits (NaN and Inf above all)
+__device__ __forceinline__ __half kv4_scale(uint32_t amax_bits, float& inv) {
+    if (amax_bits >= 0x7F800000u) { inv = 0.0f; return __ushort_as_half(0x7FFF); }          // NaN: the row says so wherever it is seen
+    const float s = __fmul_rn(__uint_as_float(amax_bits), 1.0f / 7.0f);
+    const __half h = __float2half_rn(fminf(s, 65504.0f));
+    inv = __half2float(h) > 0.0f ? __fdiv_rn(1.0f, __half2float(h)) : 0.0f;
+    return h;
+}
+__device__ __forceinline__ uint32_t kv4_code(float x, float inv) {
+    const float q = inv > 0.0f ? fminf(fmaxf(rintf(__fmul_rn(x, inv)), -7.0f), 7.0f) : 0.0f;
+    return (uint32_t)((int)q + 8);
+}
+// Values i..i+3 of a key or value row of head h, read from src and written to the cache. Eight neighbouring lanes have a group, whose
+// largest magnitude they share. turn: the position's angles, or NULL.
+__device__ __forceinline__ void kv4_write_four(const Kv4& c, const float* src, bool key, int h, int r, int i, const double2* turn) {
+    const int ng = c.hd / 32, lane = threadIdx.x & 31;
+    float x[4] = { __ldcg(src + i), __ldcg(src + i + 1), __ldcg(src + i + 2), __ldcg(src + i + 3) };
+    if (key && turn) { kv4_turn(x[0], x[1], turn[i / 2]); kv4_turn(x[2], x[3], turn[i / 2 + 1]); }
+    uint32_t m = 0;
+#pragma unroll
+    for (int u = 0; u < 4; u++) m = max(m, __float_as_uint(x[u]) & 0x7FFFFFFFu);
+    const unsigned lanes = 0xFFu << (lane & 24);
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(lanes, m, o));
+    float inv;
+    const __half s = kv4_scale(m, inv);
+    uint32_t w = 0;
+#pragma unroll
+    for (int u = 0; u < 4; u++) w |= kv4_code(x[u], inv) << (4 * u);
+    const size_t row = c.row(h, r);
+    const int place = key ? kv4_key_place(i, ng) : kv4_value_place(i, ng);                 // four values stay together in both orders
+    *reinterpret_cast<uint16_t*>((key ? c.k : c.v) + row * (c.hd / 2) + place / 2) = (uint16_t)w;
+    if ((i & 31) == 0) c.scale[row * 2 * ng + (key ? 0 : ng) + i / 32] = s;
+    if (key && i == 0 && c.weight) c.weight[row] = 0.0f;
+}
+
+// ── queries ──
+// values 8t..8t+7 of a group of one query (src: the group's first value), turned
+__device__ __forceinline__ void kv4_query(float (&x)[8], const float* src, bool on, const double2* turn) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = on ? __ldcg(src + i) : 0.0f;
+    if (on && turn) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) kv4_turn(x[i], x[i + 1], turn[i / 2]);
+    }
+}
+// The largest magnitude of a query goes to [2^13, 2^14). A power of 2 up to 2^120, in two factors: what that leaves small are queries below
+// 2^-106, whose scores are zeros beside one another anyway. back: takes it off the sums again; log2(e) makes exponents of 2 of them.
+struct Kv4Up { float a, b, back; };
+__device__ __forceinline__ Kv4Up kv4_up(uint32_t amax_bits, int hd) {
+    const int e = min(120, max(-114, 13 - ((int)(amax_bits >> 23) - 127)));
+    return { __int_as_float(((e >> 1) + 127) << 23), __int_as_float((e - (e >> 1) + 127) << 23),
+             (float)fmin((double)__int_as_float((min(126, -e) + 127) << 23) * (1.4426950408889634 / sqrt((double)hd)), 3.0e38) };
+}
+// Fragments of step s: high and low pieces of codes 2 s and 2 s + 4 of the lane's eight, and of 2 s + 1 and 2 s + 5, which reach the product 16-fold
+__device__ __forceinline__ void kv4_pieces(const float (&x)[8], int s, uint32_t (&hi)[2], uint32_t (&lo)[2]) {
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+        const float f = u ? 0.0625f : 1.0f, a = x[2 * s + u] * f, z = x[2 * s + u + 4] * f;
+        const __half2 h = __floats2half2_rn(a, z), l = __floats2half2_rn(a - __low2float(h), z - __high2float(h));
+        hi[u] = *reinterpret_cast<const uint32_t*>(&h);
+        lo[u] = *reinterpret_cast<const uint32_t*>(&l);
+    }
+}
+
 // Prepares a call's queries (q != NULL) and writes its rows (k != NULL), one launch. Defined in kv4.cu.
-struct Kv4Prep { const float *q, *k, *v; uint2* qf; float* qc; double log2_theta; int rotate; };
+struct Kv4Prep { const float *q, *k, *v; uint4* qf; float* qc; double log2_theta; int rotate; };
 int kv4_prepare(ibcu_ctx* ctx, const Kv4& c, const Kv4Columns& t, const Kv4Place& at, const Kv4Prep& w);
 // The attention of a call, with what it has to prepare. q, k, v as above (k NULL: the rows are there). Defined in kv4_attn.cu.
 int kv4_attend(ibcu_ctx* ctx, const Kv4& c, float decay, const Kv4Place& at, const float* q, const float* k, const float* v, float* out, int n_heads, int B, double log2_theta, int rotate);

@@ -12,10 +12,14 @@
 // The maximum that p refers to is that of score + L(row), 2^L a bound on the row's value scales: then P' never passes 2^14 (2^16 with the
 // slack below), whatever the scales are, and a column's numbers do not depend on rows that it does not see.
 //
-// A block has a tile of 8 or 16 columns of one KV head and a chunk of rows; its four warps take 32 rows each in turn, every
-// warp through a ring of its own that bulk copies fill (rows of a head lie one behind the other), so that no warp waits for another until the end. With
-// up to 8 columns the M = 16 rows of an instruction are 8 columns twice, high and low pieces; with more they are 16 columns
-// and every product is done twice.
+// A warp has a tile of 8 or 16 columns of one KV head and takes 32 rows at a time through a ring of its own that bulk copies fill (rows of a
+// head lie one behind the other), so that no warp waits for another before the end. Three ways (KaMode):
+//   FEW   up to 8 columns, which are the M = 16 rows of an instruction twice, as high and low pieces. One launch: the blocks prepare the queries for themselves and
+//         write the call's rows that lie in their chunk.
+//   MANY  16 columns a tile, every product done twice, once for each piece. The four warps of a block share the tile's rows and put their results together.
+//   WIDE  the same with four tiles a block, a warp for each: what is read through L2 grows, but nothing is left to put together.
+// A column's rows are cut into chunks where that fills the machine; the chunks are joined by the last block of the tile to finish, or by a launch of
+// its own where they are many.
 #include "kv4.cuh"
 #include "tc_common.cuh"
 #include <algorithm>
@@ -26,11 +30,13 @@ constexpr int KA_WARPS = 4, KA_ROWS = 32;            // warps of a block; rows o
 constexpr float KA_LOW = -3.0e38f;                   // where running maxima start (finite: nothing minus infinity)
 constexpr float KA_SLACK = 1.9f;                     // by how much a maximum may be outgrown before the sums are rescaled
 
+enum KaMode { FEW, MANY, WIDE };
+
 struct KaParams {
-    Kv4 c; Kv4Columns t; Kv4Place at;
-    const uint2* qf; const float* qc;
+    Kv4 c; Kv4Columns t; Kv4Place at; Kv4Prep w;     // w.qf, w.qc: fragments prepared (MANY, WIDE), or left for the weights (FEW, if stat)
     float* out; float2* stat;                        // stat [unit][16] or NULL: a column's softmax weight is 2^((score - x) - y)
     float* pacc; float2* pml;                        // chunk results [unit][chunk][16][hd], [unit][chunk][16] (maximum, sum)
+    int* arrived;                                    // [unit] chunks done, zero between launches; NULL: kv4_join_kernel joins them
     int want, grid_chunks;
     int* err;
 };
@@ -44,9 +50,13 @@ __host__ __device__ __forceinline__ void ka_plan(int rows, int want, int& chunk,
     n = (stages + per - 1) / per;
 }
 
-__device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_f16(float* c, const uint4& a, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16_first(float* c, const uint4& a, uint32_t b0, uint32_t b1) {          // nothing to add to
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) { const __half2 h = __floats2half2_rn(lo, hi); return *reinterpret_cast<const uint32_t*>(&h); }
@@ -89,134 +99,263 @@ __device__ __forceinline__ void unpack(uint32_t w, uint32_t* f) {
 template <int NG> struct KaStage {                   // a ring stage: 32 rows of keys, of values and of scales
     static constexpr int KEYS = 0, VALUES = KA_ROWS * 16 * NG, SCALES = 2 * VALUES, BYTES = SCALES + KA_ROWS * 4 * NG;
 };
-template <int NG, bool LARGE> struct KaSmem {
-    static constexpr int DEPTH = NG > 4 ? 2 : 3;
-    static constexpr int FRAGS = 0, QC = (LARGE ? 2 : 1) * NG * 1024, SCALES = QC + 128;
+template <int NG, int MODE> struct KaSmem {
+    static constexpr bool LARGE = MODE != FEW;
+    static constexpr int DEPTH = NG > 4 ? 2 : 3, FRAG_BYTES = (LARGE ? 2 : 1) * NG * 1024, TILES = MODE == WIDE ? KA_WARPS : 1;
+    static constexpr int FRAGS = 0, QC = TILES * FRAG_BYTES, SCALES = QC + (TILES * 64 + 127) / 128 * 128;
     static constexpr int RING = SCALES + KA_WARPS * (2 * NG + 1) * 128;
-    static constexpr int TOTAL = RING + KA_WARPS * DEPTH * KaStage<NG>::BYTES;
-    static_assert(KA_WARPS * (LARGE ? 16 : 8) * 32 * NG * 4 <= KA_WARPS * DEPTH * KaStage<NG>::BYTES, "the warps' results meet in the rings");
+    static constexpr int TOTAL = RING + KA_WARPS * DEPTH * KaStage<NG>::BYTES;       // FEW: angles of the positions follow
+    static_assert(MODE == WIDE || KA_WARPS * (LARGE ? 16 : 8) * 32 * NG * 4 <= KA_WARPS * DEPTH * KaStage<NG>::BYTES, "the warps' results meet in the rings");
 };
 
 // A stage's scales in FP32, once per row instead of once per lane that uses them: sc [2 NG + 1][32], rows in the order t * 8 + 2 i + h
 // for row 8 i + 4 h + t, so that a lane's eight rows lie side by side; the last line is L.
-template <int NG, bool VALUES>
+template <int NG>
 __device__ __forceinline__ void spread_scales(float* sc, const unsigned char* rows, int lane) {
     uint32_t w[NG];
     lds_words<NG>(w, rows + lane * 4 * NG);
     float* d = sc + (lane & 3) * 8 + (lane >> 3) * 2 + ((lane >> 2) & 1);
     uint32_t top = 0;
 #pragma unroll
-    for (int j = 0; j < (VALUES ? 2 * NG : NG); j++) {
-        const uint32_t u = j & 1 ? w[j / 2] >> 16 : w[j / 2] & 0xFFFFu;
-        if (j >= NG) top = max(top, u & 0x7FFFu);
-        d[j * 32] = __half2float(__ushort_as_half((unsigned short)u));
+    for (int j = 0; j < NG; j++) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+        d[2 * j * 32] = f.x;
+        d[(2 * j + 1) * 32] = f.y;
+        // groups NG.. are the values'
+        if (2 * j >= NG) top = max(top, w[j] & 0x7FFFu);
+        if (2 * j + 1 >= NG) top = max(top, w[j] >> 16 & 0x7FFFu);
     }
-    if (VALUES) d[2 * NG * 32] = (float)((int)(top >> 10) - 14);       // scales stay below 2^(exponent - 14)
+    d[2 * NG * 32] = (float)((int)(top >> 10) - 14);          // scales stay below 2^(exponent - 14)
+}
+// a lane's eight rows of a line of sc
+__device__ __forceinline__ void lane_rows(float (&x)[4][2], const float* line, int t) {
+    const float4 a = *reinterpret_cast<const float4*>(line + t * 8), b = *reinterpret_cast<const float4*>(line + t * 8 + 4);
+    x[0][0] = a.x; x[0][1] = a.y; x[1][0] = a.z; x[1][1] = a.w; x[2][0] = b.x; x[2][1] = b.y; x[3][0] = b.z; x[3][1] = b.w;
 }
 
-// Scores of 32 rows: s[i][h][n] for row 8 i + 4 h + t and column g (n = 0), g + 8 (n = 1), in the column's own units
-template <int NG, bool LARGE>
-__device__ __forceinline__ void score_rows(float (&s)[4][2][LARGE ? 2 : 1], const uint32_t (&kw)[4][NG], const uint2* qf, const float* sc, int lane) {
-    const int t = lane & 3;
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-            for (int n = 0; n < (LARGE ? 2 : 1); n++) s[i][h][n] = 0.0f;
+// Scores of 32 rows: s[i][h][n] for row 8 i + 4 h + t and column g (n = 0), g + 8 (n = 1), in the column's own units. keys(i, j, f): the codes
+// of group j of the lane's i-th row, unpacked.
+template <int NG, bool LARGE, typename Keys>
+__device__ __forceinline__ void score_rows(float (&s)[4][2][LARGE ? 2 : 1], Keys keys, const uint4* qf, const float* sc, int lane) {
 #pragma unroll
     for (int j = 0; j < NG; j++) {
-        uint2 a[LARGE ? 2 : 1][2][2];
-#pragma unroll
-        for (int p = 0; p < (LARGE ? 2 : 1); p++)
-#pragma unroll
-            for (int st = 0; st < 2; st++)
-#pragma unroll
-                for (int hf = 0; hf < 2; hf++) a[p][st][hf] = qf[(((p * NG + j) * 2 + st) * 2 + hf) * 32 + lane];
-        const float4 k0 = *reinterpret_cast<const float4*>(sc + j * 32 + t * 8), k1 = *reinterpret_cast<const float4*>(sc + j * 32 + t * 8 + 4);
-        const float ks[4][2] = { { k0.x, k0.y }, { k0.z, k0.w }, { k1.x, k1.y }, { k1.z, k1.w } };
+        const uint4 a0 = qf[(j * 2) * 32 + lane], a1 = qf[(j * 2 + 1) * 32 + lane];
+        uint4 l0 = a0, l1 = a1;
+        if (LARGE) { l0 = qf[((NG + j) * 2) * 32 + lane]; l1 = qf[((NG + j) * 2 + 1) * 32 + lane]; }
+        float ks[4][2];
+        lane_rows(ks, sc + j * 32, lane & 3);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             uint32_t f[4];
-            unpack(kw[i][j], f);
-            float c[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
+            keys(i, j, f);
+            float c[4];
+            mma_f16_first(c, a0, f[0], f[1]);
+            mma_f16(c, a1, f[2], f[3]);
+            if (LARGE) { mma_f16(c, l0, f[0], f[1]); mma_f16(c, l1, f[2], f[3]); }
 #pragma unroll
-            for (int p = 0; p < (LARGE ? 2 : 1); p++) {
-                mma_f16(c, a[p][0][0].x, a[p][0][1].x, a[p][0][0].y, a[p][0][1].y, f[0], f[1]);
-                mma_f16(c, a[p][1][0].x, a[p][1][1].x, a[p][1][0].y, a[p][1][1].y, f[2], f[3]);
-            }
-            if constexpr (LARGE) {
-#pragma unroll
-                for (int n = 0; n < 2; n++) { s[i][0][n] = fmaf(ks[i][0], c[2 * n], s[i][0][n]); s[i][1][n] = fmaf(ks[i][1], c[2 * n + 1], s[i][1][n]); }
-            } else {
-                s[i][0][0] = fmaf(ks[i][0], c[0] + c[2], s[i][0][0]);
-                s[i][1][0] = fmaf(ks[i][1], c[1] + c[3], s[i][1][0]);
+            for (int h = 0; h < 2; h++) {
+                if constexpr (LARGE) {
+                    s[i][h][0] = j ? fmaf(ks[i][h], c[h], s[i][h][0]) : ks[i][h] * c[h];
+                    s[i][h][1] = j ? fmaf(ks[i][h], c[2 + h], s[i][h][1]) : ks[i][h] * c[2 + h];
+                } else {
+                    s[i][h][0] = j ? fmaf(ks[i][h], c[h] + c[2 + h], s[i][h][0]) : ks[i][h] * (c[h] + c[2 + h]);
+                }
             }
         }
     }
 }
 
-template <int NG, bool LARGE>
-__global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (LARGE ? 2 : 3)) kv4_attn_kernel(const KaParams p) {
-    using S = KaSmem<NG, LARGE>;
+// Chunks first, first + step, .. of a column added up at value 4 d4, against the maximum M. at: the column's first chunk. A lane's weights are broadcast
+// to the others: nothing in the loop waits for a load but the sums.
+__device__ __forceinline__ float4 join_values(const KaParams& p, size_t at, int n, int first, int step, float M, int d4) {
+    const int lane = threadIdx.x & 31, mine = (n - first + step - 1) / step;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s0 = 0; s0 < mine; s0 += 32) {
+        const float w = s0 + lane < mine ? ex2(__ldcg(p.pml + at + (size_t)(first + (s0 + lane) * step) * 16).x - M) : 0.0f;
+        const int end = min(32, mine - s0);
+#pragma unroll 8
+        for (int s = 0; s < end; s++) {
+            const float k = __shfl_sync(0xffffffffu, w, s);
+            const float4 v = d4 < p.c.hd / 4 ? __ldcg(reinterpret_cast<const float4*>(p.pacc + (at + (size_t)(first + (s0 + s) * step) * 16) * p.c.hd) + d4) : make_float4(0.f, 0.f, 0.f, 0.f);
+            o.x = fmaf(v.x, k, o.x); o.y = fmaf(v.y, k, o.y); o.z = fmaf(v.z, k, o.z); o.w = fmaf(v.w, k, o.w);
+        }
+    }
+    return o;
+}
+// maximum and sum over the chunks, by a warp
+__device__ __forceinline__ float2 join_stat(const KaParams& p, size_t at, int n) {
+    const int lane = threadIdx.x & 31;
+    float2 own = lane < n ? __ldcg(p.pml + at + (size_t)lane * 16) : make_float2(KA_LOW, 0.0f);
+    float M = own.x;
+    for (int s = lane + 32; s < n; s += 32) M = fmaxf(M, __ldcg(p.pml + at + (size_t)s * 16).x);
+    M = warp_max(M);
+    float sum = own.y * ex2(own.x - M);
+    for (int s = lane + 32; s < n; s += 32) { const float2 v = __ldcg(p.pml + at + (size_t)s * 16); sum = fmaf(v.y, ex2(v.x - M), sum); }
+    return make_float2(M, warp_sum(sum));
+}
+__device__ __forceinline__ void join_store(const KaParams& p, int kvh, int cc, int d4, const float4& o, float inv) {
+    float* to = p.out + ((size_t)(cc / p.t.group) * p.t.n_heads + (size_t)kvh * p.t.group + cc % p.t.group) * p.c.hd + 4 * d4;
+    to[0] = o.x * inv; to[1] = o.y * inv; to[2] = o.z * inv; to[3] = o.w * inv;
+}
+// The chunks of a unit put together by its last block, a warp every fourth column.
+__device__ __forceinline__ void join_by_last(const KaParams& p, int unit, int n) {
+    const int lane = threadIdx.x & 31, kvh = unit / p.t.ntiles, c0 = unit % p.t.ntiles * p.t.cols(), q4 = p.c.hd / 4;
+    for (int col = threadIdx.x >> 5; col < p.t.cols() && (c0 + col) / p.t.group < p.t.B; col += KA_WARPS) {
+        const size_t at = (size_t)unit * p.grid_chunks * 16 + col;
+        const float2 st = join_stat(p, at, n);
+        for (int d0 = 0; d0 < q4; d0 += 32) {
+            const float4 o = join_values(p, at, n, 0, 1, st.x, d0 + lane);
+            if (d0 + lane < q4) join_store(p, kvh, c0 + col, d0 + lane, o, 1.0f / st.y);
+        }
+        if (lane == 0 && p.stat) p.stat[(size_t)unit * 16 + col] = make_float2(st.x, log2f(st.y) - 14.0f);
+    }
+}
+// grid (columns of a tile, units): the same by a launch of its own, a block a column, where there are many chunks
+__global__ void __launch_bounds__(128) kv4_join_kernel(const KaParams p) {
+    __shared__ float4 part[4][64];
+    pdl_launch_dependents();
+    pdl_wait();
+    int row0, pos0, chunk, n;
+    if (!kv4_place(p.at, p.t.B, p.c.max_rows, p.err, row0, pos0)) return;
+    ka_plan(row0 + p.t.B, p.want, chunk, n);
+    const int unit = blockIdx.y, kvh = unit / p.t.ntiles, cc = unit % p.t.ntiles * p.t.cols() + blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q4 = p.c.hd / 4;
+    if (n == 1 || cc / p.t.group >= p.t.B) return;
+    const size_t at = (size_t)unit * p.grid_chunks * 16 + blockIdx.x;
+    const float2 st = join_stat(p, at, n);
+    for (int d0 = 0; d0 < q4; d0 += 32) part[warp][d0 + lane] = join_values(p, at, n, warp, 4, st.x, d0 + lane);
+    __syncthreads();
+    if (threadIdx.x < q4) {
+        float4 o = part[0][threadIdx.x];
+        for (int w = 1; w < 4; w++) { const float4 v = part[w][threadIdx.x]; o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w; }
+        join_store(p, kvh, cc, threadIdx.x, o, 1.0f / st.y);
+    }
+    if (threadIdx.x == 0 && p.stat) p.stat[(size_t)unit * 16 + blockIdx.x] = make_float2(st.x, log2f(st.y) - 14.0f);
+}
+
+template <int NG, int MODE>
+__global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (MODE == FEW ? 3 : 2)) kv4_attn_kernel(const KaParams p) {
+    using S = KaSmem<NG, MODE>;
     using St = KaStage<NG>;
-    constexpr int NC = LARGE ? 2 : 1, COLS = 8 * NC, HD = 32 * NG;
+    constexpr bool LARGE = S::LARGE;
+    constexpr int NC = LARGE ? 2 : 1, COLS = 8 * NC, HD = 32 * NG, EACH = MODE == WIDE ? 1 : KA_WARPS;          // EACH: a warp takes every EACH-th stage
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ unsigned long long full[KA_WARPS][S::DEPTH];
-    __shared__ int abort_flag;
+    __shared__ int abort_flag, last;
+    __shared__ float2 ml[KA_WARPS][16];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int tile = p.t.ntiles - 1 - blockIdx.x % p.t.ntiles, kvh = blockIdx.x / p.t.ntiles, sp = blockIdx.y;   // tiles that see most rows first
+    // tiles that see most rows first
+    const int per_head = (p.t.ntiles + S::TILES - 1) / S::TILES, kvh = blockIdx.x / per_head, sp = blockIdx.y;
+    const int tile = p.t.ntiles - 1 - (blockIdx.x % per_head * S::TILES + (MODE == WIDE ? warp : 0));
     const int unit = kvh * p.t.ntiles + tile, c0 = tile * COLS;
     if (tid == 0) {
         abort_flag = 0;
         for (int w = 0; w < KA_WARPS; w++) for (int d = 0; d < S::DEPTH; d++) mbar_init(smem_u32(&full[w][d]), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    double2* turn = reinterpret_cast<double2*>(smem + S::TOTAL);
+    int row0 = p.at.row0, pos0 = p.at.pos0;
+    if (MODE == FEW) {
+        if (p.w.rotate && !p.at.at) kv4_angles(turn, p.t.B, pos0, HD, p.w.log2_theta);             // beside the end of the launch ahead
+        pdl_wait();
+        pdl_launch_dependents();
+    }
     __syncthreads();
-    // Launches ahead of the preparing one have ended when this one starts, since that one lets it start behind its own wait: what they wrote (a
+    // MANY, WIDE: launches ahead of the preparing one have ended when this one starts, since that one lets it start behind its own wait. What they wrote (a
     // device position, rows of earlier calls) may be read before this launch's own wait.
-    int row0, pos0;
     if (!kv4_place(p.at, p.t.B, p.c.max_rows, p.err, row0, pos0)) return;
+    if (MODE == FEW && p.w.rotate && p.at.at) kv4_angles(turn, p.t.B, pos0, HD, p.w.log2_theta);
     int chunk, n_chunks;
     ka_plan(row0 + p.t.B, p.want, chunk, n_chunks);
     if (sp >= n_chunks) return;
-    const int lim0 = row0 + c0 / p.t.group;                                                        // the last row that the tile's first column sees
-    const int t0 = sp * chunk, t1 = min(t0 + chunk, row0 + min(p.t.B - 1, (c0 + COLS - 1) / p.t.group) + 1);
-    const int stages = t1 > t0 ? (t1 - t0 + KA_ROWS - 1) / KA_ROWS : 0, mine = stages > warp ? (stages - warp + KA_WARPS - 1) / KA_WARPS : 0;
+    const int lim0 = row0 + max(c0, 0) / p.t.group;                                                // the last row that the tile's first column sees
+    const int t0 = sp * chunk, t1 = tile < 0 ? 0 : min(t0 + chunk, row0 + min(p.t.B - 1, (c0 + COLS - 1) / p.t.group) + 1);
+    const int skip = MODE == WIDE ? 0 : warp, stages = t1 > t0 ? (t1 - t0 + KA_ROWS - 1) / KA_ROWS : 0, mine = stages > skip ? (stages - skip + EACH - 1) / EACH : 0;
     unsigned char* ring = smem + S::RING + warp * S::DEPTH * St::BYTES;
     const size_t plane = p.c.row(kvh, 0);
     auto issue = [&](int n) {                                                                      // one lane: the n-th stage of this warp; whole groups of 8 rows, which the planes have
-        const int r = t0 + (warp + n * KA_WARPS) * KA_ROWS, rows = min(KA_ROWS, (t1 - r + 7) & ~7), d = n % S::DEPTH;
+        const int r = t0 + (skip + n * EACH) * KA_ROWS, rows = min(KA_ROWS, (t1 - r + 7) & ~7), d = n % S::DEPTH;
         const uint32_t bar = smem_u32(&full[warp][d]), to = smem_u32(ring + d * St::BYTES);
         mbar_expect_tx(bar, (uint32_t)rows * 36 * NG);
         bulk_load(to + St::KEYS, p.c.k + (plane + r) * (16 * NG), (uint32_t)rows * 16 * NG, bar);
         bulk_load(to + St::VALUES, p.c.v + (plane + r) * (16 * NG), (uint32_t)rows * 16 * NG, bar);
         bulk_load(to + St::SCALES, p.c.scale + (plane + r) * (2 * NG), (uint32_t)rows * 4 * NG, bar);
     };
+    const int old = p.w.k ? row0 : t1;                                                             // rows below were there before this call
     int issued = 0;
     if (lane == 0)
-        for (; issued < min(mine, (int)S::DEPTH) && t0 + (warp + issued * KA_WARPS) * KA_ROWS + KA_ROWS <= row0; issued++) issue(issued);
-    pdl_wait();
-    pdl_launch_dependents();
-    if (lane == 0) {
-        asm volatile("fence.proxy.async.global;" ::: "memory");                                    // rows that the preparing launch wrote
-        for (; issued < min(mine, (int)S::DEPTH); issued++) issue(issued);
+        for (; issued < min(mine, (int)S::DEPTH) && t0 + (skip + issued * EACH) * KA_ROWS + KA_ROWS <= old; issued++) issue(issued);
+    uint4* qf = reinterpret_cast<uint4*>(smem + S::FRAGS + (MODE == WIDE ? warp * S::FRAG_BYTES : 0));
+    float* qc = reinterpret_cast<float*>(smem + S::QC) + (MODE == WIDE ? warp * 16 : 0);
+    if constexpr (MODE == FEW) {
+        __shared__ uint32_t amax[KA_WARPS][8];
+        __syncthreads();
+        if (p.w.k) {                                                                               // the call's rows of this chunk
+            const int r0 = max(t0, row0), r1 = min(t1, row0 + p.t.B);
+            for (int e = tid; e < (r1 - r0) * 2 * (HD / 4); e += 32 * KA_WARPS) {
+                const int f = e / (HD / 4), r = r0 + f / 2, b = r - row0;
+                const bool key = f % 2 == 0;
+                kv4_write_four(p.c, (key ? p.w.k : p.w.v) + ((size_t)b * p.c.n_kv + kvh) * HD, key, kvh, r, e % (HD / 4) * 4, p.w.rotate ? turn + b * (HD / 2) : nullptr);
+            }
+            asm volatile("fence.proxy.async.global;" ::: "memory");                                // the bulk copies read them
+        }
+        constexpr int JT = (NG + KA_WARPS - 1) / KA_WARPS;                                         // a warp has every fourth group of all columns
+        const int b = g / p.t.group;
+        const bool on = b < p.t.B;
+        const float* src = p.w.q + ((size_t)b * p.t.n_heads + (size_t)kvh * p.t.group + g % p.t.group) * HD + 8 * t;
+        float x[JT][8];
+        uint32_t m = 0;
+#pragma unroll
+        for (int jj = 0; jj < JT; jj++) {
+            const int j = warp + jj * KA_WARPS;
+            if (j >= NG) break;
+            kv4_query(x[jj], src + 32 * j, on, p.w.rotate ? turn + b * (HD / 2) + 16 * j + 4 * t : nullptr);
+#pragma unroll
+            for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(x[jj][i]) & 0x7FFFFFFFu);
+        }
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        if (t == 0) amax[warp][g] = m;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < KA_WARPS; w++) m = max(m, amax[w][g]);
+        const Kv4Up up = kv4_up(m, HD);
+        const bool leave = p.stat && sp == 0;
+        if (warp == 0 && t == 0) { qc[g] = up.back; if (leave) p.w.qc[(size_t)unit * 16 + g] = up.back; }
+#pragma unroll
+        for (int jj = 0; jj < JT; jj++) {
+            const int j = warp + jj * KA_WARPS;
+            if (j >= NG) break;
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[jj][i] = x[jj][i] * up.a * up.b;
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                uint32_t hi[2], lo[2];
+                kv4_pieces(x[jj], s, hi, lo);
+                const uint4 v = make_uint4(hi[0], lo[0], hi[1], lo[1]);
+                qf[(j * 2 + s) * 32 + lane] = v;
+                if (leave) p.w.qf[unit * kv4_frags(NG, false) + (j * 2 + s) * 32 + lane] = v;
+            }
+        }
+    } else {
+        pdl_wait();
+        pdl_launch_dependents();
+        if (lane == 0) asm volatile("fence.proxy.async.global;" ::: "memory");                     // rows that the preparing launch wrote
+        const int n = MODE == WIDE ? 32 : 32 * KA_WARPS, e0 = MODE == WIDE ? lane : tid;
+        if (tile >= 0) {
+            const uint4* src = p.w.qf + unit * kv4_frags(NG, true);
+            for (int e = e0; e < NG * 128; e += n) qf[e] = __ldcg(src + e);
+            if (e0 < 16) qc[e0] = __ldcg(p.w.qc + (size_t)unit * 16 + e0);
+        }
     }
-    uint2* qf = reinterpret_cast<uint2*>(smem + S::FRAGS);
-    float* qc = reinterpret_cast<float*>(smem + S::QC);
-    {
-        const uint4* src = reinterpret_cast<const uint4*>(p.qf + unit * kv4_frag_uint2(NG, LARGE));
-        for (int e = tid; e < NC * NG * 64; e += 32 * KA_WARPS) reinterpret_cast<uint4*>(qf)[e] = __ldcg(src + e);
-        if (tid < COLS) qc[tid] = __ldcg(p.qc + (size_t)unit * 16 + tid);
-    }
-    __syncthreads();
+    if (lane == 0) for (; issued < min(mine, (int)S::DEPTH); issued++) issue(issued);
+    if (MODE == WIDE) __syncwarp(); else __syncthreads();
     float* sc = reinterpret_cast<float*>(smem + S::SCALES) + warp * (2 * NG + 1) * 32;
     float f[NC], m[NC], l[NC], acc[NG][4][4];
     int lim[NC];
 #pragma unroll
     for (int n = 0; n < NC; n++) {
         f[n] = qc[g + 8 * n]; m[n] = KA_LOW; l[n] = 0.0f;
-        lim[n] = row0 + (c0 + g + 8 * n) / p.t.group;
+        lim[n] = row0 + (max(c0, 0) + g + 8 * n) / p.t.group;
     }
 #pragma unroll
     for (int j = 0; j < NG; j++)
@@ -229,16 +368,16 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (LARGE ? 2 : 3)) k
     int d = 0;
     bool wide = false;
     for (int it = 0; it < mine; it++) {
-        const int r0 = t0 + (warp + it * KA_WARPS) * KA_ROWS;
+        const int r0 = t0 + (skip + it * EACH) * KA_ROWS;
         if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&full[warp][d]), phase, &abort_flag, IBCU_KV4_WAIT_ERR))) break;
         const unsigned char* stage = ring + d * St::BYTES;
-        spread_scales<NG, true>(sc, stage + St::SCALES, lane);
+        spread_scales<NG>(sc, stage + St::SCALES, lane);
         uint32_t kw[4][NG], vw[4][2][(NG + 1) / 2];
 #pragma unroll
         for (int i = 0; i < 4; i++) lds_words<NG>(kw[i], stage + St::KEYS + (8 * i + (g >> 1) + 4 * (g & 1)) * 16 * NG + t * 4 * NG);
         __syncwarp();
         float s[4][2][NC];
-        score_rows<NG, LARGE>(s, kw, qf, sc, lane);
+        score_rows<NG, LARGE>(s, [&](int i, int j, uint32_t* to) { unpack(kw[i][j], to); }, qf, sc, lane);
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -249,10 +388,9 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (LARGE ? 2 : 3)) k
 
         auto weigh = [&](auto masked) {
             constexpr bool MASK = decltype(masked)::value;
-            const float4 l0 = *reinterpret_cast<const float4*>(sc + 2 * NG * 32 + t * 8), l1 = *reinterpret_cast<const float4*>(sc + 2 * NG * 32 + t * 8 + 4);
-            const float L[4][2] = { { l0.x, l0.y }, { l0.z, l0.w }, { l1.x, l1.y }, { l1.z, l1.w } };
+            float L[4][2], top[NC];
+            lane_rows(L, sc + 2 * NG * 32, t);
             auto seen = [&](int i, int h, int n) { return !MASK || r0 + 8 * i + 4 * h + t <= lim[n]; };
-            float top[NC];
             bool grow = false;
 #pragma unroll
             for (int n = 0; n < NC; n++) {
@@ -314,8 +452,8 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (LARGE ? 2 : 3)) k
             }
 #pragma unroll
             for (int j = 0; j < NG; j++) {
-                const float4 v0 = *reinterpret_cast<const float4*>(sc + (NG + j) * 32 + t * 8), v1 = *reinterpret_cast<const float4*>(sc + (NG + j) * 32 + t * 8 + 4);
-                const float vs[4][2] = { { v0.x, v0.y }, { v0.z, v0.w }, { v1.x, v1.y }, { v1.z, v1.w } };
+                float vs[4][2];
+                lane_rows(vs, sc + (NG + j) * 32, t);
 #pragma unroll
                 for (int u = 0; u < 2; u++) {                                                      // 16 rows: pieces 2 u and 2 u + 1
                     uint32_t hi[2][NC], lo[2][NC];
@@ -330,18 +468,16 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (LARGE ? 2 : 3)) k
                             const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[i][n]));
                             lo[i][n] = pack_half(a - back.x, b - back.y);
                         }
-                    uint32_t x0 = __byte_perm(vw[2 * u][0][j / 2], vw[2 * u][1][j / 2], j & 1 ? 0x7632 : 0x5410);
-                    uint32_t x1 = __byte_perm(vw[2 * u + 1][0][j / 2], vw[2 * u + 1][1][j / 2], j & 1 ? 0x7632 : 0x5410);
                     uint32_t b0[4], b1[4];
-                    unpack(x0, b0);
-                    unpack(x1, b1);
+                    unpack(__byte_perm(vw[2 * u][0][j / 2], vw[2 * u][1][j / 2], j & 1 ? 0x7632 : 0x5410), b0);
+                    unpack(__byte_perm(vw[2 * u + 1][0][j / 2], vw[2 * u + 1][1][j / 2], j & 1 ? 0x7632 : 0x5410), b1);
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         if constexpr (LARGE) {
-                            mma_f16(acc[j][i], hi[0][0], hi[0][1], hi[1][0], hi[1][1], b0[i], b1[i]);
-                            mma_f16(acc[j][i], lo[0][0], lo[0][1], lo[1][0], lo[1][1], b0[i], b1[i]);
+                            mma_f16(acc[j][i], make_uint4(hi[0][0], hi[0][1], hi[1][0], hi[1][1]), b0[i], b1[i]);
+                            mma_f16(acc[j][i], make_uint4(lo[0][0], lo[0][1], lo[1][0], lo[1][1]), b0[i], b1[i]);
                         } else {
-                            mma_f16(acc[j][i], hi[0][0], lo[0][0], hi[1][0], lo[1][0], b0[i], b1[i]);
+                            mma_f16(acc[j][i], make_uint4(hi[0][0], lo[0][0], hi[1][0], lo[1][0]), b0[i], b1[i]);
                         }
                     }
                 }
@@ -352,14 +488,56 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (LARGE ? 2 : 3)) k
         __syncwarp();                                                                              // the scales may be overwritten
     }
 
-    // the four warps' results meet in the rings: [warp][column][value], and maxima and sums
-    __shared__ float2 ml[KA_WARPS][16];
 #pragma unroll
     for (int n = 0; n < NC; n++) {
         l[n] += __shfl_xor_sync(0xffffffffu, l[n], 1);
         l[n] += __shfl_xor_sync(0xffffffffu, l[n], 2);
-        if (t == 0) ml[warp][g + 8 * n] = make_float2(m[n], l[n]);
     }
+    // values 8t..8t+7 of group j of column g + 8 n
+    auto values = [&](int n, int j, float (&o)[8]) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const float a = LARGE ? acc[j][i][2 * n + u] : acc[j][i][u] + acc[j][i][u + 2];
+                o[4 * u + i] = i & 1 ? a * 0.0625f : a;
+            }
+    };
+    auto give_up = [&]() {                                     // by one thread of the block, when its waits are over
+        if (!*(volatile int*)&abort_flag) return;
+        *p.err = IBCU_KV4_WAIT_ERR;
+        for (int i = 0; i < 1000; i++) __nanosleep(1000);      // copies still on their way into this block's shared memory land before it goes
+    };
+    if constexpr (MODE == WIDE) {
+#pragma unroll
+        for (int n = 0; n < NC; n++) {
+            const int c = c0 + g + 8 * n, b = c / p.t.group;
+            if (tile < 0 || b >= p.t.B) continue;
+            float* to = p.out + ((size_t)b * p.t.n_heads + (size_t)kvh * p.t.group + c % p.t.group) * HD + 8 * t;
+            const float inv = 1.0f / l[n];
+            const bool vec = ((uintptr_t)p.out & 15) == 0;
+#pragma unroll
+            for (int j = 0; j < NG; j++) {
+                float o[8];
+                values(n, j, o);
+                if (vec) {
+                    *reinterpret_cast<float4*>(to + 32 * j) = make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+                    *reinterpret_cast<float4*>(to + 32 * j + 4) = make_float4(o[4] * inv, o[5] * inv, o[6] * inv, o[7] * inv);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) to[32 * j + i] = o[i] * inv;
+                }
+            }
+            if (t == 0 && p.stat) p.stat[(size_t)unit * 16 + g + 8 * n] = make_float2(m[n], log2f(l[n]) - 14.0f);
+        }
+        __syncthreads();
+        if (tid == 0) give_up();
+        return;
+    }
+
+    // the four warps' results meet in the rings: [warp][column][value], and maxima and sums
+#pragma unroll
+    for (int n = 0; n < NC; n++) if (t == 0) ml[warp][g + 8 * n] = make_float2(m[n], l[n]);
     __syncthreads();
     float* meet = reinterpret_cast<float*>(smem + S::RING);
 #pragma unroll
@@ -367,26 +545,17 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (LARGE ? 2 : 3)) k
 #pragma unroll
         for (int j = 0; j < NG; j++) {
             float o[8];
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const float a = LARGE ? acc[j][i][2 * n + u] : acc[j][i][u] + acc[j][i][u + 2];
-                    o[4 * u + i] = i & 1 ? a * 0.0625f : a;
-                }
+            values(n, j, o);
             float4* to = reinterpret_cast<float4*>(meet + ((size_t)warp * COLS + g + 8 * n) * HD + 32 * j + 8 * t);
             to[0] = make_float4(o[0], o[1], o[2], o[3]);
             to[1] = make_float4(o[4], o[5], o[6], o[7]);
         }
     __syncthreads();
-    if (tid == 0 && abort_flag) {
-        *p.err = abort_flag;
-        for (int i = 0; i < 1000; i++) __nanosleep(1000);      // copies still on their way into this block's shared memory land before it goes
-    }
+    if (tid == 0) give_up();
     for (int e = tid; e < COLS * HD / 4; e += 32 * KA_WARPS) {
         const int col = e / (HD / 4), d4 = e % (HD / 4), c = c0 + col, b = c / p.t.group;
         if (b >= p.t.B) break;
-        float M = ml[0][col].x, wsum = 0.0f;
+        float M = ml[0][col].x, sum = 0.0f;
 #pragma unroll
         for (int w = 1; w < KA_WARPS; w++) M = fmaxf(M, ml[w][col].x);
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -394,114 +563,115 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (LARGE ? 2 : 3)) k
         for (int w = 0; w < KA_WARPS; w++) {
             const float k = ex2(ml[w][col].x - M);
             const float4 v = *reinterpret_cast<const float4*>(meet + ((size_t)w * COLS + col) * HD + 4 * d4);
-            wsum = fmaf(ml[w][col].y, k, wsum);
+            sum = fmaf(ml[w][col].y, k, sum);
             o.x = fmaf(v.x, k, o.x); o.y = fmaf(v.y, k, o.y); o.z = fmaf(v.z, k, o.z); o.w = fmaf(v.w, k, o.w);
         }
         if (n_chunks == 1) {
             float* to = p.out + ((size_t)b * p.t.n_heads + (size_t)kvh * p.t.group + c % p.t.group) * HD + 4 * d4;
-            const float inv = 1.0f / wsum;
+            const float inv = 1.0f / sum;
             to[0] = o.x * inv; to[1] = o.y * inv; to[2] = o.z * inv; to[3] = o.w * inv;
-            if (d4 == 0 && p.stat) p.stat[(size_t)unit * 16 + col] = make_float2(M, log2f(wsum) - 14.0f);
+            if (d4 == 0 && p.stat) p.stat[(size_t)unit * 16 + col] = make_float2(M, log2f(sum) - 14.0f);
         } else {
             const size_t at = ((size_t)unit * p.grid_chunks + sp) * 16 + col;
             *reinterpret_cast<float4*>(p.pacc + at * HD + 4 * d4) = o;
-            if (d4 == 0) p.pml[at] = make_float2(M, wsum);
+            if (d4 == 0) p.pml[at] = make_float2(M, sum);
+        }
+    }
+    if (n_chunks > 1 && p.arrived) {
+        __threadfence();                                       // this block's chunk, ahead of its arrival
+        __syncthreads();
+        if (tid == 0) last = atomicAdd(p.arrived + unit, 1) == n_chunks - 1;
+        __syncthreads();
+        if (last) {
+            __threadfence();
+            if (tid == 0) p.arrived[unit] = 0;
+            join_by_last(p, unit, n_chunks);
         }
     }
 }
 
-// grid (columns of a tile, units): the chunks of a column joined
-__global__ void __launch_bounds__(128) kv4_join_kernel(const KaParams p) {
-    extern __shared__ __align__(16) float4 part[];            // [threads]
-    pdl_launch_dependents();
-    pdl_wait();
-    int row0, pos0, chunk, n;
-    if (!kv4_place(p.at, p.t.B, p.c.max_rows, p.err, row0, pos0)) return;
-    ka_plan(row0 + p.t.B, p.want, chunk, n);
-    const int unit = blockIdx.y, kvh = unit / p.t.ntiles, tile = unit % p.t.ntiles, col = blockIdx.x, cc = tile * p.t.cols() + col, b = cc / p.t.group;
-    if (n == 1 || b >= p.t.B) return;
-    const int q4 = p.c.hd / 4, lanes = min(q4, 64), ways = 128 / lanes, way = threadIdx.x / lanes, tid = threadIdx.x;
-    const size_t base = (size_t)unit * p.grid_chunks * 16 + col;
-    float M = KA_LOW;
-    for (int s = tid & 31; s < n; s += 32) M = fmaxf(M, __ldcg(&p.pml[base + (size_t)s * 16].x));
-    M = warp_max(M);
-    float sum = 0.0f;
-    for (int s = tid & 31; s < n; s += 32) { const float2 v = __ldcg(&p.pml[base + (size_t)s * 16]); sum = fmaf(v.y, ex2(v.x - M), sum); }
-    sum = warp_sum(sum);
-    const float inv = 1.0f / sum;
-    if (way < ways) {
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        const int d4 = tid % lanes;
-#pragma unroll 4
-        for (int s = way; s < n; s += ways) {
-            const float k = ex2(__ldcg(&p.pml[base + (size_t)s * 16].x) - M);
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(p.pacc + (base + (size_t)s * 16) * p.c.hd) + d4);
-            o.x = fmaf(v.x, k, o.x); o.y = fmaf(v.y, k, o.y); o.z = fmaf(v.z, k, o.z); o.w = fmaf(v.w, k, o.w);
-        }
-        part[tid] = o;
+// Attention that the rows draw. grid (128 rows, KV heads, parts of the tiles): a warp holds the unpacked keys of 32 rows and walks the columns that see them,
+// whose fragments come through a ring; the scores are computed again, which costs less than writing them down once there are several columns. The
+// parts of a row are added in order.
+constexpr int KW_DEPTH = 3;
+template <int NG, bool LARGE> struct KwSmem {
+    static constexpr int FRAG_BYTES = (LARGE ? 2 : 1) * NG * 1024, QC = FRAG_BYTES, STAT = QC + 64, STAGE = STAT + 128 + 64;
+    static constexpr int SCALES = KW_DEPTH * STAGE, TOTAL = SCALES + KA_WARPS * NG * 128;
+};
+template <int NG, bool LARGE>
+__global__ void __launch_bounds__(32 * KA_WARPS) kv4_weight_kernel(const KaParams p, float decay, float* __restrict__ parts) {
+    using S = KwSmem<NG, LARGE>;
+    constexpr int NC = LARGE ? 2 : 1, COLS = 8 * NC;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ unsigned long long full[KW_DEPTH];
+    __shared__ int abort_flag;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, kvh = blockIdx.y;
+    if (tid == 0) {
+        abort_flag = 0;
+        for (int d = 0; d < KW_DEPTH; d++) mbar_init(smem_u32(&full[d]), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
-    if (tid < q4) {
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int w = 0; w < ways; w++) { const float4 v = part[w * lanes + tid]; o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w; }
-        float* to = p.out + ((size_t)b * p.t.n_heads + (size_t)kvh * p.t.group + cc % p.t.group) * p.c.hd + 4 * tid;
-        to[0] = o.x * inv; to[1] = o.y * inv; to[2] = o.z * inv; to[3] = o.w * inv;
-    }
-    if (tid == 0 && p.stat) p.stat[(size_t)unit * 16 + col] = make_float2(M, log2f(sum) - 14.0f);
-}
-
-// Attention that the rows draw. grid (128 rows, KV heads, parts of the tiles): a warp holds the keys of 32 rows and walks the columns that see them; the
-// scores are computed again, which costs less than writing them down once there are several columns. The parts of a row are added in order.
-template <int NG, bool LARGE>
-__global__ void __launch_bounds__(128) kv4_weight_kernel(const KaParams p, float decay, float* __restrict__ parts) {
-    constexpr int NC = LARGE ? 2 : 1, COLS = 8 * NC;
-    __shared__ __align__(16) uint2 qf[NC * NG * 128];
-    __shared__ float qc[16];
-    __shared__ float2 st[16];
-    __shared__ __align__(16) float scales[4][NG * 32];
     pdl_launch_dependents();
     pdl_wait();
     int row0, pos0;
     if (!kv4_place(p.at, p.t.B, p.c.max_rows, p.err, row0, pos0)) return;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, kvh = blockIdx.y, R = row0 + p.t.B;
-    const int r0 = blockIdx.x * 128 + warp * 32;
+    const int R = row0 + p.t.B, r0 = blockIdx.x * 128 + warp * 32;
     if ((int)blockIdx.x * 128 >= R) return;
-    float* sc = scales[warp];
-    uint32_t kw[4][NG];
+    const int first = max(0, (int)blockIdx.x * 128 - row0) * p.t.group / COLS + blockIdx.z;       // tiles that see a row of the block, every gridDim.z-th
+    const int n = first < p.t.ntiles ? (p.t.ntiles - first + gridDim.z - 1) / gridDim.z : 0;
+    auto issue = [&](int i) {
+        const int unit = kvh * p.t.ntiles + first + i * gridDim.z, d = i % KW_DEPTH;
+        const uint32_t bar = smem_u32(&full[d]), to = smem_u32(smem + d * S::STAGE);
+        mbar_expect_tx(bar, S::FRAG_BYTES + 64 + 128);
+        bulk_load(to, p.w.qf + unit * kv4_frags(NG, LARGE), S::FRAG_BYTES, bar);
+        bulk_load(to + S::QC, p.w.qc + (size_t)unit * 16, 64, bar);
+        bulk_load(to + S::STAT, p.stat + (size_t)unit * 16, 128, bar);
+    };
+    if (tid == 0) {
+        asm volatile("fence.proxy.async.global;" ::: "memory");                                    // the launches ahead wrote them
+        for (int i = 0; i < min(n, KW_DEPTH); i++) issue(i);
+    }
+    float* sc = reinterpret_cast<float*>(smem + S::SCALES) + warp * NG * 32;
+    uint32_t kf[4][NG][4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const int r = min(r0 + 8 * i + (g >> 1) + 4 * (g & 1), R - 1);
         const uint32_t* src = reinterpret_cast<const uint32_t*>(p.c.k + p.c.row(kvh, r) * (16 * NG)) + t * NG;
 #pragma unroll
-        for (int j = 0; j < NG; j++) kw[i][j] = __ldcg(src + j);
+        for (int j = 0; j < NG; j++) unpack(__ldcg(src + j), kf[i][j]);
     }
     {
         const __half* src = p.c.scale + p.c.row(kvh, min(r0 + lane, R - 1)) * (2 * NG);
         float* d = sc + (lane & 3) * 8 + (lane >> 3) * 2 + ((lane >> 2) & 1);
         for (int j = 0; j < NG; j++) d[j * 32] = __half2float(__ushort_as_half(__ldcg(reinterpret_cast<const unsigned short*>(src) + j)));
     }
+    __syncwarp();
     float w[4][2] = {};
-    const int first = max(0, (int)blockIdx.x * 128 - row0) * p.t.group / COLS;                    // the first tile that sees a row of the block
-    for (int tile = first + blockIdx.z; tile < p.t.ntiles; tile += gridDim.z) {
-        const int unit = kvh * p.t.ntiles + tile, c0 = tile * COLS;
-        __syncthreads();
-        const uint4* src = reinterpret_cast<const uint4*>(p.qf + unit * kv4_frag_uint2(NG, LARGE));
-        for (int e = tid; e < NC * NG * 64; e += 128) reinterpret_cast<uint4*>(qf)[e] = __ldcg(src + e);
-        if (tid < COLS) qc[tid] = __ldcg(p.qc + (size_t)unit * 16 + tid);
-        if (tid < COLS) st[tid] = __ldcg(p.stat + (size_t)unit * 16 + tid);
-        __syncthreads();
+    int d = 0;
+    uint32_t phase = 0;
+    for (int i = 0; i < n; i++) {
+        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&full[d]), phase, &abort_flag, IBCU_KV4_WAIT_ERR))) { __syncthreads(); continue; }      // the barrier below is everyone's
+        const unsigned char* stage = smem + d * S::STAGE;
         float s[4][2][NC];
-        score_rows<NG, LARGE>(s, kw, qf, sc, lane);
+        score_rows<NG, LARGE>(s, [&](int k, int j, uint32_t* to) {
 #pragma unroll
-        for (int n = 0; n < NC; n++) {
-            const int c = c0 + g + 8 * n, b = c / p.t.group, lim = b < p.t.B ? row0 + b : -1;
-            const float f = qc[g + 8 * n];
-            const float2 off = st[g + 8 * n];
+            for (int u = 0; u < 4; u++) to[u] = kf[k][j][u];
+        }, reinterpret_cast<const uint4*>(stage), sc, lane);
+        const int c0 = (first + i * gridDim.z) * COLS;
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+        for (int k = 0; k < NC; k++) {
+            const int b = (c0 + g + 8 * k) / p.t.group, lim = b < p.t.B ? row0 + b : -1;
+            const float f = reinterpret_cast<const float*>(stage + S::QC)[g + 8 * k];
+            const float2 off = reinterpret_cast<const float2*>(stage + S::STAT)[g + 8 * k];
 #pragma unroll
-                for (int h = 0; h < 2; h++) if (r0 + 8 * i + 4 * h + t <= lim) w[i][h] += ex2((__fmul_rn(s[i][h][n], f) - off.x) - off.y);
+            for (int q = 0; q < 4; q++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) if (r0 + 8 * q + 4 * h + t <= lim) w[q][h] += ex2((__fmul_rn(s[q][h][k], f) - off.x) - off.y);
         }
+        __syncthreads();
+        if (tid == 0 && i + KW_DEPTH < n) issue(i + KW_DEPTH);
+        if (++d == KW_DEPTH) { d = 0; phase ^= 1; }
     }
 #pragma unroll
     for (int i = 0; i < 4; i++)
@@ -518,6 +688,10 @@ __global__ void __launch_bounds__(128) kv4_weight_kernel(const KaParams p, float
                 else p.c.weight[at] = (decay == 0.0f ? 0.0f : decay * __ldcg(p.c.weight + at)) + x;
             }
         }
+    if (tid == 0 && *(volatile int*)&abort_flag) {
+        *p.err = IBCU_KV4_WAIT_ERR;
+        for (int i = 0; i < 1000; i++) __nanosleep(1000);
+    }
 }
 __global__ void __launch_bounds__(256) kv4_weight_join_kernel(const KaParams p, float decay, const float* __restrict__ parts, int n) {
     pdl_launch_dependents();
@@ -532,20 +706,26 @@ __global__ void __launch_bounds__(256) kv4_weight_join_kernel(const KaParams p, 
     p.c.weight[at] = (decay == 0.0f ? 0.0f : decay * __ldcg(p.c.weight + at)) + x;
 }
 
-template <int NG, bool LARGE>
-int launch_attention(ibcu_ctx* ctx, const KaParams& p, int units, int chunks, int rows, float decay, float* parts, int n_parts) {
-    static SmemOptIn opt;
-    if (int rc = ibcu_allow_smem(ctx, opt, kv4_attn_kernel<NG, LARGE>, KaSmem<NG, LARGE>::TOTAL)) return rc;
-    int rc = ibcu_launch(ctx, kv4_attn_kernel<NG, LARGE>, dim3(units, chunks), dim3(32 * KA_WARPS), KaSmem<NG, LARGE>::TOTAL, 1, true, p);
-    if (!rc && chunks > 1) rc = ibcu_launch(ctx, kv4_join_kernel, dim3(p.t.cols(), units), dim3(128), 128 * sizeof(float4), 1, true, p);
+// what a call launches
+struct KaCall { int mode, blocks, chunks, rows, n_parts; float decay; float* parts; };
+
+template <int NG, int MODE>
+int launch_attention(ibcu_ctx* ctx, const KaParams& p, const KaCall& k) {
+    static SmemOptIn opt, opt_w;
+    const size_t smem = KaSmem<NG, MODE>::TOTAL + (MODE == FEW && p.w.rotate ? (size_t)p.t.B * 16 * NG * sizeof(double2) : 0);
+    if (int rc = ibcu_allow_smem(ctx, opt, kv4_attn_kernel<NG, MODE>, smem)) return rc;
+    int rc = ibcu_launch(ctx, kv4_attn_kernel<NG, MODE>, dim3(k.blocks, k.chunks), dim3(32 * KA_WARPS), smem, 1, true, p);
+    if (!rc && k.chunks > 1 && !p.arrived) rc = ibcu_launch(ctx, kv4_join_kernel, dim3(std::min(p.t.cols(), p.t.B * p.t.group), p.c.n_kv * p.t.ntiles), dim3(128), 0, 1, true, p);
     if (rc || !p.stat) return rc;
-    rc = ibcu_launch(ctx, kv4_weight_kernel<NG, LARGE>, dim3((rows + 127) / 128, p.c.n_kv, n_parts), dim3(128), 0, 1, true, p, decay, n_parts > 1 ? parts : (float*)nullptr);
-    if (!rc && n_parts > 1) rc = ibcu_launch(ctx, kv4_weight_join_kernel, dim3((rows + 255) / 256, p.c.n_kv), dim3(256), 0, 1, true, p, decay, (const float*)parts, n_parts);
+    constexpr bool LARGE = MODE != FEW;
+    if ((rc = ibcu_allow_smem(ctx, opt_w, kv4_weight_kernel<NG, LARGE>, KwSmem<NG, LARGE>::TOTAL))) return rc;
+    rc = ibcu_launch(ctx, kv4_weight_kernel<NG, LARGE>, dim3((k.rows + 127) / 128, p.c.n_kv, k.n_parts), dim3(32 * KA_WARPS), KwSmem<NG, LARGE>::TOTAL, 1, true, p, k.decay, k.n_parts > 1 ? k.parts : (float*)nullptr);
+    if (!rc && k.n_parts > 1) rc = ibcu_launch(ctx, kv4_weight_join_kernel, dim3((k.rows + 255) / 256, p.c.n_kv), dim3(256), 0, 1, true, p, k.decay, (const float*)k.parts, k.n_parts);
     return rc;
 }
 template <int NG>
-int launch_attention(ibcu_ctx* ctx, const KaParams& p, int units, int chunks, int rows, float decay, float* parts, int n_parts) {
-    return p.t.large ? launch_attention<NG, true>(ctx, p, units, chunks, rows, decay, parts, n_parts) : launch_attention<NG, false>(ctx, p, units, chunks, rows, decay, parts, n_parts);
+int launch_attention(ibcu_ctx* ctx, const KaParams& p, const KaCall& k) {
+    return k.mode == FEW ? launch_attention<NG, FEW>(ctx, p, k) : k.mode == MANY ? launch_attention<NG, MANY>(ctx, p, k) : launch_attention<NG, WIDE>(ctx, p, k);
 }
 
 }  // namespace
@@ -556,34 +736,50 @@ int kv4_attend(ibcu_ctx* ctx, const Kv4& c, float decay, const Kv4Place& at, con
     const int large = columns > 8, ntiles = (int)((columns + (large ? 15 : 7)) / (large ? 16 : 8)), units = c.n_kv * ntiles;
     const int rows = at.at ? c.max_rows : at.row0 + B;
     const Kv4Columns t = { n_heads, group, B, large, ntiles };
-    int want = std::max(1, (large ? 2 : 3) * ctx->sm_count / units), chunk, chunks;
-    ka_plan(rows, want, chunk, chunks);
-    if (at.at) chunks = std::min(want, (rows + KA_ROWS - 1) / KA_ROWS);                            // shorter contexts have more, shorter chunks
+    KaCall call;
+    memset(&call, 0, sizeof call);
+    call.rows = rows; call.decay = decay;
+    // Four tiles a block once those fill the machine.
+    const int wide_blocks = c.n_kv * ((ntiles + KA_WARPS - 1) / KA_WARPS);
+    call.mode = !large ? FEW : wide_blocks >= ctx->sm_count ? WIDE : MANY;
+    call.blocks = call.mode == WIDE ? wide_blocks : units;
+    const int stages = (rows + KA_ROWS - 1) / KA_ROWS;
+    int want = call.mode == WIDE ? 1 : std::max(1, (large ? 2 : 3) * ctx->sm_count / units), chunk;
+    // The last block of a tile joins its chunks if a warp of it has at most 32 to read; a launch of its own is worth it beyond (one of several thousand
+    // rows with sixteen columns rather has fewer chunks).
+    const int a_warp = (int)(std::min(columns, (long)t.cols()) + 3) / 4;
+    if (large && want > 32 / a_warp && stages <= 128) want = 32 / a_warp;
+    ka_plan(rows, want, chunk, call.chunks);
+    if (at.at) call.chunks = std::min(want, stages);                                               // shorter contexts have more, shorter chunks
+    const bool by_last = call.chunks > 1 && call.chunks * a_warp <= 32;
     const int row_blocks = (rows + 127) / 128;
-    int n_parts = c.weight ? std::min(std::min(ntiles, 16), std::max(1, 6 * ctx->sm_count / (row_blocks * c.n_kv))) : 1;
+    call.n_parts = c.weight && ntiles >= 16 ? std::min(std::min(ntiles, 16), std::max(1, 6 * ctx->sm_count / (row_blocks * c.n_kv))) : 1;
     auto round_up = [](size_t n) { return (n + 255) & ~(size_t)255; };
-    const size_t b_qf = round_up(units * kv4_frag_uint2(ng, large) * sizeof(uint2)), b_qc = round_up((size_t)units * 16 * sizeof(float));
-    const size_t b_stat = c.weight ? round_up((size_t)units * 16 * sizeof(float2)) : 0, b_ml = chunks > 1 ? round_up((size_t)units * chunks * 16 * sizeof(float2)) : 0;
-    const size_t b_acc = chunks > 1 ? round_up((size_t)units * chunks * 16 * c.hd * sizeof(float)) : 0, b_parts = n_parts > 1 ? round_up((size_t)n_parts * c.n_kv * c.max_rows * sizeof(float)) : 0;
+    const bool frags = large || c.weight;
+    const size_t b_qf = frags ? round_up(units * kv4_frags(ng, large) * sizeof(uint4)) : 0, b_qc = frags ? round_up((size_t)units * 16 * sizeof(float)) : 0;
+    const size_t b_stat = c.weight ? round_up((size_t)units * 16 * sizeof(float2)) : 0, b_ml = call.chunks > 1 ? round_up((size_t)units * call.chunks * 16 * sizeof(float2)) : 0;
+    const size_t b_acc = call.chunks > 1 ? round_up((size_t)units * call.chunks * 16 * c.hd * sizeof(float)) : 0, b_parts = call.n_parts > 1 ? round_up((size_t)call.n_parts * c.n_kv * c.max_rows * sizeof(float)) : 0;
     if (int rc = ibcu_reserve(ctx, &ctx->scratch, &ctx->scratch_bytes, b_qf + b_qc + b_stat + b_ml + b_acc + b_parts)) return rc;
+    if (by_last) { if (int rc = ibcu_reserve_zeroed(ctx, &ctx->kv4_arrived, &ctx->kv4_arrived_bytes, (size_t)units * sizeof(int))) return rc; }
     char* s = (char*)ctx->scratch;
     auto take = [&](size_t n) { char* r = s; s += n; return r; };
     KaParams p;
     memset(&p, 0, sizeof p);
     p.c = c; p.t = t; p.at = at;
-    uint2* qf = (uint2*)take(b_qf); float* qc = (float*)take(b_qc);
-    p.qf = qf; p.qc = qc;
+    uint4* qf = (uint4*)take(b_qf); float* qc = (float*)take(b_qc);
+    p.w = Kv4Prep{ q, k, v, qf, qc, log2_theta, rotate };
     p.stat = (float2*)take(b_stat); if (!c.weight) p.stat = nullptr;
     p.pml = (float2*)take(b_ml); p.pacc = (float*)take(b_acc);
-    float* parts = (float*)take(b_parts);
-    p.out = out; p.want = want; p.grid_chunks = chunks; p.err = ctx->kern_err;
-    if (int rc = kv4_prepare(ctx, c, t, at, Kv4Prep{ q, k, v, qf, qc, log2_theta, rotate })) return rc;
+    call.parts = (float*)take(b_parts);
+    p.arrived = by_last ? (int*)ctx->kv4_arrived : nullptr;
+    p.out = out; p.want = want; p.grid_chunks = call.chunks; p.err = ctx->kern_err;
+    if (large) { if (int rc = kv4_prepare(ctx, c, t, at, p.w)) return rc; }
     switch (ng) {
-        case 1: return launch_attention<1>(ctx, p, units, chunks, rows, decay, parts, n_parts);
-        case 2: return launch_attention<2>(ctx, p, units, chunks, rows, decay, parts, n_parts);
-        case 3: return launch_attention<3>(ctx, p, units, chunks, rows, decay, parts, n_parts);
-        case 4: return launch_attention<4>(ctx, p, units, chunks, rows, decay, parts, n_parts);
-        case 6: return launch_attention<6>(ctx, p, units, chunks, rows, decay, parts, n_parts);
-        default: return launch_attention<8>(ctx, p, units, chunks, rows, decay, parts, n_parts);
+        case 1: return launch_attention<1>(ctx, p, call);
+        case 2: return launch_attention<2>(ctx, p, call);
+        case 3: return launch_attention<3>(ctx, p, call);
+        case 4: return launch_attention<4>(ctx, p, call);
+        case 6: return launch_attention<6>(ctx, p, call);
+        default: return launch_attention<8>(ctx, p, call);
     }
 }
