@@ -19,11 +19,11 @@ __device__ __forceinline__ float held(const uint8_t* row, int place, float s) { 
 __device__ __forceinline__ float scale_at(const Kv4& c, size_t i) { return __half2float(__ushort_as_half(__ldcg(reinterpret_cast<const unsigned short*>(c.scale) + i))); }
 
 // One launch ahead of the attention of more than eight columns, and that of ibcu_kv4_write: blocks below qblocks turn a tile of 16 columns into
-// fragments, the others write the rows of a position, whose heads share its angles.
+// fragments or their part of an image, the others write the rows of a position, whose heads share its angles.
 struct PrepParams { Kv4 c; Kv4Columns t; Kv4Place at; Kv4Prep w; int qblocks, wparts; int* err; };
 
 __global__ void __launch_bounds__(128) kv4_prep_kernel(const PrepParams p) {
-    extern __shared__ __align__(16) double2 turn[];           // [positions of the block][hd / 2]; then [8 columns a warp][hd] turned queries
+    extern __shared__ __align__(16) double2 turn[];           // [positions of the block][hd / 2]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hd = p.c.hd, half = hd / 2, ng = hd / 32;
     const bool queries = (int)blockIdx.x < p.qblocks;
     const int kvh = blockIdx.x / p.t.ntiles, c0 = blockIdx.x % p.t.ntiles * 16, wb = blockIdx.x - p.qblocks;
@@ -38,37 +38,72 @@ __global__ void __launch_bounds__(128) kv4_prep_kernel(const PrepParams p) {
     pdl_launch_dependents();                                  // not earlier: the attention reads rows of earlier calls ahead of its own wait
     __syncthreads();
     if (queries) {
-        if (warp >= 2) return;
-        // a warp prepares eight columns, lane = column * 4 + t: values 8t..8t+7 of every group
-        const int g = lane >> 2, t = lane & 3, col = c0 + warp * 8 + g, b = col / p.t.group;
-        float* qr = reinterpret_cast<float*>(turn + (p.w.rotate ? (size_t)min(16, 15 / p.t.group + 2) * half : 0)) + ((size_t)warp * 8 + g) * hd + 8 * t;
-        const bool on = b < p.t.B;
-        const float* src = p.w.q + ((size_t)b * p.t.n_heads + (size_t)kvh * p.t.group + col % p.t.group) * hd + 8 * t;
-        const double2* angles = on && p.w.rotate ? turn + (b - b0) * half + 4 * t : nullptr;
-        uint32_t m = 0;
-        for (int j = 0; j < ng; j++) {
-            float x[8];
-            kv4_query(x, src + 32 * j, on, angles ? angles + 16 * j : nullptr);
+        // lane = column g and column g + 8, piece t: values 8t..8t+7 of every group; a warp has every fourth group
+        __shared__ uint32_t amax[4][16];
+        const int g = lane >> 2, t = lane & 3;
+        float x[2][2][8];
+        uint32_t m[2] = { 0, 0 };
 #pragma unroll
-            for (int i = 0; i < 8; i++) { m = max(m, __float_as_uint(x[i]) & 0x7FFFFFFFu); qr[32 * j + i] = x[i]; }
+        for (int n = 0; n < 2; n++) {
+            const int col = c0 + g + 8 * n, b = col / p.t.group;
+            const bool on = b < p.t.B;
+            const float* src = p.w.q + ((size_t)b * p.t.n_heads + (size_t)kvh * p.t.group + col % p.t.group) * hd + 8 * t;
+            const double2* angles = on && p.w.rotate ? turn + (b - b0) * half + 4 * t : nullptr;
+#pragma unroll
+            for (int jj = 0; jj < 2; jj++) {
+                const int j = warp + 4 * jj;
+                if (j >= ng) break;
+                kv4_query(x[n][jj], src + 32 * j, on, angles ? angles + 16 * j : nullptr);
+#pragma unroll
+                for (int i = 0; i < 8; i++) m[n] = max(m[n], __float_as_uint(x[n][jj][i]) & 0x7FFFFFFFu);
+            }
+            m[n] = max(m[n], __shfl_xor_sync(0xffffffffu, m[n], 1));
+            m[n] = max(m[n], __shfl_xor_sync(0xffffffffu, m[n], 2));
+            if (t == 0) amax[warp][g + 8 * n] = m[n];
         }
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        const Kv4Up up = kv4_up(m, hd);
-        if (t == 0) p.w.qc[(size_t)blockIdx.x * 16 + warp * 8 + g] = up.back;
-        uint32_t* qf = reinterpret_cast<uint32_t*>(p.w.qf + blockIdx.x * kv4_frags(ng, true)) + lane * 4 + warp;
-        for (int j = 0; j < ng; j++) {
-            float x[8];
+        __syncthreads();
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = qr[32 * j + i] * up.a * up.b;
+        for (int n = 0; n < 2; n++) {
 #pragma unroll
-            for (int s = 0; s < 2; s++) {
-                uint32_t hi[2], lo[2];
-                kv4_pieces(x, s, hi, lo);
-                uint32_t* to = qf + (j * 2 + s) * 128;
-                to[0] = hi[0]; to[2] = hi[1];
-                to += ng * 256;
-                to[0] = lo[0]; to[2] = lo[1];
+            for (int w = 0; w < 4; w++) m[n] = max(m[n], amax[w][g + 8 * n]);
+            const Kv4Up up = kv4_up(m[n], hd);
+            if (warp == 0 && t == 0) p.w.qc[(size_t)blockIdx.x * 16 + g + 8 * n] = up.back;
+#pragma unroll
+            for (int jj = 0; jj < 2; jj++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[n][jj][i] = x[n][jj][i] * up.a * up.b;
+        }
+#pragma unroll
+        for (int jj = 0; jj < 2; jj++) {
+            const int j = warp + 4 * jj;
+            if (j >= ng) break;
+            if (p.t.large == 2) {
+                const int piece = t * ng + j;
+                unsigned char* image = reinterpret_cast<unsigned char*>(p.w.qf) + (size_t)(blockIdx.x / 8) * (ng * 16384) + (piece >> 3) * 16384;
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    const int col = blockIdx.x % 8 * 16 + g + 8 * n;
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const __half2 h = __floats2half2_rn(x[n][jj][i], x[n][jj][i + 4]), l = __floats2half2_rn(x[n][jj][i] - __low2float(h), x[n][jj][i + 4] - __high2float(h));
+                        hi[i] = *reinterpret_cast<const uint32_t*>(&h);
+                        lo[i] = *reinterpret_cast<const uint32_t*>(&l);
+                    }
+                    unsigned char* at = image + col * 128 + (((piece & 7) ^ (col & 7)) << 4);
+                    *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    *reinterpret_cast<uint4*>(at + ng / 2 * 16384) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                }
+            } else {
+                uint4* qf = p.w.qf + blockIdx.x * kv4_frags(ng, true) + lane;
+#pragma unroll
+                for (int s = 0; s < 2; s++) {
+                    uint32_t hi[2][2], lo[2][2];
+#pragma unroll
+                    for (int n = 0; n < 2; n++) kv4_pieces(x[n][jj], s, hi[n], lo[n]);
+                    qf[(j * 2 + s) * 32] = make_uint4(hi[0][0], hi[1][0], hi[0][1], hi[1][1]);
+                    qf[((ng + j) * 2 + s) * 32] = make_uint4(lo[0][0], lo[1][0], lo[0][1], lo[1][1]);
+                }
             }
         }
         return;
@@ -293,7 +328,7 @@ double log2_of(float theta) { return theta > 0.0f ? log2((double)theta) : 0.0; }
 int kv4_prepare(ibcu_ctx* ctx, const Kv4& c, const Kv4Columns& t, const Kv4Place& at, const Kv4Prep& w) {
     PrepParams p = { c, t, at, w, w.q ? c.n_kv * t.ntiles : 0, t.B <= 8 ? c.n_kv : 1, ctx->kern_err };
     const int nb = w.q ? std::min(16, 15 / t.group + 2) : 1;  // positions that a block may have to do with
-    const size_t smem = (w.rotate ? (size_t)nb * c.hd / 2 * sizeof(double2) : 0) + (w.q ? (size_t)16 * c.hd * sizeof(float) : 0);
+    const size_t smem = w.rotate ? (size_t)nb * c.hd / 2 * sizeof(double2) : 0;
     return ibcu_launch(ctx, kv4_prep_kernel, dim3(p.qblocks + (w.k ? t.B * p.wparts : 0)), dim3(128), smem, 1, true, p);
 }
 

@@ -14,8 +14,11 @@ struct Kv4 {
 // value: [unit = KV head * tiles + tile][part][group of 32][step][lane] uint4. Tiles of 16 have two parts, high and low pieces, with columns 0-7 in the
 // fragments' even registers and 8-15 in the odd ones; a tile of 8 has one, with high and low pieces there. Beside them
 // qc [unit][16]: the factor that turns a column's sums into exponents of 2.
+// Prompts (kv4_prompt.cu) go in tiles of 128 columns, eight of 16 side by side, as operand images instead: [KV head * tiles + tile][part][64 values][column]
+// rows of 128 bytes in the 128-byte swizzle, a row's 16-byte pieces in the order of a key row's words (piece t * (hd / 32) + j: values 32 j + 8 t..), the eight values of a
+// piece as 0, 4, 1, 5, 2, 6, 3, 7.
 struct Kv4Columns {
-    int n_heads, group, B, large, ntiles;
+    int n_heads, group, B, large, ntiles;                      // large: tiles of 16; 2: as images, ntiles a multiple of 8
     __host__ __device__ int cols() const { return large ? 16 : 8; }
 };
 __host__ __device__ constexpr size_t kv4_frags(int ng, bool large) { return (size_t)(large ? 2 : 1) * ng * 64; }     // uint4s of a unit
@@ -56,7 +59,7 @@ __device__ __forceinline__ void kv4_turn(float& x0, float& x1, const double2 cs)
 __device__ __forceinline__ __half kv4_scale(uint32_t amax_bits, float& inv) {
     if (amax_bits >= 0x7F800000u) { inv = 0.0f; return __ushort_as_half(0x7FFF); }          // NaN: the row says so wherever it is seen
     const float s = __fmul_rn(__uint_as_float(amax_bits), 1.0f / 7.0f);
-    const __half h = __float2half_rn(fminf(s, 65504.0f));
+    const __half h = __float2half_rn(fminf(s, 8192.0f));                                    // seven of them, the largest value, are an fp16 too
     inv = __half2float(h) > 0.0f ? __fdiv_rn(1.0f, __half2float(h)) : 0.0f;
     return h;
 }
@@ -120,5 +123,8 @@ __device__ __forceinline__ void kv4_pieces(const float (&x)[8], int s, uint32_t 
 // Prepares a call's queries (q != NULL) and writes its rows (k != NULL), one launch. Defined in kv4.cu.
 struct Kv4Prep { const float *q, *k, *v; uint4* qf; float* qc; double log2_theta; int rotate; };
 int kv4_prepare(ibcu_ctx* ctx, const Kv4& c, const Kv4Columns& t, const Kv4Place& at, const Kv4Prep& w);
+// A prompt's attention over images that are prepared: kv4_prompt.cu, for head_dim 64 and 128. stat, parts: for the weights, or NULL.
+int kv4_prompt_parts(ibcu_ctx* ctx, const Kv4& c, int tiles, int rows);
+int kv4_prompt(ibcu_ctx* ctx, const Kv4& c, const Kv4Columns& t, const Kv4Place& at, const unsigned char* image, const float* qc, float* out, float2* stat, int rows, float* parts, int n_parts);
 // The attention of a call, with what it has to prepare. q, k, v as above (k NULL: the rows are there). Defined in kv4_attn.cu.
 int kv4_attend(ibcu_ctx* ctx, const Kv4& c, float decay, const Kv4Place& at, const float* q, const float* k, const float* v, float* out, int n_heads, int B, double log2_theta, int rotate);

@@ -739,6 +739,23 @@ int kv4_attend(ibcu_ctx* ctx, const Kv4& c, float decay, const Kv4Place& at, con
     KaCall call;
     memset(&call, 0, sizeof call);
     call.rows = rows; call.decay = decay;
+    if ((c.hd == 64 || c.hd == 128) && large && c.n_kv * (columns / 128) >= ctx->sm_count / 4) {          // a prompt
+        Kv4Columns tp = t;
+        tp.ntiles = (int)((columns + 127) / 128) * 8;
+        tp.large = 2;
+        const size_t tiles = (size_t)c.n_kv * tp.ntiles / 8, b_image = tiles * ng * 16384, b_qc = tiles * 512, b_stat = c.weight ? tiles * 1024 : 0;
+        const int n_parts = c.weight ? kv4_prompt_parts(ctx, c, tp.ntiles / 8, rows) : 0;
+        if (int rc = ibcu_reserve(ctx, &ctx->scratch, &ctx->scratch_bytes, b_image + b_qc + b_stat + (size_t)n_parts * c.n_kv * c.max_rows * sizeof(float))) return rc;
+        char* s = (char*)ctx->scratch;
+        float* qc = (float*)(s + b_image); float2* stat = c.weight ? (float2*)(s + b_image + b_qc) : nullptr; float* parts = (float*)(s + b_image + b_qc + b_stat);
+        if (int rc = kv4_prepare(ctx, c, tp, at, Kv4Prep{ q, k, v, (uint4*)s, qc, log2_theta, rotate })) return rc;
+        if (int rc = kv4_prompt(ctx, c, tp, at, (const unsigned char*)s, qc, out, stat, rows, parts, n_parts)) return rc;
+        if (!c.weight) return IBCU_OK;
+        KaParams p;
+        memset(&p, 0, sizeof p);
+        p.c = c; p.t = tp; p.at = at; p.err = ctx->kern_err;
+        return ibcu_launch(ctx, kv4_weight_join_kernel, dim3((rows + 255) / 256, c.n_kv), dim3(256), 0, 1, true, p, decay, (const float*)parts, n_parts);
+    }
     // Four tiles a block once those fill the machine.
     const int wide_blocks = c.n_kv * ((ntiles + KA_WARPS - 1) / KA_WARPS);
     call.mode = !large ? FEW : wide_blocks >= ctx->sm_count ? WIDE : MANY;

@@ -1,0 +1,529 @@
+// Attention over the 4-bit KV cache for prompts, on tcgen05 (kind::f16, FP32 accumulators in tensor memory), keeping FP32's accuracy.
+//
+// A block has 128 columns of a KV head (a column is a query head at a position) and walks the rows, 64 at a time:
+//     S [128 columns x 64 rows] = Q K'^T,   P = 2^(S f - m + 14),   O [128 columns x values] += P V'
+// K' = ks (n - 8) and V' = vs (n - 8) are held values, an 11-bit scale times a 4-bit code: 15 bits, which two fp16 pieces hold exactly. Q and P are
+// two pieces of 11 bits. Each product is three instructions a step, high.high + low.high + high.low; low.low is 2^-23 of the result.
+// (On mma.sync the scales stay FP32 factors outside the products, two instructions a step, but their rate is a third; 16
+// columns share an unpacked row there, 128 here. A prompt of 2048, 32 heads of 128 over 8: 370 us that way.)
+//
+// Warps: 4 softmax, a thread a column; 4 that turn key codes into the pieces of K', 4 for V' (transposed: the rows are the
+// contraction); 1 issues the products, 1 the copies. Everything is double buffered, and S of the next rows is computed while the softmax is at these.
+// A V' of a row with a NaN scale would reach columns that do not see the row (0 * NaN), so NaN goes into the row's K' instead, and with it
+// into every column that does see it.
+#include "kv4.cuh"
+#include "tc_common.cuh"
+#include <algorithm>
+
+namespace {
+
+constexpr int PK_ROWS = 64, PK_COLS = 128, PK_RAW = 3;
+constexpr int PK_KEY_WARP = 4, PK_VALUE_WARP = 8, PK_MMA_WARP = 12, PK_TMA_WARP = 13, PK_THREADS = 14 * 32;
+constexpr float PK_LOW = -3.0e38f, PK_SLACK = 1.9f;            // see kv4_attn.cu
+
+struct PkParams {
+    Kv4 c; Kv4Columns t; Kv4Place at;
+    const unsigned char* image; const float* qc;
+    float* out; float2* stat;
+    int tiles;                                                 // of 128 columns, a KV head
+    int* err;
+};
+template <int NG> struct PkSmem {
+    static constexpr int KB = NG / 2, HD = 32 * NG;            // KB: blocks of 64 values, a swizzled row of 128 bytes each
+    static constexpr int IMAGE = 2 * KB * 16384, KEYS = 2 * KB * 8192, VALUES = 2 * HD * 128, RAW_BYTES = PK_ROWS * 36 * NG;
+    static constexpr int Q = 0, K = Q + IMAGE, V = K + 2 * KEYS, RAW = V + 2 * VALUES, TOTAL = RAW + PK_RAW * RAW_BYTES;
+};
+struct PkShared {
+    unsigned long long q_full, raw_full[PK_RAW], raw_empty[PK_RAW], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], s_empty[2], p_full[2], pv_done[2], drained;
+    uint32_t tmem_base;
+    int abort_flag;
+};
+
+__device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 :: "r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+__device__ __forceinline__ __half2 half2_of(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
+
+// The eight codes of a word less their bias of 8, as pairs 0 and 4, 1 and 5, 2 and 6, 3 and 7: under the exponent of 1024 a code n is the fp16 1024 + n
+__device__ __forceinline__ void codes_of(uint32_t w, __half2 (&f)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) f[i] = __hsub2(half2_of((w >> (4 * i) & 0x000F000Fu) | 0x64006400u), half2_of(0x64086408u));
+}
+// codes times scales as two pieces, exact together
+__device__ __forceinline__ void held_pieces(const __half2 f, const __half2 scale, uint32_t& high, uint32_t& low) {
+    const __half2 h = __hmul2(f, scale);
+    high = bits(h);
+    low = bits(__hfma2(f, scale, __hneg2(h)));
+}
+__device__ __forceinline__ bool is_nan(uint32_t half_bits) { return (half_bits & 0x7FFFu) > 0x7C00u; }
+
+// Piece t of a key row (the values 8t..8t+7 of every group) into the operand image: rows of 128 bytes, 16-byte pieces swizzled, blocks of 64 values
+// `block` bytes apart, the low pieces `part` bytes behind the high ones. scales: the row's, keys' and values'.
+template <int NG>
+__device__ __forceinline__ void place_key(unsigned char* to, int block, int part, int r, int t, const uint32_t (&w)[NG], const uint32_t (&scales)[NG]) {
+    bool bad = false;
+#pragma unroll
+    for (int j = NG / 2; j < NG; j++) bad = bad || is_nan(scales[j]) || is_nan(scales[j] >> 16);
+#pragma unroll
+    for (int j = 0; j < NG; j++) {
+        const uint32_t s = bad ? 0x7FFFu : (j & 1 ? scales[j / 2] >> 16 : scales[j / 2] & 0xFFFFu);
+        const __half2 s2 = half2_of(s | s << 16);
+        __half2 f[4];
+        codes_of(w[j], f);
+        uint4 high, low;
+        held_pieces(f[0], s2, high.x, low.x); held_pieces(f[1], s2, high.y, low.y); held_pieces(f[2], s2, high.z, low.z); held_pieces(f[3], s2, high.w, low.w);
+        const int piece = t * NG + j;
+        unsigned char* at = to + (piece >> 3) * block + r * 128 + (((piece & 7) ^ (r & 7)) << 4);
+        *reinterpret_cast<uint4*>(at) = high;
+        *reinterpret_cast<uint4*>(at + part) = low;
+    }
+}
+template <int N> __device__ __forceinline__ void load_words(uint32_t (&d)[N], const unsigned char* s) {
+    if constexpr (N == 4) { const uint4 v = *reinterpret_cast<const uint4*>(s); d[0] = v.x; d[1] = v.y; d[2] = v.z; d[3] = v.w; }
+    else { const uint2 v = *reinterpret_cast<const uint2*>(s); d[0] = v.x; d[1] = v.y; }
+}
+
+template <int NG>
+__global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParams p) {
+    using S = PkSmem<NG>;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    PkShared* sh = reinterpret_cast<PkShared*>(smem + S::TOTAL);
+    volatile int* abort_flag = &sh->abort_flag;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int kvh = blockIdx.x % p.c.n_kv, tile = p.tiles - 1 - blockIdx.x / p.c.n_kv, unit = kvh * p.tiles + tile, c0 = tile * PK_COLS;          // most rows first
+    if (tid == 0) {
+        auto init = [&](unsigned long long& b, int n) { mbar_init(smem_u32(&b), n); };
+        init(sh->q_full, 1); init(sh->drained, 1);
+        for (int i = 0; i < PK_RAW; i++) { init(sh->raw_full[i], 1); init(sh->raw_empty[i], 8); }
+        for (int i = 0; i < 2; i++) {
+            init(sh->k_full[i], 4); init(sh->k_empty[i], 1); init(sh->v_full[i], 4); init(sh->v_empty[i], 1);
+            init(sh->s_full[i], 1); init(sh->s_empty[i], 4); init(sh->p_full[i], 4); init(sh->pv_done[i], 1);
+        }
+        sh->abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    if (warp == PK_MMA_WARP) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&sh->tmem_base)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        pdl_launch_dependents();                               // not before this block holds its tensor memory: see linear_tc.cu
+    }
+    pdl_wait();
+    int row0, pos0;
+    const bool there = kv4_place(p.at, p.t.B, p.c.max_rows, p.err, row0, pos0);
+    const int rows = there ? row0 + min(p.t.B - 1, (c0 + PK_COLS - 1) / p.t.group) + 1 : 0, n = (rows + PK_ROWS - 1) / PK_ROWS;
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem_o = sh->tmem_base, tmem_s = tmem_o + S::HD, tmem_p = tmem_s + 2 * PK_ROWS;          // 128 + 2 x 64 + 2 x 64 columns
+
+    if (warp == PK_TMA_WARP) {
+        if (elect_one() && n) {
+            asm volatile("fence.proxy.async.global;" ::: "memory");
+            mbar_expect_tx(smem_u32(&sh->q_full), S::IMAGE);
+            for (int e = 0; e < S::IMAGE; e += 16384) bulk_load(smem_u32(smem + S::Q + e), p.image + (size_t)unit * S::IMAGE + e, 16384, smem_u32(&sh->q_full));
+            const size_t plane = p.c.row(kvh, 0);
+            int s = 0; uint32_t ph = 1;
+            for (int i = 0; i < n; i++) {
+                if (!mbar_wait(smem_u32(&sh->raw_empty[s]), ph, abort_flag, 1)) break;
+                const int r = i * PK_ROWS, have = min(PK_ROWS, (rows - r + 7) & ~7);            // whole groups of 8 rows, which the planes have
+                const uint32_t bar = smem_u32(&sh->raw_full[s]), to = smem_u32(smem + S::RAW + s * S::RAW_BYTES);
+                mbar_expect_tx(bar, (uint32_t)have * 36 * NG);
+                bulk_load(to, p.c.k + (plane + r) * (16 * NG), (uint32_t)have * 16 * NG, bar);
+                bulk_load(to + PK_ROWS * 16 * NG, p.c.v + (plane + r) * (16 * NG), (uint32_t)have * 16 * NG, bar);
+                bulk_load(to + PK_ROWS * 32 * NG, p.c.scale + (plane + r) * (2 * NG), (uint32_t)have * 4 * NG, bar);
+                if (++s == PK_RAW) { s = 0; ph ^= 1; }
+            }
+        }
+        __syncwarp();
+    } else if (warp == PK_MMA_WARP) {
+        if (elect_one() && n) {
+            constexpr uint32_t idesc = (1u << 4) | (8u << 24);                                    // FP32 accumulators, fp16 operands, 128 rows
+            constexpr uint32_t idesc_s = idesc | ((PK_ROWS / 8) << 17), idesc_o = idesc | ((S::HD / 8) << 17);
+            bool ok = mbar_wait(smem_u32(&sh->q_full), 0u, abort_flag, 2);
+            const uint64_t q = smem_desc_sw128(smem_u32(smem + S::Q));
+            auto scores = [&](int i) {
+                const int b = i & 1;
+                const uint32_t ph = (uint32_t)(i >> 1) & 1u;
+                if (!mbar_wait(smem_u32(&sh->k_full[b]), ph, abort_flag, 3) || !mbar_wait(smem_u32(&sh->s_empty[b]), ph ^ 1u, abort_flag, 4)) return false;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint64_t k = smem_desc_sw128(smem_u32(smem + S::K + b * S::KEYS));
+#pragma unroll
+                for (int m = 0; m < 3; m++)                                                       // high.high, low.high, high.low
+#pragma unroll
+                    for (int st = 0; st < S::HD / 16; st++)
+                        mma_f16_ss(tmem_s + b * PK_ROWS, q + (((m == 1) * S::KB + st / 4) * 16384 >> 4) + st % 4 * 2, k + (((m == 2) * S::KB + st / 4) * 8192 >> 4) + st % 4 * 2, idesc_s,
+                                   m || st ? 1u : 0u);
+                mma_commit(smem_u32(&sh->k_empty[b]));
+                mma_commit(smem_u32(&sh->s_full[b]));
+                return true;
+            };
+            ok = ok && scores(0);
+            for (int i = 0; i < n && ok; i++) {
+                if (i + 1 < n) ok = scores(i + 1);
+                const int b = i & 1;
+                const uint32_t ph = (uint32_t)(i >> 1) & 1u;
+                ok = ok && mbar_wait(smem_u32(&sh->v_full[b]), ph, abort_flag, 5) && mbar_wait(smem_u32(&sh->p_full[b]), ph, abort_flag, 6);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint64_t v = smem_desc_sw128(smem_u32(smem + S::V + b * S::VALUES));
+#pragma unroll
+                for (int m = 0; m < 3; m++)
+#pragma unroll
+                    for (int st = 0; st < PK_ROWS / 16; st++)
+                        mma_f16_ts(tmem_o, tmem_p + b * PK_ROWS + (m == 1) * (PK_ROWS / 2) + st * 8, v + ((m == 2) * S::HD * 128 >> 4) + st * 2, idesc_o, i || m || st ? 1u : 0u);
+                mma_commit(smem_u32(&sh->v_empty[b]));
+                mma_commit(smem_u32(&sh->pv_done[b]));
+            }
+            mma_commit(smem_u32(&sh->drained));
+            mbar_wait(smem_u32(&sh->drained), 0u, abort_flag, 7);
+        }
+        __syncwarp();
+    } else if (warp >= PK_KEY_WARP) {
+        const bool keys = warp < PK_VALUE_WARP;
+        const int w = warp & 3;
+        int s = 0; uint32_t ph = 0;
+        for (int i = 0; i < n; i++) {
+            const int b = i & 1;
+            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->raw_full[s]), ph, abort_flag, 8) &&
+                                         mbar_wait(smem_u32(keys ? &sh->k_empty[b] : &sh->v_empty[b]), (uint32_t)((i >> 1) & 1) ^ 1u, abort_flag, 9))) break;
+            const unsigned char* raw = smem + S::RAW + s * S::RAW_BYTES;
+            const unsigned char* scales = raw + PK_ROWS * 32 * NG;
+            if (keys) {
+                // lanes: eight rows by the four pieces; the swizzle spreads the rows' pieces over the banks
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const int r = 8 * (w + 4 * u) + (lane & 7), t = lane >> 3;
+                    uint32_t k[NG], sc[NG];
+                    load_words<NG>(k, raw + r * 16 * NG + t * 4 * NG);
+                    load_words<NG>(sc, scales + r * 4 * NG);
+                    place_key<NG>(smem + S::K + b * S::KEYS, 8192, S::KB * 8192, r, t, k, sc);
+                }
+            } else {
+                // lanes: four pairs of rows by the eight pieces of a row; transposed, value 32 j + 4 g + i is line (4 j + i) 8 + g of 64 rows
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const int chunk = w + 4 * u, g = lane >> 2, a = 8 * chunk + 2 * (lane & 3);
+                    uint32_t va[NG / 2], vb[NG / 2], sa[NG], sb[NG];
+                    if constexpr (NG == 4) {
+                        load_words<2>(va, raw + PK_ROWS * 16 * NG + a * 16 * NG + g * 2 * NG);
+                        load_words<2>(vb, raw + PK_ROWS * 16 * NG + (a + 1) * 16 * NG + g * 2 * NG);
+                    } else {
+                        va[0] = *reinterpret_cast<const uint32_t*>(raw + PK_ROWS * 16 * NG + a * 16 * NG + g * 2 * NG);
+                        vb[0] = *reinterpret_cast<const uint32_t*>(raw + PK_ROWS * 16 * NG + (a + 1) * 16 * NG + g * 2 * NG);
+                    }
+                    load_words<NG>(sa, scales + a * 4 * NG);
+                    load_words<NG>(sb, scales + (a + 1) * 4 * NG);
+                    const bool in_a = i * PK_ROWS + a < rows, in_b = i * PK_ROWS + a + 1 < rows;
+#pragma unroll
+                    for (int j = 0; j < NG; j++) {
+                        uint32_t ha = j & 1 ? sa[(NG + j) / 2] >> 16 : sa[(NG + j) / 2] & 0xFFFFu, hb = j & 1 ? sb[(NG + j) / 2] >> 16 : sb[(NG + j) / 2] & 0xFFFFu;
+                        if (!in_a || is_nan(ha)) ha = 0;
+                        if (!in_b || is_nan(hb)) hb = 0;
+                        const __half2 s2 = half2_of(ha | hb << 16);
+                        __half2 f[4];
+                        codes_of(__byte_perm(va[j / 2], vb[j / 2], j & 1 ? 0x7632 : 0x5410), f);
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            uint32_t high, low;
+                            held_pieces(f[q], s2, high, low);
+                            unsigned char* at = smem + S::V + b * S::VALUES + ((4 * j + q) * 8 + g) * 128 + ((chunk ^ g) << 4) + (lane & 3) * 4;
+                            *reinterpret_cast<uint32_t*>(at) = high;
+                            *reinterpret_cast<uint32_t*>(at + S::HD * 128) = low;
+                        }
+                    }
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");                        // the tensor cores read these stores
+            __syncwarp();
+            if (lane == 0) { mbar_arrive(smem_u32(keys ? &sh->k_full[b] : &sh->v_full[b])); mbar_arrive(smem_u32(&sh->raw_empty[s])); }
+            if (++s == PK_RAW) { s = 0; ph ^= 1; }
+        }
+    } else {
+        const int c = c0 + tid, b_col = c / p.t.group;
+        const bool on = b_col < p.t.B;
+        const int lim = row0 + b_col, lim0 = row0 + (c0 + (tid & ~31)) / p.t.group;              // last rows that this column, the warp's first column, see
+        const float f = on ? __ldcg(p.qc + (size_t)unit * PK_COLS + tid) : 0.0f;
+        const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+        float m = PK_LOW, l = 0.0f;
+        bool wide = false, alive = true;
+        for (int i = 0; i < n; i++) {
+            const int b = i & 1;
+            const uint32_t ph = (uint32_t)(i >> 1) & 1u;
+            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->s_full[b]), ph, abort_flag, 10))) { alive = false; break; }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            uint32_t s[64];
+            tmem_ld32(tmem_s + lanes + b * PK_ROWS, s);
+            tmem_ld32(tmem_s + lanes + b * PK_ROWS + 32, s + 32);
+            tmem_wait_ld(s);
+            tmem_wait_ld(s + 32);
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sh->s_empty[b]));
+            if (i * PK_ROWS + PK_ROWS - 1 > lim0) {
+#pragma unroll
+                for (int u = 0; u < 64; u++) if (i * PK_ROWS + u > lim) s[u] = 0xFF800000u;
+            }
+            float t4[4] = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };
+#pragma unroll
+            for (int u = 0; u < 64; u++) t4[u & 3] = fmaxf(t4[u & 3], __uint_as_float(s[u]));
+            const float top = fmaxf(PK_LOW, fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * f);
+            if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->pv_done[b]), ph ^ 1u, abort_flag, 11))) { alive = false; break; }          // this half of P is free
+            if (__any_sync(0xffffffffu, top > m + PK_SLACK)) {
+                const float now = fmaxf(m, top), corr = ex2(m - now);
+                m = now;
+                l *= corr;
+                wide = fabsf(now) > 524288.0f;
+                if (i) {
+                    if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->pv_done[b ^ 1]), (uint32_t)((i - 1) >> 1) & 1u, abort_flag, 12))) { alive = false; break; }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+                    for (int d = 0; d < S::HD; d += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(tmem_o + lanes + d, o);
+                        tmem_wait_ld(o);
+#pragma unroll
+                        for (int u = 0; u < 32; u++) o[u] = __float_as_uint(__uint_as_float(o[u]) * corr);
+                        tmem_st32(tmem_o + lanes + d, o);
+                    }
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                }
+            }
+            const float off = 14.0f - m;
+            if (__any_sync(0xffffffffu, wide)) {               // beyond 2^19 a fused product would show the maximum's own rounding
+#pragma unroll
+                for (int u = 0; u < 64; u++) s[u] = __float_as_uint(ex2((__fmul_rn(__uint_as_float(s[u]), f) - m) + 14.0f));
+            } else {
+#pragma unroll
+                for (int u = 0; u < 64; u++) s[u] = __float_as_uint(ex2(fmaf(__uint_as_float(s[u]), f, off)));
+            }
+            float l4[4] = { 0.f, 0.f, 0.f, 0.f };
+#pragma unroll
+            for (int u = 0; u < 64; u++) l4[u & 3] += __uint_as_float(s[u]);
+            l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {                      // 32 rows: 16 columns of tensor memory a piece
+                uint32_t high[16], low[16];
+#pragma unroll
+                for (int u = 0; u < 16; u++) {
+                    const float a = __uint_as_float(s[32 * h + 2 * u]), z = __uint_as_float(s[32 * h + 2 * u + 1]);
+                    const __half2 x = __floats2half2_rn(a, z);
+                    const float2 back = __half22float2(x);
+                    high[u] = bits(x);
+                    low[u] = bits(__floats2half2_rn(a - back.x, z - back.y));
+                }
+                tmem_st16(tmem_p + lanes + b * PK_ROWS + 16 * h, high);
+                tmem_st16(tmem_p + lanes + b * PK_ROWS + PK_ROWS / 2 + 16 * h, low);
+            }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sh->p_full[b]));
+        }
+        if (n && alive && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->pv_done[(n - 1) & 1]), (uint32_t)((n - 1) >> 1) & 1u, abort_flag, 13))) {
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const float inv = 1.0f / l;
+            float* to = p.out + ((size_t)b_col * p.t.n_heads + (size_t)kvh * p.t.group + c % p.t.group) * S::HD;
+            const bool vec = ((uintptr_t)p.out & 15) == 0;
+#pragma unroll 1
+            for (int j = 0; j < NG; j++) {
+                uint32_t o[32];
+                tmem_ld32(tmem_o + lanes + 32 * j, o);
+                tmem_wait_ld(o);
+                if (!on) continue;
+#pragma unroll
+                for (int g = 0; g < 8; g++) {
+                    const float4 x = make_float4(__uint_as_float(o[g]) * inv, __uint_as_float(o[8 + g]) * inv, __uint_as_float(o[16 + g]) * inv, __uint_as_float(o[24 + g]) * inv);
+                    float* at = to + 32 * j + 4 * g;
+                    if (vec) *reinterpret_cast<float4*>(at) = x;
+                    else { at[0] = x.x; at[1] = x.y; at[2] = x.z; at[3] = x.w; }
+                }
+            }
+            if (on && p.stat) p.stat[(size_t)unit * PK_COLS + tid] = make_float2(m, log2f(l) - 14.0f);
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == PK_MMA_WARP) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem_o), "r"(512u) : "memory");
+    }
+    if (tid == 0 && sh->abort_flag) {
+        *p.err = IBCU_KV4_WAIT_ERR;
+        for (int i = 0; i < 1000; i++) __nanosleep(1000);      // copies still on their way into this block's shared memory land before it goes
+    }
+}
+
+// Attention that the rows draw: S^T [128 rows x 128 columns] = K' Q^T again, a thread a row, which adds up its softmax weights over the columns that
+// see it. grid (128 rows, KV heads, parts of the column tiles); K' is made once, the columns' images come through a ring. Writes parts [part][KV head][max_rows].
+constexpr int PW_MMA_WARP = 4, PW_TMA_WARP = 5, PW_THREADS = 6 * 32;
+template <int NG> struct PwSmem {
+    static constexpr int KB = NG / 2, IMAGE = 2 * KB * 16384, STAGE = IMAGE + 2048;              // a tile's image, 128 factors, 128 pairs of its softmax
+    static constexpr int K = 0, RING = IMAGE, TOTAL = RING + 2 * STAGE;
+};
+struct PwShared { unsigned long long full[2], empty[2], d_full[2], d_empty[2], k_full, drained; uint32_t tmem_base; int abort_flag; };
+
+template <int NG>
+__global__ void __launch_bounds__(PW_THREADS, 1) kv4_prompt_weight_kernel(const PkParams p, float* __restrict__ parts) {
+    using S = PwSmem<NG>;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    PwShared* sh = reinterpret_cast<PwShared*>(smem + S::TOTAL);
+    volatile int* abort_flag = &sh->abort_flag;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kvh = blockIdx.y, r0 = blockIdx.x * 128;
+    if (tid == 0) {
+        auto init = [&](unsigned long long& b, int n) { mbar_init(smem_u32(&b), n); };
+        for (int i = 0; i < 2; i++) { init(sh->full[i], 1); init(sh->empty[i], 5); init(sh->d_full[i], 1); init(sh->d_empty[i], 4); }
+        init(sh->k_full, 4); init(sh->drained, 1);
+        sh->abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    if (warp == PW_MMA_WARP) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&sh->tmem_base)), "r"(256u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        pdl_launch_dependents();
+    }
+    pdl_wait();
+    int row0, pos0;
+    const bool there = kv4_place(p.at, p.t.B, p.c.max_rows, p.err, row0, pos0);
+    const int R = there ? row0 + p.t.B : 0, first = max(0, r0 - row0) * p.t.group / PK_COLS + blockIdx.z;       // tiles that see a row of the block, every gridDim.z-th
+    const int n = r0 < R && first < p.tiles ? (p.tiles - first + (int)gridDim.z - 1) / (int)gridDim.z : 0;
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = sh->tmem_base;
+    if (warp == PW_TMA_WARP) {
+        if (elect_one() && n) {
+            asm volatile("fence.proxy.async.global;" ::: "memory");
+            for (int i = 0; i < n; i++) {
+                const int s = i & 1;
+                if (!mbar_wait(smem_u32(&sh->empty[s]), (uint32_t)((i >> 1) & 1) ^ 1u, abort_flag, 1)) break;
+                const size_t unit = (size_t)kvh * p.tiles + first + i * (int)gridDim.z;
+                const uint32_t bar = smem_u32(&sh->full[s]), to = smem_u32(smem + S::RING + s * S::STAGE);
+                mbar_expect_tx(bar, S::IMAGE + 512 + 1024);
+                for (int e = 0; e < S::IMAGE; e += 16384) bulk_load(to + e, p.image + unit * S::IMAGE + e, 16384, bar);
+                bulk_load(to + S::IMAGE, p.qc + unit * PK_COLS, 512, bar);
+                bulk_load(to + S::IMAGE + 512, p.stat + unit * PK_COLS, 1024, bar);
+            }
+        }
+        __syncwarp();
+    } else if (warp == PW_MMA_WARP) {
+        if (elect_one() && n) {
+            constexpr uint32_t idesc = (1u << 4) | (8u << 24) | ((PK_COLS / 8) << 17);
+            bool ok = mbar_wait(smem_u32(&sh->k_full), 0u, abort_flag, 2);
+            const uint64_t k = smem_desc_sw128(smem_u32(smem + S::K));
+            for (int i = 0; i < n && ok; i++) {
+                const int s = i & 1;
+                const uint32_t ph = (uint32_t)(i >> 1) & 1u;
+                ok = mbar_wait(smem_u32(&sh->full[s]), ph, abort_flag, 3) && mbar_wait(smem_u32(&sh->d_empty[s]), ph ^ 1u, abort_flag, 4);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint64_t q = smem_desc_sw128(smem_u32(smem + S::RING + s * S::STAGE));
+#pragma unroll
+                for (int m = 0; m < 3; m++)
+#pragma unroll
+                    for (int st = 0; st < 2 * NG; st++)
+                        mma_f16_ss(tmem + s * PK_COLS, k + (((m == 2) * S::KB + st / 4) * 16384 >> 4) + st % 4 * 2, q + (((m == 1) * S::KB + st / 4) * 16384 >> 4) + st % 4 * 2, idesc, m || st ? 1u : 0u);
+                mma_commit(smem_u32(&sh->empty[s]));
+                mma_commit(smem_u32(&sh->d_full[s]));
+            }
+            mma_commit(smem_u32(&sh->drained));
+            mbar_wait(smem_u32(&sh->drained), 0u, abort_flag, 5);
+        }
+        __syncwarp();
+    } else if (n) {
+#pragma unroll 1
+        for (int u = 0; u < 4; u++) {                          // keys: eight rows by the four pieces a warp at a time
+            const int r = 8 * (warp + 4 * u) + (lane & 7), t = lane >> 3;
+            const size_t row = p.c.row(kvh, min(r0 + r, R - 1));
+            uint32_t w[NG], sc[NG];
+#pragma unroll
+            for (int j = 0; j < NG; j++) {
+                w[j] = __ldcg(reinterpret_cast<const uint32_t*>(p.c.k + row * (16 * NG)) + t * NG + j);
+                sc[j] = __ldcg(reinterpret_cast<const uint32_t*>(p.c.scale + row * (2 * NG)) + j);
+            }
+            place_key<NG>(smem + S::K, 16384, S::KB * 16384, r, t, w, sc);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh->k_full));
+        const int r = r0 + tid;
+        float sum = 0.0f;
+        for (int i = 0; i < n; i++) {
+            const int s = i & 1, tile = first + i * (int)gridDim.z, c0 = tile * PK_COLS;
+            const uint32_t ph = (uint32_t)(i >> 1) & 1u;
+            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->full[s]), ph, abort_flag, 6) && mbar_wait(smem_u32(&sh->d_full[s]), ph, abort_flag, 7))) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const float* f = reinterpret_cast<const float*>(smem + S::RING + s * S::STAGE + S::IMAGE);
+            const float2* st = reinterpret_cast<const float2*>(f + 128);
+            // columns from which on the row is seen, and how many there are
+            const int from = max(0, r - row0) * p.t.group - c0, upto = p.t.B * p.t.group - c0;
+            const bool whole = __all_sync(0xffffffffu, from <= 0) && upto >= PK_COLS;
+#pragma unroll 1
+            for (int c = 0; c < PK_COLS; c += 32) {
+                uint32_t x[32];
+                tmem_ld32(tmem + ((uint32_t)(warp * 32) << 16) + s * PK_COLS + c, x);
+                tmem_wait_ld(x);
+                float part[2] = { 0.0f, 0.0f };
+#pragma unroll
+                for (int u = 0; u < 32; u += 2) {
+                    const float2 ff = *reinterpret_cast<const float2*>(f + c + u);
+                    const float4 ss = *reinterpret_cast<const float4*>(st + c + u);
+                    const float a = ex2((__fmul_rn(__uint_as_float(x[u]), ff.x) - ss.x) - ss.y), b = ex2((__fmul_rn(__uint_as_float(x[u + 1]), ff.y) - ss.z) - ss.w);
+                    part[0] += whole || (c + u >= from && c + u < upto) ? a : 0.0f;
+                    part[1] += whole || (c + u + 1 >= from && c + u + 1 < upto) ? b : 0.0f;
+                }
+                sum += part[0] + part[1];
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) { mbar_arrive(smem_u32(&sh->d_empty[s])); mbar_arrive(smem_u32(&sh->empty[s])); }
+        }
+        if (r < R) parts[((size_t)blockIdx.z * p.c.n_kv + kvh) * p.c.max_rows + r] = sum;
+    } else if (r0 + tid < R) {
+        parts[((size_t)blockIdx.z * p.c.n_kv + kvh) * p.c.max_rows + r0 + tid] = 0.0f;
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == PW_MMA_WARP) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(256u) : "memory");
+    }
+    if (tid == 0 && sh->abort_flag) {
+        *p.err = IBCU_KV4_WAIT_ERR;
+        for (int i = 0; i < 1000; i++) __nanosleep(1000);
+    }
+}
+
+template <int NG>
+int launch_prompt(ibcu_ctx* ctx, const PkParams& p, int rows, float* parts, int n_parts) {
+    static SmemOptIn opt, opt_w;
+    constexpr size_t smem = PkSmem<NG>::TOTAL + sizeof(PkShared), smem_w = PwSmem<NG>::TOTAL + sizeof(PwShared);
+    static_assert(smem <= 227 * 1024 && smem_w <= 227 * 1024, "a block's shared memory");
+    if (int rc = ibcu_allow_smem(ctx, opt, kv4_prompt_kernel<NG>, smem)) return rc;
+    if (int rc = ibcu_launch(ctx, kv4_prompt_kernel<NG>, dim3(p.c.n_kv * p.tiles), dim3(PK_THREADS), smem, 1, true, p)) return rc;
+    if (!p.stat) return IBCU_OK;
+    if (int rc = ibcu_allow_smem(ctx, opt_w, kv4_prompt_weight_kernel<NG>, smem_w)) return rc;
+    return ibcu_launch(ctx, kv4_prompt_weight_kernel<NG>, dim3((rows + 127) / 128, p.c.n_kv, n_parts), dim3(PW_THREADS), smem_w, 1, true, p, parts);
+}
+
+}  // namespace
+
+int kv4_prompt_parts(ibcu_ctx* ctx, const Kv4& c, int tiles, int rows) {
+    return std::min(std::min(tiles, 16), std::max(1, 8 * ctx->sm_count / (((rows + 127) / 128) * c.n_kv)));
+}
+int kv4_prompt(ibcu_ctx* ctx, const Kv4& c, const Kv4Columns& t, const Kv4Place& at, const unsigned char* image, const float* qc, float* out, float2* stat, int rows, float* parts, int n_parts) {
+    PkParams p;
+    memset(&p, 0, sizeof p);
+    p.c = c; p.t = t; p.at = at; p.image = image; p.qc = qc; p.out = out; p.stat = stat; p.tiles = t.ntiles / 8; p.err = ctx->kern_err;
+    return c.hd == 128 ? launch_prompt<4>(ctx, p, rows, parts, n_parts) : launch_prompt<2>(ctx, p, rows, parts, n_parts);
+}

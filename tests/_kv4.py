@@ -20,7 +20,7 @@ def quantise(x):
     amax = np.abs(y).max(-1)
     bad = ~np.isfinite(y).all(-1)
     with np.errstate(all="ignore"):
-        s = np.minimum(np.where(bad, np.float32(0), amax) * (np.float32(1) / np.float32(7)), np.float32(65504)).astype(np.float16)
+        s = np.minimum(np.where(bad, np.float32(0), amax) * (np.float32(1) / np.float32(7)), np.float32(8192)).astype(np.float16)
         inv = np.where(s > 0, np.float32(1) / s.astype(np.float32), np.float32(0)).astype(np.float32)
         c = np.clip(np.rint(np.where(bad[..., None], np.float32(0), y) * inv[..., None]), -7, 7)
     s[bad] = np.nan

@@ -74,7 +74,7 @@ def test_groups_out_of_the_ordinary(backend):
     """Zeros, values below the smallest scale, beyond the largest, Inf and NaN: each group by itself."""
     be, rng = backend, np.random.default_rng(1)
     x = rng.standard_normal((1, 256), dtype=np.float32).reshape(8, 32)
-    x[0] = 0; x[1] *= 1e-9; x[2] *= 1e-6; x[3] *= 1e38; x[4, 3] = np.inf; x[5, 31] = np.nan; x[6] *= 65504 * 7; x[7, 0] = -np.inf
+    x[0] = 0; x[1] *= 1e-9; x[2] *= 1e-6; x[3] *= 1e38; x[4, 3] = np.inf; x[5, 31] = np.nan; x[6] *= 8192 * 7; x[7, 0] = -np.inf
     x = x.reshape(1, 256)
     t = be.make_kv4(1, 256, 8)
     dx = be.upload(x)
@@ -83,7 +83,7 @@ def test_groups_out_of_the_ordinary(backend):
     k, v, sc = get(be, t)
     assert np.array_equal(k[0, 2], _kv4.pack(c, True)[0]) and np.array_equal(v[0, 2], _kv4.pack(c, False)[0])
     assert same(sc[0, 2], np.concatenate([s, s], -1)[0])
-    assert np.isnan(s[0, [4, 5, 7]]).all() and s[0, 0] == 0 and s[0, 1] == 0 and s[0, 2] > 0 and s[0, 3] == 65504
+    assert np.isnan(s[0, [4, 5, 7]]).all() and s[0, 0] == 0 and s[0, 1] == 0 and s[0, 2] > 0 and s[0, 3] == 8192
 
 
 SHAPES = [(1, 1, 32, 0, 1), (32, 8, 128, 0, 1), (32, 8, 128, 511, 1), (32, 4, 64, 3001, 6), (8, 1, 256, 100, 9), (6, 2, 96, 33, 5), (12, 12, 64, 257, 3), (10, 2, 192, 60, 8),
@@ -115,8 +115,15 @@ def test_attention_and_weights(backend, n_heads, n_kv, hd, row0, B):
         assert np.array_equal(be.download(dq, np.float32, q.size), q.reshape(-1))
 
 
+@pytest.mark.parametrize("n_heads,n_kv,hd,row0,B", [(32, 8, 128, 0, 200), (16, 16, 64, 37, 400), (32, 4, 64, 1000, 333), (48, 48, 128, 61, 129), (32, 8, 128, 1, 257)])
+def test_prompts(backend, n_heads, n_kv, hd, row0, B):
+    """Enough columns for tiles of 128 on the tensor cores: tiles and rows that end anywhere, groups that do not divide a tile's positions."""
+    test_attention_and_weights(backend, n_heads, n_kv, hd, row0, B)
+
+
 @pytest.mark.parametrize("n_heads,n_kv,hd,row0,pos0,B,theta", [(32, 8, 128, 512, 512, 1, 10000.0), (32, 4, 64, 0, 0, 1, 10000.0), (8, 2, 128, 100, 5000, 4, 500000.0),
-                                                                (6, 6, 96, 31, 31, 33, 10000.0), (4, 1, 256, 15, 70000, 2, 10000.0), (5, 1, 32, 3, 3, 1, 0.0), (32, 8, 128, 0, 0, 150, 10000.0)])
+                                                                (6, 6, 96, 31, 31, 33, 10000.0), (4, 1, 256, 15, 70000, 2, 10000.0), (5, 1, 32, 3, 3, 1, 0.0), (32, 8, 128, 0, 0, 150, 10000.0),
+                                                                (32, 8, 128, 5, 5, 200, 10000.0), (12, 12, 64, 70, 9000, 600, 500000.0)])
 def test_decode_step(backend, n_heads, n_kv, hd, row0, pos0, B, theta):
     """One call: queries and keys rotated, the rows written as ibcu_kv4_write writes them, attention over them; inputs left alone."""
     be, rng = backend, np.random.default_rng(row0 + B)
@@ -140,7 +147,8 @@ def test_decode_step(backend, n_heads, n_kv, hd, row0, pos0, B, theta):
         assert np.array_equal(be.download(d, np.float32, x.size), x.reshape(-1))
 
 
-@pytest.mark.parametrize("n_heads,n_kv,hd,row0,B,at", [(8, 2, 64, 0, 6, 3), (4, 4, 128, 29, 9, 30), (4, 1, 256, 60, 8, 67), (8, 8, 64, 0, 80, 33), (32, 8, 128, 200, 3, 201)])
+@pytest.mark.parametrize("n_heads,n_kv,hd,row0,B,at", [(8, 2, 64, 0, 6, 3), (4, 4, 128, 29, 9, 30), (4, 1, 256, 60, 8, 67), (8, 8, 64, 0, 80, 33), (32, 8, 128, 200, 3, 201), (32, 8, 128, 100, 300, 250),
+                                                       (32, 4, 64, 0, 300, 130)])
 def test_a_later_row_does_not_reach_an_earlier_position(backend, n_heads, n_kv, hd, row0, B, at):
     """Row `at` holds NaN in key and value: positions that do not see it keep their bits, the others show it."""
     be, rng = backend, np.random.default_rng(at)
