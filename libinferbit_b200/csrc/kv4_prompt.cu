@@ -31,7 +31,7 @@ struct PkParams {
 template <int NG> struct PkSmem {
     static constexpr int KB = NG / 2, HD = 32 * NG;            // KB: blocks of 64 values, a swizzled row of 128 bytes each
     static constexpr int IMAGE = 2 * KB * 16384, KEYS = 2 * KB * 8192, VALUES = 2 * HD * 128, RAW_BYTES = PK_ROWS * 36 * NG;
-    static constexpr int Q = 0, K = Q + IMAGE, V = K + 2 * KEYS, RAW = V + 2 * VALUES, TOTAL = RAW + PK_RAW * RAW_BYTES;
+    static constexpr int K = 0, V = K + 2 * KEYS, RAW = V + 2 * VALUES, TOTAL = RAW + PK_RAW * RAW_BYTES;
 };
 struct PkShared {
     unsigned long long q_full, raw_full[PK_RAW], raw_empty[PK_RAW], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], s_empty[2], p_full[2], pv_done[2], drained;
@@ -39,11 +39,6 @@ struct PkShared {
     int abort_flag;
 };
 
-__device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
-}
 __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
                  "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
@@ -102,7 +97,7 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
     const int kvh = blockIdx.x % p.c.n_kv, tile = p.tiles - 1 - blockIdx.x / p.c.n_kv, unit = kvh * p.tiles + tile, c0 = tile * PK_COLS;          // most rows first
     if (tid == 0) {
         auto init = [&](unsigned long long& b, int n) { mbar_init(smem_u32(&b), n); };
-        init(sh->q_full, 1); init(sh->drained, 1);
+        init(sh->q_full, 4); init(sh->drained, 1);
         for (int i = 0; i < PK_RAW; i++) { init(sh->raw_full[i], 1); init(sh->raw_empty[i], 8); }
         for (int i = 0; i < 2; i++) {
             init(sh->k_full[i], 4); init(sh->k_empty[i], 1); init(sh->v_full[i], 4); init(sh->v_empty[i], 1);
@@ -124,13 +119,11 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem_o = sh->tmem_base, tmem_s = tmem_o + S::HD, tmem_p = tmem_s + 2 * PK_ROWS;          // 128 + 2 x 64 + 2 x 64 columns
+    const uint32_t tmem_o = sh->tmem_base, tmem_s = tmem_o + S::HD, tmem_p = tmem_s + 2 * PK_ROWS, tmem_q = tmem_p + 2 * PK_ROWS;          // 128 + 2 x 64 + 2 x 64 + 2 x 64 columns
 
     if (warp == PK_TMA_WARP) {
         if (elect_one() && n) {
             asm volatile("fence.proxy.async.global;" ::: "memory");
-            mbar_expect_tx(smem_u32(&sh->q_full), S::IMAGE);
-            for (int e = 0; e < S::IMAGE; e += 16384) bulk_load(smem_u32(smem + S::Q + e), p.image + (size_t)unit * S::IMAGE + e, 16384, smem_u32(&sh->q_full));
             const size_t plane = p.c.row(kvh, 0);
             int s = 0; uint32_t ph = 1;
             for (int i = 0; i < n; i++) {
@@ -150,7 +143,6 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
             constexpr uint32_t idesc = (1u << 4) | (8u << 24);                                    // FP32 accumulators, fp16 operands, 128 rows
             constexpr uint32_t idesc_s = idesc | ((PK_ROWS / 8) << 17), idesc_o = idesc | ((S::HD / 8) << 17);
             bool ok = mbar_wait(smem_u32(&sh->q_full), 0u, abort_flag, 2);
-            const uint64_t q = smem_desc_sw128(smem_u32(smem + S::Q));
             auto scores = [&](int i) {
                 const int b = i & 1;
                 const uint32_t ph = (uint32_t)(i >> 1) & 1u;
@@ -161,7 +153,7 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
                 for (int m = 0; m < 3; m++)                                                       // high.high, low.high, high.low
 #pragma unroll
                     for (int st = 0; st < S::HD / 16; st++)
-                        mma_f16_ss(tmem_s + b * PK_ROWS, q + (((m == 1) * S::KB + st / 4) * 16384 >> 4) + st % 4 * 2, k + (((m == 2) * S::KB + st / 4) * 8192 >> 4) + st % 4 * 2, idesc_s,
+                        mma_f16_ts(tmem_s + b * PK_ROWS, tmem_q + (m == 1) * (S::HD / 2) + st * 8, k + (((m == 2) * S::KB + st / 4) * 8192 >> 4) + st % 4 * 2, idesc_s,
                                    m || st ? 1u : 0u);
                 mma_commit(smem_u32(&sh->k_empty[b]));
                 mma_commit(smem_u32(&sh->s_full[b]));
@@ -254,6 +246,27 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
         const int lim = row0 + b_col, lim0 = row0 + (c0 + (tid & ~31)) / p.t.group;              // last rows that this column, the warp's first column, see
         const float f = on ? __ldcg(p.qc + (size_t)unit * PK_COLS + tid) : 0.0f;
         const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+        // the queries' pieces into tensor memory: the scores' A operand (from shared memory it would be read again for every 64 rows, and with what the
+        // dequantisers write that is more than shared memory gives)
+        if (n) {
+            const unsigned char* image = p.image + (size_t)unit * S::IMAGE + tid * 128;
+#pragma unroll 1
+            for (int part = 0; part < 2; part += 1)
+#pragma unroll 1
+                for (int kb = 0; kb < S::KB; kb++) {
+                    uint32_t x[32];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const uint4 v = __ldcg(reinterpret_cast<const uint4*>(image + (part * S::KB + kb) * 16384 + ((e ^ (tid & 7)) << 4)));
+                        x[4 * e] = v.x; x[4 * e + 1] = v.y; x[4 * e + 2] = v.z; x[4 * e + 3] = v.w;
+                    }
+                    tmem_st32(tmem_q + lanes + part * (S::HD / 2) + kb * 32, x);
+                }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sh->q_full));
+        }
         float m = PK_LOW, l = 0.0f;
         bool wide = false, alive = true;
         for (int i = 0; i < n; i++) {
@@ -363,14 +376,15 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
     }
 }
 
-// Attention that the rows draw: S^T [128 rows x 128 columns] = K' Q^T again, a thread a row, which adds up its softmax weights over the columns that
-// see it. grid (128 rows, KV heads, parts of the column tiles); K' is made once, the columns' images come through a ring. Writes parts [part][KV head][max_rows].
-constexpr int PW_MMA_WARP = 4, PW_TMA_WARP = 5, PW_THREADS = 6 * 32;
+// Attention that the rows draw: S^T [128 rows x 128 columns] = K' Q^T again, two threads a row, which add up its softmax weights over the columns that
+// see it. grid (128 rows, KV heads, parts of the column tiles); K' is made once and stays in tensor memory, the columns' images come through a ring. Writes
+// parts [part][KV head][max_rows].
+constexpr int PW_SUM_WARPS = 8, PW_MMA_WARP = 8, PW_TMA_WARP = 9, PW_THREADS = 10 * 32;
 template <int NG> struct PwSmem {
-    static constexpr int KB = NG / 2, IMAGE = 2 * KB * 16384, STAGE = IMAGE + 2048;              // a tile's image, 128 factors, 128 pairs of its softmax
-    static constexpr int K = 0, RING = IMAGE, TOTAL = RING + 2 * STAGE;
+    static constexpr int KB = NG / 2, IMAGE = 2 * KB * 16384, STAGE = IMAGE + 2048, DEPTH = 3;   // a tile's image, 128 factors, 128 pairs of its softmax
+    static constexpr int TOTAL = DEPTH * STAGE;
 };
-struct PwShared { unsigned long long full[2], empty[2], d_full[2], d_empty[2], k_full, drained; uint32_t tmem_base; int abort_flag; };
+struct PwShared { unsigned long long full[3], empty[3], d_full[2], d_empty[2], k_full, drained; uint32_t tmem_base; int abort_flag; float half[128]; };
 
 template <int NG>
 __global__ void __launch_bounds__(PW_THREADS, 1) kv4_prompt_weight_kernel(const PkParams p, float* __restrict__ parts) {
@@ -381,14 +395,15 @@ __global__ void __launch_bounds__(PW_THREADS, 1) kv4_prompt_weight_kernel(const 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kvh = blockIdx.y, r0 = blockIdx.x * 128;
     if (tid == 0) {
         auto init = [&](unsigned long long& b, int n) { mbar_init(smem_u32(&b), n); };
-        for (int i = 0; i < 2; i++) { init(sh->full[i], 1); init(sh->empty[i], 5); init(sh->d_full[i], 1); init(sh->d_empty[i], 4); }
+        for (int i = 0; i < S::DEPTH; i++) { init(sh->full[i], 1); init(sh->empty[i], PW_SUM_WARPS + 1); }
+        for (int i = 0; i < 2; i++) { init(sh->d_full[i], 1); init(sh->d_empty[i], PW_SUM_WARPS); }
         init(sh->k_full, 4); init(sh->drained, 1);
         sh->abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
     if (warp == PW_MMA_WARP) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&sh->tmem_base)), "r"(256u) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&sh->tmem_base)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         pdl_launch_dependents();
     }
@@ -400,19 +415,20 @@ __global__ void __launch_bounds__(PW_THREADS, 1) kv4_prompt_weight_kernel(const 
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = sh->tmem_base;
+    const uint32_t tmem = sh->tmem_base, tmem_k = tmem + 2 * PK_COLS;                            // two accumulators, then high and low pieces of K'
     if (warp == PW_TMA_WARP) {
         if (elect_one() && n) {
             asm volatile("fence.proxy.async.global;" ::: "memory");
+            int s = 0; uint32_t ph = 1;
             for (int i = 0; i < n; i++) {
-                const int s = i & 1;
-                if (!mbar_wait(smem_u32(&sh->empty[s]), (uint32_t)((i >> 1) & 1) ^ 1u, abort_flag, 1)) break;
+                if (!mbar_wait(smem_u32(&sh->empty[s]), ph, abort_flag, 1)) break;
                 const size_t unit = (size_t)kvh * p.tiles + first + i * (int)gridDim.z;
-                const uint32_t bar = smem_u32(&sh->full[s]), to = smem_u32(smem + S::RING + s * S::STAGE);
+                const uint32_t bar = smem_u32(&sh->full[s]), to = smem_u32(smem + s * S::STAGE);
                 mbar_expect_tx(bar, S::IMAGE + 512 + 1024);
                 for (int e = 0; e < S::IMAGE; e += 16384) bulk_load(to + e, p.image + unit * S::IMAGE + e, 16384, bar);
                 bulk_load(to + S::IMAGE, p.qc + unit * PK_COLS, 512, bar);
                 bulk_load(to + S::IMAGE + 512, p.stat + unit * PK_COLS, 1024, bar);
+                if (++s == S::DEPTH) { s = 0; ph ^= 1; }
             }
         }
         __syncwarp();
@@ -420,83 +436,105 @@ __global__ void __launch_bounds__(PW_THREADS, 1) kv4_prompt_weight_kernel(const 
         if (elect_one() && n) {
             constexpr uint32_t idesc = (1u << 4) | (8u << 24) | ((PK_COLS / 8) << 17);
             bool ok = mbar_wait(smem_u32(&sh->k_full), 0u, abort_flag, 2);
-            const uint64_t k = smem_desc_sw128(smem_u32(smem + S::K));
+            int s = 0; uint32_t phs = 0;
             for (int i = 0; i < n && ok; i++) {
-                const int s = i & 1;
-                const uint32_t ph = (uint32_t)(i >> 1) & 1u;
-                ok = mbar_wait(smem_u32(&sh->full[s]), ph, abort_flag, 3) && mbar_wait(smem_u32(&sh->d_empty[s]), ph ^ 1u, abort_flag, 4);
+                const int b = i & 1;
+                ok = mbar_wait(smem_u32(&sh->full[s]), phs, abort_flag, 3) && mbar_wait(smem_u32(&sh->d_empty[b]), ((uint32_t)(i >> 1) & 1u) ^ 1u, abort_flag, 4);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint64_t q = smem_desc_sw128(smem_u32(smem + S::RING + s * S::STAGE));
+                const uint64_t q = smem_desc_sw128(smem_u32(smem + s * S::STAGE));
 #pragma unroll
                 for (int m = 0; m < 3; m++)
 #pragma unroll
                     for (int st = 0; st < 2 * NG; st++)
-                        mma_f16_ss(tmem + s * PK_COLS, k + (((m == 2) * S::KB + st / 4) * 16384 >> 4) + st % 4 * 2, q + (((m == 1) * S::KB + st / 4) * 16384 >> 4) + st % 4 * 2, idesc, m || st ? 1u : 0u);
+                        mma_f16_ts(tmem + b * PK_COLS, tmem_k + (m == 2) * 16 * NG + st * 8, q + (((m == 1) * S::KB + st / 4) * 16384 >> 4) + st % 4 * 2, idesc, m || st ? 1u : 0u);
                 mma_commit(smem_u32(&sh->empty[s]));
-                mma_commit(smem_u32(&sh->d_full[s]));
+                mma_commit(smem_u32(&sh->d_full[b]));
+                if (++s == S::DEPTH) { s = 0; phs ^= 1; }
             }
             mma_commit(smem_u32(&sh->drained));
             mbar_wait(smem_u32(&sh->drained), 0u, abort_flag, 5);
         }
         __syncwarp();
-    } else if (n) {
-#pragma unroll 1
-        for (int u = 0; u < 4; u++) {                          // keys: eight rows by the four pieces a warp at a time
-            const int r = 8 * (warp + 4 * u) + (lane & 7), t = lane >> 3;
-            const size_t row = p.c.row(kvh, min(r0 + r, R - 1));
-            uint32_t w[NG], sc[NG];
-#pragma unroll
-            for (int j = 0; j < NG; j++) {
-                w[j] = __ldcg(reinterpret_cast<const uint32_t*>(p.c.k + row * (16 * NG)) + t * NG + j);
-                sc[j] = __ldcg(reinterpret_cast<const uint32_t*>(p.c.scale + row * (2 * NG)) + j);
-            }
-            place_key<NG>(smem + S::K, 16384, S::KB * 16384, r, t, w, sc);
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh->k_full));
-        const int r = r0 + tid;
+    } else {
+        const int quarter = warp & 3, half = warp >> 2, own = quarter * 32 + lane, r = r0 + own;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         float sum = 0.0f;
-        for (int i = 0; i < n; i++) {
-            const int s = i & 1, tile = first + i * (int)gridDim.z, c0 = tile * PK_COLS;
-            const uint32_t ph = (uint32_t)(i >> 1) & 1u;
-            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->full[s]), ph, abort_flag, 6) && mbar_wait(smem_u32(&sh->d_full[s]), ph, abort_flag, 7))) break;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const float* f = reinterpret_cast<const float*>(smem + S::RING + s * S::STAGE + S::IMAGE);
-            const float2* st = reinterpret_cast<const float2*>(f + 128);
-            // columns from which on the row is seen, and how many there are
-            const int from = max(0, r - row0) * p.t.group - c0, upto = p.t.B * p.t.group - c0;
-            const bool whole = __all_sync(0xffffffffu, from <= 0) && upto >= PK_COLS;
-#pragma unroll 1
-            for (int c = 0; c < PK_COLS; c += 32) {
-                uint32_t x[32];
-                tmem_ld32(tmem + ((uint32_t)(warp * 32) << 16) + s * PK_COLS + c, x);
-                tmem_wait_ld(x);
-                float part[2] = { 0.0f, 0.0f };
+        if (n) {
+            if (half == 0) {
+                const size_t row = p.c.row(kvh, min(r, R - 1));
+                uint32_t sc[NG];
 #pragma unroll
-                for (int u = 0; u < 32; u += 2) {
-                    const float2 ff = *reinterpret_cast<const float2*>(f + c + u);
-                    const float4 ss = *reinterpret_cast<const float4*>(st + c + u);
-                    const float a = ex2((__fmul_rn(__uint_as_float(x[u]), ff.x) - ss.x) - ss.y), b = ex2((__fmul_rn(__uint_as_float(x[u + 1]), ff.y) - ss.z) - ss.w);
-                    part[0] += whole || (c + u >= from && c + u < upto) ? a : 0.0f;
-                    part[1] += whole || (c + u + 1 >= from && c + u + 1 < upto) ? b : 0.0f;
+                for (int j = 0; j < NG; j++) sc[j] = __ldcg(reinterpret_cast<const uint32_t*>(p.c.scale + row * (2 * NG)) + j);
+                bool bad = false;
+#pragma unroll
+                for (int j = NG / 2; j < NG; j++) bad = bad || is_nan(sc[j]) || is_nan(sc[j] >> 16);
+#pragma unroll 1
+                for (int t = 0; t < 4; t += 2) {               // pieces of a key row, two at a time: 8 NG columns of tensor memory a part
+                    uint32_t high[8 * NG], low[8 * NG];
+#pragma unroll
+                    for (int e = 0; e < 2 * NG; e++) {
+                        const int j = e % NG;
+                        const uint32_t w = __ldcg(reinterpret_cast<const uint32_t*>(p.c.k + row * (16 * NG)) + t * NG + e), k = bad ? 0x7FFFu : (j & 1 ? sc[j / 2] >> 16 : sc[j / 2] & 0xFFFFu);
+                        __half2 f[4];
+                        codes_of(w, f);
+#pragma unroll
+                        for (int u = 0; u < 4; u++) held_pieces(f[u], half2_of(k | k << 16), high[4 * e + u], low[4 * e + u]);
+                    }
+                    if constexpr (NG == 4) {
+                        tmem_st32(tmem_k + lanes + t * 4 * NG, high);
+                        tmem_st32(tmem_k + lanes + 16 * NG + t * 4 * NG, low);
+                    } else {
+                        tmem_st16(tmem_k + lanes + t * 4 * NG, high);
+                        tmem_st16(tmem_k + lanes + 16 * NG + t * 4 * NG, low);
+                    }
                 }
-                sum += part[0] + part[1];
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sh->k_full));
             }
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) { mbar_arrive(smem_u32(&sh->d_empty[s])); mbar_arrive(smem_u32(&sh->empty[s])); }
+            int s = 0; uint32_t phs = 0;
+            for (int i = 0; i < n; i++) {
+                const int b = i & 1, c0 = (first + i * (int)gridDim.z) * PK_COLS;
+                if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->full[s]), phs, abort_flag, 6) && mbar_wait(smem_u32(&sh->d_full[b]), (uint32_t)(i >> 1) & 1u, abort_flag, 7))) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const float* f = reinterpret_cast<const float*>(smem + s * S::STAGE + S::IMAGE);
+                const float2* st = reinterpret_cast<const float2*>(f + 128);
+                // columns from which on the row is seen, and how many there are
+                const int from = max(0, r - row0) * p.t.group - c0, upto = p.t.B * p.t.group - c0;
+                const bool whole = __all_sync(0xffffffffu, from <= 0) && upto >= PK_COLS;
+#pragma unroll 1
+                for (int c = half * 64; c < half * 64 + 64; c += 32) {
+                    uint32_t x[32];
+                    tmem_ld32(tmem + lanes + b * PK_COLS + c, x);
+                    tmem_wait_ld(x);
+                    float part[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
+#pragma unroll
+                    for (int u = 0; u < 32; u += 2) {
+                        const float2 ff = *reinterpret_cast<const float2*>(f + c + u);
+                        const float4 ss = *reinterpret_cast<const float4*>(st + c + u);
+                        const float y = ex2((__fmul_rn(__uint_as_float(x[u]), ff.x) - ss.x) - ss.y), z = ex2((__fmul_rn(__uint_as_float(x[u + 1]), ff.y) - ss.z) - ss.w);
+                        part[u & 2] += whole || (c + u >= from && c + u < upto) ? y : 0.0f;
+                        part[(u & 2) + 1] += whole || (c + u + 1 >= from && c + u + 1 < upto) ? z : 0.0f;
+                    }
+                    sum += (part[0] + part[1]) + (part[2] + part[3]);
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) { mbar_arrive(smem_u32(&sh->d_empty[b])); mbar_arrive(smem_u32(&sh->empty[s])); }
+                if (++s == S::DEPTH) { s = 0; phs ^= 1; }
+            }
         }
-        if (r < R) parts[((size_t)blockIdx.z * p.c.n_kv + kvh) * p.c.max_rows + r] = sum;
-    } else if (r0 + tid < R) {
-        parts[((size_t)blockIdx.z * p.c.n_kv + kvh) * p.c.max_rows + r0 + tid] = 0.0f;
+        if (half) sh->half[own] = sum;
+        asm volatile("bar.sync 2, %0;" :: "n"(PW_SUM_WARPS * 32) : "memory");
+        if (!half && r < R) parts[((size_t)blockIdx.z * p.c.n_kv + kvh) * p.c.max_rows + r] = sum + sh->half[own];
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (warp == PW_MMA_WARP) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(256u) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512u) : "memory");
     }
     if (tid == 0 && sh->abort_flag) {
         *p.err = IBCU_KV4_WAIT_ERR;
@@ -519,7 +557,7 @@ int launch_prompt(ibcu_ctx* ctx, const PkParams& p, int rows, float* parts, int 
 }  // namespace
 
 int kv4_prompt_parts(ibcu_ctx* ctx, const Kv4& c, int tiles, int rows) {
-    return std::min(std::min(tiles, 16), std::max(1, 8 * ctx->sm_count / (((rows + 127) / 128) * c.n_kv)));
+    return std::min(std::min(tiles, 16), std::max(1, (3 * ctx->sm_count) / (((rows + 127) / 128) * c.n_kv)));
 }
 int kv4_prompt(ibcu_ctx* ctx, const Kv4& c, const Kv4Columns& t, const Kv4Place& at, const unsigned char* image, const float* qc, float* out, float2* stat, int rows, float* parts, int n_parts) {
     PkParams p;
