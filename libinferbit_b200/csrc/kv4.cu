@@ -14,9 +14,7 @@
 
 namespace {
 
-__device__ __forceinline__ float held(const uint8_t* row, int place, float s) { return (float)((__ldcg(row + (place >> 1)) >> ((place & 1) * 4) & 15) - 8) * s; }
-
-__device__ __forceinline__ float scale_at(const Kv4& c, size_t i) { return __half2float(__ushort_as_half(__ldcg(reinterpret_cast<const unsigned short*>(c.scale) + i))); }
+__device__ __forceinline__ float scale_at(const __half* p) { return __half2float(__ushort_as_half(__ldcg(reinterpret_cast<const unsigned short*>(p)))); }
 
 // One launch ahead of the attention of more than eight columns, and that of ibcu_kv4_write: blocks below qblocks turn a tile of 16 columns into
 // fragments or their part of an image, the others write the rows of a position, whose heads share its angles.
@@ -108,24 +106,45 @@ __global__ void __launch_bounds__(128) kv4_prep_kernel(const PrepParams p) {
         }
         return;
     }
-    const int quads = hd / 4, heads = (p.c.n_kv - wb % p.wparts + p.wparts - 1) / p.wparts;          // heads wparts apart
-    for (int e = tid; e < 2 * heads * quads; e += 128) {
-        const bool key = e < heads * quads;
-        const int f = key ? e : e - heads * quads, h = wb % p.wparts + f / quads * p.wparts;
-        kv4_write_four(p.c, (key ? p.w.k : p.w.v) + ((size_t)b0 * p.c.n_kv + h) * hd, key, h, row0 + b0, f % quads * 4, p.w.rotate ? turn : nullptr);
+    // heads wparts apart; a thread has four values of a row, up to four times ahead of their use
+    const int quads = hd / 4, heads = (p.c.n_kv - wb % p.wparts + p.wparts - 1) / p.wparts, total = 2 * heads * quads;
+    for (int e0 = tid; e0 < total; e0 += 512) {
+        float x[4][4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int e = e0 + u * 128, f = e < heads * quads ? e : e - heads * quads, h = wb % p.wparts + f / quads * p.wparts;
+            if (e < total) kv4_load_four(x[u], (e < heads * quads ? p.w.k : p.w.v) + ((size_t)b0 * p.c.n_kv + h) * hd + f % quads * 4);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int e = e0 + u * 128, f = e < heads * quads ? e : e - heads * quads, h = wb % p.wparts + f / quads * p.wparts;
+            if (e < total) kv4_write_four(p.c, x[u], e < heads * quads, h, row0 + b0, f % quads * 4, p.w.rotate ? turn : nullptr);
+        }
     }
 }
 
-// grid (rows, KV heads): the values that the cache holds
-__global__ void __launch_bounds__(128) kv4_read_kernel(Kv4 c, float* __restrict__ k, float* __restrict__ v, int row0) {
+// The values that the cache holds: a thread has a word of eight codes of a key row and the word at the same place of the value row
+__global__ void __launch_bounds__(256) kv4_read_kernel(Kv4 c, float* __restrict__ k, float* __restrict__ v, int row0, int n) {
     pdl_launch_dependents();
     pdl_wait();
-    const int b = blockIdx.x, h = blockIdx.y, ng = c.hd / 32;
-    const size_t row = c.row(h, row0 + b);
-    for (int i = threadIdx.x; i < c.hd; i += blockDim.x) {
-        const size_t o = ((size_t)b * c.n_kv + h) * c.hd + i;
-        k[o] = held(c.k + row * (c.hd / 2), kv4_key_place(i, ng), scale_at(c, row * 2 * ng + i / 32));
-        v[o] = held(c.v + row * (c.hd / 2), kv4_value_place(i, ng), scale_at(c, row * 2 * ng + ng + i / 32));
+    const int ng = c.hd / 32, words = 4 * ng, per_row = c.n_kv * words;
+    const bool vec = (((uintptr_t)k | (uintptr_t)v) & 15) == 0;
+    auto put = [&](float* to, uint32_t codes, float s) {      // the four lowest codes
+        const float x[4] = { (float)((int)(codes & 15) - 8) * s, (float)((int)(codes >> 4 & 15) - 8) * s, (float)((int)(codes >> 8 & 15) - 8) * s, (float)((int)(codes >> 12 & 15) - 8) * s };
+        if (vec) *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
+        else { to[0] = x[0]; to[1] = x[1]; to[2] = x[2]; to[3] = x[3]; }
+    };
+    for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < (long)n * per_row; e += (long)gridDim.x * 256) {
+        const int b = (int)(e / per_row), h = (int)(e % per_row) / words, w = (int)(e % per_row) % words;
+        const size_t row = c.row(h, row0 + b), out = ((size_t)b * c.n_kv + h) * c.hd;
+        const uint32_t kw = __ldcg(reinterpret_cast<const uint32_t*>(c.k) + row * words + w), vw = __ldcg(reinterpret_cast<const uint32_t*>(c.v) + row * words + w);
+        const __half* sc = c.scale + row * 2 * ng;
+        const int j = w % ng, t = w / ng, u0 = 2 * w, u1 = 2 * w + 1;                  // the key's group and piece; the value row's units of four codes
+        const float ks = scale_at(sc + j), v0 = scale_at(sc + ng + u0 % ng), v1 = scale_at(sc + ng + u1 % ng);
+        put(k + out + 32 * j + 8 * t, kw, ks);
+        put(k + out + 32 * j + 8 * t + 4, kw >> 16, ks);
+        put(v + out + 32 * (u0 % ng) + 4 * (u0 / ng), vw, v0);
+        put(v + out + 32 * (u1 % ng) + 4 * (u1 / ng), vw >> 16, v1);
     }
 }
 
@@ -346,7 +365,8 @@ extern "C" int ibcu_kv4_read(ibcu_ctx* ctx, const ibcu_kv4_t* cache, float* k, f
     if (int rc = check_cache(ctx, cache, "ibcu_kv4_read")) return rc;
     IBCU_REQUIRE(ctx, k && v, "ibcu_kv4_read: null pointer");
     if (int rc = check_rows(ctx, cache, row0, n, "ibcu_kv4_read")) return rc;
-    return ibcu_launch(ctx, kv4_read_kernel, dim3(n, cache->n_kv_heads), dim3(128), 0, 1, true, planes(cache), k, v, row0);
+    const long words = (long)n * cache->n_kv_heads * (cache->head_dim / 8);
+    return ibcu_launch(ctx, kv4_read_kernel, dim3((int)std::min((words + 255) / 256, 16L * ctx->sm_count)), dim3(256), 0, 1, true, planes(cache), k, v, row0, n);
 }
 
 static int check_heads(ibcu_ctx* ctx, const ibcu_kv4_t* cache, int n_heads, int B, const char* call) {

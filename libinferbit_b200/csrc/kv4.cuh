@@ -67,11 +67,15 @@ __device__ __forceinline__ uint32_t kv4_code(float x, float inv) {
     const float q = inv > 0.0f ? fminf(fmaxf(rintf(__fmul_rn(x, inv)), -7.0f), 7.0f) : 0.0f;
     return (uint32_t)((int)q + 8);
 }
-// Values i..i+3 of a key or value row of head h, read from src and written to the cache. Eight neighbouring lanes have a group, whose
-// largest magnitude they share. turn: the position's angles, or NULL.
-__device__ __forceinline__ void kv4_write_four(const Kv4& c, const float* src, bool key, int h, int r, int i, const double2* turn) {
+// four values of a row, at any address
+__device__ __forceinline__ void kv4_load_four(float (&x)[4], const float* src) {
+    if (((uintptr_t)src & 15) == 0) { const float4 v = __ldcg(reinterpret_cast<const float4*>(src)); x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w; }
+    else { x[0] = __ldcg(src); x[1] = __ldcg(src + 1); x[2] = __ldcg(src + 2); x[3] = __ldcg(src + 3); }
+}
+// Values i..i+3 of a key or value row of head h into the cache. Eight neighbouring lanes have a group, whose largest magnitude they
+// share. turn: the position's angles, or NULL.
+__device__ __forceinline__ void kv4_write_four(const Kv4& c, float (&x)[4], bool key, int h, int r, int i, const double2* turn) {
     const int ng = c.hd / 32, lane = threadIdx.x & 31;
-    float x[4] = { __ldcg(src + i), __ldcg(src + i + 1), __ldcg(src + i + 2), __ldcg(src + i + 3) };
     if (key && turn) { kv4_turn(x[0], x[1], turn[i / 2]); kv4_turn(x[2], x[3], turn[i / 2 + 1]); }
     uint32_t m = 0;
 #pragma unroll

@@ -294,7 +294,9 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (MODE == FEW ? 3 :
             for (int e = tid; e < (r1 - r0) * 2 * (HD / 4); e += 32 * KA_WARPS) {
                 const int f = e / (HD / 4), r = r0 + f / 2, b = r - row0;
                 const bool key = f % 2 == 0;
-                kv4_write_four(p.c, (key ? p.w.k : p.w.v) + ((size_t)b * p.c.n_kv + kvh) * HD, key, kvh, r, e % (HD / 4) * 4, p.w.rotate ? turn + b * (HD / 2) : nullptr);
+                float x4[4];
+                kv4_load_four(x4, (key ? p.w.k : p.w.v) + ((size_t)b * p.c.n_kv + kvh) * HD + e % (HD / 4) * 4);
+                kv4_write_four(p.c, x4, key, kvh, r, e % (HD / 4) * 4, p.w.rotate ? turn + b * (HD / 2) : nullptr);
             }
             asm volatile("fence.proxy.async.global;" ::: "memory");                                // the bulk copies read them
         }
@@ -762,13 +764,11 @@ int kv4_attend(ibcu_ctx* ctx, const Kv4& c, float decay, const Kv4Place& at, con
     call.blocks = call.mode == WIDE ? wide_blocks : units;
     const int stages = (rows + KA_ROWS - 1) / KA_ROWS;
     int want = call.mode == WIDE ? 1 : std::max(1, (large ? 2 : 3) * ctx->sm_count / units), chunk;
-    // The last block of a tile joins its chunks if a warp of it has at most 32 to read; a launch of its own is worth it beyond (one of several thousand
-    // rows with sixteen columns rather has fewer chunks).
-    const int a_warp = (int)(std::min(columns, (long)t.cols()) + 3) / 4;
-    if (large && want > 32 / a_warp && stages <= 128) want = 32 / a_warp;
+    // The last block of a tile joins its chunks where every warp of it has one column of them to read, a launch of its own elsewhere.
+    const bool few_chunks = std::min(columns, (long)t.cols()) <= KA_WARPS;
     ka_plan(rows, want, chunk, call.chunks);
     if (at.at) call.chunks = std::min(want, stages);                                               // shorter contexts have more, shorter chunks
-    const bool by_last = call.chunks > 1 && call.chunks * a_warp <= 32;
+    const bool by_last = call.chunks > 1 && call.chunks <= 32 && few_chunks;
     const int row_blocks = (rows + 127) / 128;
     call.n_parts = c.weight && ntiles >= 16 ? std::min(std::min(ntiles, 16), std::max(1, 6 * ctx->sm_count / (row_blocks * c.n_kv))) : 1;
     auto round_up = [](size_t n) { return (n + 255) & ~(size_t)255; };
