@@ -12,25 +12,70 @@ namespace {
 // float4s, which the thread keeps between the maximum and the codes (up to QR_KEEP of them; further ones are read twice). Bound by memory: 511 rows of 14336
 // took 12 us one value at a time.
 constexpr int QR_KEEP = 8;
+__device__ __forceinline__ uint32_t size_of(const float4& v) {
+    return max(max(__float_as_uint(v.x) & 0x7FFFFFFFu, __float_as_uint(v.y) & 0x7FFFFFFFu), max(__float_as_uint(v.z) & 0x7FFFFFFFu, __float_as_uint(v.w) & 0x7FFFFFFFu));
+}
+// a token's scale and what turns its values into codes, from the bits of its largest magnitude
+__device__ __forceinline__ float token_scale(uint32_t m, float& inv) {
+    if (m < 0x0D800000u) { inv = 0.0f; return 0.0f; }         // below 2^-100: zeros
+    if (m >= 0x7F800000u) { inv = 0.0f; return __uint_as_float(0x7FFFFFFFu); }           // NaN or Inf: all results of the token are NaN
+    const float s = __fmul_rn(__uint_as_float(m), 1.0f / 127.0f);
+    inv = __fdiv_rn(1.0f, s);
+    return s;
+}
+__device__ __forceinline__ int code_of(float v, float inv) { return inv > 0.0f ? (int)rintf(__fmul_rn(v, inv)) & 255 : 0; }
+__device__ __forceinline__ uint32_t codes_of(const float4& v, float inv) { return (uint32_t)(code_of(v.x, inv) | code_of(v.y, inv) << 8 | code_of(v.z, inv) << 16 | code_of(v.w, inv) << 24); }
+
+// Rows of `n` bytes that begin anywhere, `from` apart, into rows `to` apart (a multiple of 16): TMA wants rows that start on 16 bytes.
+struct AlignJob { const uint8_t* src; uint8_t* dst; long from, to, rows; int n; };
+__device__ void align_rows(const AlignJob& j, long block, long blocks) {
+    const int per = (int)(j.to / 16);
+    for (long e = block * blockDim.x + threadIdx.x; e < j.rows * per; e += blocks * blockDim.x) {
+        const long r = e / per;
+        const int c = (int)(e % per) * 16;
+        const uint8_t* a = j.src + r * j.from + c;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (c + 16 < j.n) {                                   // aligned words and a shift; the last word is not past the row's end
+            const uint32_t* w = reinterpret_cast<const uint32_t*>((uintptr_t)a & ~(uintptr_t)3);
+            const uint32_t sh = (uint32_t)((uintptr_t)a & 3) * 8;
+            uint32_t x[5];
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = __ldcg(w + i);
+            x[4] = sh ? __ldcg(w + 4) : 0u;
+            v = make_uint4(__funnelshift_r(x[0], x[1], sh), __funnelshift_r(x[1], x[2], sh), __funnelshift_r(x[2], x[3], sh), __funnelshift_r(x[3], x[4], sh));
+        } else {
+            uint8_t b[16];
+            for (int i = 0; i < 16; i++) b[i] = c + i < j.n ? __ldcg(a + i) : (uint8_t)0;
+            memcpy(&v, b, 16);
+        }
+        *reinterpret_cast<uint4*>(j.dst + r * j.to + c) = v;
+    }
+}
+// What a call has to copy beside quantising its tokens: blocks behind the tokens' share the jobs.
+struct AlignJobs { AlignJob j[5]; int n, blocks; };
+
 template <bool VEC>
-__global__ void __launch_bounds__(512) quantize_rows_kernel(const float* __restrict__ x, int8_t* __restrict__ q, float* __restrict__ scale, int N, int ldq) {
+__global__ void __launch_bounds__(512) quantize_rows_kernel(const float* __restrict__ x, int8_t* __restrict__ q, float* __restrict__ scale, int N, int ldq, int B, const AlignJobs jobs) {
     __shared__ uint32_t red[16];
     pdl_launch_dependents();
     pdl_wait();
+    if ((int)blockIdx.x >= B) {
+        for (int i = 0; i < jobs.n; i++) align_rows(jobs.j[i], blockIdx.x - B, jobs.blocks);
+        return;
+    }
     const size_t b = blockIdx.x;
     const float* xb = x + b * N;
     int8_t* qb = q + b * ldq;
     const int tid = threadIdx.x, nth = blockDim.x, n4 = N / 4;
     const float4* x4 = reinterpret_cast<const float4*>(xb);
-    auto size4 = [](const float4& v) { return max(max(__float_as_uint(v.x) & 0x7FFFFFFFu, __float_as_uint(v.y) & 0x7FFFFFFFu), max(__float_as_uint(v.z) & 0x7FFFFFFFu, __float_as_uint(v.w) & 0x7FFFFFFFu)); };
     float4 kept[QR_KEEP];
     uint32_t m = 0;
     if (VEC) {
 #pragma unroll
         for (int u = 0; u < QR_KEEP; u++) kept[u] = tid + u * nth < n4 ? __ldcg(x4 + tid + u * nth) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int u = 0; u < QR_KEEP; u++) m = max(m, size4(kept[u]));
-        for (int i = tid + QR_KEEP * nth; i < n4; i += nth) m = max(m, size4(__ldcg(x4 + i)));
+        for (int u = 0; u < QR_KEEP; u++) m = max(m, size_of(kept[u]));
+        for (int i = tid + QR_KEEP * nth; i < n4; i += nth) m = max(m, size_of(__ldcg(x4 + i)));
     } else {
         for (int i = tid; i < N; i += nth) m = max(m, __float_as_uint(__ldcg(xb + i)) & 0x7FFFFFFFu);
     }
@@ -38,18 +83,16 @@ __global__ void __launch_bounds__(512) quantize_rows_kernel(const float* __restr
     if ((tid & 31) == 0) red[tid >> 5] = m;
     __syncthreads();
     for (int w = 0; w < nth / 32; w++) m = max(m, red[w]);
-    float s = __fmul_rn(__uint_as_float(m), 1.0f / 127.0f), inv = __fdiv_rn(1.0f, s);
-    if (m < 0x0D800000u) { s = 0.0f; inv = 0.0f; }            // below 2^-100: zeros
-    if (m >= 0x7F800000u) { s = __uint_as_float(0x7FFFFFFFu); inv = 0.0f; }      // NaN or Inf: all results of the token are NaN
-    auto code = [&](float v) { return inv > 0.0f ? (int)rintf(__fmul_rn(v, inv)) & 255 : 0; };
+    float inv;
+    const float s = token_scale(m, inv);
     if (VEC) {
-        auto put = [&](int i, const float4& v) { reinterpret_cast<uint32_t*>(qb)[i] = (uint32_t)(code(v.x) | code(v.y) << 8 | code(v.z) << 16 | code(v.w) << 24); };
+        auto put = [&](int i, const float4& v) { reinterpret_cast<uint32_t*>(qb)[i] = codes_of(v, inv); };
 #pragma unroll
         for (int u = 0; u < QR_KEEP; u++) if (tid + u * nth < n4) put(tid + u * nth, kept[u]);
         for (int i = tid + QR_KEEP * nth; i < n4; i += nth) put(i, __ldcg(x4 + i));
         for (int i = N + tid; i < ldq; i += nth) qb[i] = 0;
     } else {
-        for (int i = tid; i < ldq; i += nth) qb[i] = i < N ? (int8_t)code(__ldcg(xb + i)) : (int8_t)0;
+        for (int i = tid; i < ldq; i += nth) qb[i] = i < N ? (int8_t)code_of(__ldcg(xb + i), inv) : (int8_t)0;
     }
     if (tid == 0) scale[b] = s;
 }
@@ -294,30 +337,91 @@ __global__ void __launch_bounds__(W8_THREADS, 1) w8a8_tc_kernel(const __grid_con
     }
 }
 
-// Rows of `n` bytes that begin anywhere, `from` apart, into rows `to` apart (a multiple of 16): TMA wants rows that start on 16 bytes.
-__global__ void __launch_bounds__(256) align_rows_kernel(const uint8_t* __restrict__ src, long from, uint8_t* __restrict__ dst, long to, int n, long rows) {
+// ── few tokens ──
+// Up to four tokens are bound by the weights' bytes and, for one matrix, by latency: one launch, a warp a row, whose bytes are all on
+// their way before the launch ahead has ended; meanwhile every block quantises the tokens for itself (or copies their codes), then four products a dp4a. 4096 x 4096
+// at one token: W8F us against 10.3 for the quantiser and the tensor cores.
+constexpr int WF_WARPS = 8, WF_AHEAD = 8, WF_TOKENS = 4;
+struct WfParams { ibcu_linear_t t[4]; int n, row_start[5], N, B; const float* x; const int8_t* xq; const float* sx; };
+
+template <int B>
+__global__ void __launch_bounds__(WF_WARPS * 32) w8a8_few_kernel(const WfParams p) {
+    extern __shared__ __align__(16) int8_t codes[];           // [B][N]
+    __shared__ uint32_t red[WF_WARPS];
+    __shared__ float scale[B];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n16 = p.N / 16, rows = p.row_start[p.n], step = gridDim.x * WF_WARPS;
+    auto tensor_of = [&](int row) { int ti = 0; for (int i = 1; i < p.n; i++) if (row >= p.row_start[i]) ti = i; return ti; };
+    int row = blockIdx.x * WF_WARPS + warp;
+    uint4 w[WF_AHEAD];
+    auto fetch = [&](int first) {                             // WF_AHEAD pieces of the row a lane
+        const int ti = tensor_of(row);
+        const uint4* src = reinterpret_cast<const uint4*>((const int8_t*)p.t[ti].w + (size_t)(row - p.row_start[ti]) * p.N);
+#pragma unroll
+        for (int u = 0; u < WF_AHEAD; u++) {
+            const int i = first + lane + 32 * u;
+            w[u] = i < n16 ? ld_stream_u4(src + i) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    if (row < rows) fetch(0);
     pdl_launch_dependents();
     pdl_wait();
-    const int per = (int)(to / 16);
-    for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < rows * per; e += (long)gridDim.x * 256) {
-        const long r = e / per;
-        const int c = (int)(e % per) * 16;
-        const uint8_t* a = src + r * from + c;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (c + 16 < n) {                                     // aligned words and a shift; the last word is not past the row's end
-            const uint32_t* w = reinterpret_cast<const uint32_t*>((uintptr_t)a & ~(uintptr_t)3);
-            const uint32_t sh = (uint32_t)((uintptr_t)a & 3) * 8;
-            uint32_t x[5];
+    if (p.x) {
+        const int n4 = p.N / 4;
+        for (int b = 0; b < B; b++) {
+            const float4* x4 = reinterpret_cast<const float4*>(p.x + (size_t)b * p.N);
+            float4 kept[4];
+            uint32_t m = 0;
 #pragma unroll
-            for (int i = 0; i < 4; i++) x[i] = __ldcg(w + i);
-            x[4] = sh ? __ldcg(w + 4) : 0u;
-            v = make_uint4(__funnelshift_r(x[0], x[1], sh), __funnelshift_r(x[1], x[2], sh), __funnelshift_r(x[2], x[3], sh), __funnelshift_r(x[3], x[4], sh));
-        } else {
-            uint8_t b[16];
-            for (int i = 0; i < 16; i++) b[i] = c + i < n ? __ldcg(a + i) : (uint8_t)0;
-            memcpy(&v, b, 16);
+            for (int u = 0; u < 4; u++) kept[u] = tid + u * 256 < n4 ? __ldcg(x4 + tid + u * 256) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int u = 0; u < 4; u++) m = max(m, size_of(kept[u]));
+            for (int i = tid + 1024; i < n4; i += 256) m = max(m, size_of(__ldcg(x4 + i)));
+            m = __reduce_max_sync(0xffffffffu, m);
+            if (lane == 0) red[warp] = m;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < WF_WARPS; i++) m = max(m, red[i]);
+            float inv;
+            const float s = token_scale(m, inv);
+            uint32_t* to = reinterpret_cast<uint32_t*>(codes + (size_t)b * p.N);
+#pragma unroll
+            for (int u = 0; u < 4; u++) if (tid + u * 256 < n4) to[tid + u * 256] = codes_of(kept[u], inv);
+            for (int i = tid + 1024; i < n4; i += 256) to[i] = codes_of(__ldcg(x4 + i), inv);
+            if (tid == 0) scale[b] = s;
+            __syncthreads();
         }
-        *reinterpret_cast<uint4*>(dst + r * to + c) = v;
+    } else {
+        for (int i = tid; i < B * n16; i += 256) reinterpret_cast<uint4*>(codes)[i] = __ldcg(reinterpret_cast<const uint4*>(p.xq) + i);
+        if (tid < B) scale[tid] = __ldcg(p.sx + tid);
+        __syncthreads();
+    }
+    for (; row < rows; row += step) {
+        int sum[B] = {};
+        for (int first = 0; first < n16; first += 32 * WF_AHEAD) {
+            if (first || row != (int)(blockIdx.x * WF_WARPS + warp)) fetch(first);
+#pragma unroll
+            for (int u = 0; u < WF_AHEAD; u++) {
+                const int i = first + lane + 32 * u;
+                if (i >= n16) break;
+#pragma unroll
+                for (int b = 0; b < B; b++) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(codes + (size_t)b * p.N + 16 * i);
+                    sum[b] = __dp4a((int)w[u].x, (int)x.x, sum[b]); sum[b] = __dp4a((int)w[u].y, (int)x.y, sum[b]);
+                    sum[b] = __dp4a((int)w[u].z, (int)x.z, sum[b]); sum[b] = __dp4a((int)w[u].w, (int)x.w, sum[b]);
+                }
+            }
+        }
+        const ibcu_linear_t& t = p.t[tensor_of(row)];
+        const int r = row - p.row_start[tensor_of(row)];
+        int mine = 0;
+#pragma unroll
+        for (int b = 0; b < B; b++) { const int v = __reduce_add_sync(0xffffffffu, sum[b]); if (lane == b) mine = v; }
+        if (lane < B) {
+            const float sw = t.scales_fp32 ? reinterpret_cast<const float*>(t.scales)[r] : __half2float(reinterpret_cast<const __half*>(t.scales)[r]);
+            float* o = t.out + (size_t)lane * t.out_stride + r;
+            const float y = (float)mine * (sw * scale[lane]);
+            *o = t.epilogue == IBCU_EPI_ADD ? __ldcg(o) + y : y;
+        }
     }
 }
 
@@ -332,9 +436,30 @@ int check_call(ibcu_ctx* ctx, const ibcu_linear_t* ts, int n, int N, int B, cons
     return IBCU_OK;
 }
 
-int quantize(ibcu_ctx* ctx, const float* x, int8_t* q, float* scale, int N, int ldq, int B) {
+int quantize(ibcu_ctx* ctx, const float* x, int8_t* q, float* scale, int N, int ldq, int B, const AlignJobs& jobs) {
     const bool vec = N % 4 == 0 && ldq % 4 == 0 && ((uintptr_t)x & 15) == 0 && ((uintptr_t)q & 3) == 0;
-    return ibcu_launch(ctx, vec ? quantize_rows_kernel<true> : quantize_rows_kernel<false>, dim3(B), dim3(N > 8192 || (B < ctx->sm_count && N >= 2048) ? 512 : 256), 0, 1, true, x, q, scale, N, ldq);
+    return ibcu_launch(ctx, vec ? quantize_rows_kernel<true> : quantize_rows_kernel<false>, dim3(B + (jobs.n ? jobs.blocks : 0)), dim3(N > 8192 || (B < ctx->sm_count && N >= 2048) ? 512 : 256), 0, 1, true,
+                       x, q, scale, N, ldq, B, jobs);
+}
+
+// Few tokens: IBCU_DECLINED where the call is not one for that kernel. x: FP32 tokens, or their codes and scales. Every block quantises for itself while that is 16384 values.
+int product_few(ibcu_ctx* ctx, const ibcu_linear_t* ts, int n, const float* x, const int8_t* xq, const float* sx, int N, int B) {
+    if (B > WF_TOKENS || N % 16 || (long)B * N > (x ? 16384 : 65536) || ((uintptr_t)(x ? (const void*)x : xq) & 15)) return IBCU_DECLINED;
+    WfParams p;
+    memset(&p, 0, sizeof p);
+    for (int i = 0; i < n; i++) {
+        if ((uintptr_t)ts[i].w & 15) return IBCU_DECLINED;
+        p.t[i] = ts[i];
+        if ((long)p.row_start[i] + ts[i].M > 0x7FFF0000L) return IBCU_DECLINED;
+        p.row_start[i + 1] = p.row_start[i] + ts[i].M;
+    }
+    p.n = n; p.N = N; p.B = B; p.x = x; p.xq = xq; p.sx = sx;
+    auto kern = B == 1 ? w8a8_few_kernel<1> : B == 2 ? w8a8_few_kernel<2> : B == 3 ? w8a8_few_kernel<3> : w8a8_few_kernel<4>;
+    static SmemOptIn opt[WF_TOKENS];
+    const size_t smem = (size_t)B * N;
+    if (int rc = ibcu_allow_smem(ctx, opt[B - 1], kern, smem)) return rc;
+    const int fit = std::max(1, std::min(4, (int)(220 * 1024 / (smem + 1024))));
+    return ibcu_launch(ctx, kern, dim3(std::min((p.row_start[n] + WF_WARPS - 1) / WF_WARPS, fit * ctx->sm_count)), dim3(WF_WARPS * 32), smem, 1, true, p);
 }
 
 // How a call is cut: tokens in tiles of equal size (up to 256), and columns over S blocks where the tiles leave SMs idle.
@@ -355,7 +480,8 @@ W8Cut w8_cut(int sm_count, long row_tiles, int nkb, int B) {
     return best;
 }
 
-int product(ibcu_ctx* ctx, const ibcu_linear_t* ts, int n, const int8_t* xq, const float* sx, int N, int ldq, int B, const char* call) {
+// x: FP32 tokens, whose codes and scales go into xq (rows ldq apart) and sx first; NULL: they are there
+int product(ibcu_ctx* ctx, const ibcu_linear_t* ts, int n, const float* x, int8_t* xq, float* sx, int N, int ldq, int B, const char* call) {
     const size_t pitch = (N + 15) & ~15;
     IBCU_REQUIRE(ctx, tensor_map_encoder(), "%s: the driver has no tensor maps", call);
     // operands whose rows do not start on 16 bytes: copies whose rows do
@@ -364,16 +490,20 @@ int product(ibcu_ctx* ctx, const ibcu_linear_t* ts, int n, const int8_t* xq, con
     for (int i = 0; i < n; i++)
         if ((copy[i] = N % 16 || ((uintptr_t)ts[i].w & 15))) { at[i] = need; need += ((size_t)ts[i].M * pitch + 255) & ~(size_t)255; }
     if ((copy[4] = ldq % 16 || ((uintptr_t)xq & 15))) { at[4] = need; need += ((size_t)B * pitch + 255) & ~(size_t)255; }
+    AlignJobs jobs;
+    memset(&jobs, 0, sizeof jobs);
     if (need) {
         if (int rc = ibcu_reserve(ctx, &ctx->scratch, &ctx->scratch_bytes, need)) return rc;
+        long pieces = 0;
         for (int i = 0; i < 5; i++) {
             if (!copy[i]) continue;
             const long rows = i < 4 ? ts[i].M : B;
-            const int grid = (int)std::min((rows * (long)(pitch / 16) + 255) / 256, 16L * ctx->sm_count);
-            if (int rc = ibcu_launch(ctx, align_rows_kernel, dim3(grid), dim3(256), 0, 1, true, (const uint8_t*)(i < 4 ? ts[i].w : xq), (long)(i < 4 ? N : ldq),
-                                     (uint8_t*)ctx->scratch + at[i], (long)pitch, N, rows)) return rc;
+            jobs.j[jobs.n++] = { (const uint8_t*)(i < 4 ? ts[i].w : xq), (uint8_t*)ctx->scratch + at[i], i < 4 ? N : ldq, (long)pitch, rows, N };
+            pieces = std::max(pieces, rows * (long)(pitch / 16));
         }
+        jobs.blocks = (int)std::min((pieces + 255) / 256, 8L * ctx->sm_count);
     }
+    if (x || need) { if (int rc = quantize(ctx, x, xq, sx, N, ldq, x ? B : 0, jobs)) return rc; }
     W8Maps maps;
     W8Params p;
     memset(&p, 0, sizeof p);
@@ -412,27 +542,28 @@ extern "C" int ibcu_quantize_rows_int8(ibcu_ctx* ctx, const float* x, int8_t* q,
     IBCU_CHECK_CTX(ctx);
     IBCU_REQUIRE(ctx, x && q && scale, "ibcu_quantize_rows_int8: null pointer");
     IBCU_REQUIRE(ctx, N >= 1 && B >= 1, "ibcu_quantize_rows_int8: N=%d B=%d", N, B);
-    return quantize(ctx, x, q, scale, N, N, B);
+    AlignJobs none;
+    memset(&none, 0, sizeof none);
+    return quantize(ctx, x, q, scale, N, N, B, none);
 }
 
 extern "C" int ibcu_linear_w8a8(ibcu_ctx* ctx, const ibcu_linear_t* tensors, int n_tensors, const int8_t* xq, const float* sx, int N, int B) {
     IBCU_CHECK_CTX(ctx);
     if (int rc = check_call(ctx, tensors, n_tensors, N, B, "ibcu_linear_w8a8")) return rc;
     IBCU_REQUIRE(ctx, xq && sx, "ibcu_linear_w8a8: null pointer");
-    return product(ctx, tensors, n_tensors, xq, sx, N, N, B, "ibcu_linear_w8a8");
+    const int rc = product_few(ctx, tensors, n_tensors, nullptr, xq, sx, N, B);
+    if (rc != IBCU_DECLINED) return rc;
+    return product(ctx, tensors, n_tensors, nullptr, const_cast<int8_t*>(xq), const_cast<float*>(sx), N, N, B, "ibcu_linear_w8a8");
 }
 
 extern "C" int ibcu_linear_w8a8_fp32(ibcu_ctx* ctx, const ibcu_linear_t* tensors, int n_tensors, const float* x, int N, int B) {
     IBCU_CHECK_CTX(ctx);
     if (int rc = check_call(ctx, tensors, n_tensors, N, B, "ibcu_linear_w8a8_fp32")) return rc;
     IBCU_REQUIRE(ctx, x, "ibcu_linear_w8a8_fp32: null pointer");
+    int rc = product_few(ctx, tensors, n_tensors, x, nullptr, nullptr, N, B);
+    if (rc != IBCU_DECLINED) return rc;
     const int ldq = (N + 15) & ~15;
     const size_t qb = ((size_t)B * ldq + 255) & ~(size_t)255;
-    int rc = ibcu_reserve(ctx, &ctx->xpack, &ctx->xpack_bytes, qb + (size_t)B * sizeof(float));
-    if (rc) return rc;
-    int8_t* q = (int8_t*)ctx->xpack;
-    float* sx = (float*)((char*)ctx->xpack + qb);
-    rc = quantize(ctx, x, q, sx, N, ldq, B);
-    if (!rc) rc = product(ctx, tensors, n_tensors, q, sx, N, ldq, B, "ibcu_linear_w8a8_fp32");
-    return rc;
+    if ((rc = ibcu_reserve(ctx, &ctx->xpack, &ctx->xpack_bytes, qb + (size_t)B * sizeof(float)))) return rc;
+    return product(ctx, tensors, n_tensors, x, (int8_t*)ctx->xpack, (float*)((char*)ctx->xpack + qb), N, ldq, B, "ibcu_linear_w8a8_fp32");
 }
