@@ -122,6 +122,42 @@ struct W8Shared {
     float sx[2][256];
 };
 
+// A tile's results from tensor memory, by eight warps: this thread's output row, 32 tokens at a time or the last 16. Each warp's store of a token is 128 bytes.
+__device__ __forceinline__ void write_tile(const ibcu_linear_t& W, uint32_t tmem, int row, int tok0, int tokens, int NT, float sw, const float* sx) {
+    const int warp = threadIdx.x >> 5;
+    const bool have = row < W.M;
+    const size_t ld = (size_t)W.out_stride;
+    const uint32_t from = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    for (int c = (warp >> 2) * 32; c < NT; c += W8_OUT_WARPS * 8) {          // 32 tokens at a time, or the last 16
+        uint32_t acc[32];
+        if (NT - c >= 32) { tmem_ld32(from + c, acc); tmem_wait_ld(acc); }
+        else tmem_ld16(from + c, acc);
+        const int n = have ? min(32, tokens - c) : 0;
+        float* o = W.out + (size_t)(tok0 + c) * ld + row;
+        auto finish = [&](auto whole, auto add) {
+#pragma unroll
+            for (int u0 = 0; u0 < 32; u0 += 8) {
+                float old[8];
+#pragma unroll
+                for (int u = 0; u < 8; u++) old[u] = decltype(add)::value && (decltype(whole)::value || u0 + u < n) ? __ldcg(o + (size_t)u * ld) : 0.0f;
+                const float4 s0 = *reinterpret_cast<const float4*>(sx + c + u0), s1 = *reinterpret_cast<const float4*>(sx + c + u0 + 4);
+                const float f[8] = { s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w };
+#pragma unroll
+                for (int u = 0; u < 8; u++) {
+                    const float y = (float)(int)acc[u0 + u] * (sw * f[u]);
+                    if (decltype(whole)::value || u0 + u < n) o[(size_t)u * ld] = decltype(add)::value ? old[u] + y : y;
+                }
+                o += 8 * ld;
+                if (!decltype(whole)::value && u0 + 8 >= n) break;
+            }
+        };
+        if (W.epilogue == IBCU_EPI_ADD) { if (n == 32) finish(std::true_type(), std::true_type()); else if (n > 0) finish(std::false_type(), std::true_type()); }
+        else if (n == 32) finish(std::true_type(), std::false_type());
+        else if (n > 0) finish(std::false_type(), std::false_type());
+        __syncwarp();
+    }
+}
+
 // tokens of a tile whose sums meet in one block of S, in fours
 __host__ __device__ __forceinline__ int w8_share(int NT, int S) { return (NT / 4 + S - 1) / S * 4; }
 
@@ -153,10 +189,8 @@ __global__ void __launch_bounds__(W8_THREADS, 1) w8a8_tc_kernel(const __grid_con
 
     // Blocks at work at the same time start at different blocks of columns: those that share rows or tokens would otherwise read the same
     // lines at the same moment and queue for them. (Integer sums: the order is free.)
-    auto column = [&](int tile, int i) {
-        const int k = i + (tile / p.token_tiles + tile % p.token_tiles * 4) % nk;
-        return (k0 + (k < nk ? k : k - nk)) * 128;
-    };
+    auto turn_of = [&](int tile) { return (tile / p.token_tiles + tile % p.token_tiles * 4) % nk; };
+    auto column = [&](int turn, int i) { const int k = i + turn; return (k0 + (k < nk ? k : k - nk)) * 128; };
 
     if (warp == W8_MMA_WARP) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&sh->tmem_base)), "r"((uint32_t)p.tmem_cols) : "memory");
@@ -170,9 +204,10 @@ __global__ void __launch_bounds__(W8_THREADS, 1) w8a8_tc_kernel(const __grid_con
         const int ahead = p.early_weights && first < tiles ? min(p.stages, nk) : 0;
         if (one && ahead) {
             place(first, ti, row0, tok0);
+            const int turn = turn_of(first);
             for (int s = 0; s < ahead; s++) {
                 mbar_expect_tx(smem_u32(&sh->full[s]), (uint32_t)stage_bytes);
-                tma_load_2d(smem_u32(w8_smem + (size_t)s * stage_bytes), &maps.w[ti], column(first, s), row0, smem_u32(&sh->full[s]));
+                tma_load_2d(smem_u32(w8_smem + (size_t)s * stage_bytes), &maps.w[ti], column(turn, s), row0, smem_u32(&sh->full[s]));
             }
         }
         __syncwarp();
@@ -184,15 +219,16 @@ __global__ void __launch_bounds__(W8_THREADS, 1) w8a8_tc_kernel(const __grid_con
             long n = 0;
             for (int tile = first; tile < tiles && ok; tile += step) {
                 place(tile, ti, row0, tok0);
+                const int turn = turn_of(tile);
                 for (int i = 0; i < nk; i++, n++) {
                     const uint32_t at = smem_u32(w8_smem + (size_t)s * stage_bytes), bar = smem_u32(&sh->full[s]);
                     if (n >= ahead) {
                         ok = mbar_wait(smem_u32(&sh->empty[s]), ph, abort_flag, 1);
                         if (!ok) break;
                         mbar_expect_tx(bar, (uint32_t)stage_bytes);
-                        tma_load_2d(at, &maps.w[ti], column(tile, i), row0, bar);
+                        tma_load_2d(at, &maps.w[ti], column(turn, i), row0, bar);
                     }
-                    tma_load_2d(at + 16384, &maps.x, column(tile, i), tok0, bar);
+                    tma_load_2d(at + 16384, &maps.x, column(turn, i), tok0, bar);
                     if (++s == p.stages) { s = 0; ph ^= 1; }
                 }
             }
@@ -249,36 +285,7 @@ __global__ void __launch_bounds__(W8_THREADS, 1) w8a8_tc_kernel(const __grid_con
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (S > 1) break;                        // one tile a cluster; its parts meet below
             if (!there) continue;                    // gave up: the barrier above is still everyone's
-            const size_t ld = (size_t)W.out_stride;
-            const uint32_t from = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)((j & 1) * p.NT);
-            for (int c = (warp >> 2) * 32; c < p.NT; c += W8_OUT_WARPS * 8) {          // 32 tokens at a time, or the last 16
-                uint32_t acc[32];
-                if (p.NT - c >= 32) { tmem_ld32(from + c, acc); tmem_wait_ld(acc); }
-                else tmem_ld16(from + c, acc);
-                if (!have) continue;
-                const int n = min(32, tokens - c);
-                float* o = W.out + (size_t)(tok0 + c) * ld + row;
-                auto finish = [&](auto whole, auto add) {
-#pragma unroll
-                    for (int u0 = 0; u0 < 32; u0 += 8) {
-                        float old[8];
-#pragma unroll
-                        for (int u = 0; u < 8; u++) old[u] = decltype(add)::value && (decltype(whole)::value || u0 + u < n) ? __ldcg(o + (size_t)u * ld) : 0.0f;
-                        const float4 s0 = *reinterpret_cast<const float4*>(sx + c + u0), s1 = *reinterpret_cast<const float4*>(sx + c + u0 + 4);
-                        const float f[8] = { s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w };
-#pragma unroll
-                        for (int u = 0; u < 8; u++) {
-                            const float y = (float)(int)acc[u0 + u] * (sw * f[u]);
-                            if (decltype(whole)::value || u0 + u < n) o[(size_t)u * ld] = decltype(add)::value ? old[u] + y : y;
-                        }
-                        o += 8 * ld;
-                        if (!decltype(whole)::value && u0 + 8 >= n) break;
-                    }
-                };
-                if (W.epilogue == IBCU_EPI_ADD) { if (n == 32) finish(std::true_type(), std::true_type()); else finish(std::false_type(), std::true_type()); }
-                else if (n == 32) finish(std::true_type(), std::false_type());
-                else if (n > 0) finish(std::false_type(), std::false_type());
-            }
+            write_tile(W, tmem + (uint32_t)((j & 1) * p.NT), row, tok0, tokens, p.NT, sw, sx);
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&sh->acc_empty[j & 1]));
@@ -334,6 +341,144 @@ __global__ void __launch_bounds__(W8_THREADS, 1) w8a8_tc_kernel(const __grid_con
     if (tid == 0 && sh->abort_flag) {
         *p.err = 420 + sh->abort_flag;
         for (int i = 0; i < 1000; i++) __nanosleep(1000);      // copies still on their way into this block's shared memory land before it goes
+    }
+}
+
+// The same product by pairs of blocks (cta_group::2): 256 output rows by up to 256 tokens, each block with 128 of the rows and half of the tokens' codes in its
+// shared memory, results of its rows in its tensor memory. A block of columns is 32 KB a block instead of 48 for as many products, which the copies keep
+// ahead of (48 took 707 cycles of the copies for 524 of products). The first block issues the products; both blocks' copies report to its
+// barriers, and its commits to both.
+__global__ void __launch_bounds__(W8_THREADS, 1) w8a8_pair_kernel(const __grid_constant__ W8Maps maps, const W8Params p) {
+    extern __shared__ __align__(1024) unsigned char w8_smem[];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = blockIdx.x & 1, first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    const int tiles = p.tile_start[p.n_tensors] * p.token_tiles, nk = p.nkb, half = p.NT / 2;
+    const int stage_bytes = 16384 + half * 128;
+    W8Shared* sh = reinterpret_cast<W8Shared*>(w8_smem + (size_t)p.stages * stage_bytes);
+    volatile int* abort_flag = &sh->abort_flag;
+    if (tid == 0) {
+        for (int s = 0; s < W8_MAX_STAGES; s++) { mbar_init(smem_u32(&sh->full[s]), 1); mbar_init(smem_u32(&sh->empty[s]), 1); }
+        for (int s = 0; s < 2; s++) { mbar_init(smem_u32(&sh->acc_full[s]), 1); mbar_init(smem_u32(&sh->acc_empty[s]), 2 * W8_OUT_WARPS); }
+        mbar_init(smem_u32(&sh->drained), 1);
+        sh->abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    cluster_arrive(); cluster_wait();                // the other block runs and its barriers are there
+    auto place = [&](int tile, int& ti, int& row0, int& tok0) {
+        const int rt = tile / p.token_tiles;
+        tok0 = tile % p.token_tiles * p.NT;
+        ti = 0;
+#pragma unroll
+        for (int i = 1; i < 4; i++) if (i < p.n_tensors && rt >= p.tile_start[i]) ti = i;
+        row0 = (rt - p.tile_start[ti]) * 256 + rank * 128;
+    };
+    auto turn_of = [&](int tile) { return (tile / p.token_tiles + tile % p.token_tiles * 4) % nk; };          // see w8a8_tc_kernel
+    auto column = [&](int turn, int i) { const int k = i + turn; return (k < nk ? k : k - nk) * 128; };
+    if (warp == W8_MMA_WARP) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&sh->tmem_base)), "r"((uint32_t)p.tmem_cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        pdl_launch_dependents();                     // not before this block holds its tensor memory: see linear_tc.cu
+    }
+    if (warp == W8_TMA_WARP) {
+        const bool one = elect_one();
+        int ti, row0, tok0;
+        const int ahead = p.early_weights && first < tiles ? min(p.stages, nk) : 0;
+        if (one && ahead) {
+            place(first, ti, row0, tok0);
+            const int turn = turn_of(first);
+            for (int s = 0; s < ahead; s++) {
+                if (rank == 0) mbar_expect_tx(smem_u32(&sh->full[s]), 2u * (uint32_t)stage_bytes);
+                tma_load_2d_pair(smem_u32(w8_smem + (size_t)s * stage_bytes), &maps.w[ti], column(turn, s), row0, peer_address(smem_u32(&sh->full[s]), 0));
+            }
+        }
+        __syncwarp();
+        pdl_wait();
+        if (one) {
+            asm volatile("fence.proxy.async.global;" ::: "memory");
+            int s = 0; uint32_t ph = 1;
+            bool ok = true;
+            long n = 0;
+            for (int tile = first; tile < tiles && ok; tile += step) {
+                place(tile, ti, row0, tok0);
+                const int turn = turn_of(tile);
+                for (int i = 0; i < nk; i++, n++) {
+                    const uint32_t at = smem_u32(w8_smem + (size_t)s * stage_bytes), bar = peer_address(smem_u32(&sh->full[s]), 0);
+                    if (n >= ahead) {
+                        ok = mbar_wait(smem_u32(&sh->empty[s]), ph, abort_flag, 1);
+                        if (!ok) break;
+                        if (rank == 0) mbar_expect_tx(smem_u32(&sh->full[s]), 2u * (uint32_t)stage_bytes);
+                        tma_load_2d_pair(at, &maps.w[ti], column(turn, i), row0, bar);
+                    }
+                    tma_load_2d_pair(at + 16384, &maps.x, column(turn, i), tok0 + rank * half, bar);
+                    if (++s == p.stages) { s = 0; ph ^= 1; }
+                }
+            }
+        }
+        __syncwarp();
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    if (warp != W8_TMA_WARP) asm volatile("bar.sync 1, %0;" :: "n"(W8_THREADS - 32) : "memory");
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = warp == W8_TMA_WARP ? 0u : sh->tmem_base;
+    if (warp == W8_MMA_WARP) {
+        pdl_wait();
+        if (rank == 0 && elect_one()) {
+            // s32 accumulators, both operands signed bytes, 256 rows
+            const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(p.NT >> 3) << 17) | (16u << 24);
+            int s = 0, j = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int tile = first; tile < tiles && ok; tile += step, j++) {
+                ok = mbar_wait(smem_u32(&sh->acc_empty[j & 1]), (uint32_t)((j >> 1) & 1) ^ 1u, abort_flag, 2);
+                const uint32_t d = tmem + (uint32_t)((j & 1) * p.NT);
+                for (int i = 0; i < nk && ok; i++) {
+                    ok = mbar_wait(smem_u32(&sh->full[s]), ph, abort_flag, 3);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t at = smem_u32(w8_smem + (size_t)s * stage_bytes);
+                    const uint64_t ad = smem_desc_sw128(at), bd = smem_desc_sw128(at + 16384);
+#pragma unroll
+                    for (int m = 0; m < 4; m++) mma_i8_pair(d, ad + m * 2, bd + m * 2, idesc, (i | m) ? 1u : 0u);
+                    mma_commit_pair(smem_u32(&sh->empty[s]));
+                    if (++s == p.stages) { s = 0; ph ^= 1; }
+                }
+                if (ok) mma_commit_pair(smem_u32(&sh->acc_full[j & 1]));
+            }
+            mma_commit_pair(smem_u32(&sh->drained));
+            mbar_wait(smem_u32(&sh->drained), 0u, abort_flag, 4);              // nothing is left in the tensor pipe
+        }
+        __syncwarp();
+    } else if (warp < W8_OUT_WARPS) {
+        pdl_wait();
+        int j = 0;
+        for (int tile = first; tile < tiles; tile += step, j++) {
+            int ti, row0, tok0;
+            place(tile, ti, row0, tok0);
+            const ibcu_linear_t& W = p.t[ti];
+            const int row = row0 + (tid & 127), tokens = min(p.NT, p.B - tok0);
+            const float sw = row >= W.M ? 0.0f : W.scales_fp32 ? reinterpret_cast<const float*>(W.scales)[row] : __half2float(reinterpret_cast<const __half*>(W.scales)[row]);
+            float* sx = sh->sx[j & 1];
+            if (tid < p.NT) sx[tid] = tid < tokens ? __ldcg(p.sx + tok0 + tid) : 0.0f;
+            asm volatile("bar.sync 2, %0;" :: "n"(W8_OUT_WARPS * 32) : "memory");
+            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->acc_full[j & 1]), (uint32_t)((j >> 1) & 1), abort_flag, 5))) continue;          // gave up: the barrier above is still everyone's
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            write_tile(W, tmem + (uint32_t)((j & 1) * p.NT), row, tok0, tokens, p.NT, sw, sx);
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive_peer(peer_address(smem_u32(&sh->acc_empty[j & 1]), 0));
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (tid == 0 && sh->abort_flag) {
+        *p.err = 440 + sh->abort_flag;
+        for (int i = 0; i < 1000; i++) __nanosleep(1000);      // copies still on their way into this block's shared memory land before it goes
+    }
+    __syncthreads();
+    cluster_arrive(); cluster_wait();                // neither block's barriers or tensor memory are needed any more
+    if (warp == W8_MMA_WARP) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"((uint32_t)p.tmem_cols) : "memory");
     }
 }
 
@@ -463,9 +608,9 @@ int product_few(ibcu_ctx* ctx, const ibcu_linear_t* ts, int n, const float* x, c
 }
 
 // How a call is cut: tokens in tiles of equal size (up to 256), and columns over S blocks where the tiles leave SMs idle.
-struct W8Cut { int NT, token_tiles, S; };
-W8Cut w8_cut(int sm_count, long row_tiles, int nkb, int B) {
-    W8Cut best = { 0, 0, 1 };
+struct W8Cut { int NT, token_tiles, S, pairs; };
+W8Cut w8_cut(int sm_count, long row_tiles, long pair_tiles, int nkb, int B) {
+    W8Cut best = { 0, 0, 1, 0 };
     double least = 1e30;
     for (int n = (B + 255) / 256; n <= (B + 255) / 256 + 3; n++) {
         const int NT = ((B + n - 1) / n + 15) / 16 * 16, tt = (B + NT - 1) / NT;
@@ -476,8 +621,13 @@ W8Cut w8_cut(int sm_count, long row_tiles, int nkb, int B) {
             // Cycles: a block of columns is as long as its bytes are on their way, 70 of them a cycle (the products of 256 tokens take 524 of the 702); then
             // the results, or S blocks' sums that meet. Over 13 shapes of 8 to 511 tokens within 7 % of the best of all cuts, 2 % on the mean.
             const double t = waves * ((double)((nkb + S - 1) / S) * (16384 + 128 * NT) / 70.0 + (S > 1 ? 1800 + 24 * NT : 900 + 4 * NT));
-            if (t < least) { least = t; best = { NT, tt, S }; }
+            if (t < least) { least = t; best = { NT, tt, S, 0 }; }
         }
+        // pairs of blocks: half the tokens' codes a block, until the products are what a block of columns takes
+        const int NP = (NT + 31) / 32 * 32, tp = (B + NP - 1) / NP;
+        const double waves = (double)((pair_tiles * tp + sm_count / 2 - 1) / (sm_count / 2));
+        const double t = waves * (nkb * std::max((16384 + 64 * NP) / 70.0, 2.1 * NP) + 1200 + 4 * NP);
+        if (t < least) { least = t; best = { NP, tp, 1, 1 }; }
     }
     return best;
 }
@@ -520,20 +670,29 @@ int product(ibcu_ctx* ctx, const ibcu_linear_t* ts, int n, const float* x, int8_
     for (int i = n; i < 4; i++) maps.w[i] = maps.w[0];
     p.n_tensors = n; p.B = B; p.nkb = (N + 127) / 128; p.sx = sx; p.err = ctx->kern_err;
     const long row_tiles = p.tile_start[n];
-    const W8Cut cut = w8_cut(ctx->sm_count, row_tiles, p.nkb, B);
+    long pair_tiles = 0;
+    for (int i = 0; i < n; i++) pair_tiles += (ts[i].M + 255) / 256;
+    const W8Cut cut = w8_cut(ctx->sm_count, row_tiles, pair_tiles, p.nkb, B);
+    const bool pairs = cut.pairs;
     p.NT = cut.NT; p.token_tiles = cut.token_tiles; p.S = cut.S;
-    ok = ok && tensor_map_bytes(&maps.x, copy[4] ? (uint8_t*)ctx->scratch + at[4] : (const uint8_t*)xq, B, N, copy[4] ? (long)pitch : ldq, p.NT);
+    ok = ok && tensor_map_bytes(&maps.x, copy[4] ? (uint8_t*)ctx->scratch + at[4] : (const uint8_t*)xq, B, N, copy[4] ? (long)pitch : ldq, pairs ? p.NT / 2 : p.NT);
     IBCU_REQUIRE(ctx, ok, "%s: no tensor map for N=%d", call, N);
-    const int stage = 16384 + p.NT * 128, room = 227 * 1024 - (int)sizeof(W8Shared) - 1024;
+    if (pairs) for (int i = 0; i < n; i++) p.tile_start[i + 1] = p.tile_start[i] + (ts[i].M + 255) / 256;
+    const int stage = 16384 + (pairs ? p.NT / 2 : p.NT) * 128, room = 227 * 1024 - (int)sizeof(W8Shared) - 1024;
     p.stages = std::min(std::min(W8_MAX_STAGES, room / stage), std::max(2, (p.nkb + p.S - 1) / p.S * 2));
     size_t rings = (size_t)p.stages * stage;
     const size_t meet = p.S > 1 ? (size_t)p.S * w8_share(p.NT, p.S) * 512 : 0;
     if (rings < meet) { p.stages = (int)((meet + stage - 1) / stage); rings = (size_t)p.stages * stage; }
     for (p.tmem_cols = 32; p.tmem_cols < 2 * p.NT; p.tmem_cols *= 2) {}
-    const long tiles = row_tiles * p.token_tiles;
+    const long tiles = (pairs ? pair_tiles : row_tiles) * p.token_tiles;
     const int grid = p.S > 1 ? (int)tiles * p.S : (int)std::min(tiles, (long)ctx->sm_count);
-    static SmemOptIn opt;
     const size_t smem = rings + sizeof(W8Shared);
+    if (pairs) {
+        static SmemOptIn opt_pair;
+        if (int rc = ibcu_allow_smem(ctx, opt_pair, w8a8_pair_kernel, smem)) return rc;
+        return ibcu_launch(ctx, w8a8_pair_kernel, dim3(2 * (int)std::min(tiles, (long)ctx->sm_count / 2)), dim3(W8_THREADS), smem, 2, true, maps, p);
+    }
+    static SmemOptIn opt;
     if (int rc = ibcu_allow_smem(ctx, opt, w8a8_tc_kernel, smem)) return rc;
     return ibcu_launch(ctx, w8a8_tc_kernel, dim3(grid), dim3(W8_THREADS), smem, p.S, true, maps, p);
 }
