@@ -156,6 +156,14 @@ int  ib_b200_model_set_norms(ib_b200_model* m, int layer, const uint16_t* input_
 int  ib_b200_model_set_embedding(ib_b200_model* m, const void* embed, const uint16_t* embed_scale, const uint16_t* final_norm);
 int  ib_b200_model_set_kv(ib_b200_model* m, int layer, const float* k, const float* v, int n_pos);
 int  ib_b200_model_get_kv(ib_b200_model* m, int layer, float* k, float* v, int n_pos);
+/* Holds the model's KV cache in 4 bits (ibcu_kv4_t: 4.5 bits a value instead of 32) from here on; what the FP32 cache held goes with it.
+ * weights != 0: the attention that every row draws is summed up for ib_b200_model_evict. Needs head_dim 32, 64, 96, 128, 192 or
+ * 256. ib_b200_model_fill_random, _set_kv and _get_kv work on the values that the cache holds. The step's answers are those of attention over them. */
+int  ib_b200_model_kv4(ib_b200_model* m, int weights);
+/* Cuts the 4-bit cache, which holds positions up to n_pos - 1, to `keep` rows in every layer and KV head (ibcu_kv4_evict: the first
+ * `sink` and last `recent` stay, of the others those that drew most attention). Steps go on at positions n_pos and up; max_ctx bounds the
+ * rows, no longer the positions. Rows are then no positions any more: _set_kv and _get_kv count rows. */
+int  ib_b200_model_evict(ib_b200_model* m, int n_pos, int keep, int sink, int recent);
 /* B consecutive positions pos0.. of one sequence (B == 1: forward_single_ex, src/forward.c:518-664;
  * B > 1: forward_batch, :682-846). tokens and logits are host arrays; logits [B*vocab] may be NULL.
  * The launch sequence is captured into a CUDA graph per batch size on first use and replayed for every

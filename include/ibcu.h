@@ -290,6 +290,11 @@ int ibcu_attention_kv4(ibcu_ctx* ctx, const ibcu_kv4_t* cache, const float* q, f
  * attention over rows 0..row0+b. q, k and v hold the raw projections and are left as they are. */
 int ibcu_attention_decode_kv4(ibcu_ctx* ctx, const ibcu_kv4_t* cache, const float* q, const float* k, const float* v, float* out,
                               int n_heads, int row0, int pos0, int B, float theta);
+/* The same step with its place read from device memory when the kernels run: at_dev = { row0, pos0 }. Grid and scratch are sized for
+ * max_rows, so that a launch captured into a CUDA graph serves every step (row0 + B <= max_rows). A place outside the cache writes nothing;
+ * the next ibcu_sync returns IBCU_ERR_PARAM. */
+int ibcu_attention_decode_kv4_at(ibcu_ctx* ctx, const ibcu_kv4_t* cache, const float* q, const float* k, const float* v, float* out,
+                                 int n_heads, const int* at_dev, int B, float theta);
 /* Cuts rows 0..rows-1 of a cache down to `keep` of them, for every KV head by its own weights: the first `sink` and the last
  * `recent` rows stay, and of the others those with the largest weight (equal weights: the lower row; NaN counts as less than any
  * number). Kept rows go to rows 0..keep-1 of dst in their old order, weights with them. dst may be the same cache (cut in place),

@@ -105,6 +105,8 @@ IBCU_SYMBOLS = {
     "ibcu_attention_kv4": (C.c_int, [C.c_void_p, C.POINTER(Kv4T), C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int]),
     "ibcu_attention_decode_kv4": (C.c_int, [C.c_void_p, C.POINTER(Kv4T), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                             C.c_int, C.c_int, C.c_int, C.c_int, C.c_float]),
+    "ibcu_attention_decode_kv4_at": (C.c_int, [C.c_void_p, C.POINTER(Kv4T), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                               C.c_int, C.c_void_p, C.c_int, C.c_float]),
     "ibcu_kv4_evict": (C.c_int, [C.c_void_p, C.POINTER(Kv4T), C.POINTER(Kv4T), C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p]),
     "ibcu_int4g_matmul_fp32": (C.c_int, [C.c_void_p, C.POINTER(Int4gT), C.c_void_p, C.c_void_p, C.c_float]),
     "ibcu_pq_lm_head_topk": (C.c_int, [C.c_void_p, C.POINTER(PqT), C.c_void_p, C.c_int, C.c_void_p, C.c_void_p]),
@@ -244,6 +246,8 @@ HOST_SYMBOLS = {
     "ib_b200_model_set_embedding": (_i, [_vp, _vp, _vp, _vp]),
     "ib_b200_model_set_kv": (_i, [_vp, _i, _vp, _vp, _i]),
     "ib_b200_model_get_kv": (_i, [_vp, _i, _vp, _vp, _i]),
+    "ib_b200_model_kv4": (_i, [_vp, _i]),
+    "ib_b200_model_evict": (_i, [_vp, _i, _i, _i, _i]),
     "ib_b200_forward_step": (_i, [_vp, _vp, _i, _i, _vp]),
     "ib_b200_forward_step_last": (_i, [_vp, _vp, _i, _i, _vp]),
     "ib_b200_forward_step_device": (_i, [_vp, _i, _i]),

@@ -394,6 +394,17 @@ extern "C" int ibcu_attention_decode_kv4(ibcu_ctx* ctx, const ibcu_kv4_t* cache,
     return kv4_attend(ctx, planes(cache), cache->decay, Kv4Place{ row0, pos0, nullptr }, q, k, v, out, n_heads, B, log2_of(theta), theta > 0.0f);
 }
 
+extern "C" int ibcu_attention_decode_kv4_at(ibcu_ctx* ctx, const ibcu_kv4_t* cache, const float* q, const float* k, const float* v, float* out,
+                                            int n_heads, const int* at_dev, int B, float theta) {
+    IBCU_CHECK_CTX(ctx);
+    if (int rc = check_cache(ctx, cache, "ibcu_attention_decode_kv4_at")) return rc;
+    IBCU_REQUIRE(ctx, q && k && v && out && at_dev, "ibcu_attention_decode_kv4_at: null pointer");
+    if (int rc = check_rows(ctx, cache, 0, B, "ibcu_attention_decode_kv4_at")) return rc;
+    if (int rc = check_heads(ctx, cache, n_heads, B, "ibcu_attention_decode_kv4_at")) return rc;
+    if (int rc = check_rotation(ctx, 0, B, theta, "ibcu_attention_decode_kv4_at")) return rc;
+    return kv4_attend(ctx, planes(cache), cache->decay, Kv4Place{ 0, 0, at_dev }, q, k, v, out, n_heads, B, log2_of(theta), theta > 0.0f);
+}
+
 extern "C" int ibcu_kv4_evict(ibcu_ctx* ctx, const ibcu_kv4_t* src, const ibcu_kv4_t* dst, int rows, int keep, int sink, int recent, int32_t* kept) {
     IBCU_CHECK_CTX(ctx);
     if (int rc = check_cache(ctx, src, "ibcu_kv4_evict")) return rc;

@@ -534,9 +534,7 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (MODE == FEW ? 3 :
         }
         __syncthreads();
         if (tid == 0) give_up();
-        return;
-    }
-
+    } else {
     // the four warps' results meet in the rings: [warp][column][value], and maxima and sums
 #pragma unroll
     for (int n = 0; n < NC; n++) if (t == 0) ml[warp][g + 8 * n] = make_float2(m[n], l[n]);
@@ -589,6 +587,7 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (MODE == FEW ? 3 :
             if (tid == 0) p.arrived[unit] = 0;
             join_by_last(p, unit, n_chunks);
         }
+    }
     }
 }
 

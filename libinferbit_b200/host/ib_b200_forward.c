@@ -23,7 +23,7 @@ typedef struct {
     int row0, rows;           /* this rank's slice */
 } lin;
 
-typedef struct { lin t[7]; void *in_norm, *post_norm, *k_cache, *v_cache; } layer;
+typedef struct { lin t[7]; void *in_norm, *post_norm, *k_cache, *v_cache; ibcu_kv4_t kv4; } layer;
 
 struct ib_b200_model {
     ibcu_ctx* ctx;
@@ -37,7 +37,9 @@ struct ib_b200_model {
     float *x, *xb, *q, *k, *v, *att, *hg, *hu, *logits;
     float* amax;              /* [BMAX][AMAX_PARTS] pieces of max|silu(gate)*up| per position */
     int32_t* tokens;
-    int32_t* pos_dev;         /* position of the first token of the step, read by the attention kernels */
+    int32_t* pos_dev;         /* position of the first token of the step, read by the attention kernels; 4-bit cache: its row, then its position */
+    int kv4;                  /* the cache is held in 4 bits */
+    int evicted, next_pos;    /* 4-bit cache: row = position - evicted; positions below next_pos are cut rows now */
     void* pin;                /* pinned staging for tokens / logits */
     size_t pin_bytes;
     struct { int B, last_only, id; } graphs[MAX_GRAPHS];
@@ -127,6 +129,7 @@ void ib_b200_model_free(ib_b200_model* m) {
         layer* y = &m->L[l];
         for (int i = 0; i < 7; i++) { ibcu_free(m->ctx, y->t[i].w); ibcu_free(m->ctx, y->t[i].scale); }
         ibcu_free(m->ctx, y->in_norm); ibcu_free(m->ctx, y->post_norm); ibcu_free(m->ctx, y->k_cache); ibcu_free(m->ctx, y->v_cache);
+        ibcu_free(m->ctx, y->kv4.k); ibcu_free(m->ctx, y->kv4.v); ibcu_free(m->ctx, y->kv4.scale); ibcu_free(m->ctx, y->kv4.weight);
     }
     ibcu_free(m->ctx, m->head.w); ibcu_free(m->ctx, m->head.scale);
     void* v[] = { m->embed, m->embed_scale, m->final_norm, m->x, m->xb, m->q, m->k, m->v, m->att, m->hg, m->hu, m->logits, m->tokens, m->amax, m->pos_dev };
@@ -140,6 +143,64 @@ size_t ib_b200_model_weight_bytes(const ib_b200_model* m) { return m ? m->weight
 void*  ib_b200_model_tokens(ib_b200_model* m) { return m ? m->tokens : NULL; }
 float* ib_b200_model_logits(ib_b200_model* m) { return m ? m->logits : NULL; }
 void   ib_b200_model_use_graph(ib_b200_model* m, int on) { if (m) m->use_graph = on ? 1 : 0; }
+
+int ib_b200_model_kv4(ib_b200_model* m, int weights) {
+    if (!m || m->kv4) return IBCU_ERR_PARAM;
+    const ib_b200_model_cfg* c = &m->c;
+    const int hd = c->head_dim, max_rows = (c->max_ctx + 7) / 8 * 8;
+    if (hd % 32 || hd > 256 || hd == 160 || hd == 224) return IBCU_ERR_PARAM;
+    int rc = ibcu_sync(m->ctx);
+    for (int g = 0; g < m->n_graphs; g++) ibcu_graph_destroy(m->ctx, m->graphs[g].id);        /* they read and write the FP32 cache */
+    m->n_graphs = 0;
+    const size_t rows = (size_t)c->n_kv_heads * max_rows;
+    for (int l = 0; l < c->n_layers && !rc; l++) {
+        ibcu_kv4_t* t = &m->L[l].kv4;
+        t->n_kv_heads = c->n_kv_heads; t->head_dim = hd; t->max_rows = max_rows; t->decay = 1.0f;
+        rc = dmalloc(m, (void**)&t->k, rows * hd / 2);
+        if (!rc) rc = dmalloc(m, (void**)&t->v, rows * hd / 2);
+        if (!rc) rc = dmalloc(m, (void**)&t->scale, rows * hd / 8);
+        if (!rc && weights) rc = dmalloc(m, (void**)&t->weight, rows * sizeof(float));
+    }
+    if (rc) {                                                 /* the FP32 cache stays */
+        for (int l = 0; l < c->n_layers; l++) {
+            ibcu_kv4_t* t = &m->L[l].kv4;
+            ibcu_free(m->ctx, t->k); ibcu_free(m->ctx, t->v); ibcu_free(m->ctx, t->scale); ibcu_free(m->ctx, t->weight);
+            memset(t, 0, sizeof *t);
+        }
+        return rc;
+    }
+    for (int l = 0; l < c->n_layers; l++) {
+        layer* y = &m->L[l];
+        ibcu_free(m->ctx, y->k_cache); ibcu_free(m->ctx, y->v_cache);
+        y->k_cache = y->v_cache = NULL;
+    }
+    m->kv4 = 1;
+    return 0;
+}
+
+int ib_b200_model_evict(ib_b200_model* m, int n_pos, int keep, int sink, int recent) {
+    if (!m || !m->kv4 || n_pos < m->next_pos || n_pos - m->evicted < 1 || n_pos - m->evicted > m->c.max_ctx) return IBCU_ERR_PARAM;
+    const int rows = n_pos - m->evicted;
+    if (keep < 1 || keep > rows || sink < 0 || recent < 0 || sink > keep - recent) return IBCU_ERR_PARAM;
+    int rc = 0;
+    for (int l = 0; l < m->c.n_layers && !rc; l++) rc = ibcu_kv4_evict(m->ctx, &m->L[l].kv4, &m->L[l].kv4, rows, keep, sink, recent, NULL);
+    if (!rc) { m->evicted = n_pos - keep; m->next_pos = n_pos; }
+    return rc;
+}
+
+/* n rows of FP32 keys and values, rotated already, into a layer's 4-bit cache: from the host, or (host pointers NULL) made by the counter-based generator */
+static int kv4_put(ib_b200_model* m, int l, const float* k, const float* v, int n, uint64_t seed) {
+    const size_t kv = (size_t)m->c.n_kv_heads * m->c.head_dim, bytes = (size_t)n * kv * sizeof(float);
+    float* d[2] = { NULL, NULL };
+    int rc = dmalloc(m, (void**)&d[0], bytes);
+    if (!rc) rc = dmalloc(m, (void**)&d[1], bytes);
+    for (int i = 0; i < 2 && !rc; i++)
+        rc = k ? ibcu_memcpy_h2d(m->ctx, d[i], i ? v : k, bytes) : ibcu_fill_hash_f32_normal_at(m->ctx, d[i], (size_t)n * kv, seed + (uint64_t)i, 0.0f, 1.0f, 0);
+    if (!rc) rc = ibcu_kv4_write(m->ctx, &m->L[l].kv4, d[0], d[1], 0, 0, n, 0.0f);
+    if (!rc) rc = ibcu_sync(m->ctx);
+    ibcu_free(m->ctx, d[0]); ibcu_free(m->ctx, d[1]);
+    return rc;
+}
 
 static lin* pick(ib_b200_model* m, int layer_i, int which) {
     if (which == IB_B200_HEAD) return &m->head;
@@ -173,8 +234,9 @@ int ib_b200_model_fill_random(ib_b200_model* m, uint64_t seed, int kv_fill) {
             rc = ibcu_fill_hash_fp16_uniform(m->ctx, y->in_norm, (size_t)H, ls + 1, 0.9f, 1.1f);
             if (!rc) rc = ibcu_fill_hash_fp16_uniform(m->ctx, y->post_norm, (size_t)H, ls + 2, 0.9f, 1.1f);
             /* earlier positions of the KV cache: bell-shaped values of unit variance */
-            if (!rc && kv_fill) rc = ibcu_fill_hash_f32_normal_at(m->ctx, (float*)y->k_cache, (size_t)kv_fill * kv, ls + 3, 0.0f, 1.0f, 0);
-            if (!rc && kv_fill) rc = ibcu_fill_hash_f32_normal_at(m->ctx, (float*)y->v_cache, (size_t)kv_fill * kv, ls + 4, 0.0f, 1.0f, 0);
+            if (!rc && kv_fill && m->kv4) rc = kv4_put(m, l, NULL, NULL, kv_fill, ls + 3);
+            if (!rc && kv_fill && !m->kv4) rc = ibcu_fill_hash_f32_normal_at(m->ctx, (float*)y->k_cache, (size_t)kv_fill * kv, ls + 3, 0.0f, 1.0f, 0);
+            if (!rc && kv_fill && !m->kv4) rc = ibcu_fill_hash_f32_normal_at(m->ctx, (float*)y->v_cache, (size_t)kv_fill * kv, ls + 4, 0.0f, 1.0f, 0);
         }
     }
     uint64_t es = seed * 104729ull;
@@ -231,6 +293,7 @@ int ib_b200_model_set_embedding(ib_b200_model* m, const void* e, const uint16_t*
 }
 int ib_b200_model_set_kv(ib_b200_model* m, int l, const float* k, const float* v, int n) {
     if (!m || !k || !v || l < 0 || l >= m->c.n_layers || n < 0 || n > m->c.max_ctx) return IBCU_ERR_PARAM;
+    if (m->kv4) return n ? kv4_put(m, l, k, v, n, 0) : 0;
     const size_t b = (size_t)n * m->c.n_kv_heads * m->c.head_dim * sizeof(float);
     int rc = ibcu_memcpy_h2d(m->ctx, m->L[l].k_cache, k, b);
     if (!rc) rc = ibcu_memcpy_h2d(m->ctx, m->L[l].v_cache, v, b);
@@ -240,6 +303,17 @@ int ib_b200_model_set_kv(ib_b200_model* m, int l, const float* k, const float* v
 int ib_b200_model_get_kv(ib_b200_model* m, int l, float* k, float* v, int n) {
     if (!m || !k || !v || l < 0 || l >= m->c.n_layers || n < 0 || n > m->c.max_ctx) return IBCU_ERR_PARAM;
     const size_t b = (size_t)n * m->c.n_kv_heads * m->c.head_dim * sizeof(float);
+    if (m->kv4) {
+        float* d[2] = { NULL, NULL };
+        int rc = n ? dmalloc(m, (void**)&d[0], b) : 0;
+        if (!rc && n) rc = dmalloc(m, (void**)&d[1], b);
+        if (!rc && n) rc = ibcu_kv4_read(m->ctx, &m->L[l].kv4, d[0], d[1], 0, n);
+        if (!rc && n) rc = ibcu_memcpy_d2h(m->ctx, k, d[0], b);
+        if (!rc && n) rc = ibcu_memcpy_d2h(m->ctx, v, d[1], b);
+        if (!rc) rc = ibcu_sync(m->ctx);
+        ibcu_free(m->ctx, d[0]); ibcu_free(m->ctx, d[1]);
+        return rc;
+    }
     int rc = ibcu_memcpy_d2h(m->ctx, k, m->L[l].k_cache, b);
     if (!rc) rc = ibcu_memcpy_d2h(m->ctx, v, m->L[l].v_cache, b);
     if (!rc) rc = ibcu_sync(m->ctx);
@@ -289,7 +363,8 @@ static int issue(ib_b200_model* m, int pos0, int B, int head_last) {
         float* qkv_out[3] = { m->q, m->k, m->v };
         rc = linear_group(m, qkv, qkv_out, 3, m->x, H, B, &n1, IBCU_EPI_STORE);
         /* RoPE, the KV-cache write and the attention itself are one step on the device */
-        if (!rc) rc = m->dyn_pos
+        if (!rc && m->kv4) rc = ibcu_attention_decode_kv4_at(ctx, &y->kv4, m->q, m->k, m->v, m->att, c->n_heads, m->pos_dev, B, c->theta);
+        else if (!rc) rc = m->dyn_pos
             ? ibcu_attention_decode_at(ctx, m->q, m->k, m->v, (float*)y->k_cache, (float*)y->v_cache, m->att,
                                        c->n_heads, c->n_kv_heads, c->head_dim, m->pos_dev, c->max_ctx, B, c->theta)
             : ibcu_attention_decode(ctx, m->q, m->k, m->v, (float*)y->k_cache, (float*)y->v_cache, m->att,
@@ -319,10 +394,11 @@ static int issue(ib_b200_model* m, int pos0, int B, int head_last) {
 }
 
 static int step_device(ib_b200_model* m, int pos0, int B, int head_last) {
-    if (!m || B < 1 || B > BMAX || pos0 < 0 || pos0 + B > m->c.max_ctx) return IBCU_ERR_PARAM;   /* src/forward.c:696-699, 857-862 */
-    int rc = ibcu_store_i32(m->ctx, m->pos_dev, pos0);
+    if (!m || B < 1 || B > BMAX || pos0 < 0 || pos0 < m->next_pos || pos0 - m->evicted > m->c.max_ctx - B) return IBCU_ERR_PARAM;   /* src/forward.c:696-699, 857-862 */
+    int rc = ibcu_store_i32(m->ctx, m->pos_dev, pos0 - m->evicted);
+    if (!rc && m->kv4) rc = ibcu_store_i32(m->ctx, m->pos_dev + 1, pos0);
     if (rc) return rc;
-    if (!m->use_graph || !m->dyn_pos) return issue(m, pos0, B, head_last);
+    if (!m->use_graph || (!m->dyn_pos && !m->kv4)) return issue(m, pos0, B, head_last);
     for (int g = 0; g < m->n_graphs; g++)
         if (m->graphs[g].B == B && m->graphs[g].last_only == head_last) return ibcu_graph_launch(m->ctx, m->graphs[g].id);
     /* first use of this batch size: run once eagerly (sizes scratch), then capture for replay */

@@ -34,6 +34,7 @@ def test_caches(bad):
     assert refused(lib.ibcu_kv4_read, t, P, P, 0, 1)
     assert refused(lib.ibcu_attention_kv4, t, P, P, 4, 0, 1)
     assert refused(lib.ibcu_attention_decode_kv4, t, P, P, P, P, 4, 0, 0, 1, 10000.0)
+    assert refused(lib.ibcu_attention_decode_kv4_at, t, P, P, P, P, 4, P, 1, 10000.0)
     assert refused(lib.ibcu_kv4_evict, t, good, 8, 4, 0, 0, None) and refused(lib.ibcu_kv4_evict, good, t, 8, 4, 0, 0, None)
 
 
@@ -83,3 +84,13 @@ def test_evictions_between_unlike_caches():
     assert refused(lib.ibcu_kv4_evict, cache(), cache(weight=P), 8, 4, 0, 0, None)                    # no weights to go by
     assert refused(lib.ibcu_kv4_evict, cache(weight=P), cache(n_kv_heads=1), 8, 4, 0, 0, None)
     assert refused(lib.ibcu_kv4_evict, cache(weight=P), cache(head_dim=32), 8, 4, 0, 0, None)
+
+
+def test_evictions_into_a_cache_that_shares_some_planes():
+    assert refused(lib.ibcu_kv4_evict, cache(weight=P), cache(weight=P, k=8 * P), 8, 4, 0, 0, None)
+    assert refused(lib.ibcu_kv4_evict, cache(weight=P), cache(weight=P, max_rows=32), 8, 4, 0, 0, None)
+
+
+@pytest.mark.parametrize("heads,at,B,theta", [(4, None, 1, 1.0), (4, P, 65, 1.0), (4, P, 0, 1.0), (3, P, 1, 1.0), (4, P, 1, -1.0)])
+def test_places_on_the_device(heads, at, B, theta):
+    assert refused(lib.ibcu_attention_decode_kv4_at, cache(), P, P, P, P, heads, at, B, theta)

@@ -248,3 +248,58 @@ def test_prompt_then_eviction_then_decode(backend):
     assert np.all(np.abs(after[3][:, :keep + 3] - total) <= 1e-5 * total + 1e-9)
     for a, b in zip(after[:3], held[:3]):
         assert np.array_equal(raw(a[:, :keep + 3]), raw(b))
+
+
+@pytest.mark.parametrize("n_heads,n_kv,hd,B,max_rows", [(32, 8, 128, 1, 1024), (8, 1, 64, 1, 4096), (16, 4, 64, 6, 600), (32, 8, 128, 40, 256), (32, 8, 128, 200, 512)])
+def test_captured_at_a_device_place(backend, n_heads, n_kv, hd, B, max_rows):
+    """One captured step serves every place: from an empty cache to a full one, rows and positions apart, weights summed up; the same as
+    the launch for one place. A larger call in between makes the scratch grow, which the graph must survive."""
+    import ctypes as C
+    be, rng = backend, np.random.default_rng(B + hd)
+    theta = 10000.0
+    planes = _kv4.random_planes(rng, n_kv, hd, max_rows, max_rows)
+    w0 = rng.uniform(0, 1, (n_kv, max_rows)).astype(np.float32)
+    draw = lambda heads: rng.standard_normal((B, heads * hd), dtype=np.float32)
+    q, k, v = draw(n_heads), draw(n_kv), draw(n_kv)
+    d, o, at = [be.upload(x) for x in (q, k, v)], be.alloc(q.nbytes), be.upload(np.zeros(2, np.int32))
+    t = put(be, *planes, weight=w0)
+    call = lambda: be._check(be.lib.ibcu_attention_decode_kv4_at(be.ctx, t, *(x.ptr for x in d), o.ptr, n_heads, at.ptr, B, theta))
+    call(); be.sync()
+    gid = C.c_int()
+    be._check(be.lib.ibcu_graph_begin(be.ctx)); call(); be._check(be.lib.ibcu_graph_end(be.ctx, C.byref(gid)))
+    try:
+        for i, (row0, pos0) in enumerate([(0, 0), (5, 9000), (max_rows // 2 + 3, max_rows // 2 + 3), (max_rows - B, 77)]):
+            for b, a in zip(t._keep, planes):
+                be.write(b, a.view(np.uint16) if a.dtype == np.float16 else a)
+            be.write(t._keep[3], w0)
+            be.write(at, np.array([row0, pos0], np.int32))
+            if i == 2:
+                big = put(be, *_kv4.random_planes(rng, 8, 128, 2000, 2000), weight=np.zeros((8, 2000)))
+                x = be.upload(rng.standard_normal((300, 32 * 128), dtype=np.float32))
+                be._check(be.lib.ibcu_attention_kv4(be.ctx, big, x.ptr, be.alloc(300 * 32 * 128 * 4).ptr, 32, 1700, 300))
+            be._check(be.lib.ibcu_graph_launch(be.ctx, gid)); be.sync()
+            got, after = be.download(o, np.float32, q.size).reshape(q.shape), get(be, t)
+            held = [p.copy() for p in planes]
+            kc, ks = _kv4.quantise(rows_of(_kv4.rotate(k, n_kv, pos0, theta).astype(np.float32), n_kv))
+            vc, vs = _kv4.quantise(rows_of(v, n_kv))
+            new = slice(row0, row0 + B)
+            held[0][:, new], held[1][:, new], held[2][:, new] = _kv4.pack(kc, True), _kv4.pack(vc, False), np.concatenate([ks, vs], -1)
+            for a, b in zip(after, held):
+                assert np.array_equal(raw(a), raw(b))
+            R = row0 + B
+            want, weight, tol, wtol = _kv4.attention(_kv4.rotate(q, n_heads, pos0, theta).astype(np.float32).astype(np.float64), _kv4.plane_values(*(h[:, :R] for h in held)), n_heads, row0)
+            assert np.all(np.abs(got - want) <= tol), (row0, np.max(np.abs(got - want) / tol))
+            full = weight + np.where(np.arange(R) < row0, w0[:, :R], 0)
+            assert np.all(np.abs(after[3][:, :R] - full) <= wtol + 3 * 2.0 ** -24 * full)
+            assert np.array_equal(after[3][:, R:], w0[:, R:])
+        # a place outside the cache writes nothing and is reported
+        for row0, pos0 in ((max_rows - B + 1, 0), (-1, 0), (0, -5)):
+            before = get(be, t)
+            be.write(at, np.array([row0, pos0], np.int32))
+            be._check(be.lib.ibcu_graph_launch(be.ctx, gid))
+            assert be.lib.ibcu_sync(be.ctx) == -1 and b"outside the cache" in be.lib.ibcu_last_error(be.ctx)
+            be.lib.ibcu_clear_error(be.ctx)
+            for a, b in zip(get(be, t), before):
+                assert np.array_equal(raw(a), raw(b))
+    finally:
+        be._check(be.lib.ibcu_graph_destroy(be.ctx, gid))
