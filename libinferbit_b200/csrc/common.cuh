@@ -37,7 +37,6 @@ struct ibcu_ctx {
     void*  xpack;      size_t xpack_bytes;      // activation limbs + per-slice scales and limb sums of the current linear call
     void*  scratch;    size_t scratch_bytes;    // partial sums (split-K slices, attention chunks, k-means per-block partials)
     void*  pq_acc;     size_t pq_acc_bytes;     // PQ matvec: arrival counters + fixed-point row accumulators, zero between calls
-    void*  kv4_arrived; size_t kv4_arrived_bytes; // 4-bit cache: chunks of a tile that are done, zero between calls
     void*  retired[IBCU_MAX_RETIRED]; int n_retired;   // outgrown scratch that an instantiated graph may still use
     cudaEvent_t events[IBCU_MAX_EVENTS];
     cudaGraphExec_t graphs[IBCU_MAX_GRAPHS];
@@ -118,9 +117,6 @@ constexpr int IBCU_DECLINED = 1;
 // holds instantiated graphs the outgrown buffer is kept (their kernels carry its address) until the
 // last graph is destroyed.
 int ibcu_reserve(ibcu_ctx* ctx, void** buf, size_t* have, size_t want);
-
-// The same for buffers that the kernels leave zeroed: zero when they are new.
-int ibcu_reserve_zeroed(ibcu_ctx* ctx, void** buf, size_t* have, size_t want);
 
 // Opt `kernel` in to `smem` bytes of dynamic shared memory; `opt` is that kernel's own, static at the place of the launch.
 template <typename K>

@@ -37,13 +37,6 @@ int ibcu_reserve(ibcu_ctx* ctx, void** buf, size_t* have, size_t want) {
     return IBCU_OK;
 }
 
-int ibcu_reserve_zeroed(ibcu_ctx* ctx, void** buf, size_t* have, size_t want) {
-    if (*have >= want) return IBCU_OK;
-    if (int rc = ibcu_reserve(ctx, buf, have, want < 4096 ? 4096 : want)) return rc;
-    IBCU_CUDA(ctx, cudaMemsetAsync(*buf, 0, *have, ctx->stream));
-    return IBCU_OK;
-}
-
 extern "C" int ibcu_device_count(void) {
     int n = 0;
     if (cudaGetDeviceCount(&n) != cudaSuccess) { cudaGetLastError(); return 0; }
@@ -94,7 +87,6 @@ extern "C" void ibcu_ctx_destroy(ibcu_ctx* ctx) {
     if (ctx->xpack) cudaFree(ctx->xpack);
     if (ctx->scratch) cudaFree(ctx->scratch);
     if (ctx->pq_acc) cudaFree(ctx->pq_acc);
-    if (ctx->kv4_arrived) cudaFree(ctx->kv4_arrived);
     if (ctx->kern_err) cudaFreeHost(ctx->kern_err);
     if (ctx->spin_flag) cudaFreeHost(ctx->spin_flag);
     cudaStreamDestroy(ctx->stream);
@@ -170,7 +162,6 @@ static int ibcu_collect_kernel_errors(ibcu_ctx* ctx) {
         const int e = *(volatile int*)ctx->kern_err;
         *(volatile int*)ctx->kern_err = 0;
         if (e >= IBCU_PQ_TC_ERR && e < IBCU_PQ_TC_ERR + 100 && ctx->pq_acc) IBCU_CUDA(ctx, cudaMemsetAsync(ctx->pq_acc, 0, ctx->pq_acc_bytes, ctx->stream));
-        if (e == IBCU_KV4_WAIT_ERR && ctx->kv4_arrived) IBCU_CUDA(ctx, cudaMemsetAsync(ctx->kv4_arrived, 0, ctx->kv4_arrived_bytes, ctx->stream));
         if (e == IBCU_KV4_PLACE_ERR) return ibcu_fail(ctx, IBCU_ERR_PARAM, "a row or position read on the device lies outside the cache: nothing was written");
         return ibcu_fail(ctx, IBCU_ERR_CUDA, "a kernel gave up a bounded wait (code %d): its results are not valid", e);
     }

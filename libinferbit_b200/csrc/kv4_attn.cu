@@ -13,13 +13,19 @@
 // slack below), whatever the scales are, and a column's numbers do not depend on rows that it does not see.
 //
 // A warp has a tile of 8 or 16 columns of one KV head and takes 32 rows at a time through a ring of its own that bulk copies fill (rows of a
-// head lie one behind the other), so that no warp waits for another before the end. Three ways (KaMode):
-//   FEW   up to 8 columns, which are the M = 16 rows of an instruction twice, as high and low pieces. One launch: the blocks prepare the queries for themselves and
-//         write the call's rows that lie in their chunk.
-//   MANY  16 columns a tile, every product done twice, once for each piece. The four warps of a block share the tile's rows and put their results together.
-//   WIDE  the same with four tiles a block, a warp for each: what is read through L2 grows, but nothing is left to put together.
-// A column's rows are cut into chunks where that fills the machine; the chunks are joined by the last block of the tile to finish, or by a launch of
-// its own where they are many.
+// head lie one behind the other), so that no warp waits for another before the end; the four warps of a block share the tile's rows and put their
+// results together. Tiles of
+//   4     keys and values as the M = 16 rows of an instruction, the columns' high and low pieces as its N = 8: a group of up to four query heads and one token.
+//         728 instructions for 32 rows of 128 values, against 973 with tiles of eight;
+//   8     the columns, as high and low pieces, are the M = 16 rows;
+//   16    every product is done twice, once for each piece (LARGE), after a launch that prepares the queries and writes the call's rows. Blocks of the
+//         others do both for themselves, in their one launch.
+// A column's rows are cut into chunks where that fills the machine. The chunks' blocks stand in clusters, which put their results together in shared
+// memory; up to eight chunks are one cluster, the results of more clusters are put together by a launch of its own. (32 heads of 128 values over
+// 8 KV heads, one token after 512 rows: 6.4 us, against 8.6 with a second launch and 9.7 with the last block of a tile to finish doing it; after 4000: 9.0
+// against 10.3 with clusters of four and a second launch.)
+// What bounds it: instructions, 4 codes a lane being five to unpack. After 32767 rows 18.4 us, 2.1 TB/s of cache, of which 11 us are the start, the ring's first
+// copies and the joins; after 262143 rows 78 us, 3.9 TB/s.
 #include "kv4.cuh"
 #include "tc_common.cuh"
 #include <algorithm>
@@ -27,25 +33,22 @@
 namespace {
 
 constexpr int KA_WARPS = 4, KA_ROWS = 32;            // warps of a block; rows of a ring stage
+constexpr int KA_CLUSTER = 8;                        // blocks of a cluster at most
 constexpr float KA_LOW = -3.0e38f;                   // where running maxima start (finite: nothing minus infinity)
 constexpr float KA_SLACK = 1.9f;                     // by how much a maximum may be outgrown before the sums are rescaled
 
-enum KaMode { FEW, MANY, WIDE };
-
 struct KaParams {
-    Kv4 c; Kv4Columns t; Kv4Place at; Kv4Prep w;     // w.qf, w.qc: fragments prepared (MANY, WIDE), or left for the weights (FEW, if stat)
+    Kv4 c; Kv4Columns t; Kv4Place at; Kv4Prep w;     // w.qf, w.qc: fragments prepared (LARGE), or left for the weights (few, if stat)
     float* out; float2* stat;                        // stat [unit][16] or NULL: a column's softmax weight is 2^((score - x) - y)
-    float* pacc; float2* pml;                        // chunk results [unit][chunk][16][hd], [unit][chunk][16] (maximum, sum)
-    int* arrived;                                    // [unit] chunks done, zero between launches; NULL: kv4_join_kernel joins them
-    int want, grid_chunks;
+    float* pacc; float2* pml;                        // results of clusters [unit][cluster][16][hd], [unit][cluster][16] (maximum, sum)
+    int want, grid_chunks, cluster;                  // chunks at most; blocks a tile, whole clusters of them
     int* err;
 };
 
-// `rows` rows in at most `want` chunks of whole stages; chunks of more than a stage a warp are whole rounds of the warps
+// `rows` rows in at most `want` chunks of whole rounds of the warps
 __host__ __device__ __forceinline__ void ka_plan(int rows, int want, int& chunk, int& n) {
     const int stages = (rows + KA_ROWS - 1) / KA_ROWS;
-    int per = (stages + want - 1) / want;
-    if (per > KA_WARPS) per = (per + KA_WARPS - 1) / KA_WARPS * KA_WARPS;
+    const int per = ((stages + want - 1) / want + KA_WARPS - 1) / KA_WARPS * KA_WARPS;
     chunk = per * KA_ROWS;
     n = (stages + per - 1) / per;
 }
@@ -58,6 +61,7 @@ __device__ __forceinline__ void mma_f16_first(float* c, const uint4& a, uint32_t
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                  : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.0f));
 }
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t a) { uint32_t d; asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a)); return d; }
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) { const __half2 h = __floats2half2_rn(lo, hi); return *reinterpret_cast<const uint32_t*>(&h); }
 
@@ -87,34 +91,37 @@ __device__ __forceinline__ void lds_units(uint32_t* d, const unsigned char* s) {
         }
     }
 }
+// (w & mask) | base as the one instruction that it is (the compiler makes two of it, which were 128 of the 855 of a stage)
+__device__ __forceinline__ uint32_t under(uint32_t w, uint32_t mask, uint32_t base) { uint32_t d; asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(w), "r"(mask), "r"(base)); return d; }
 // The eight codes of a word less their bias, as four pairs: codes 0 and 4, 1 and 5 (16-fold), 2 and 6, 3 and 7 (16-fold)
 __device__ __forceinline__ void unpack(uint32_t w, uint32_t* f) {
     auto less = [](uint32_t a, uint32_t b) { const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b)); return *reinterpret_cast<const uint32_t*>(&d); };
     constexpr uint32_t BASE = 0x64006400u, EIGHT = 0x64086408u, EIGHT16 = 0x64806480u;       // 1024, 1024 + 8, 1024 + 16 * 8
-    f[0] = less((w & 0x000F000Fu) | BASE, EIGHT); f[1] = less((w & 0x00F000F0u) | BASE, EIGHT16);
+    f[0] = less(under(w, 0x000F000Fu, BASE), EIGHT); f[1] = less(under(w, 0x00F000F0u, BASE), EIGHT16);
     w >>= 8;
-    f[2] = less((w & 0x000F000Fu) | BASE, EIGHT); f[3] = less((w & 0x00F000F0u) | BASE, EIGHT16);
+    f[2] = less(under(w, 0x000F000Fu, BASE), EIGHT); f[3] = less(under(w, 0x00F000F0u, BASE), EIGHT16);
 }
 
 template <int NG> struct KaStage {                   // a ring stage: 32 rows of keys, of values and of scales
     static constexpr int KEYS = 0, VALUES = KA_ROWS * 16 * NG, SCALES = 2 * VALUES, BYTES = SCALES + KA_ROWS * 4 * NG;
 };
-template <int NG, int MODE> struct KaSmem {
-    static constexpr bool LARGE = MODE != FEW;
-    static constexpr int DEPTH = NG > 4 ? 2 : 3, FRAG_BYTES = (LARGE ? 2 : 1) * NG * 1024, TILES = MODE == WIDE ? KA_WARPS : 1;
-    static constexpr int FRAGS = 0, QC = TILES * FRAG_BYTES, SCALES = QC + (TILES * 64 + 127) / 128 * 128;
+template <int NG, int COLS> struct KaSmem {
+    static constexpr bool LARGE = COLS == 16;
+    static constexpr int DEPTH = NG > 4 || COLS == 4 ? 2 : 3, FRAG_BYTES = (LARGE ? 2 : 1) * NG * 1024;
+    static constexpr int FRAGS = 0, QC = FRAG_BYTES, SCALES = QC + 128;
     static constexpr int RING = SCALES + KA_WARPS * (2 * NG + 1) * 128;
-    static constexpr int TOTAL = RING + KA_WARPS * DEPTH * KaStage<NG>::BYTES;       // FEW: angles of the positions follow
-    static_assert(MODE == WIDE || KA_WARPS * (LARGE ? 16 : 8) * 32 * NG * 4 <= KA_WARPS * DEPTH * KaStage<NG>::BYTES, "the warps' results meet in the rings");
+    static constexpr int TOTAL = RING + KA_WARPS * DEPTH * KaStage<NG>::BYTES;       // few: angles of the positions follow
+    static_assert(KA_WARPS * COLS * 32 * NG * 4 <= KA_WARPS * DEPTH * KaStage<NG>::BYTES, "the warps' results meet in the rings");
 };
 
 // A stage's scales in FP32, once per row instead of once per lane that uses them: sc [2 NG + 1][32], rows in the order t * 8 + 2 i + h
 // for row 8 i + 4 h + t, so that a lane's eight rows lie side by side; the last line is L.
-template <int NG>
+// (FOUR: row 8 i + (g >> 1) + 4 (g & 1) at g * 4 + i.)
+template <int NG, bool FOUR>
 __device__ __forceinline__ void spread_scales(float* sc, const unsigned char* rows, int lane) {
     uint32_t w[NG];
     lds_words<NG>(w, rows + lane * 4 * NG);
-    float* d = sc + (lane & 3) * 8 + (lane >> 3) * 2 + ((lane >> 2) & 1);
+    float* d = sc + (FOUR ? (lane & 3) * 8 + ((lane >> 2) & 1) * 4 + (lane >> 3) : (lane & 3) * 8 + (lane >> 3) * 2 + ((lane >> 2) & 1));
     uint32_t top = 0;
 #pragma unroll
     for (int j = 0; j < NG; j++) {
@@ -133,7 +140,29 @@ __device__ __forceinline__ void lane_rows(float (&x)[4][2], const float* line, i
     x[0][0] = a.x; x[0][1] = a.y; x[1][0] = a.z; x[1][1] = a.w; x[2][0] = b.x; x[2][1] = b.y; x[3][0] = b.z; x[3][1] = b.w;
 }
 
-// Scores of 32 rows: s[i][h][n] for row 8 i + 4 h + t and column g (n = 0), g + 8 (n = 1), in the column's own units. keys(i, j, f): the codes
+// Scores of 32 rows for up to four columns. s[i]: row 8 i + (g >> 1) + 4 (g & 1), column t, in the column's own units.
+template <int NG>
+__device__ __forceinline__ void score_rows_four(float (&s)[4][1][1], const uint32_t (&kw)[4][NG], const uint2* qf, const float* sc, int lane) {
+#pragma unroll
+    for (int j = 0; j < NG; j++) {
+        const uint2 b0 = qf[(j * 2) * 32 + lane], b1 = qf[(j * 2 + 1) * 32 + lane];
+        const float4 line = *reinterpret_cast<const float4*>(sc + j * 32 + (lane >> 2) * 4);
+        const float ks[4] = { line.x, line.y, line.z, line.w };
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            uint32_t u[4], w[4];
+            unpack(kw[i][j], u);
+            unpack(kw[i + 1][j], w);
+            float c[4];
+            mma_f16_first(c, make_uint4(u[0], w[0], u[1], w[1]), b0.x, b0.y);
+            mma_f16(c, make_uint4(u[2], w[2], u[3], w[3]), b1.x, b1.y);
+            s[i][0][0] = j ? fmaf(ks[i], c[0] + c[1], s[i][0][0]) : ks[i] * (c[0] + c[1]);
+            s[i + 1][0][0] = j ? fmaf(ks[i + 1], c[2] + c[3], s[i + 1][0][0]) : ks[i + 1] * (c[2] + c[3]);
+        }
+    }
+}
+
+// For more columns: s[i][h][n] for row 8 i + 4 h + t and column g (n = 0), g + 8 (n = 1), in the column's own units. keys(i, j, f): the codes
 // of group j of the lane's i-th row, unpacked.
 template <int NG, bool LARGE, typename Keys>
 __device__ __forceinline__ void score_rows(float (&s)[4][2][LARGE ? 2 : 1], Keys keys, const uint4* qf, const float* sc, int lane) {
@@ -165,7 +194,7 @@ __device__ __forceinline__ void score_rows(float (&s)[4][2][LARGE ? 2 : 1], Keys
     }
 }
 
-// Chunks first, first + step, .. of a column added up at value 4 d4, against the maximum M. at: the column's first chunk. A lane's weights are broadcast
+// Results of clusters first, first + step, .. of a column added up at value 4 d4, against the maximum M. at: the column's first. A lane's weights are broadcast
 // to the others: nothing in the loop waits for a load but the sums.
 __device__ __forceinline__ float4 join_values(const KaParams& p, size_t at, int n, int first, int step, float M, int d4) {
     const int lane = threadIdx.x & 31, mine = (n - first + step - 1) / step;
@@ -182,7 +211,7 @@ __device__ __forceinline__ float4 join_values(const KaParams& p, size_t at, int 
     }
     return o;
 }
-// maximum and sum over the chunks, by a warp
+// maximum and sum over the clusters, by a warp
 __device__ __forceinline__ float2 join_stat(const KaParams& p, size_t at, int n) {
     const int lane = threadIdx.x & 31;
     float2 own = lane < n ? __ldcg(p.pml + at + (size_t)lane * 16) : make_float2(KA_LOW, 0.0f);
@@ -197,20 +226,7 @@ __device__ __forceinline__ void join_store(const KaParams& p, int kvh, int cc, i
     float* to = p.out + ((size_t)(cc / p.t.group) * p.t.n_heads + (size_t)kvh * p.t.group + cc % p.t.group) * p.c.hd + 4 * d4;
     to[0] = o.x * inv; to[1] = o.y * inv; to[2] = o.z * inv; to[3] = o.w * inv;
 }
-// The chunks of a unit put together by its last block, a warp every fourth column.
-__device__ __forceinline__ void join_by_last(const KaParams& p, int unit, int n) {
-    const int lane = threadIdx.x & 31, kvh = unit / p.t.ntiles, c0 = unit % p.t.ntiles * p.t.cols(), q4 = p.c.hd / 4;
-    for (int col = threadIdx.x >> 5; col < p.t.cols() && (c0 + col) / p.t.group < p.t.B; col += KA_WARPS) {
-        const size_t at = (size_t)unit * p.grid_chunks * 16 + col;
-        const float2 st = join_stat(p, at, n);
-        for (int d0 = 0; d0 < q4; d0 += 32) {
-            const float4 o = join_values(p, at, n, 0, 1, st.x, d0 + lane);
-            if (d0 + lane < q4) join_store(p, kvh, c0 + col, d0 + lane, o, 1.0f / st.y);
-        }
-        if (lane == 0 && p.stat) p.stat[(size_t)unit * 16 + col] = make_float2(st.x, log2f(st.y) - 14.0f);
-    }
-}
-// grid (columns of a tile, units): the same by a launch of its own, a block a column, where there are many chunks
+// grid (columns of a tile, units), a block a column
 __global__ void __launch_bounds__(128) kv4_join_kernel(const KaParams p) {
     __shared__ float4 part[4][64];
     pdl_launch_dependents();
@@ -218,9 +234,10 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const KaParams p) {
     int row0, pos0, chunk, n;
     if (!kv4_place(p.at, p.t.B, p.c.max_rows, p.err, row0, pos0)) return;
     ka_plan(row0 + p.t.B, p.want, chunk, n);
+    n = (n + p.cluster - 1) / p.cluster;
     const int unit = blockIdx.y, kvh = unit / p.t.ntiles, cc = unit % p.t.ntiles * p.t.cols() + blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q4 = p.c.hd / 4;
     if (n == 1 || cc / p.t.group >= p.t.B) return;
-    const size_t at = (size_t)unit * p.grid_chunks * 16 + blockIdx.x;
+    const size_t at = (size_t)unit * (p.grid_chunks / p.cluster) * 16 + blockIdx.x;
     const float2 st = join_stat(p, at, n);
     for (int d0 = 0; d0 < q4; d0 += 32) part[warp][d0 + lane] = join_values(p, at, n, warp, 4, st.x, d0 + lane);
     __syncthreads();
@@ -232,20 +249,20 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const KaParams p) {
     if (threadIdx.x == 0 && p.stat) p.stat[(size_t)unit * 16 + blockIdx.x] = make_float2(st.x, log2f(st.y) - 14.0f);
 }
 
-template <int NG, int MODE>
-__global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (MODE == FEW ? 3 : 2)) kv4_attn_kernel(const KaParams p) {
-    using S = KaSmem<NG, MODE>;
+template <int NG, int COLS>
+__global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (COLS == 16 ? 2 : 3)) kv4_attn_kernel(const KaParams p) {
+    using S = KaSmem<NG, COLS>;
     using St = KaStage<NG>;
-    constexpr bool LARGE = S::LARGE;
-    constexpr int NC = LARGE ? 2 : 1, COLS = 8 * NC, HD = 32 * NG, EACH = MODE == WIDE ? 1 : KA_WARPS;          // EACH: a warp takes every EACH-th stage
+    constexpr bool LARGE = COLS == 16, FOUR = COLS == 4;
+    constexpr int NC = LARGE ? 2 : 1, HD = 32 * NG;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ unsigned long long full[KA_WARPS][S::DEPTH];
-    __shared__ int abort_flag, last;
-    __shared__ float2 ml[KA_WARPS][16];
+    __shared__ int abort_flag;
+    __shared__ float2 ml[KA_WARPS][16], own[16];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     // tiles that see most rows first
-    const int per_head = (p.t.ntiles + S::TILES - 1) / S::TILES, kvh = blockIdx.x / per_head, sp = blockIdx.y;
-    const int tile = p.t.ntiles - 1 - (blockIdx.x % per_head * S::TILES + (MODE == WIDE ? warp : 0));
+    const int place = blockIdx.x / p.grid_chunks, kvh = place / p.t.ntiles, tile = p.t.ntiles - 1 - place % p.t.ntiles, sp = blockIdx.x % p.grid_chunks;
+    const int rank = sp % p.cluster, peers_from = sp - rank;
     const int unit = kvh * p.t.ntiles + tile, c0 = tile * COLS;
     if (tid == 0) {
         abort_flag = 0;
@@ -254,26 +271,26 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (MODE == FEW ? 3 :
     }
     double2* turn = reinterpret_cast<double2*>(smem + S::TOTAL);
     int row0 = p.at.row0, pos0 = p.at.pos0;
-    if (MODE == FEW) {
+    if (!LARGE) {
         if (p.w.rotate && !p.at.at) kv4_angles(turn, p.t.B, pos0, HD, p.w.log2_theta);             // beside the end of the launch ahead
         pdl_wait();
         pdl_launch_dependents();
     }
     __syncthreads();
-    // MANY, WIDE: launches ahead of the preparing one have ended when this one starts, since that one lets it start behind its own wait. What they wrote (a
+    // LARGE: launches ahead of the preparing one have ended when this one starts, since that one lets it start behind its own wait. What they wrote (a
     // device position, rows of earlier calls) may be read before this launch's own wait.
     if (!kv4_place(p.at, p.t.B, p.c.max_rows, p.err, row0, pos0)) return;
-    if (MODE == FEW && p.w.rotate && p.at.at) kv4_angles(turn, p.t.B, pos0, HD, p.w.log2_theta);
+    if (!LARGE && p.w.rotate && p.at.at) kv4_angles(turn, p.t.B, pos0, HD, p.w.log2_theta);
     int chunk, n_chunks;
     ka_plan(row0 + p.t.B, p.want, chunk, n_chunks);
-    if (sp >= n_chunks) return;
-    const int lim0 = row0 + max(c0, 0) / p.t.group;                                                // the last row that the tile's first column sees
-    const int t0 = sp * chunk, t1 = tile < 0 ? 0 : min(t0 + chunk, row0 + min(p.t.B - 1, (c0 + COLS - 1) / p.t.group) + 1);
-    const int skip = MODE == WIDE ? 0 : warp, stages = t1 > t0 ? (t1 - t0 + KA_ROWS - 1) / KA_ROWS : 0, mine = stages > skip ? (stages - skip + EACH - 1) / EACH : 0;
+    if (peers_from >= n_chunks) return;                                                            // all of the cluster
+    const int lim0 = row0 + c0 / p.t.group;                                                // the last row that the tile's first column sees
+    const int t0 = sp * chunk, t1 = min(min(t0 + chunk, n_chunks * chunk), row0 + min(p.t.B - 1, (c0 + COLS - 1) / p.t.group) + 1);
+    const int stages = t1 > t0 ? (t1 - t0 + KA_ROWS - 1) / KA_ROWS : 0, mine = stages > warp ? (stages - warp + KA_WARPS - 1) / KA_WARPS : 0;     // a warp takes every fourth stage
     unsigned char* ring = smem + S::RING + warp * S::DEPTH * St::BYTES;
     const size_t plane = p.c.row(kvh, 0);
     auto issue = [&](int n) {                                                                      // one lane: the n-th stage of this warp; whole groups of 8 rows, which the planes have
-        const int r = t0 + (skip + n * EACH) * KA_ROWS, rows = min(KA_ROWS, (t1 - r + 7) & ~7), d = n % S::DEPTH;
+        const int r = t0 + (warp + n * KA_WARPS) * KA_ROWS, rows = min(KA_ROWS, (t1 - r + 7) & ~7), d = n % S::DEPTH;
         const uint32_t bar = smem_u32(&full[warp][d]), to = smem_u32(ring + d * St::BYTES);
         mbar_expect_tx(bar, (uint32_t)rows * 36 * NG);
         bulk_load(to + St::KEYS, p.c.k + (plane + r) * (16 * NG), (uint32_t)rows * 16 * NG, bar);
@@ -283,10 +300,10 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (MODE == FEW ? 3 :
     const int old = p.w.k ? row0 : t1;                                                             // rows below were there before this call
     int issued = 0;
     if (lane == 0)
-        for (; issued < min(mine, (int)S::DEPTH) && t0 + (skip + issued * EACH) * KA_ROWS + KA_ROWS <= old; issued++) issue(issued);
-    uint4* qf = reinterpret_cast<uint4*>(smem + S::FRAGS + (MODE == WIDE ? warp * S::FRAG_BYTES : 0));
-    float* qc = reinterpret_cast<float*>(smem + S::QC) + (MODE == WIDE ? warp * 16 : 0);
-    if constexpr (MODE == FEW) {
+        for (; issued < min(mine, (int)S::DEPTH) && t0 + (warp + issued * KA_WARPS) * KA_ROWS + KA_ROWS <= old; issued++) issue(issued);
+    uint4* qf = reinterpret_cast<uint4*>(smem + S::FRAGS);
+    float* qc = reinterpret_cast<float*>(smem + S::QC);
+    if constexpr (!LARGE) {
         __shared__ uint32_t amax[KA_WARPS][8];
         __syncthreads();
         if (p.w.k) {                                                                               // the call's rows of this chunk
@@ -301,9 +318,9 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (MODE == FEW ? 3 :
             asm volatile("fence.proxy.async.global;" ::: "memory");                                // the bulk copies read them
         }
         constexpr int JT = (NG + KA_WARPS - 1) / KA_WARPS;                                         // a warp has every fourth group of all columns
-        const int b = g / p.t.group;
+        const int column = FOUR ? g >> 1 : g, b = column / p.t.group;                              // FOUR: high pieces in even g, low ones in odd
         const bool on = b < p.t.B;
-        const float* src = p.w.q + ((size_t)b * p.t.n_heads + (size_t)kvh * p.t.group + g % p.t.group) * HD + 8 * t;
+        const float* src = p.w.q + ((size_t)b * p.t.n_heads + (size_t)kvh * p.t.group + column % p.t.group) * HD + 8 * t;
         float x[JT][8];
         uint32_t m = 0;
 #pragma unroll
@@ -316,13 +333,13 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (MODE == FEW ? 3 :
         }
         m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
         m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        if (t == 0) amax[warp][g] = m;
+        if (t == 0) amax[warp][column] = m;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < KA_WARPS; w++) m = max(m, amax[w][g]);
+        for (int w = 0; w < KA_WARPS; w++) m = max(m, amax[w][column]);
         const Kv4Up up = kv4_up(m, HD);
         const bool leave = p.stat && sp == 0;
-        if (warp == 0 && t == 0) { qc[g] = up.back; if (leave) p.w.qc[(size_t)unit * 16 + g] = up.back; }
+        if (warp == 0 && t == 0) { qc[column] = up.back; if (leave) p.w.qc[(size_t)unit * 16 + (FOUR && (g & 1) ? 4 : 0) + column] = up.back; }
 #pragma unroll
         for (int jj = 0; jj < JT; jj++) {
             const int j = warp + jj * KA_WARPS;
@@ -334,35 +351,39 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (MODE == FEW ? 3 :
                 uint32_t hi[2], lo[2];
                 kv4_pieces(x[jj], s, hi, lo);
                 const uint4 v = make_uint4(hi[0], lo[0], hi[1], lo[1]);
-                qf[(j * 2 + s) * 32 + lane] = v;
-                if (leave) p.w.qf[unit * kv4_frags(NG, false) + (j * 2 + s) * 32 + lane] = v;
+                if (FOUR) reinterpret_cast<uint2*>(qf)[(j * 2 + s) * 32 + lane] = g & 1 ? make_uint2(lo[0], lo[1]) : make_uint2(hi[0], hi[1]);
+                else qf[(j * 2 + s) * 32 + lane] = v;
+                if (leave) {                                                                       // columns of 8, the upper four of FOUR empty
+                    uint4* to = p.w.qf + unit * kv4_frags(NG, false) + (j * 2 + s) * 32;
+                    if (!FOUR) to[lane] = v;
+                    else to[((g & 1) * 4 + column) * 4 + t] = g & 1 ? make_uint4(0, 0, 0, 0) : v;
+                }
             }
         }
     } else {
         pdl_wait();
         pdl_launch_dependents();
         if (lane == 0) asm volatile("fence.proxy.async.global;" ::: "memory");                     // rows that the preparing launch wrote
-        const int n = MODE == WIDE ? 32 : 32 * KA_WARPS, e0 = MODE == WIDE ? lane : tid;
-        if (tile >= 0) {
-            const uint4* src = p.w.qf + unit * kv4_frags(NG, true);
-            for (int e = e0; e < NG * 128; e += n) qf[e] = __ldcg(src + e);
-            if (e0 < 16) qc[e0] = __ldcg(p.w.qc + (size_t)unit * 16 + e0);
-        }
+        const uint4* src = p.w.qf + unit * kv4_frags(NG, true);
+        for (int e = tid; e < NG * 128; e += 32 * KA_WARPS) qf[e] = __ldcg(src + e);
+        if (tid < 16) qc[tid] = __ldcg(p.w.qc + (size_t)unit * 16 + tid);
     }
     if (lane == 0) for (; issued < min(mine, (int)S::DEPTH); issued++) issue(issued);
-    if (MODE == WIDE) __syncwarp(); else __syncthreads();
+    __syncthreads();
     float* sc = reinterpret_cast<float*>(smem + S::SCALES) + warp * (2 * NG + 1) * 32;
-    float f[NC], m[NC], l[NC], acc[NG][4][4];
+    constexpr int NA = FOUR ? 2 : 4;
+    float f[NC], m[NC], l[NC], acc[NG][NA][4];
     int lim[NC];
 #pragma unroll
     for (int n = 0; n < NC; n++) {
-        f[n] = qc[g + 8 * n]; m[n] = KA_LOW; l[n] = 0.0f;
-        lim[n] = row0 + (max(c0, 0) + g + 8 * n) / p.t.group;
+        const int column = FOUR ? t : g + 8 * n;
+        f[n] = qc[column]; m[n] = KA_LOW; l[n] = 0.0f;
+        lim[n] = row0 + (c0 + column) / p.t.group;
     }
 #pragma unroll
     for (int j = 0; j < NG; j++)
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < NA; i++)
 #pragma unroll
             for (int u = 0; u < 4; u++) acc[j][i][u] = 0.0f;
 
@@ -370,16 +391,17 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (MODE == FEW ? 3 :
     int d = 0;
     bool wide = false;
     for (int it = 0; it < mine; it++) {
-        const int r0 = t0 + (skip + it * EACH) * KA_ROWS;
+        const int r0 = t0 + (warp + it * KA_WARPS) * KA_ROWS;
         if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&full[warp][d]), phase, &abort_flag, IBCU_KV4_WAIT_ERR))) break;
         const unsigned char* stage = ring + d * St::BYTES;
-        spread_scales<NG>(sc, stage + St::SCALES, lane);
+        spread_scales<NG, FOUR>(sc, stage + St::SCALES, lane);
         uint32_t kw[4][NG], vw[4][2][(NG + 1) / 2];
 #pragma unroll
         for (int i = 0; i < 4; i++) lds_words<NG>(kw[i], stage + St::KEYS + (8 * i + (g >> 1) + 4 * (g & 1)) * 16 * NG + t * 4 * NG);
         __syncwarp();
-        float s[4][2][NC];
-        score_rows<NG, LARGE>(s, [&](int i, int j, uint32_t* to) { unpack(kw[i][j], to); }, qf, sc, lane);
+        float s[4][FOUR ? 1 : 2][NC];
+        if constexpr (FOUR) score_rows_four<NG>(s, kw, reinterpret_cast<const uint2*>(qf), sc, lane);
+        else score_rows<NG, LARGE>(s, [&](int i, int j, uint32_t* to) { unpack(kw[i][j], to); }, qf, sc, lane);
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -390,9 +412,12 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (MODE == FEW ? 3 :
 
         auto weigh = [&](auto masked) {
             constexpr bool MASK = decltype(masked)::value;
-            float L[4][2], top[NC];
-            lane_rows(L, sc + 2 * NG * 32, t);
-            auto seen = [&](int i, int h, int n) { return !MASK || r0 + 8 * i + 4 * h + t <= lim[n]; };
+            constexpr int NH = FOUR ? 1 : 2;                                                       // rows of a lane in eight
+            float L[4][NH], top[NC];
+            if constexpr (FOUR) { const float4 x = *reinterpret_cast<const float4*>(sc + 2 * NG * 32 + g * 4); L[0][0] = x.x; L[1][0] = x.y; L[2][0] = x.z; L[3][0] = x.w; }
+            else lane_rows(L, sc + 2 * NG * 32, t);
+            auto seen = [&](int i, int h, int n) { return !MASK || r0 + 8 * i + (FOUR ? (g >> 1) + 4 * (g & 1) : 4 * h + t) <= lim[n]; };
+            constexpr int OVER0 = FOUR ? 4 : 1, OVER1 = FOUR ? 32 : 4;                              // lanes of a column
             bool grow = false;
 #pragma unroll
             for (int n = 0; n < NC; n++) {
@@ -400,18 +425,18 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (MODE == FEW ? 3 :
 #pragma unroll
                 for (int i = 0; i < 4; i++)
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
+                    for (int h = 0; h < NH; h++) {
                         s[i][h][n] *= f[n];
                         if (seen(i, h, n)) top[n] = fmaxf(top[n], s[i][h][n] + L[i][h]);
                     }
-                top[n] = fmaxf(top[n], __shfl_xor_sync(0xffffffffu, top[n], 1));
-                top[n] = fmaxf(top[n], __shfl_xor_sync(0xffffffffu, top[n], 2));
                 grow = grow || top[n] > m[n] + KA_SLACK;
             }
             if (__any_sync(0xffffffffu, grow)) {
                 wide = false;
 #pragma unroll
                 for (int n = 0; n < NC; n++) {
+#pragma unroll
+                    for (int o = OVER0; o < OVER1; o *= 2) top[n] = fmaxf(top[n], __shfl_xor_sync(0xffffffffu, top[n], o));
                     const float now = fmaxf(m[n], top[n]), corr = ex2(m[n] - now);
                     m[n] = now;
                     wide = wide || fabsf(now) > 524288.0f;
@@ -419,7 +444,7 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (MODE == FEW ? 3 :
 #pragma unroll
                     for (int j = 0; j < NG; j++) {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
+                        for (int i = 0; i < NA; i++) {
                             if (LARGE) { acc[j][i][2 * n] *= corr; acc[j][i][2 * n + 1] *= corr; }
                             else { acc[j][i][0] *= corr; acc[j][i][1] *= corr; acc[j][i][2] *= corr; acc[j][i][3] *= corr; }
                         }
@@ -431,7 +456,7 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (MODE == FEW ? 3 :
 #pragma unroll
                 for (int i = 0; i < 4; i++)
 #pragma unroll
-                    for (int h = 0; h < 2; h++) s[i][h][n] -= m[n];
+                    for (int h = 0; h < NH; h++) s[i][h][n] -= m[n];
             // Beyond 2^19 (log2 units; such a softmax has one row) the maximum itself is rounded by more than the slack allows for.
             if (__any_sync(0xffffffffu, wide)) {
 #pragma unroll
@@ -439,47 +464,71 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (MODE == FEW ? 3 :
 #pragma unroll
                     for (int i = 0; i < 4; i++)
 #pragma unroll
-                        for (int h = 0; h < 2; h++) s[i][h][n] = s[i][h][n] > 1.0f - L[i][h] ? 1.0f - L[i][h] : s[i][h][n];
+                        for (int h = 0; h < NH; h++) s[i][h][n] = s[i][h][n] > 1.0f - L[i][h] ? 1.0f - L[i][h] : s[i][h][n];
             }
 #pragma unroll
             for (int n = 0; n < NC; n++) {
 #pragma unroll
                 for (int i = 0; i < 4; i++)
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
+                    for (int h = 0; h < NH; h++) {
                         const float e = seen(i, h, n) ? ex2(s[i][h][n] + 14.0f) : 0.0f;
                         s[i][h][n] = e;
                         l[n] += e;
                     }
             }
+            if constexpr (FOUR) {
 #pragma unroll
-            for (int j = 0; j < NG; j++) {
-                float vs[4][2];
-                lane_rows(vs, sc + (NG + j) * 32, t);
-#pragma unroll
-                for (int u = 0; u < 2; u++) {                                                      // 16 rows: pieces 2 u and 2 u + 1
-                    uint32_t hi[2][NC], lo[2][NC];
-#pragma unroll
-                    for (int i = 0; i < 2; i++)
-#pragma unroll
-                        for (int n = 0; n < NC; n++) {
-                            float a = s[2 * u + i][0][n] * vs[2 * u + i][0], b = s[2 * u + i][1][n] * vs[2 * u + i][1];
-                            if (!seen(2 * u + i, 0, n)) a = 0.0f;                                  // the row's scale may be NaN
-                            if (!seen(2 * u + i, 1, n)) b = 0.0f;
-                            hi[i][n] = pack_half(a, b);
-                            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[i][n]));
-                            lo[i][n] = pack_half(a - back.x, b - back.y);
-                        }
-                    uint32_t b0[4], b1[4];
-                    unpack(__byte_perm(vw[2 * u][0][j / 2], vw[2 * u][1][j / 2], j & 1 ? 0x7632 : 0x5410), b0);
-                    unpack(__byte_perm(vw[2 * u + 1][0][j / 2], vw[2 * u + 1][1][j / 2], j & 1 ? 0x7632 : 0x5410), b1);
+                for (int j = 0; j < NG; j++) {
+                    const float4 line = *reinterpret_cast<const float4*>(sc + (NG + j) * 32 + g * 4);
+                    const float vs[4] = { line.x, line.y, line.z, line.w };
+                    uint32_t b[4];                                                                 // [rows 8 i ..][columns' pieces], transposed
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        if constexpr (LARGE) {
-                            mma_f16(acc[j][i], make_uint4(hi[0][0], hi[0][1], hi[1][0], hi[1][1]), b0[i], b1[i]);
-                            mma_f16(acc[j][i], make_uint4(lo[0][0], lo[0][1], lo[1][0], lo[1][1]), b0[i], b1[i]);
-                        } else {
-                            mma_f16(acc[j][i], make_uint4(hi[0][0], lo[0][0], hi[1][0], lo[1][0]), b0[i], b1[i]);
+                        float a = s[i][0][0] * vs[i];
+                        if (!seen(i, 0, 0)) a = 0.0f;                                              // the row's scale may be NaN
+                        const float hi = __uint_as_float(__float_as_uint(a) & 0xFFFFE000u);        // eleven bits, cut off: the low piece has the same sign and what is left to 2^-22
+                        b[i] = transpose_8x8(pack_half(hi, a - hi));
+                    }
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        uint32_t x[4], y[4];
+                        unpack(__byte_perm(vw[2 * u][0][j / 2], vw[2 * u][1][j / 2], j & 1 ? 0x7632 : 0x5410), x);
+                        unpack(__byte_perm(vw[2 * u + 1][0][j / 2], vw[2 * u + 1][1][j / 2], j & 1 ? 0x7632 : 0x5410), y);
+                        mma_f16(acc[j][0], make_uint4(x[0], x[2], y[0], y[2]), b[2 * u], b[2 * u + 1]);
+                        mma_f16(acc[j][1], make_uint4(x[1], x[3], y[1], y[3]), b[2 * u], b[2 * u + 1]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < NG; j++) {
+                    float vs[4][2];
+                    lane_rows(vs, sc + (NG + j) * 32, t);
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {                                                      // 16 rows: pieces 2 u and 2 u + 1
+                        uint32_t hi[2][NC], lo[2][NC];
+#pragma unroll
+                        for (int i = 0; i < 2; i++)
+#pragma unroll
+                            for (int n = 0; n < NC; n++) {
+                                float a = s[2 * u + i][0][n] * vs[2 * u + i][0], b = s[2 * u + i][1][n] * vs[2 * u + i][1];
+                                if (!seen(2 * u + i, 0, n)) a = 0.0f;                                  // the row's scale may be NaN
+                                if (!seen(2 * u + i, 1, n)) b = 0.0f;
+                                hi[i][n] = pack_half(a, b);
+                                const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[i][n]));
+                                lo[i][n] = pack_half(a - back.x, b - back.y);
+                            }
+                        uint32_t b0[4], b1[4];
+                        unpack(__byte_perm(vw[2 * u][0][j / 2], vw[2 * u][1][j / 2], j & 1 ? 0x7632 : 0x5410), b0);
+                        unpack(__byte_perm(vw[2 * u + 1][0][j / 2], vw[2 * u + 1][1][j / 2], j & 1 ? 0x7632 : 0x5410), b1);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            if constexpr (LARGE) {
+                                mma_f16(acc[j][i], make_uint4(hi[0][0], hi[0][1], hi[1][0], hi[1][1]), b0[i], b1[i]);
+                                mma_f16(acc[j][i], make_uint4(lo[0][0], lo[0][1], lo[1][0], lo[1][1]), b0[i], b1[i]);
+                            } else {
+                                mma_f16(acc[j][i], make_uint4(hi[0][0], lo[0][0], hi[1][0], lo[1][0]), b0[i], b1[i]);
+                            }
                         }
                     }
                 }
@@ -491,104 +540,91 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (MODE == FEW ? 3 :
     }
 
 #pragma unroll
-    for (int n = 0; n < NC; n++) {
-        l[n] += __shfl_xor_sync(0xffffffffu, l[n], 1);
-        l[n] += __shfl_xor_sync(0xffffffffu, l[n], 2);
-    }
-    // values 8t..8t+7 of group j of column g + 8 n
-    auto values = [&](int n, int j, float (&o)[8]) {
+    for (int n = 0; n < NC; n++)
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const float a = LARGE ? acc[j][i][2 * n + u] : acc[j][i][u] + acc[j][i][u + 2];
-                o[4 * u + i] = i & 1 ? a * 0.0625f : a;
-            }
-    };
+        for (int o = FOUR ? 4 : 1; o < (FOUR ? 32 : 4); o *= 2) l[n] += __shfl_xor_sync(0xffffffffu, l[n], o);
     auto give_up = [&]() {                                     // by one thread of the block, when its waits are over
         if (!*(volatile int*)&abort_flag) return;
         *p.err = IBCU_KV4_WAIT_ERR;
         for (int i = 0; i < 1000; i++) __nanosleep(1000);      // copies still on their way into this block's shared memory land before it goes
     };
-    if constexpr (MODE == WIDE) {
-#pragma unroll
-        for (int n = 0; n < NC; n++) {
-            const int c = c0 + g + 8 * n, b = c / p.t.group;
-            if (tile < 0 || b >= p.t.B) continue;
-            float* to = p.out + ((size_t)b * p.t.n_heads + (size_t)kvh * p.t.group + c % p.t.group) * HD + 8 * t;
-            const float inv = 1.0f / l[n];
-            const bool vec = ((uintptr_t)p.out & 15) == 0;
-#pragma unroll
-            for (int j = 0; j < NG; j++) {
-                float o[8];
-                values(n, j, o);
-                if (vec) {
-                    *reinterpret_cast<float4*>(to + 32 * j) = make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-                    *reinterpret_cast<float4*>(to + 32 * j + 4) = make_float4(o[4] * inv, o[5] * inv, o[6] * inv, o[7] * inv);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) to[32 * j + i] = o[i] * inv;
-                }
-            }
-            if (t == 0 && p.stat) p.stat[(size_t)unit * 16 + g + 8 * n] = make_float2(m[n], log2f(l[n]) - 14.0f);
-        }
-        __syncthreads();
-        if (tid == 0) give_up();
-    } else {
     // the four warps' results meet in the rings: [warp][column][value], and maxima and sums
 #pragma unroll
-    for (int n = 0; n < NC; n++) if (t == 0) ml[warp][g + 8 * n] = make_float2(m[n], l[n]);
+    for (int n = 0; n < NC; n++) if (FOUR ? g == 0 : t == 0) ml[warp][FOUR ? t : g + 8 * n] = make_float2(m[n], l[n]);
     __syncthreads();
     float* meet = reinterpret_cast<float*>(smem + S::RING);
 #pragma unroll
-    for (int n = 0; n < NC; n++)
+    for (int j = 0; j < NG; j++) {
+        if constexpr (FOUR)                                                                        // values 4g..4g+3 of group j of column t
+            *reinterpret_cast<float4*>(meet + ((size_t)warp * COLS + t) * HD + 32 * j + 4 * g) = make_float4(
+                acc[j][0][0] + acc[j][0][1], (acc[j][1][0] + acc[j][1][1]) * 0.0625f, acc[j][0][2] + acc[j][0][3], (acc[j][1][2] + acc[j][1][3]) * 0.0625f);
+        else {
 #pragma unroll
-        for (int j = 0; j < NG; j++) {
-            float o[8];
-            values(n, j, o);
-            float4* to = reinterpret_cast<float4*>(meet + ((size_t)warp * COLS + g + 8 * n) * HD + 32 * j + 8 * t);
-            to[0] = make_float4(o[0], o[1], o[2], o[3]);
-            to[1] = make_float4(o[4], o[5], o[6], o[7]);
+            for (int n = 0; n < NC; n++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {                                                      // values 8t+4u..8t+4u+3 of group j of column g + 8 n
+                    auto value = [&](int i) { return LARGE ? acc[j][i][2 * n + u] : acc[j][i][u] + acc[j][i][u + 2]; };
+                    *reinterpret_cast<float4*>(meet + ((size_t)warp * COLS + g + 8 * n) * HD + 32 * j + 8 * t + 4 * u) = make_float4(value(0), value(1) * 0.0625f, value(2), value(3) * 0.0625f);
+                }
         }
+    }
     __syncthreads();
     if (tid == 0) give_up();
+    auto store = [&](int col, int d4, const float4& o, float M, float sum) {
+        const int c = c0 + col;
+        if (n_chunks <= p.cluster) {
+            join_store(p, kvh, c, d4, o, 1.0f / sum);
+            if (d4 == 0 && p.stat) p.stat[(size_t)unit * 16 + col] = make_float2(M, log2f(sum) - 14.0f);
+        } else {
+            const size_t at = ((size_t)unit * (p.grid_chunks / p.cluster) + sp / p.cluster) * 16 + col;
+            *reinterpret_cast<float4*>(p.pacc + at * HD + 4 * d4) = o;
+            if (d4 == 0) p.pml[at] = make_float2(M, sum);
+        }
+    };
+    auto add = [](float4& o, float& sum, const float4& v, const float2& of, float M) {
+        const float k = ex2(of.x - M);
+        sum = fmaf(of.y, k, sum);
+        o.x = fmaf(v.x, k, o.x); o.y = fmaf(v.y, k, o.y); o.z = fmaf(v.z, k, o.z); o.w = fmaf(v.w, k, o.w);
+    };
     for (int e = tid; e < COLS * HD / 4; e += 32 * KA_WARPS) {
-        const int col = e / (HD / 4), d4 = e % (HD / 4), c = c0 + col, b = c / p.t.group;
-        if (b >= p.t.B) break;
+        const int col = e / (HD / 4), d4 = e % (HD / 4);
+        if ((c0 + col) / p.t.group >= p.t.B) break;
         float M = ml[0][col].x, sum = 0.0f;
 #pragma unroll
         for (int w = 1; w < KA_WARPS; w++) M = fmaxf(M, ml[w][col].x);
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < KA_WARPS; w++) {
-            const float k = ex2(ml[w][col].x - M);
-            const float4 v = *reinterpret_cast<const float4*>(meet + ((size_t)w * COLS + col) * HD + 4 * d4);
-            sum = fmaf(ml[w][col].y, k, sum);
-            o.x = fmaf(v.x, k, o.x); o.y = fmaf(v.y, k, o.y); o.z = fmaf(v.z, k, o.z); o.w = fmaf(v.w, k, o.w);
-        }
-        if (n_chunks == 1) {
-            float* to = p.out + ((size_t)b * p.t.n_heads + (size_t)kvh * p.t.group + c % p.t.group) * HD + 4 * d4;
-            const float inv = 1.0f / sum;
-            to[0] = o.x * inv; to[1] = o.y * inv; to[2] = o.z * inv; to[3] = o.w * inv;
-            if (d4 == 0 && p.stat) p.stat[(size_t)unit * 16 + col] = make_float2(M, log2f(sum) - 14.0f);
-        } else {
-            const size_t at = ((size_t)unit * p.grid_chunks + sp) * 16 + col;
-            *reinterpret_cast<float4*>(p.pacc + at * HD + 4 * d4) = o;
-            if (d4 == 0) p.pml[at] = make_float2(M, sum);
+        for (int w = 0; w < KA_WARPS; w++) add(o, sum, *reinterpret_cast<const float4*>(meet + ((size_t)w * COLS + col) * HD + 4 * d4), ml[w][col], M);
+        if (p.cluster == 1) store(col, d4, o, M, sum);
+        else {
+            *reinterpret_cast<float4*>(meet + (size_t)col * HD + 4 * d4) = o;                      // read by this thread alone until here
+            if (d4 == 0) own[col] = make_float2(M, sum);
         }
     }
-    if (n_chunks > 1 && p.arrived) {
-        __threadfence();                                       // this block's chunk, ahead of its arrival
-        __syncthreads();
-        if (tid == 0) last = atomicAdd(p.arrived + unit, 1) == n_chunks - 1;
-        __syncthreads();
-        if (last) {
-            __threadfence();
-            if (tid == 0) p.arrived[unit] = 0;
-            join_by_last(p, unit, n_chunks);
+    if (p.cluster == 1) return;
+    // and the blocks of a cluster in one another's shared memory, each with its part of the values
+    cluster_arrive(); cluster_wait();
+    const int peers = min(p.cluster, n_chunks - peers_from);
+    for (int e = rank * 32 * KA_WARPS + tid; e < COLS * HD / 4; e += p.cluster * 32 * KA_WARPS) {
+        const int col = e / (HD / 4), d4 = e % (HD / 4);
+        if ((c0 + col) / p.t.group >= p.t.B) break;
+        float2 of[KA_CLUSTER];
+        float4 v[KA_CLUSTER];
+#pragma unroll
+        for (int r = 0; r < KA_CLUSTER; r++) {
+            if (r >= peers) break;
+            of[r] = peer_load_f2(smem_u32(&own[col]), r);
+            v[r] = peer_load_f4(smem_u32(meet + (size_t)col * HD + 4 * d4), r);
         }
+        float M = of[0].x, sum = 0.0f;
+#pragma unroll
+        for (int r = 1; r < KA_CLUSTER; r++) if (r < peers) M = fmaxf(M, of[r].x);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int r = 0; r < KA_CLUSTER; r++) if (r < peers) add(o, sum, v[r], of[r], M);
+        store(col, d4, o, M, sum);
     }
-    }
+    cluster_arrive(); cluster_wait();                          // nobody reads this block's shared memory any more
 }
 
 // Attention that the rows draw. grid (128 rows, KV heads, parts of the tiles): a warp holds the unpacked keys of 32 rows and walks the columns that see them,
@@ -708,17 +744,17 @@ __global__ void __launch_bounds__(256) kv4_weight_join_kernel(const KaParams p, 
 }
 
 // what a call launches
-struct KaCall { int mode, blocks, chunks, rows, n_parts; float decay; float* parts; };
+struct KaCall { int cols, chunks, rows, n_parts; float decay; float* parts; };
 
-template <int NG, int MODE>
+template <int NG, int COLS>
 int launch_attention(ibcu_ctx* ctx, const KaParams& p, const KaCall& k) {
     static SmemOptIn opt, opt_w;
-    const size_t smem = KaSmem<NG, MODE>::TOTAL + (MODE == FEW && p.w.rotate ? (size_t)p.t.B * 16 * NG * sizeof(double2) : 0);
-    if (int rc = ibcu_allow_smem(ctx, opt, kv4_attn_kernel<NG, MODE>, smem)) return rc;
-    int rc = ibcu_launch(ctx, kv4_attn_kernel<NG, MODE>, dim3(k.blocks, k.chunks), dim3(32 * KA_WARPS), smem, 1, true, p);
-    if (!rc && k.chunks > 1 && !p.arrived) rc = ibcu_launch(ctx, kv4_join_kernel, dim3(std::min(p.t.cols(), p.t.B * p.t.group), p.c.n_kv * p.t.ntiles), dim3(128), 0, 1, true, p);
+    constexpr bool LARGE = COLS == 16;
+    const size_t smem = KaSmem<NG, COLS>::TOTAL + (!LARGE && p.w.rotate ? (size_t)p.t.B * 16 * NG * sizeof(double2) : 0);
+    if (int rc = ibcu_allow_smem(ctx, opt, kv4_attn_kernel<NG, COLS>, smem)) return rc;
+    int rc = ibcu_launch(ctx, kv4_attn_kernel<NG, COLS>, dim3(p.c.n_kv * p.t.ntiles * k.chunks), dim3(32 * KA_WARPS), smem, p.cluster, true, p);
+    if (!rc && k.chunks > p.cluster) rc = ibcu_launch(ctx, kv4_join_kernel, dim3(std::min(p.t.cols(), p.t.B * p.t.group), p.c.n_kv * p.t.ntiles), dim3(128), 0, 1, true, p);
     if (rc || !p.stat) return rc;
-    constexpr bool LARGE = MODE != FEW;
     if ((rc = ibcu_allow_smem(ctx, opt_w, kv4_weight_kernel<NG, LARGE>, KwSmem<NG, LARGE>::TOTAL))) return rc;
     rc = ibcu_launch(ctx, kv4_weight_kernel<NG, LARGE>, dim3((k.rows + 127) / 128, p.c.n_kv, k.n_parts), dim3(32 * KA_WARPS), KwSmem<NG, LARGE>::TOTAL, 1, true, p, k.decay, k.n_parts > 1 ? k.parts : (float*)nullptr);
     if (!rc && k.n_parts > 1) rc = ibcu_launch(ctx, kv4_weight_join_kernel, dim3((k.rows + 255) / 256, p.c.n_kv), dim3(256), 0, 1, true, p, k.decay, (const float*)k.parts, k.n_parts);
@@ -726,7 +762,7 @@ int launch_attention(ibcu_ctx* ctx, const KaParams& p, const KaCall& k) {
 }
 template <int NG>
 int launch_attention(ibcu_ctx* ctx, const KaParams& p, const KaCall& k) {
-    return k.mode == FEW ? launch_attention<NG, FEW>(ctx, p, k) : k.mode == MANY ? launch_attention<NG, MANY>(ctx, p, k) : launch_attention<NG, WIDE>(ctx, p, k);
+    return k.cols == 16 ? launch_attention<NG, 16>(ctx, p, k) : k.cols == 8 ? launch_attention<NG, 8>(ctx, p, k) : launch_attention<NG, 4>(ctx, p, k);
 }
 
 }  // namespace
@@ -739,7 +775,7 @@ int kv4_attend(ibcu_ctx* ctx, const Kv4& c, float decay, const Kv4Place& at, con
     const Kv4Columns t = { n_heads, group, B, large, ntiles };
     KaCall call;
     memset(&call, 0, sizeof call);
-    call.rows = rows; call.decay = decay;
+    call.rows = rows; call.decay = decay; call.cols = large ? 16 : columns > 4 ? 8 : 4;
     if ((c.hd == 64 || c.hd == 128) && large && c.n_kv * (columns / 128) >= ctx->sm_count / 4) {          // a prompt
         Kv4Columns tp = t;
         tp.ntiles = (int)((columns + 127) / 128) * 8;
@@ -757,26 +793,28 @@ int kv4_attend(ibcu_ctx* ctx, const Kv4& c, float decay, const Kv4Place& at, con
         p.c = c; p.t = tp; p.at = at; p.err = ctx->kern_err;
         return ibcu_launch(ctx, kv4_weight_join_kernel, dim3((rows + 255) / 256, c.n_kv), dim3(256), 0, 1, true, p, decay, (const float*)parts, n_parts);
     }
-    // Four tiles a block once those fill the machine.
-    const int wide_blocks = c.n_kv * ((ntiles + KA_WARPS - 1) / KA_WARPS);
-    call.mode = !large ? FEW : wide_blocks >= ctx->sm_count ? WIDE : MANY;
-    call.blocks = call.mode == WIDE ? wide_blocks : units;
     const int stages = (rows + KA_ROWS - 1) / KA_ROWS;
-    int want = call.mode == WIDE ? 1 : std::max(1, (large ? 2 : 3) * ctx->sm_count / units), chunk;
-    // The last block of a tile joins its chunks where every warp of it has one column of them to read, a launch of its own elsewhere.
-    const bool few_chunks = std::min(columns, (long)t.cols()) <= KA_WARPS;
+    // Blocks an SM that chunks are cut for: what fits, but two where a stage is short beside a block's start (one token of 32 heads over 8 of 64 values after 32767
+    // rows: 14.8 us, 17.3 with three; of 128 values 21.9 with two, 18.4 with three). One cluster of eight, and so no second launch, for contexts that leave each
+    // of its warps four stages at most (after 4000 rows 9.0 against 10.3 us, after 8000 12.4 against 11.9). Clusters of four beyond, since those of eight leave places of the
+    // machine empty (32767 rows: 28 against 20.7 us), unless there is an SM for each block (one KV head: 12.6 against 14.3).
+    int want = std::max(1, (large || (columns <= 4 && ng <= 2) || ng > 4 ? 2 : 3) * ctx->sm_count / units), chunk;
+    if (stages <= KA_CLUSTER * KA_WARPS * 4) want = std::min(want, KA_CLUSTER);
+    if (want > KA_CLUSTER) want = want / 4 * 4;
     ka_plan(rows, want, chunk, call.chunks);
-    if (at.at) call.chunks = std::min(want, stages);                                               // shorter contexts have more, shorter chunks
-    const bool by_last = call.chunks > 1 && call.chunks <= 32 && few_chunks;
+    if (at.at) call.chunks = std::min(want, (stages + KA_WARPS - 1) / KA_WARPS);                   // shorter contexts may have more, shorter chunks
+    int cluster = 1;
+    while (cluster < std::min(call.chunks, call.chunks > KA_CLUSTER && (long)units * call.chunks > ctx->sm_count ? 4 : KA_CLUSTER)) cluster *= 2;
+    call.chunks = (call.chunks + cluster - 1) / cluster * cluster;
+    const int joined = call.chunks / cluster;
     const int row_blocks = (rows + 127) / 128;
     call.n_parts = c.weight && ntiles >= 16 ? std::min(std::min(ntiles, 16), std::max(1, 6 * ctx->sm_count / (row_blocks * c.n_kv))) : 1;
     auto round_up = [](size_t n) { return (n + 255) & ~(size_t)255; };
     const bool frags = large || c.weight;
     const size_t b_qf = frags ? round_up(units * kv4_frags(ng, large) * sizeof(uint4)) : 0, b_qc = frags ? round_up((size_t)units * 16 * sizeof(float)) : 0;
-    const size_t b_stat = c.weight ? round_up((size_t)units * 16 * sizeof(float2)) : 0, b_ml = call.chunks > 1 ? round_up((size_t)units * call.chunks * 16 * sizeof(float2)) : 0;
-    const size_t b_acc = call.chunks > 1 ? round_up((size_t)units * call.chunks * 16 * c.hd * sizeof(float)) : 0, b_parts = call.n_parts > 1 ? round_up((size_t)call.n_parts * c.n_kv * c.max_rows * sizeof(float)) : 0;
+    const size_t b_stat = c.weight ? round_up((size_t)units * 16 * sizeof(float2)) : 0, b_ml = joined > 1 ? round_up((size_t)units * joined * 16 * sizeof(float2)) : 0;
+    const size_t b_acc = joined > 1 ? round_up((size_t)units * joined * 16 * c.hd * sizeof(float)) : 0, b_parts = call.n_parts > 1 ? round_up((size_t)call.n_parts * c.n_kv * c.max_rows * sizeof(float)) : 0;
     if (int rc = ibcu_reserve(ctx, &ctx->scratch, &ctx->scratch_bytes, b_qf + b_qc + b_stat + b_ml + b_acc + b_parts)) return rc;
-    if (by_last) { if (int rc = ibcu_reserve_zeroed(ctx, &ctx->kv4_arrived, &ctx->kv4_arrived_bytes, (size_t)units * sizeof(int))) return rc; }
     char* s = (char*)ctx->scratch;
     auto take = [&](size_t n) { char* r = s; s += n; return r; };
     KaParams p;
@@ -787,8 +825,7 @@ int kv4_attend(ibcu_ctx* ctx, const Kv4& c, float decay, const Kv4Place& at, con
     p.stat = (float2*)take(b_stat); if (!c.weight) p.stat = nullptr;
     p.pml = (float2*)take(b_ml); p.pacc = (float*)take(b_acc);
     call.parts = (float*)take(b_parts);
-    p.arrived = by_last ? (int*)ctx->kv4_arrived : nullptr;
-    p.out = out; p.want = want; p.grid_chunks = call.chunks; p.err = ctx->kern_err;
+    p.out = out; p.want = want; p.grid_chunks = call.chunks; p.cluster = cluster; p.err = ctx->kern_err;
     if (large) { if (int rc = kv4_prepare(ctx, c, t, at, p.w)) return rc; }
     switch (ng) {
         case 1: return launch_attention<1>(ctx, p, call);

@@ -127,6 +127,20 @@ __device__ __forceinline__ uint32_t peer_load_u32(uint32_t addr, uint32_t rank) 
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(remote) : "memory");
     return v;
 }
+__device__ __forceinline__ float2 peer_load_f2(uint32_t addr, uint32_t rank) {
+    uint32_t remote;
+    float2 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(remote) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 peer_load_f4(uint32_t addr, uint32_t rank) {
+    uint32_t remote;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote) : "memory");
+    return v;
+}
 // ── pairs of blocks (cta_group::2) ──
 __device__ __forceinline__ uint32_t peer_address(uint32_t addr, uint32_t rank) {
     uint32_t remote;
