@@ -16,109 +16,149 @@ namespace {
 
 __device__ __forceinline__ float scale_at(const __half* p) { return __half2float(__ushort_as_half(__ldcg(reinterpret_cast<const unsigned short*>(p)))); }
 
-// One launch ahead of the attention of more than eight columns, and that of ibcu_kv4_write: blocks below qblocks turn a tile of 16 columns into
-// fragments or their part of an image, the others write the rows of a position, whose heads share its angles.
-struct PrepParams { Kv4 c; Kv4Columns t; Kv4Place at; Kv4Prep w; int qblocks, wparts; int* err; };
+// One launch ahead of the attention of more than eight columns, and that of ibcu_kv4_write: blocks below qblocks turn a tile of 16 columns of every
+// qparts-th KV head into fragments or their part of an image, the others write the rows of a position. Heads share a position's angles. Bound by
+// instructions: eighteen a value of a row, PREPQ a value of a query.
+struct PrepParams { Kv4 c; Kv4Columns t; Kv4Place at; Kv4Prep w; int qblocks, qparts, wparts; int* err; };
 
+template <int NG>
 __global__ void __launch_bounds__(128) kv4_prep_kernel(const PrepParams p) {
-    extern __shared__ __align__(16) double2 turn[];           // [positions of the block][hd / 2]
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hd = p.c.hd, half = hd / 2, ng = hd / 32;
+    constexpr int HD = 32 * NG, HALF = HD / 2, JT = (NG + 3) / 4;
+    extern __shared__ __align__(16) double2 turn[];           // [positions of the block][HALF]
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const bool queries = (int)blockIdx.x < p.qblocks;
-    const int kvh = blockIdx.x / p.t.ntiles, c0 = blockIdx.x % p.t.ntiles * 16, wb = blockIdx.x - p.qblocks;
-    const int b0 = queries ? c0 / p.t.group : wb / p.wparts, b1 = queries ? min(p.t.B - 1, (c0 + 15) / p.t.group) : b0;
+    // a block of a few rows is short: no division that it can do without
+    int tile = 0, c0 = 0, b0 = blockIdx.x - p.qblocks, b1, part = 0;
+    if (queries) {
+        tile = blockIdx.x % p.t.ntiles;
+        c0 = tile * 16;
+        b0 = c0 / p.t.group;
+        b1 = min(p.t.B - 1, (c0 + 15) / p.t.group);
+    } else {
+        if (p.wparts > 1) { part = b0 % p.wparts; b0 /= p.wparts; }
+        b1 = b0;
+    }
     int row0 = p.at.row0, pos0 = p.at.pos0;
     if (p.at.at) {
         pdl_wait();
         if (!kv4_place(p.at, p.t.B, p.c.max_rows, p.err, row0, pos0)) return;
     }
-    if (p.w.rotate) kv4_angles(turn, b1 - b0 + 1, pos0 + b0, hd, p.w.log2_theta);
+    if (p.w.rotate) kv4_angles(turn, b1 - b0 + 1, pos0 + b0, HD, p.w.log2_theta);
     if (!p.at.at) pdl_wait();
     pdl_launch_dependents();                                  // not earlier: the attention reads rows of earlier calls ahead of its own wait
     __syncthreads();
+    if ((NG == 2 || NG == 4) && queries && p.t.large == 2) {
+        // a warp has four columns, eight lanes each, whose pieces are whole sectors of the image
+        const int col = warp * 4 + (lane >> 3), pl = lane & 7, b = (c0 + col) / p.t.group, head = (c0 + col) % p.t.group, at = tile % 8 * 16 + col;
+        const bool on = b < p.t.B;
+        const double2* angles = p.w.rotate ? turn + (b - b0) * HALF : nullptr;
+#pragma unroll 2
+        for (int kvh = blockIdx.x / p.t.ntiles; kvh < p.c.n_kv; kvh += p.qparts) {
+            const size_t unit = (size_t)kvh * p.t.ntiles + tile;
+            const float* src = p.w.q + ((size_t)b * p.t.n_heads + (size_t)kvh * p.t.group + head) * HD;
+            constexpr int PL = NG < 4 ? 1 : NG / 2;           // pieces of a lane
+            float x[PL][8];
+            uint32_t m = 0;
+#pragma unroll
+            for (int u = 0; u < PL; u++) {
+                const int piece = pl + 8 * u, i = piece % NG * 32 + piece / NG * 8;
+                kv4_query(x[u], src + i, on, angles ? angles + i / 2 : nullptr);
+#pragma unroll
+                for (int n = 0; n < 8; n++) m = max(m, __float_as_uint(x[u][n]) & 0x7FFFFFFFu);
+            }
+#pragma unroll
+            for (int o = 1; o < 8; o *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const Kv4Up up = kv4_up(m, HD);
+            if (pl == 0) p.w.qc[unit * 16 + col] = up.back;
+            unsigned char* image = reinterpret_cast<unsigned char*>(p.w.qf) + unit / 8 * (NG * 16384) + at * 128 + ((pl ^ (at & 7)) << 4);
+#pragma unroll
+            for (int u = 0; u < PL; u++) {
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float a = x[u][i] * up.a * up.b, z = x[u][i + 4] * up.a * up.b;
+                    const __half2 h = __floats2half2_rn(a, z), l = __floats2half2_rn(a - __low2float(h), z - __high2float(h));
+                    hi[i] = *reinterpret_cast<const uint32_t*>(&h);
+                    lo[i] = *reinterpret_cast<const uint32_t*>(&l);
+                }
+                *reinterpret_cast<uint4*>(image + u * 16384) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                *reinterpret_cast<uint4*>(image + (NG / 2 + u) * 16384) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
+        }
+        return;
+    }
     if (queries) {
         // lane = column g and column g + 8, piece t: values 8t..8t+7 of every group; a warp has every fourth group
-        __shared__ uint32_t amax[4][16];
+        __shared__ uint32_t amax[2][4][16];
         const int g = lane >> 2, t = lane & 3;
-        float x[2][2][8];
-        uint32_t m[2] = { 0, 0 };
+        int b[2], head[2];
 #pragma unroll
-        for (int n = 0; n < 2; n++) {
-            const int col = c0 + g + 8 * n, b = col / p.t.group;
-            const bool on = b < p.t.B;
-            const float* src = p.w.q + ((size_t)b * p.t.n_heads + (size_t)kvh * p.t.group + col % p.t.group) * hd + 8 * t;
-            const double2* angles = on && p.w.rotate ? turn + (b - b0) * half + 4 * t : nullptr;
+        for (int n = 0; n < 2; n++) { const int col = c0 + g + 8 * n; b[n] = col / p.t.group; head[n] = col % p.t.group; }
+        int turns = 0;
+        for (int kvh = blockIdx.x / p.t.ntiles; kvh < p.c.n_kv; kvh += p.qparts, turns ^= 1) {
+            const size_t unit = (size_t)kvh * p.t.ntiles + tile;
+            float x[2][JT][8];
+            uint32_t m[2] = { 0, 0 };
 #pragma unroll
-            for (int jj = 0; jj < 2; jj++) {
-                const int j = warp + 4 * jj;
-                if (j >= ng) break;
-                kv4_query(x[n][jj], src + 32 * j, on, angles ? angles + 16 * j : nullptr);
+            for (int n = 0; n < 2; n++) {
+                const bool on = b[n] < p.t.B;
+                const float* src = p.w.q + ((size_t)b[n] * p.t.n_heads + (size_t)kvh * p.t.group + head[n]) * HD + 8 * t;
+                const double2* angles = p.w.rotate ? turn + (b[n] - b0) * HALF + 4 * t : nullptr;
 #pragma unroll
-                for (int i = 0; i < 8; i++) m[n] = max(m[n], __float_as_uint(x[n][jj][i]) & 0x7FFFFFFFu);
-            }
-            m[n] = max(m[n], __shfl_xor_sync(0xffffffffu, m[n], 1));
-            m[n] = max(m[n], __shfl_xor_sync(0xffffffffu, m[n], 2));
-            if (t == 0) amax[warp][g + 8 * n] = m[n];
-        }
-        __syncthreads();
+                for (int jj = 0; jj < JT; jj++) {
+                    const int j = warp + 4 * jj;
+                    if (j >= NG) break;
+                    kv4_query(x[n][jj], src + 32 * j, on, angles ? angles + 16 * j : nullptr);
 #pragma unroll
-        for (int n = 0; n < 2; n++) {
-#pragma unroll
-            for (int w = 0; w < 4; w++) m[n] = max(m[n], amax[w][g + 8 * n]);
-            const Kv4Up up = kv4_up(m[n], hd);
-            if (warp == 0 && t == 0) p.w.qc[(size_t)blockIdx.x * 16 + g + 8 * n] = up.back;
-#pragma unroll
-            for (int jj = 0; jj < 2; jj++)
-#pragma unroll
-                for (int i = 0; i < 8; i++) x[n][jj][i] = x[n][jj][i] * up.a * up.b;
-        }
-#pragma unroll
-        for (int jj = 0; jj < 2; jj++) {
-            const int j = warp + 4 * jj;
-            if (j >= ng) break;
-            if (p.t.large == 2) {
-                const int piece = t * ng + j;
-                unsigned char* image = reinterpret_cast<unsigned char*>(p.w.qf) + (size_t)(blockIdx.x / 8) * (ng * 16384) + (piece >> 3) * 16384;
-#pragma unroll
-                for (int n = 0; n < 2; n++) {
-                    const int col = blockIdx.x % 8 * 16 + g + 8 * n;
-                    uint32_t hi[4], lo[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const __half2 h = __floats2half2_rn(x[n][jj][i], x[n][jj][i + 4]), l = __floats2half2_rn(x[n][jj][i] - __low2float(h), x[n][jj][i + 4] - __high2float(h));
-                        hi[i] = *reinterpret_cast<const uint32_t*>(&h);
-                        lo[i] = *reinterpret_cast<const uint32_t*>(&l);
-                    }
-                    unsigned char* at = image + col * 128 + (((piece & 7) ^ (col & 7)) << 4);
-                    *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    *reinterpret_cast<uint4*>(at + ng / 2 * 16384) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    for (int i = 0; i < 8; i++) m[n] = max(m[n], __float_as_uint(x[n][jj][i]) & 0x7FFFFFFFu);
                 }
-            } else {
-                uint4* qf = p.w.qf + blockIdx.x * kv4_frags(ng, true) + lane;
+                m[n] = max(m[n], __shfl_xor_sync(0xffffffffu, m[n], 1));
+                m[n] = max(m[n], __shfl_xor_sync(0xffffffffu, m[n], 2));
+                if (t == 0) amax[turns][warp][g + 8 * n] = m[n];
+            }
+            __syncthreads();
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+#pragma unroll
+                for (int w = 0; w < 4; w++) m[n] = max(m[n], amax[turns][w][g + 8 * n]);
+                const Kv4Up up = kv4_up(m[n], HD);
+                if (warp == 0 && t == 0) p.w.qc[unit * 16 + g + 8 * n] = up.back;
+#pragma unroll
+                for (int jj = 0; jj < JT; jj++)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) x[n][jj][i] = x[n][jj][i] * up.a * up.b;
+            }
+#pragma unroll
+            for (int jj = 0; jj < JT; jj++) {
+                const int j = warp + 4 * jj;
+                if (j >= NG) break;
+                uint4* qf = p.w.qf + unit * kv4_frags(NG, true) + lane;
 #pragma unroll
                 for (int s = 0; s < 2; s++) {
                     uint32_t hi[2][2], lo[2][2];
 #pragma unroll
                     for (int n = 0; n < 2; n++) kv4_pieces(x[n][jj], s, hi[n], lo[n]);
                     qf[(j * 2 + s) * 32] = make_uint4(hi[0][0], hi[1][0], hi[0][1], hi[1][1]);
-                    qf[((ng + j) * 2 + s) * 32] = make_uint4(lo[0][0], lo[1][0], lo[0][1], lo[1][1]);
+                    qf[((NG + j) * 2 + s) * 32] = make_uint4(lo[0][0], lo[1][0], lo[0][1], lo[1][1]);
                 }
             }
         }
         return;
     }
-    // heads wparts apart; a thread has four values of a row, up to four times ahead of their use
-    const int quads = hd / 4, heads = (p.c.n_kv - wb % p.wparts + p.wparts - 1) / p.wparts, total = 2 * heads * quads;
-    for (int e0 = tid; e0 < total; e0 += 512) {
-        float x[4][4];
+    // heads wparts apart; a thread has eight values of a row, twice ahead of their use
+    constexpr int OCTS = HD / 8;
+    const int keys = (p.wparts > 1 ? 1 : p.c.n_kv) * OCTS;     // wparts: 1, or the KV heads
+    for (int e0 = tid; e0 < 2 * keys; e0 += 256) {
+        float x[2][8];
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const int e = e0 + u * 128, f = e < heads * quads ? e : e - heads * quads, h = wb % p.wparts + f / quads * p.wparts;
-            if (e < total) kv4_load_four(x[u], (e < heads * quads ? p.w.k : p.w.v) + ((size_t)b0 * p.c.n_kv + h) * hd + f % quads * 4);
+        for (int u = 0; u < 2; u++) {
+            const int e = e0 + u * 128, f = e < keys ? e : e - keys;
+            if (e < 2 * keys) kv4_load_eight(x[u], (e < keys ? p.w.k : p.w.v) + ((size_t)b0 * p.c.n_kv + part + f / OCTS * p.wparts) * HD + f % OCTS * 8);
         }
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const int e = e0 + u * 128, f = e < heads * quads ? e : e - heads * quads, h = wb % p.wparts + f / quads * p.wparts;
-            if (e < total) kv4_write_four(p.c, x[u], e < heads * quads, h, row0 + b0, f % quads * 4, p.w.rotate ? turn : nullptr);
+        for (int u = 0; u < 2; u++) {
+            const int e = e0 + u * 128, f = e < keys ? e : e - keys;
+            if (e < 2 * keys) kv4_write_eight<NG>(p.c, x[u], e < keys, part + f / OCTS * p.wparts, row0 + b0, f % OCTS * 8, p.w.rotate ? turn : nullptr);
         }
     }
 }
@@ -345,10 +385,12 @@ double log2_of(float theta) { return theta > 0.0f ? log2((double)theta) : 0.0; }
 }  // namespace
 
 int kv4_prepare(ibcu_ctx* ctx, const Kv4& c, const Kv4Columns& t, const Kv4Place& at, const Kv4Prep& w) {
-    PrepParams p = { c, t, at, w, w.q ? c.n_kv * t.ntiles : 0, t.B <= 8 ? c.n_kv : 1, ctx->kern_err };
+    PrepParams p = { c, t, at, w, 0, std::min(c.n_kv, (4 * ctx->sm_count + t.ntiles - 1) / t.ntiles), t.B <= 8 ? c.n_kv : 1, ctx->kern_err };
+    if (w.q) p.qblocks = p.qparts * t.ntiles;
     const int nb = w.q ? std::min(16, 15 / t.group + 2) : 1;  // positions that a block may have to do with
     const size_t smem = w.rotate ? (size_t)nb * c.hd / 2 * sizeof(double2) : 0;
-    return ibcu_launch(ctx, kv4_prep_kernel, dim3(p.qblocks + (w.k ? t.B * p.wparts : 0)), dim3(128), smem, 1, true, p);
+    auto kern = c.hd == 32 ? kv4_prep_kernel<1> : c.hd == 64 ? kv4_prep_kernel<2> : c.hd == 96 ? kv4_prep_kernel<3> : c.hd == 128 ? kv4_prep_kernel<4> : c.hd == 192 ? kv4_prep_kernel<6> : kv4_prep_kernel<8>;
+    return ibcu_launch(ctx, kern, dim3(p.qblocks + (w.k ? t.B * p.wparts : 0)), dim3(128), smem, 1, true, p);
 }
 
 extern "C" int ibcu_kv4_write(ibcu_ctx* ctx, const ibcu_kv4_t* cache, const float* k, const float* v, int row0, int pos0, int B, float theta) {

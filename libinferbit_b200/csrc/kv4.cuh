@@ -60,38 +60,52 @@ __device__ __forceinline__ __half kv4_scale(uint32_t amax_bits, float& inv) {
     if (amax_bits >= 0x7F800000u) { inv = 0.0f; return __ushort_as_half(0x7FFF); }          // NaN: the row says so wherever it is seen
     const float s = __fmul_rn(__uint_as_float(amax_bits), 1.0f / 7.0f);
     const __half h = __float2half_rn(fminf(s, 8192.0f));                                    // seven of them, the largest value, are an fp16 too
-    inv = __half2float(h) > 0.0f ? __fdiv_rn(1.0f, __half2float(h)) : 0.0f;
+    inv = __half2float(h) > 0.0f ? __frcp_rn(__half2float(h)) : 0.0f;
     return h;
 }
-__device__ __forceinline__ uint32_t kv4_code(float x, float inv) {
-    const float q = inv > 0.0f ? fminf(fmaxf(rintf(__fmul_rn(x, inv)), -7.0f), 7.0f) : 0.0f;
-    return (uint32_t)((int)q + 8);
-}
-// four values of a row, at any address
-__device__ __forceinline__ void kv4_load_four(float (&x)[4], const float* src) {
-    if (((uintptr_t)src & 15) == 0) { const float4 v = __ldcg(reinterpret_cast<const float4*>(src)); x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w; }
-    else { x[0] = __ldcg(src); x[1] = __ldcg(src + 1); x[2] = __ldcg(src + 2); x[3] = __ldcg(src + 3); }
-}
-// Values i..i+3 of a key or value row of head h into the cache. Eight neighbouring lanes have a group, whose largest magnitude they
-// share. turn: the position's angles, or NULL.
-__device__ __forceinline__ void kv4_write_four(const Kv4& c, float (&x)[4], bool key, int h, int r, int i, const double2* turn) {
-    const int ng = c.hd / 32, lane = threadIdx.x & 31;
-    if (key && turn) { kv4_turn(x[0], x[1], turn[i / 2]); kv4_turn(x[2], x[3], turn[i / 2 + 1]); }
-    uint32_t m = 0;
-#pragma unroll
-    for (int u = 0; u < 4; u++) m = max(m, __float_as_uint(x[u]) & 0x7FFFFFFFu);
-    const unsigned lanes = 0xFFu << (lane & 24);
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(lanes, m, o));
-    float inv;
-    const __half s = kv4_scale(m, inv);
+// Eight codes. What is added lifts a value's integer part to the lowest bits, rounded to even as rint does.
+__device__ __forceinline__ uint32_t kv4_codes(const float (&x)[8], float inv) {
     uint32_t w = 0;
 #pragma unroll
-    for (int u = 0; u < 4; u++) w |= kv4_code(x[u], inv) << (4 * u);
+    for (int u = 0; u < 8; u++) w |= (__float_as_uint(__fadd_rn(fminf(fmaxf(__fmul_rn(x[u], inv), -7.0f), 7.0f), 12582920.0f)) & 15u) << (4 * u);
+    return inv > 0.0f ? w : 0x88888888u;
+}
+// eight values of a row, at any address
+__device__ __forceinline__ void kv4_load_eight(float (&x)[8], const float* src) {
+    if (((uintptr_t)src & 15) == 0) {                          // else every lane's sector is fetched eight times
+        const float4 a = __ldcg(reinterpret_cast<const float4*>(src)), b = __ldcg(reinterpret_cast<const float4*>(src) + 1);
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = __ldcg(src + i);
+    }
+}
+// Values i..i+7 of a key or value row of head h into the cache. Four neighbouring lanes have a group, whose largest magnitude they
+// share. turn: the position's angles, or NULL.
+template <int NG>
+__device__ __forceinline__ void kv4_write_eight(const Kv4& c, float (&x)[8], bool key, int h, int r, int i, const double2* turn) {
+    const int lane = threadIdx.x & 31;
+    if (key && turn) {
+#pragma unroll
+        for (int u = 0; u < 8; u += 2) kv4_turn(x[u], x[u + 1], turn[(i + u) / 2]);
+    }
+    uint32_t m = 0;
+#pragma unroll
+    for (int u = 0; u < 8; u++) m = max(m, __float_as_uint(x[u]) & 0x7FFFFFFFu);
+    const unsigned lanes = 0xFu << (lane & 28);
+    m = max(m, __shfl_xor_sync(lanes, m, 1));
+    m = max(m, __shfl_xor_sync(lanes, m, 2));
+    float inv;
+    const __half s = kv4_scale(m, inv);
+    const uint32_t w = kv4_codes(x, inv);
     const size_t row = c.row(h, r);
-    const int place = key ? kv4_key_place(i, ng) : kv4_value_place(i, ng);                 // four values stay together in both orders
-    *reinterpret_cast<uint16_t*>((key ? c.k : c.v) + row * (c.hd / 2) + place / 2) = (uint16_t)w;
-    if ((i & 31) == 0) c.scale[row * 2 * ng + (key ? 0 : ng) + i / 32] = s;
+    uint8_t* to = (key ? c.k : c.v) + row * (16 * NG);
+    if (key) *reinterpret_cast<uint32_t*>(to + kv4_key_place(i, NG) / 2) = w;               // a word of the key's order, two pieces of the value's
+    else {
+        *reinterpret_cast<uint16_t*>(to + kv4_value_place(i, NG) / 2) = (uint16_t)w;
+        *reinterpret_cast<uint16_t*>(to + kv4_value_place(i + 4, NG) / 2) = (uint16_t)(w >> 16);
+    }
+    if ((i & 31) == 0) c.scale[row * 2 * NG + (key ? 0 : NG) + i / 32] = s;
     if (key && i == 0 && c.weight) c.weight[row] = 0.0f;
 }
 
@@ -99,8 +113,10 @@ __device__ __forceinline__ void kv4_write_four(const Kv4& c, float (&x)[4], bool
 // values 8t..8t+7 of a group of one query (src: the group's first value), turned
 __device__ __forceinline__ void kv4_query(float (&x)[8], const float* src, bool on, const double2* turn) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = on ? __ldcg(src + i) : 0.0f;
-    if (on && turn) {
+    for (int i = 0; i < 8; i++) x[i] = 0.0f;
+    if (!on) return;
+    kv4_load_eight(x, src);
+    if (turn) {
 #pragma unroll
         for (int i = 0; i < 8; i += 2) kv4_turn(x[i], x[i + 1], turn[i / 2]);
     }

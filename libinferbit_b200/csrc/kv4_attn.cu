@@ -24,7 +24,7 @@
 // memory; up to eight chunks are one cluster, the results of more clusters are put together by a launch of its own. (32 heads of 128 values over
 // 8 KV heads, one token after 512 rows: 6.4 us, against 8.6 with a second launch and 9.7 with the last block of a tile to finish doing it; after 4000: 9.0
 // against 10.3 with clusters of four and a second launch.)
-// What bounds it: instructions, 4 codes a lane being five to unpack. After 32767 rows 18.4 us, 2.1 TB/s of cache, of which 11 us are the start, the ring's first
+// What bounds it: instructions, of which a word of eight codes takes nine to unpack. After 32767 rows 18.4 us, 2.1 TB/s of cache, of which 11 us are the start, the ring's first
 // copies and the joins; after 262143 rows 78 us, 3.9 TB/s.
 #include "kv4.cuh"
 #include "tc_common.cuh"
@@ -308,12 +308,12 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (COLS == 16 ? 2 : 
         __syncthreads();
         if (p.w.k) {                                                                               // the call's rows of this chunk
             const int r0 = max(t0, row0), r1 = min(t1, row0 + p.t.B);
-            for (int e = tid; e < (r1 - r0) * 2 * (HD / 4); e += 32 * KA_WARPS) {
-                const int f = e / (HD / 4), r = r0 + f / 2, b = r - row0;
+            for (int e = tid; e < (r1 - r0) * 2 * (HD / 8); e += 32 * KA_WARPS) {
+                const int f = e / (HD / 8), r = r0 + f / 2, b = r - row0, i = e % (HD / 8) * 8;
                 const bool key = f % 2 == 0;
-                float x4[4];
-                kv4_load_four(x4, (key ? p.w.k : p.w.v) + ((size_t)b * p.c.n_kv + kvh) * HD + e % (HD / 4) * 4);
-                kv4_write_four(p.c, x4, key, kvh, r, e % (HD / 4) * 4, p.w.rotate ? turn + b * (HD / 2) : nullptr);
+                float x[8];
+                kv4_load_eight(x, (key ? p.w.k : p.w.v) + ((size_t)b * p.c.n_kv + kvh) * HD + i);
+                kv4_write_eight<NG>(p.c, x, key, kvh, r, i, p.w.rotate ? turn + b * (HD / 2) : nullptr);
             }
             asm volatile("fence.proxy.async.global;" ::: "memory");                                // the bulk copies read them
         }
