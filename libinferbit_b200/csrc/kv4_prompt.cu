@@ -7,7 +7,7 @@
 // (On mma.sync the scales stay FP32 factors outside the products, two instructions a step, but their rate is a third; 16
 // columns share an unpacked row there, 128 here. A prompt of 2048, 32 heads of 128 over 8: 370 us that way.)
 //
-// Warps: 4 softmax, a thread a column; 4 that turn key codes into the pieces of K', 4 for V' (transposed: the rows are the
+// Warps: 8 softmax, two threads a column; 4 that turn key codes into the pieces of K', 4 for V' (transposed: the rows are the
 // contraction); 1 issues the products, 1 the copies. Everything is double buffered, and S of the next rows is computed while the softmax is at these.
 // A V' of a row with a NaN scale would reach columns that do not see the row (0 * NaN), so NaN goes into the row's K' instead, and with it
 // into every column that does see it.
@@ -18,7 +18,7 @@
 namespace {
 
 constexpr int PK_ROWS = 64, PK_COLS = 128, PK_RAW = 3;
-constexpr int PK_KEY_WARP = 4, PK_VALUE_WARP = 8, PK_MMA_WARP = 12, PK_TMA_WARP = 13, PK_THREADS = 14 * 32;
+constexpr int PK_KEY_WARP = 8, PK_VALUE_WARP = 12, PK_MMA_WARP = 16, PK_TMA_WARP = 17, PK_THREADS = 18 * 32;
 constexpr float PK_LOW = -3.0e38f, PK_SLACK = 1.9f;            // see kv4_attn.cu
 
 struct PkParams {
@@ -37,6 +37,7 @@ struct PkShared {
     unsigned long long q_full, raw_full[PK_RAW], raw_empty[PK_RAW], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], s_empty[2], p_full[2], pv_done[2], drained;
     uint32_t tmem_base;
     int abort_flag;
+    float meet[2][PK_COLS];                                    // maxima, at last sums, of a column's two threads
 };
 
 __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
@@ -44,6 +45,13 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uin
                  "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
                  :: "r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
 }
+// whether any thread of the pair of warps says so
+__device__ __forceinline__ bool pair_any(int id, bool x) {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\tbarrier.cta.red.or.pred q, %1, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(r) : "r"(id), "r"((uint32_t)x) : "memory");
+    return r;
+}
+__device__ __forceinline__ void pair_sync(int id) { asm volatile("barrier.cta.sync %0, 64;" :: "r"(id) : "memory"); }
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 __device__ __forceinline__ __half2 half2_of(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
@@ -51,7 +59,11 @@ __device__ __forceinline__ __half2 half2_of(uint32_t u) { return *reinterpret_ca
 // The eight codes of a word less their bias of 8, as pairs 0 and 4, 1 and 5, 2 and 6, 3 and 7: under the exponent of 1024 a code n is the fp16 1024 + n
 __device__ __forceinline__ void codes_of(uint32_t w, __half2 (&f)[4]) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) f[i] = __hsub2(half2_of((w >> (4 * i) & 0x000F000Fu) | 0x64006400u), half2_of(0x64086408u));
+    for (int i = 0; i < 4; i++) {
+        uint32_t n;                                            // (w >> 4 i & mask) | base as one instruction
+        asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(n) : "r"(w >> (4 * i)), "r"(0x000F000Fu), "r"(0x64006400u));
+        f[i] = __hsub2(half2_of(n), half2_of(0x64086408u));
+    }
 }
 // codes times scales as two pieces, exact together
 __device__ __forceinline__ void held_pieces(const __half2 f, const __half2 scale, uint32_t& high, uint32_t& low) {
@@ -97,11 +109,11 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
     const int kvh = blockIdx.x % p.c.n_kv, tile = p.tiles - 1 - blockIdx.x / p.c.n_kv, unit = kvh * p.tiles + tile, c0 = tile * PK_COLS;          // most rows first
     if (tid == 0) {
         auto init = [&](unsigned long long& b, int n) { mbar_init(smem_u32(&b), n); };
-        init(sh->q_full, 4); init(sh->drained, 1);
+        init(sh->q_full, 8); init(sh->drained, 1);
         for (int i = 0; i < PK_RAW; i++) { init(sh->raw_full[i], 1); init(sh->raw_empty[i], 8); }
         for (int i = 0; i < 2; i++) {
             init(sh->k_full[i], 4); init(sh->k_empty[i], 1); init(sh->v_full[i], 4); init(sh->v_empty[i], 1);
-            init(sh->s_full[i], 1); init(sh->s_empty[i], 4); init(sh->p_full[i], 4); init(sh->pv_done[i], 1);
+            init(sh->s_full[i], 1); init(sh->s_empty[i], 8); init(sh->p_full[i], 8); init(sh->pv_done[i], 1);
         }
         sh->abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -202,7 +214,7 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
                 }
             } else {
                 // lanes: four pairs of rows by the eight pieces of a row; transposed, value 32 j + 4 g + i is line (4 j + i) 8 + g of 64 rows
-#pragma unroll
+#pragma unroll 1
                 for (int u = 0; u < 2; u++) {
                     const int chunk = w + 4 * u, g = lane >> 2, a = 8 * chunk + 2 * (lane & 3);
                     uint32_t va[NG / 2], vb[NG / 2], sa[NG], sb[NG];
@@ -241,66 +253,67 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
             if (++s == PK_RAW) { s = 0; ph ^= 1; }
         }
     } else {
-        const int c = c0 + tid, b_col = c / p.t.group;
+        // A column has two threads, of warps w and w + 4: each has 32 of the rows, half of the queries' copy and of the outputs.
+        const int quarter = warp & 3, half = warp >> 2, own = quarter * 32 + lane, c = c0 + own, b_col = c / p.t.group;
         const bool on = b_col < p.t.B;
-        const int lim = row0 + b_col, lim0 = row0 + (c0 + (tid & ~31)) / p.t.group;              // last rows that this column, the warp's first column, see
-        const float f = on ? __ldcg(p.qc + (size_t)unit * PK_COLS + tid) : 0.0f;
-        const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+        const int lim = row0 + b_col, lim0 = row0 + (c0 + quarter * 32) / p.t.group;             // last rows that this column, the warp's first column, see
+        const float f = on ? __ldcg(p.qc + (size_t)unit * PK_COLS + own) : 0.0f;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         // the queries' pieces into tensor memory: the scores' A operand (from shared memory it would be read again for every 64 rows, and with what the
         // dequantisers write that is more than shared memory gives)
         if (n) {
-            const unsigned char* image = p.image + (size_t)unit * S::IMAGE + tid * 128;
+            const unsigned char* image = p.image + (size_t)unit * S::IMAGE + own * 128 + half * S::KB * 16384;
 #pragma unroll 1
-            for (int part = 0; part < 2; part += 1)
-#pragma unroll 1
-                for (int kb = 0; kb < S::KB; kb++) {
-                    uint32_t x[32];
+            for (int kb = 0; kb < S::KB; kb++) {
+                uint32_t x[32];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const uint4 v = __ldcg(reinterpret_cast<const uint4*>(image + (part * S::KB + kb) * 16384 + ((e ^ (tid & 7)) << 4)));
-                        x[4 * e] = v.x; x[4 * e + 1] = v.y; x[4 * e + 2] = v.z; x[4 * e + 3] = v.w;
-                    }
-                    tmem_st32(tmem_q + lanes + part * (S::HD / 2) + kb * 32, x);
+                for (int e = 0; e < 8; e++) {
+                    const uint4 v = __ldcg(reinterpret_cast<const uint4*>(image + kb * 16384 + ((e ^ (own & 7)) << 4)));
+                    x[4 * e] = v.x; x[4 * e + 1] = v.y; x[4 * e + 2] = v.z; x[4 * e + 3] = v.w;
                 }
+                tmem_st32(tmem_q + lanes + half * (S::HD / 2) + kb * 32, x);
+            }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&sh->q_full));
         }
         float m = PK_LOW, l = 0.0f;
-        bool wide = false, alive = true;
+        bool wide = false, alive = true;                       // not alive: a wait gave up; the barriers of the pair are still both warps'
         for (int i = 0; i < n; i++) {
-            const int b = i & 1;
+            const int b = i & 1, from = i * PK_ROWS + half * 32;
             const uint32_t ph = (uint32_t)(i >> 1) & 1u;
-            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->s_full[b]), ph, abort_flag, 10))) { alive = false; break; }
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            uint32_t s[64];
-            tmem_ld32(tmem_s + lanes + b * PK_ROWS, s);
-            tmem_ld32(tmem_s + lanes + b * PK_ROWS + 32, s + 32);
-            tmem_wait_ld(s);
-            tmem_wait_ld(s + 32);
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&sh->s_empty[b]));
-            if (i * PK_ROWS + PK_ROWS - 1 > lim0) {
+            alive = alive && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->s_full[b]), ph, abort_flag, 10));
+            uint32_t s[32];
+            float top = PK_LOW;
+            if (alive) {
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                tmem_ld32(tmem_s + lanes + b * PK_ROWS + half * 32, s);
+                tmem_wait_ld(s);
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sh->s_empty[b]));
+                if (from + 31 > lim0) {
 #pragma unroll
-                for (int u = 0; u < 64; u++) if (i * PK_ROWS + u > lim) s[u] = 0xFF800000u;
+                    for (int u = 0; u < 32; u++) if (from + u > lim) s[u] = 0xFF800000u;
+                }
+                float t4[4] = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };
+#pragma unroll
+                for (int u = 0; u < 32; u++) t4[u & 3] = fmaxf(t4[u & 3], __uint_as_float(s[u]));
+                top = fmaxf(PK_LOW, fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * f);
             }
-            float t4[4] = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };
-#pragma unroll
-            for (int u = 0; u < 64; u++) t4[u & 3] = fmaxf(t4[u & 3], __uint_as_float(s[u]));
-            const float top = fmaxf(PK_LOW, fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * f);
-            if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->pv_done[b]), ph ^ 1u, abort_flag, 11))) { alive = false; break; }          // this half of P is free
-            if (__any_sync(0xffffffffu, top > m + PK_SLACK)) {
-                const float now = fmaxf(m, top), corr = ex2(m - now);
+            if (pair_any(1 + quarter, top > m + PK_SLACK)) {
+                sh->meet[half][own] = top;
+                pair_sync(1 + quarter);
+                const float now = fmaxf(m, fmaxf(top, sh->meet[half ^ 1][own])), corr = ex2(m - now);
                 m = now;
                 l *= corr;
                 wide = fabsf(now) > 524288.0f;
-                if (i) {
-                    if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->pv_done[b ^ 1]), (uint32_t)((i - 1) >> 1) & 1u, abort_flag, 12))) { alive = false; break; }
+                alive = alive && (!i || __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->pv_done[b ^ 1]), (uint32_t)((i - 1) >> 1) & 1u, abort_flag, 12)));
+                if (alive && i) {
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-                    for (int d = 0; d < S::HD; d += 32) {
+                    for (int d = half * (S::HD / 2); d < (half + 1) * (S::HD / 2); d += 32) {
                         uint32_t o[32];
                         tmem_ld32(tmem_o + lanes + d, o);
                         tmem_wait_ld(o);
@@ -311,44 +324,47 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 }
             }
+            alive = alive && (i < 2 || __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->pv_done[b]), ph ^ 1u, abort_flag, 11)));               // this half of P is free
+            if (!alive) continue;
             const float off = 14.0f - m;
             if (__any_sync(0xffffffffu, wide)) {               // beyond 2^19 a fused product would show the maximum's own rounding
 #pragma unroll
-                for (int u = 0; u < 64; u++) s[u] = __float_as_uint(ex2((__fmul_rn(__uint_as_float(s[u]), f) - m) + 14.0f));
+                for (int u = 0; u < 32; u++) s[u] = __float_as_uint(ex2((__fmul_rn(__uint_as_float(s[u]), f) - m) + 14.0f));
             } else {
 #pragma unroll
-                for (int u = 0; u < 64; u++) s[u] = __float_as_uint(ex2(fmaf(__uint_as_float(s[u]), f, off)));
+                for (int u = 0; u < 32; u++) s[u] = __float_as_uint(ex2(fmaf(__uint_as_float(s[u]), f, off)));
             }
             float l4[4] = { 0.f, 0.f, 0.f, 0.f };
 #pragma unroll
-            for (int u = 0; u < 64; u++) l4[u & 3] += __uint_as_float(s[u]);
+            for (int u = 0; u < 32; u++) l4[u & 3] += __uint_as_float(s[u]);
             l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+            uint32_t high[16], low[16];                        // 32 rows: 16 columns of tensor memory a piece
 #pragma unroll
-            for (int h = 0; h < 2; h++) {                      // 32 rows: 16 columns of tensor memory a piece
-                uint32_t high[16], low[16];
-#pragma unroll
-                for (int u = 0; u < 16; u++) {
-                    const float a = __uint_as_float(s[32 * h + 2 * u]), z = __uint_as_float(s[32 * h + 2 * u + 1]);
-                    const __half2 x = __floats2half2_rn(a, z);
-                    const float2 back = __half22float2(x);
-                    high[u] = bits(x);
-                    low[u] = bits(__floats2half2_rn(a - back.x, z - back.y));
-                }
-                tmem_st16(tmem_p + lanes + b * PK_ROWS + 16 * h, high);
-                tmem_st16(tmem_p + lanes + b * PK_ROWS + PK_ROWS / 2 + 16 * h, low);
+            for (int u = 0; u < 16; u++) {
+                const float a = __uint_as_float(s[2 * u]), z = __uint_as_float(s[2 * u + 1]);
+                const __half2 x = __floats2half2_rn(a, z);
+                const float2 back = __half22float2(x);
+                high[u] = bits(x);
+                low[u] = bits(__floats2half2_rn(a - back.x, z - back.y));
             }
+            tmem_st16(tmem_p + lanes + b * PK_ROWS + 16 * half, high);
+            tmem_st16(tmem_p + lanes + b * PK_ROWS + PK_ROWS / 2 + 16 * half, low);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&sh->p_full[b]));
         }
+        pair_sync(1 + quarter);                                // the last maxima are read
+        sh->meet[half][own] = l;
+        pair_sync(1 + quarter);
+        l += sh->meet[half ^ 1][own];
         if (n && alive && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->pv_done[(n - 1) & 1]), (uint32_t)((n - 1) >> 1) & 1u, abort_flag, 13))) {
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const float inv = 1.0f / l;
             float* to = p.out + ((size_t)b_col * p.t.n_heads + (size_t)kvh * p.t.group + c % p.t.group) * S::HD;
             const bool vec = ((uintptr_t)p.out & 15) == 0;
 #pragma unroll 1
-            for (int j = 0; j < NG; j++) {
+            for (int j = half * (NG / 2); j < (half + 1) * (NG / 2); j++) {
                 uint32_t o[32];
                 tmem_ld32(tmem_o + lanes + 32 * j, o);
                 tmem_wait_ld(o);
@@ -361,7 +377,7 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
                     else { at[0] = x.x; at[1] = x.y; at[2] = x.z; at[3] = x.w; }
                 }
             }
-            if (on && p.stat) p.stat[(size_t)unit * PK_COLS + tid] = make_float2(m, log2f(l) - 14.0f);
+            if (on && !half && p.stat) p.stat[(size_t)unit * PK_COLS + own] = make_float2(m, log2f(l) - 14.0f);
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -377,7 +393,7 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
 }
 
 // Attention that the rows draw: S^T [128 rows x 128 columns] = K' Q^T again, two threads a row, which add up its softmax weights over the columns that
-// see it. grid (128 rows, KV heads, parts of the column tiles); K' is made once and stays in tensor memory, the columns' images come through a ring. Writes
+// see it. A block for 128 rows, a KV head and a part of the column tiles; K' is made once and stays in tensor memory, the columns' images come through a ring. Writes
 // parts [part][KV head][max_rows].
 constexpr int PW_SUM_WARPS = 8, PW_MMA_WARP = 8, PW_TMA_WARP = 9, PW_THREADS = 10 * 32;
 template <int NG> struct PwSmem {
@@ -387,12 +403,13 @@ template <int NG> struct PwSmem {
 struct PwShared { unsigned long long full[3], empty[3], d_full[2], d_empty[2], k_full, drained; uint32_t tmem_base; int abort_flag; float half[128]; };
 
 template <int NG>
-__global__ void __launch_bounds__(PW_THREADS, 1) kv4_prompt_weight_kernel(const PkParams p, float* __restrict__ parts) {
+__global__ void __launch_bounds__(PW_THREADS, 1) kv4_prompt_weight_kernel(const PkParams p, float* __restrict__ parts, int n_parts) {
     using S = PwSmem<NG>;
     extern __shared__ __align__(1024) unsigned char smem[];
     PwShared* sh = reinterpret_cast<PwShared*>(smem + S::TOTAL);
     volatile int* abort_flag = &sh->abort_flag;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kvh = blockIdx.y, r0 = blockIdx.x * 128;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kvh = blockIdx.x % p.c.n_kv, own_part = blockIdx.x / p.c.n_kv % n_parts;
+    const int r0 = blockIdx.x / (p.c.n_kv * n_parts) * 128;    // rows that most tiles see first
     if (tid == 0) {
         auto init = [&](unsigned long long& b, int n) { mbar_init(smem_u32(&b), n); };
         for (int i = 0; i < S::DEPTH; i++) { init(sh->full[i], 1); init(sh->empty[i], PW_SUM_WARPS + 1); }
@@ -410,8 +427,8 @@ __global__ void __launch_bounds__(PW_THREADS, 1) kv4_prompt_weight_kernel(const 
     pdl_wait();
     int row0, pos0;
     const bool there = kv4_place(p.at, p.t.B, p.c.max_rows, p.err, row0, pos0);
-    const int R = there ? row0 + p.t.B : 0, first = max(0, r0 - row0) * p.t.group / PK_COLS + blockIdx.z;       // tiles that see a row of the block, every gridDim.z-th
-    const int n = r0 < R && first < p.tiles ? (p.tiles - first + (int)gridDim.z - 1) / (int)gridDim.z : 0;
+    const int R = there ? row0 + p.t.B : 0, first = max(0, r0 - row0) * p.t.group / PK_COLS + own_part;       // tiles that see a row of the block, every n_parts-th
+    const int n = r0 < R && first < p.tiles ? (p.tiles - first + n_parts - 1) / n_parts : 0;
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -422,7 +439,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) kv4_prompt_weight_kernel(const 
             int s = 0; uint32_t ph = 1;
             for (int i = 0; i < n; i++) {
                 if (!mbar_wait(smem_u32(&sh->empty[s]), ph, abort_flag, 1)) break;
-                const size_t unit = (size_t)kvh * p.tiles + first + i * (int)gridDim.z;
+                const size_t unit = (size_t)kvh * p.tiles + first + i * n_parts;
                 const uint32_t bar = smem_u32(&sh->full[s]), to = smem_u32(smem + s * S::STAGE);
                 mbar_expect_tx(bar, S::IMAGE + 512 + 1024);
                 for (int e = 0; e < S::IMAGE; e += 16384) bulk_load(to + e, p.image + unit * S::IMAGE + e, 16384, bar);
@@ -496,7 +513,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) kv4_prompt_weight_kernel(const 
             }
             int s = 0; uint32_t phs = 0;
             for (int i = 0; i < n; i++) {
-                const int b = i & 1, c0 = (first + i * (int)gridDim.z) * PK_COLS;
+                const int b = i & 1, c0 = (first + i * n_parts) * PK_COLS;
                 if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->full[s]), phs, abort_flag, 6) && mbar_wait(smem_u32(&sh->d_full[b]), (uint32_t)(i >> 1) & 1u, abort_flag, 7))) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const float* f = reinterpret_cast<const float*>(smem + s * S::STAGE + S::IMAGE);
@@ -528,7 +545,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) kv4_prompt_weight_kernel(const 
         }
         if (half) sh->half[own] = sum;
         asm volatile("bar.sync 2, %0;" :: "n"(PW_SUM_WARPS * 32) : "memory");
-        if (!half && r < R) parts[((size_t)blockIdx.z * p.c.n_kv + kvh) * p.c.max_rows + r] = sum + sh->half[own];
+        if (!half && r < R) parts[((size_t)own_part * p.c.n_kv + kvh) * p.c.max_rows + r] = sum + sh->half[own];
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -551,7 +568,7 @@ int launch_prompt(ibcu_ctx* ctx, const PkParams& p, int rows, float* parts, int 
     if (int rc = ibcu_launch(ctx, kv4_prompt_kernel<NG>, dim3(p.c.n_kv * p.tiles), dim3(PK_THREADS), smem, 1, true, p)) return rc;
     if (!p.stat) return IBCU_OK;
     if (int rc = ibcu_allow_smem(ctx, opt_w, kv4_prompt_weight_kernel<NG>, smem_w)) return rc;
-    return ibcu_launch(ctx, kv4_prompt_weight_kernel<NG>, dim3((rows + 127) / 128, p.c.n_kv, n_parts), dim3(PW_THREADS), smem_w, 1, true, p, parts);
+    return ibcu_launch(ctx, kv4_prompt_weight_kernel<NG>, dim3(p.c.n_kv * n_parts * ((rows + 127) / 128)), dim3(PW_THREADS), smem_w, 1, true, p, parts, n_parts);
 }
 
 }  // namespace
