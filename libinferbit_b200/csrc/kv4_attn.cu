@@ -776,7 +776,9 @@ int kv4_attend(ibcu_ctx* ctx, const Kv4& c, float decay, const Kv4Place& at, con
     KaCall call;
     memset(&call, 0, sizeof call);
     call.rows = rows; call.decay = decay; call.cols = large ? 16 : columns > 4 ? 8 : 4;
-    if ((c.hd == 64 || c.hd == 128) && large && c.n_kv * (columns / 128) >= ctx->sm_count / 4) {          // a prompt
+    // A prompt: tcgen05 (kv4_prompt.cu) takes a third of the time a row once its tiles of 128 columns have enough SMs, the tiles of 16 here fill the machine with fewer.
+    // 32 heads over 8 after 8000 rows, us here and there: of 128 values 152 and 166 with 32 tiles of 128, 245 and 166 with 40; of 64 values 126 and 145 with 48, 184 and 147 with 64.
+    if ((c.hd == 64 || c.hd == 128) && large && c.n_kv * (columns / 128) >= (c.hd == 64 ? ctx->sm_count * 3 / 8 : ctx->sm_count / 4)) {
         Kv4Columns tp = t;
         tp.ntiles = (int)((columns + 127) / 128) * 8;
         tp.large = 2;

@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(W8_THREADS, 1) w8a8_pair_kernel(const __grid_c
 // ── few tokens ──
 // Up to four tokens are bound by the weights' bytes and, for one matrix, by latency: one launch, a warp a row, whose bytes are all on
 // their way before the launch ahead has ended; meanwhile every block quantises the tokens for itself (or copies their codes), then four products a dp4a. 4096 x 4096
-// at one token: W8F us against 10.3 for the quantiser and the tensor cores.
+// at one token, replayed: 5.2 us from FP32 and 4.4 from codes, of which the weights' 16 MB are 2.6.
 constexpr int WF_WARPS = 8, WF_AHEAD = 8, WF_TOKENS = 4;
 struct WfParams { ibcu_linear_t t[4]; int n, row_start[5], N, B; const float* x; const int8_t* xq; const float* sx; };
 
@@ -587,15 +587,20 @@ int quantize(ibcu_ctx* ctx, const float* x, int8_t* q, float* scale, int N, int 
                        x, q, scale, N, ldq, B, jobs);
 }
 
-// Few tokens: IBCU_DECLINED where the call is not one for that kernel. x: FP32 tokens, or their codes and scales. Every block quantises for itself while that is 16384 values.
+// Few tokens: IBCU_DECLINED where the call is not one for that kernel. x: FP32 tokens, or their codes and scales. A token costs it the reading of its codes
+// for every row and, from FP32, its quantisation by every block, the tensor cores a launch more and a longer start. us there and here, replayed: 4096 x 4096
+// one token 7.2 and 5.2, two 7.3 and 7.0, three 7.5 and 8.9; 4096 x 8192 one 8.8 and 9.1; 2048 x 2048 four 6.8 and 5.6; with codes 4096 x 4096 four 6.3 and 6.1,
+// 4096 x 8192 two 7.7 and 6.8, three 7.6 and 8.5. Beyond two rows a warp its loads no longer run ahead: 12000 x 512 one token 4.6 and 5.6.
 int product_few(ibcu_ctx* ctx, const ibcu_linear_t* ts, int n, const float* x, const int8_t* xq, const float* sx, int N, int B) {
-    if (B > WF_TOKENS || N % 16 || (long)B * N > (x ? 16384 : 65536) || ((uintptr_t)(x ? (const void*)x : xq) & 15)) return IBCU_DECLINED;
+    double rows = 0.0;
+    for (int i = 0; i < n; i++) rows += ts[i].M;
+    if (B > WF_TOKENS || N % 16 || (long)B * N > 65536 || ((uintptr_t)(x ? (const void*)x : xq) & 15) || rows > 2.0 * WF_WARPS * 4 * ctx->sm_count ||
+        (double)B * N * (x ? rows + 3300.0 : rows) > (x ? 55e6 : 75e6)) return IBCU_DECLINED;
     WfParams p;
     memset(&p, 0, sizeof p);
     for (int i = 0; i < n; i++) {
         if ((uintptr_t)ts[i].w & 15) return IBCU_DECLINED;
         p.t[i] = ts[i];
-        if ((long)p.row_start[i] + ts[i].M > 0x7FFF0000L) return IBCU_DECLINED;
         p.row_start[i + 1] = p.row_start[i] + ts[i].M;
     }
     p.n = n; p.N = N; p.B = B; p.x = x; p.xq = xq; p.sx = sx;

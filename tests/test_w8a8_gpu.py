@@ -160,3 +160,38 @@ def test_captured_and_replayed(backend):
             check(be, w, s, o, do, *quantise(x[i]), False)
     finally:
         be._check(be.lib.ibcu_graph_destroy(be.ctx, gid))
+
+
+def run_both(be, rng, Ms, N, B, add, extra, fp32=False):
+    x = rng.standard_normal((B, N), dtype=np.float32)
+    q, sx = quantise(x)
+    for form in range(2):
+        t, w, s, o, do = tensors(be, rng, Ms, N, B, fp32, extra, add)
+        be._check(be.lib.ibcu_linear_w8a8_fp32(be.ctx, t, len(Ms), be.upload(x).ptr, N, B) if form else be.lib.ibcu_linear_w8a8(be.ctx, t, len(Ms), be.upload(q).ptr, be.upload(sx).ptr, N, B)); be.sync()
+        check(be, w, s, o, do, q, sx, add)
+
+
+@pytest.mark.parametrize("Ms,N,B,add,extra", [((5000, 5000), 1040, 700, False, 1), ((14336,), 256, 512, True, 0), ((2300, 257, 5, 4000), 1153, 1027, False, 0), ((8192,), 4096, 257, True, 7)])
+def test_large_products(backend, Ms, N, B, add, extra):
+    """Tiles by pairs of blocks, with row tiles and tokens that end inside one."""
+    run_both(backend, np.random.default_rng(B), Ms, N, B, add, extra)
+
+
+@pytest.mark.parametrize("Ms,N", [((9000,), 512), ((70, 3, 2000), 4112), ((1, 1, 1, 1), 16), ((4737,), 1024), ((2048,), 8192), ((33, 900), 16400)])
+@pytest.mark.parametrize("B", [1, 2, 3, 4])
+def test_few_tokens(backend, Ms, N, B):
+    run_both(backend, np.random.default_rng(N + B), Ms, N, B, B % 2 == 0, B - 1, B == 3)
+
+
+def test_a_row_that_is_not_finite_stays_alone_among_few(backend):
+    be, rng = backend, np.random.default_rng(9)
+    M, N, B = 300, 512, 4
+    x = rng.standard_normal((B, N), dtype=np.float32)
+    x[1, 5], x[2] = np.inf, 0
+    q, sx = quantise(x)
+    t, w, s, o, do = tensors(be, rng, [M], N, B)
+    be._check(be.lib.ibcu_linear_w8a8_fp32(be.ctx, t, 1, be.upload(x).ptr, N, B)); be.sync()
+    got = be.download(do[0], np.float32, B * M).reshape(B, M)
+    assert np.isnan(got[1]).all() and not got[2].any()
+    want = (q.astype(np.float64) @ w[0].astype(np.float64).T) * s[0].astype(np.float64) * sx.astype(np.float64)[:, None]
+    assert np.all(np.abs(got[[0, 3]] - want[[0, 3]]) <= 3.01 * HALF * np.abs(want[[0, 3]]))
