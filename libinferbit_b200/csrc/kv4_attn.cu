@@ -8,7 +8,8 @@
 //     out = sum over rows of P' (n - 8),  P' = 2^14 p vs[row][j]
 // with P' split into two pieces too. (Without the subtraction unpacking is a mask alone, n as the subnormal n * 2^-24, and the bias of 8 can be
 // taken off the sums. But those then are of codes that are all positive, hundreds of times their result after thousands of rows, and the
-// instruction's additions round towards zero: outputs after 32767 rows were 1.5e-4 off, and 1.5e-6 with the keys alone unpacked so, against 3e-7.)
+// instruction's additions round towards zero: outputs after 32767 rows were 1.5e-4 off, and 1.5e-6 with the keys alone unpacked so, against 3e-7.
+// For the same reason 32 rows are summed by themselves and added to the sums rounded: in the instruction's own sums 16000 rows of one block were 2.8e-6 off.)
 // The maximum that p refers to is that of score + L(row), 2^L a bound on the row's value scales: then P' never passes 2^14 (2^16 with the
 // slack below), whatever the scales are, and a column's numbers do not depend on rows that it does not see.
 //
@@ -490,46 +491,59 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (COLS == 16 ? 2 : 
                         const float hi = __uint_as_float(__float_as_uint(a) & 0xFFFFE000u);        // eleven bits, cut off: the low piece has the same sign and what is left to 2^-22
                         b[i] = transpose_8x8(pack_half(hi, a - hi));
                     }
+                    float part[2][4];                                                              // these rows', added to the sums rounded
 #pragma unroll
                     for (int u = 0; u < 2; u++) {
                         uint32_t x[4], y[4];
                         unpack(__byte_perm(vw[2 * u][0][j / 2], vw[2 * u][1][j / 2], j & 1 ? 0x7632 : 0x5410), x);
                         unpack(__byte_perm(vw[2 * u + 1][0][j / 2], vw[2 * u + 1][1][j / 2], j & 1 ? 0x7632 : 0x5410), y);
-                        mma_f16(acc[j][0], make_uint4(x[0], x[2], y[0], y[2]), b[2 * u], b[2 * u + 1]);
-                        mma_f16(acc[j][1], make_uint4(x[1], x[3], y[1], y[3]), b[2 * u], b[2 * u + 1]);
+#pragma unroll
+                        for (int q = 0; q < 2; q++) {
+                            if (u) mma_f16(part[q], make_uint4(x[q], x[q + 2], y[q], y[q + 2]), b[2 * u], b[2 * u + 1]);
+                            else mma_f16_first(part[q], make_uint4(x[q], x[q + 2], y[q], y[q + 2]), b[2 * u], b[2 * u + 1]);
+                        }
                     }
+#pragma unroll
+                    for (int q = 0; q < 2; q++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[j][q][e] += part[q][e];
                 }
             } else {
 #pragma unroll
                 for (int j = 0; j < NG; j++) {
                     float vs[4][2];
                     lane_rows(vs, sc + (NG + j) * 32, t);
+                    uint32_t hi[2][2][NC], lo[2][2][NC], b0[2][4], b1[2][4];                       // 16 rows each: pieces 2 u and 2 u + 1
 #pragma unroll
-                    for (int u = 0; u < 2; u++) {                                                      // 16 rows: pieces 2 u and 2 u + 1
-                        uint32_t hi[2][NC], lo[2][NC];
+                    for (int u = 0; u < 2; u++) {
 #pragma unroll
                         for (int i = 0; i < 2; i++)
 #pragma unroll
                             for (int n = 0; n < NC; n++) {
                                 float a = s[2 * u + i][0][n] * vs[2 * u + i][0], b = s[2 * u + i][1][n] * vs[2 * u + i][1];
-                                if (!seen(2 * u + i, 0, n)) a = 0.0f;                                  // the row's scale may be NaN
+                                if (!seen(2 * u + i, 0, n)) a = 0.0f;                              // the row's scale may be NaN
                                 if (!seen(2 * u + i, 1, n)) b = 0.0f;
-                                hi[i][n] = pack_half(a, b);
-                                const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[i][n]));
-                                lo[i][n] = pack_half(a - back.x, b - back.y);
+                                hi[u][i][n] = pack_half(a, b);
+                                const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[u][i][n]));
+                                lo[u][i][n] = pack_half(a - back.x, b - back.y);
                             }
-                        uint32_t b0[4], b1[4];
-                        unpack(__byte_perm(vw[2 * u][0][j / 2], vw[2 * u][1][j / 2], j & 1 ? 0x7632 : 0x5410), b0);
-                        unpack(__byte_perm(vw[2 * u + 1][0][j / 2], vw[2 * u + 1][1][j / 2], j & 1 ? 0x7632 : 0x5410), b1);
+                        unpack(__byte_perm(vw[2 * u][0][j / 2], vw[2 * u][1][j / 2], j & 1 ? 0x7632 : 0x5410), b0[u]);
+                        unpack(__byte_perm(vw[2 * u + 1][0][j / 2], vw[2 * u + 1][1][j / 2], j & 1 ? 0x7632 : 0x5410), b1[u]);
+                    }
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            if constexpr (LARGE) {
-                                mma_f16(acc[j][i], make_uint4(hi[0][0], hi[0][1], hi[1][0], hi[1][1]), b0[i], b1[i]);
-                                mma_f16(acc[j][i], make_uint4(lo[0][0], lo[0][1], lo[1][0], lo[1][1]), b0[i], b1[i]);
-                            } else {
-                                mma_f16(acc[j][i], make_uint4(hi[0][0], lo[0][0], hi[1][0], lo[1][0]), b0[i], b1[i]);
-                            }
+                    for (int i = 0; i < 4; i++) {
+                        float part[4];                                                             // these rows', added to the sums rounded
+                        if constexpr (LARGE) {
+                            mma_f16_first(part, make_uint4(lo[0][0][0], lo[0][0][1], lo[0][1][0], lo[0][1][1]), b0[0][i], b1[0][i]);
+                            mma_f16(part, make_uint4(lo[1][0][0], lo[1][0][1], lo[1][1][0], lo[1][1][1]), b0[1][i], b1[1][i]);
+                            mma_f16(part, make_uint4(hi[0][0][0], hi[0][0][1], hi[0][1][0], hi[0][1][1]), b0[0][i], b1[0][i]);
+                            mma_f16(part, make_uint4(hi[1][0][0], hi[1][0][1], hi[1][1][0], hi[1][1][1]), b0[1][i], b1[1][i]);
+                        } else {
+                            mma_f16_first(part, make_uint4(hi[0][0][0], lo[0][0][0], hi[0][1][0], lo[0][1][0]), b0[0][i], b1[0][i]);
+                            mma_f16(part, make_uint4(hi[1][0][0], lo[1][0][0], hi[1][1][0], lo[1][1][0]), b0[1][i], b1[1][i]);
                         }
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[j][i][e] += part[e];
                     }
                 }
             }

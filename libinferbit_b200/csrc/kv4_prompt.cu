@@ -9,6 +9,8 @@
 //
 // Warps: 8 softmax, two threads a column; 4 that turn key codes into the pieces of K', 4 for V' (transposed: the rows are the
 // contraction); 1 issues the products, 1 the copies. Everything is double buffered, and S of the next rows is computed while the softmax is at these.
+// The instruction cuts its sums off, towards zero, at every step: outputs after 16000 rows were 5.7e-5 off in one accumulator, 2.3e-6 after 2048. So after a run
+// of PK_RUN times 64 rows its outputs are added, rounded, to sums in shared memory.
 // A V' of a row with a NaN scale would reach columns that do not see the row (0 * NaN), so NaN goes into the row's K' instead, and with it
 // into every column that does see it.
 #include "kv4.cuh"
@@ -17,7 +19,7 @@
 
 namespace {
 
-constexpr int PK_ROWS = 64, PK_COLS = 128, PK_RAW = 3;
+constexpr int PK_ROWS = 64, PK_COLS = 128, PK_RAW = 3, PK_RUN = 4;
 constexpr int PK_KEY_WARP = 8, PK_VALUE_WARP = 12, PK_MMA_WARP = 16, PK_TMA_WARP = 17, PK_THREADS = 18 * 32;
 constexpr float PK_LOW = -3.0e38f, PK_SLACK = 1.9f;            // see kv4_attn.cu
 
@@ -31,7 +33,8 @@ struct PkParams {
 template <int NG> struct PkSmem {
     static constexpr int KB = NG / 2, HD = 32 * NG;            // KB: blocks of 64 values, a swizzled row of 128 bytes each
     static constexpr int IMAGE = 2 * KB * 16384, KEYS = 2 * KB * 8192, VALUES = 2 * HD * 128, RAW_BYTES = PK_ROWS * 36 * NG;
-    static constexpr int K = 0, V = K + 2 * KEYS, RAW = V + 2 * VALUES, TOTAL = RAW + PK_RAW * RAW_BYTES;
+    static constexpr int K = 0, V = K + 2 * KEYS, RAW = V + 2 * VALUES;
+    static constexpr int SUM = RAW + PK_RAW * RAW_BYTES, TOTAL = SUM + HD * PK_COLS * 4;         // SUM [TMEM column / 4][column] float4
 };
 struct PkShared {
     unsigned long long q_full, raw_full[PK_RAW], raw_empty[PK_RAW], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], s_empty[2], p_full[2], pv_done[2], drained;
@@ -131,7 +134,7 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem_o = sh->tmem_base, tmem_s = tmem_o + S::HD, tmem_p = tmem_s + 2 * PK_ROWS, tmem_q = tmem_p + 2 * PK_ROWS;          // 128 + 2 x 64 + 2 x 64 + 2 x 64 columns
+    const uint32_t tmem_o = sh->tmem_base, tmem_s = tmem_o + S::HD, tmem_p = tmem_s + 2 * PK_ROWS, tmem_q = tmem_p + 2 * PK_ROWS;          // 128 + 2 x 64 + 2 x 64 + 128 columns
 
     if (warp == PK_TMA_WARP) {
         if (elect_one() && n) {
@@ -162,11 +165,10 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint64_t k = smem_desc_sw128(smem_u32(smem + S::K + b * S::KEYS));
 #pragma unroll
-                for (int m = 0; m < 3; m++)                                                       // high.high, low.high, high.low
+                for (int m = 0; m < 3; m++)                                                       // low.high, high.low, high.high: small sums first, which lose least
 #pragma unroll
                     for (int st = 0; st < S::HD / 16; st++)
-                        mma_f16_ts(tmem_s + b * PK_ROWS, tmem_q + (m == 1) * (S::HD / 2) + st * 8, k + (((m == 2) * S::KB + st / 4) * 8192 >> 4) + st % 4 * 2, idesc_s,
-                                   m || st ? 1u : 0u);
+                        mma_f16_ts(tmem_s + b * PK_ROWS, tmem_q + (m == 0) * (S::HD / 2) + st * 8, k + (((m == 1) * S::KB + st / 4) * 8192 >> 4) + st % 4 * 2, idesc_s, m || st ? 1u : 0u);
                 mma_commit(smem_u32(&sh->k_empty[b]));
                 mma_commit(smem_u32(&sh->s_full[b]));
                 return true;
@@ -180,11 +182,12 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint64_t v = smem_desc_sw128(smem_u32(smem + S::V + b * S::VALUES));
+                const uint32_t more = i % PK_RUN ? 1u : 0u;
 #pragma unroll
                 for (int m = 0; m < 3; m++)
 #pragma unroll
                     for (int st = 0; st < PK_ROWS / 16; st++)
-                        mma_f16_ts(tmem_o, tmem_p + b * PK_ROWS + (m == 1) * (PK_ROWS / 2) + st * 8, v + ((m == 2) * S::HD * 128 >> 4) + st * 2, idesc_o, i || m || st ? 1u : 0u);
+                        mma_f16_ts(tmem_o, tmem_p + b * PK_ROWS + (m == 0) * (PK_ROWS / 2) + st * 8, v + ((m == 1) * S::HD * 128 >> 4) + st * 2, idesc_o, m || st ? 1u : more);
                 mma_commit(smem_u32(&sh->v_empty[b]));
                 mma_commit(smem_u32(&sh->pv_done[b]));
             }
@@ -193,6 +196,8 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
         }
         __syncwarp();
     } else if (warp >= PK_KEY_WARP) {
+        // 96 registers a thread at the launch: 256 x 80 + 256 x 112 + 64 x 96 are the 576 x 96 there
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         const bool keys = warp < PK_VALUE_WARP;
         const int w = warp & 3;
         int s = 0; uint32_t ph = 0;
@@ -254,6 +259,7 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
         }
     } else {
         // A column has two threads, of warps w and w + 4: each has 32 of the rows, half of the queries' copy and of the outputs.
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
         const int quarter = warp & 3, half = warp >> 2, own = quarter * 32 + lane, c = c0 + own, b_col = c / p.t.group;
         const bool on = b_col < p.t.B;
         const int lim = row0 + b_col, lim0 = row0 + (c0 + quarter * 32) / p.t.group;             // last rows that this column, the warp's first column, see
@@ -278,14 +284,17 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&sh->q_full));
         }
-        float m = PK_LOW, l = 0.0f;
+        float4* sums = reinterpret_cast<float4*>(smem + S::SUM) + own;
+        float m = PK_LOW, l = 0.0f, aged = 1.0f;               // aged: what the sums of earlier runs are to be multiplied by
         bool wide = false, alive = true;                       // not alive: a wait gave up; the barriers of the pair are still both warps'
         for (int i = 0; i < n; i++) {
-            const int b = i & 1, from = i * PK_ROWS + half * 32;
-            const uint32_t ph = (uint32_t)(i >> 1) & 1u;
+            const int from = i * PK_ROWS + half * 32;
+            const int b = i & 1;
+            const uint32_t ph = (uint32_t)(i >> 1) & 1u, ph_last = (uint32_t)((i - 1) >> 1) & 1u;
+            const bool begins = i % PK_RUN == 0;
             alive = alive && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->s_full[b]), ph, abort_flag, 10));
             uint32_t s[32];
-            float top = PK_LOW;
+            float top = PK_LOW, corr = 1.0f;
             if (alive) {
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 tmem_ld32(tmem_s + lanes + b * PK_ROWS + half * 32, s);
@@ -305,26 +314,28 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
             if (pair_any(1 + quarter, top > m + PK_SLACK)) {
                 sh->meet[half][own] = top;
                 pair_sync(1 + quarter);
-                const float now = fmaxf(m, fmaxf(top, sh->meet[half ^ 1][own])), corr = ex2(m - now);
+                const float now = fmaxf(m, fmaxf(top, sh->meet[half ^ 1][own]));
+                corr = ex2(m - now);
                 m = now;
                 l *= corr;
+                aged *= corr;
                 wide = fabsf(now) > 524288.0f;
-                alive = alive && (!i || __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->pv_done[b ^ 1]), (uint32_t)((i - 1) >> 1) & 1u, abort_flag, 12)));
-                if (alive && i) {
+                alive = alive && (begins || __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->pv_done[b ^ 1]), ph_last, abort_flag, 12)));
+                if (alive && !begins) {
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
                     for (int d = half * (S::HD / 2); d < (half + 1) * (S::HD / 2); d += 32) {
+                        const uint32_t at = tmem_o + lanes + d;
                         uint32_t o[32];
-                        tmem_ld32(tmem_o + lanes + d, o);
+                        tmem_ld32(at, o);
                         tmem_wait_ld(o);
 #pragma unroll
                         for (int u = 0; u < 32; u++) o[u] = __float_as_uint(__uint_as_float(o[u]) * corr);
-                        tmem_st32(tmem_o + lanes + d, o);
+                        tmem_st32(at, o);
                     }
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 }
             }
-            alive = alive && (i < 2 || __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->pv_done[b]), ph ^ 1u, abort_flag, 11)));               // this half of P is free
             if (!alive) continue;
             const float off = 14.0f - m;
             if (__any_sync(0xffffffffu, wide)) {               // beyond 2^19 a fused product would show the maximum's own rounding
@@ -347,6 +358,25 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
                 high[u] = bits(x);
                 low[u] = bits(__floats2half2_rn(a - back.x, z - back.y));
             }
+            alive = i < 2 || __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->pv_done[b]), ph ^ 1u, abort_flag, 11));       // this half of P is free
+            if (begins && i) alive = alive && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->pv_done[b ^ 1]), ph_last, abort_flag, 14));
+            if (!alive) continue;
+            if (begins && i) {                                 // a run has ended
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+                for (int d = half * (S::HD / 2); d < (half + 1) * (S::HD / 2); d += 16) {
+                    uint32_t o[16];
+                    tmem_ld16(tmem_o + lanes + d, o);
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        float4* at = sums + (d / 4 + u) * PK_COLS;
+                        const float4 old = i > PK_RUN ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
+                        *at = make_float4(fmaf(__uint_as_float(o[4 * u]), corr, old.x * aged), fmaf(__uint_as_float(o[4 * u + 1]), corr, old.y * aged),
+                                          fmaf(__uint_as_float(o[4 * u + 2]), corr, old.z * aged), fmaf(__uint_as_float(o[4 * u + 3]), corr, old.w * aged));
+                    }
+                }
+                aged = 1.0f;
+            }
             tmem_st16(tmem_p + lanes + b * PK_ROWS + 16 * half, high);
             tmem_st16(tmem_p + lanes + b * PK_ROWS + PK_ROWS / 2 + 16 * half, low);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -365,13 +395,23 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
             const bool vec = ((uintptr_t)p.out & 15) == 0;
 #pragma unroll 1
             for (int j = half * (NG / 2); j < (half + 1) * (NG / 2); j++) {
-                uint32_t o[32];
-                tmem_ld32(tmem_o + lanes + 32 * j, o);
-                tmem_wait_ld(o);
+                float o[32];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t x[16];
+                    tmem_ld16(tmem_o + lanes + 32 * j + 16 * h, x);
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        const float4 old = n > PK_RUN ? sums[(8 * j + 4 * h + u) * PK_COLS] : make_float4(0.f, 0.f, 0.f, 0.f);
+                        float* to16 = o + 16 * h + 4 * u;
+                        to16[0] = fmaf(old.x, aged, __uint_as_float(x[4 * u])); to16[1] = fmaf(old.y, aged, __uint_as_float(x[4 * u + 1]));
+                        to16[2] = fmaf(old.z, aged, __uint_as_float(x[4 * u + 2])); to16[3] = fmaf(old.w, aged, __uint_as_float(x[4 * u + 3]));
+                    }
+                }
                 if (!on) continue;
 #pragma unroll
                 for (int g = 0; g < 8; g++) {
-                    const float4 x = make_float4(__uint_as_float(o[g]) * inv, __uint_as_float(o[8 + g]) * inv, __uint_as_float(o[16 + g]) * inv, __uint_as_float(o[24 + g]) * inv);
+                    const float4 x = make_float4(o[g] * inv, o[8 + g] * inv, o[16 + g] * inv, o[24 + g] * inv);
                     float* at = to + 32 * j + 4 * g;
                     if (vec) *reinterpret_cast<float4*>(at) = x;
                     else { at[0] = x.x; at[1] = x.y; at[2] = x.z; at[3] = x.w; }
@@ -464,7 +504,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) kv4_prompt_weight_kernel(const 
                 for (int m = 0; m < 3; m++)
 #pragma unroll
                     for (int st = 0; st < 2 * NG; st++)
-                        mma_f16_ts(tmem + b * PK_COLS, tmem_k + (m == 2) * 16 * NG + st * 8, q + (((m == 1) * S::KB + st / 4) * 16384 >> 4) + st % 4 * 2, idesc, m || st ? 1u : 0u);
+                        mma_f16_ts(tmem + b * PK_COLS, tmem_k + (m == 1) * 16 * NG + st * 8, q + (((m == 0) * S::KB + st / 4) * 16384 >> 4) + st % 4 * 2, idesc, m || st ? 1u : 0u);          // small products first
                 mma_commit(smem_u32(&sh->empty[s]));
                 mma_commit(smem_u32(&sh->d_full[b]));
                 if (++s == S::DEPTH) { s = 0; phs ^= 1; }
