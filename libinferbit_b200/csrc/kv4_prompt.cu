@@ -19,7 +19,7 @@
 
 namespace {
 
-constexpr int PK_ROWS = 64, PK_COLS = 128, PK_RAW = 3, PK_RUN = 4;
+constexpr int PK_ROWS = 64, PK_COLS = 128, PK_RAW = 3, PK_RUN = 3;
 constexpr int PK_KEY_WARP = 8, PK_VALUE_WARP = 12, PK_MMA_WARP = 16, PK_TMA_WARP = 17, PK_THREADS = 18 * 32;
 constexpr float PK_LOW = -3.0e38f, PK_SLACK = 1.9f;            // see kv4_attn.cu
 
