@@ -201,7 +201,7 @@ __device__ __forceinline__ uint32_t weight_order(float w) {
 // The bound is found eight bits at a time: every block counts its rows by those bits, and adds up the blocks' counts for itself; one barrier of
 // the cluster a round, since each round has counters of its own. MOVE: the block then copies its kept rows into another cache.
 // 32 rounds of one bit by one block a head, every weight read again each time, took 330 us for 65529 rows of 8 heads.
-constexpr int CH_THREADS = 1024, CH_KEEP = 8;
+constexpr int CH_THREADS = 1024, CH_KEEP = 8, CH_CLUSTER = 8;
 template <bool IN_REGISTERS, bool MOVE>
 __global__ void __launch_bounds__(CH_THREADS) kv4_choose_kernel(Kv4 src, Kv4 dst, int32_t* __restrict__ kept, int rows, int keep, int lo, int hi, int want, int CS) {
     __shared__ uint32_t hist[4][256], total[256], totals[2], found[2];
@@ -218,7 +218,15 @@ __global__ void __launch_bounds__(CH_THREADS) kv4_choose_kernel(Kv4 src, Kv4 dst
     uint32_t key[CH_KEEP];
     if (IN_REGISTERS) {
 #pragma unroll
-        for (int i = 0; i < CH_KEEP; i++) key[i] = i < n ? weight_order(__ldcg(w + r0 + i)) : 0u;
+        for (int i = 0; i < CH_KEEP; i += 4) {
+            if (i + 4 <= n && ((uintptr_t)(w + r0) & 15) == 0) {
+                const float4 x = __ldcg(reinterpret_cast<const float4*>(w + r0 + i));
+                key[i] = weight_order(x.x); key[i + 1] = weight_order(x.y); key[i + 2] = weight_order(x.z); key[i + 3] = weight_order(x.w);
+            } else {
+#pragma unroll
+                for (int u = 0; u < 4; u++) key[i + u] = i + u < n ? weight_order(__ldcg(w + r0 + i + u)) : 0u;
+            }
+        }
     }
     // f(row, order, whether the row is one of those chosen from) for this thread's rows in order
     auto each = [&](auto f) {
@@ -238,9 +246,12 @@ __global__ void __launch_bounds__(CH_THREADS) kv4_choose_kernel(Kv4 src, Kv4 dst
             each([&](int, uint32_t k, bool in) { if (in && (k & above) == bound) atomicAdd(&hist[round][(k >> shift) & 255], 1u); });
             meet();
             if (tid < 256) {
-                uint32_t t = 0;
-                for (int r = 0; r < CS; r++) t += theirs(&hist[round][tid], r);
-                total[tid] = t;
+                uint32_t t[CH_CLUSTER], sum = 0;               // all on their way at once
+#pragma unroll
+                for (int r = 0; r < CH_CLUSTER; r++) t[r] = r < CS ? theirs(&hist[round][tid], r) : 0u;
+#pragma unroll
+                for (int r = 0; r < CH_CLUSTER; r++) sum += t[r];
+                total[tid] = sum;
             }
             __syncthreads();
             if (warp == 0) {                                  // lane l has bins 255 - 8 l .. 248 - 8 l
@@ -289,10 +300,13 @@ __global__ void __launch_bounds__(CH_THREADS) kv4_choose_kernel(Kv4 src, Kv4 dst
     meet();
     __syncthreads();
     uint32_t base = 0, eq_before = 0;                         // kept rows of the blocks below, and their rows at the bound
-    for (int r = 0; r < rank; r++) {
-        const uint32_t g = theirs(&totals[0], r), e = theirs(&totals[1], r);
-        base += g + min(e, left - min(left, eq_before));
-        eq_before += e;
+    uint32_t g[CH_CLUSTER], e[CH_CLUSTER];
+#pragma unroll
+    for (int r = 0; r < CH_CLUSTER; r++) { g[r] = r < rank ? theirs(&totals[0], r) : 0u; e[r] = r < rank ? theirs(&totals[1], r) : 0u; }
+#pragma unroll
+    for (int r = 0; r < CH_CLUSTER; r++) {
+        base += g[r] + min(e[r], left - min(left, eq_before));
+        eq_before += e[r];
     }
     const uint32_t room = left - min(left, eq_before);        // rows at the bound that stay in this block
     uint32_t at_gt = warp_gt[warp] + pgt - gt, at_eq = warp_eq[warp] + peq - eq;
@@ -464,8 +478,10 @@ extern "C" int ibcu_kv4_evict(ibcu_ctx* ctx, const ibcu_kv4_t* src, const ibcu_k
         if (rc) return rc;
         kept = (int32_t*)ctx->scratch;
     }
-    int CS = 1;                                               // a block a thousand rows, up to eight
-    while (CS < 8 && rows > 1024 * CS) CS *= 2;
+    // A block a thousand rows, up to eight, as long as all clusters run at once: 12 of eight blocks, 33 of four, 74 of two find their places (8192 rows of 32 heads
+    // by eight blocks each 38 us, by four 14).
+    int CS = 1;
+    while (CS < CH_CLUSTER && rows > 1024 * CS && nkv <= (CS == 4 ? ctx->sm_count / 12 : CS == 2 ? ctx->sm_count * 9 / 40 : ctx->sm_count / 2)) CS *= 2;
     const bool regs = (rows + CS - 1) / CS <= CH_THREADS * CH_KEEP;
     auto choose = regs ? (in_place ? kv4_choose_kernel<true, false> : kv4_choose_kernel<true, true>) : (in_place ? kv4_choose_kernel<false, false> : kv4_choose_kernel<false, true>);
     int rc = ibcu_launch(ctx, choose, dim3(CS * nkv), dim3(CH_THREADS), 0, CS, true, planes(src), planes(dst), kept, rows, keep, sink, rows - recent, keep - sink - recent, CS);
