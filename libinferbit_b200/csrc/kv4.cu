@@ -18,7 +18,8 @@ __device__ __forceinline__ float scale_at(const __half* p) { return __half2float
 
 // One launch ahead of the attention of more than eight columns, and that of ibcu_kv4_write: blocks below qblocks turn a tile of 16 columns of every
 // qparts-th KV head into fragments or their part of an image, the others write the rows of a position. Heads share a position's angles. Bound by
-// instructions: eighteen a value of a row, PREPQ a value of a query.
+// instructions: 29 for 32 values of rows, 17 of queries, and the turning. The rows of 2048 positions of 8 heads of 128 values 6.9 us (5.8 unturned, 2.9 for the
+// bytes); 11.6 with four values a thread, lengths not known at compile time and a position's angles in the order of its pairs.
 struct PrepParams { Kv4 c; Kv4Columns t; Kv4Place at; Kv4Prep w; int qblocks, qparts, wparts; int* err; };
 
 template <int NG>
@@ -62,7 +63,7 @@ __global__ void __launch_bounds__(128) kv4_prep_kernel(const PrepParams p) {
 #pragma unroll
             for (int u = 0; u < PL; u++) {
                 const int piece = pl + 8 * u, i = piece % NG * 32 + piece / NG * 8;
-                kv4_query(x[u], src + i, on, angles ? angles + i / 2 : nullptr);
+                kv4_query<NG>(x[u], src + i, on, angles, i);
 #pragma unroll
                 for (int n = 0; n < 8; n++) m = max(m, __float_as_uint(x[u][n]) & 0x7FFFFFFFu);
             }
@@ -103,12 +104,12 @@ __global__ void __launch_bounds__(128) kv4_prep_kernel(const PrepParams p) {
             for (int n = 0; n < 2; n++) {
                 const bool on = b[n] < p.t.B;
                 const float* src = p.w.q + ((size_t)b[n] * p.t.n_heads + (size_t)kvh * p.t.group + head[n]) * HD + 8 * t;
-                const double2* angles = p.w.rotate ? turn + (b[n] - b0) * HALF + 4 * t : nullptr;
+                const double2* angles = p.w.rotate ? turn + (b[n] - b0) * HALF : nullptr;
 #pragma unroll
                 for (int jj = 0; jj < JT; jj++) {
                     const int j = warp + 4 * jj;
                     if (j >= NG) break;
-                    kv4_query(x[n][jj], src + 32 * j, on, angles ? angles + 16 * j : nullptr);
+                    kv4_query<NG>(x[n][jj], src + 32 * j, on, angles, 32 * j + 8 * t);
 #pragma unroll
                     for (int i = 0; i < 8; i++) m[n] = max(m[n], __float_as_uint(x[n][jj][i]) & 0x7FFFFFFFu);
                 }
@@ -200,7 +201,8 @@ __device__ __forceinline__ uint32_t weight_order(float w) {
 // order into kept[]. A cluster of CS blocks per KV head, block r with the r-th part of the rows, a thread with `per` neighbouring ones (in registers up to CH_KEEP).
 // The bound is found eight bits at a time: every block counts its rows by those bits, and adds up the blocks' counts for itself; one barrier of
 // the cluster a round, since each round has counters of its own. MOVE: the block then copies its kept rows into another cache.
-// 32 rounds of one bit by one block a head, every weight read again each time, took 330 us for 65529 rows of 8 heads.
+// Bound by latency: four rounds of a meeting and a scan, 11 us for 4096 rows of 8 heads to 8, 14.5 for 65529, and 20 where 8192 stay (32 rounds of one bit by
+// one block a head, every weight read again each time: 330).
 constexpr int CH_THREADS = 1024, CH_KEEP = 8, CH_CLUSTER = 8;
 template <bool IN_REGISTERS, bool MOVE>
 __global__ void __launch_bounds__(CH_THREADS) kv4_choose_kernel(Kv4 src, Kv4 dst, int32_t* __restrict__ kept, int rows, int keep, int lo, int hi, int want, int CS) {

@@ -39,14 +39,14 @@ __device__ __forceinline__ bool kv4_place(const Kv4Place& p, int B, int max_rows
 __device__ __forceinline__ int kv4_key_place(int i, int ng) { return ((i & 31) / 8 * ng + i / 32) * 8 + (i & 7); }      // where value i of a row lies
 __device__ __forceinline__ int kv4_value_place(int i, int ng) { return ((i & 31) / 4 * ng + i / 32) * 4 + (i & 3); }
 
-// Angles of positions pos0, pos0 + 1, ..: turn[position][pair] = cosine and sine of position * theta^(-2 pair / hd), in 64 bits, because far positions
+// Angles of positions pos0, pos0 + 1, ..: turn[position][pair % 4][pair / 4] (threads with neighbouring eights of values read neighbours) = cosine and sine of position * theta^(-2 pair / hd), in 64 bits, because far positions
 // times a rounded frequency are off by whole steps of a 4-bit code. By all threads of a block; about a microsecond.
 __device__ __forceinline__ void kv4_angles(double2* turn, int positions, int pos0, int hd, double log2_theta) {
     const int half = hd / 2;
     for (int e = threadIdx.x; e < positions * half; e += blockDim.x) {
         double s, c;
         sincos((double)(pos0 + e / half) * exp2((double)(e % half) * (-2.0 / hd * log2_theta)), &s, &c);
-        turn[e] = make_double2(c, s);
+        turn[e / half * half + (e & 3) * (half / 4) + e % half / 4] = make_double2(c, s);
     }
 }
 // an adjacent pair, turned in 64 bits and rounded once
@@ -87,7 +87,7 @@ __device__ __forceinline__ void kv4_write_eight(const Kv4& c, float (&x)[8], boo
     const int lane = threadIdx.x & 31;
     if (key && turn) {
 #pragma unroll
-        for (int u = 0; u < 8; u += 2) kv4_turn(x[u], x[u + 1], turn[(i + u) / 2]);
+        for (int u = 0; u < 4; u++) kv4_turn(x[2 * u], x[2 * u + 1], turn[u * 4 * NG + i / 8]);
     }
     uint32_t m = 0;
 #pragma unroll
@@ -110,15 +110,16 @@ __device__ __forceinline__ void kv4_write_eight(const Kv4& c, float (&x)[8], boo
 }
 
 // ── queries ──
-// values 8t..8t+7 of a group of one query (src: the group's first value), turned
-__device__ __forceinline__ void kv4_query(float (&x)[8], const float* src, bool on, const double2* turn) {
+// values i..i+7 of one query (src: the first of them), turned by its position's angles (turn, or NULL)
+template <int NG>
+__device__ __forceinline__ void kv4_query(float (&x)[8], const float* src, bool on, const double2* turn, int i) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = 0.0f;
+    for (int u = 0; u < 8; u++) x[u] = 0.0f;
     if (!on) return;
     kv4_load_eight(x, src);
     if (turn) {
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) kv4_turn(x[i], x[i + 1], turn[i / 2]);
+        for (int u = 0; u < 4; u++) kv4_turn(x[2 * u], x[2 * u + 1], turn[u * 4 * NG + i / 8]);
     }
 }
 // The largest magnitude of a query goes to [2^13, 2^14). A power of 2 up to 2^120, in two factors: what that leaves small are queries below

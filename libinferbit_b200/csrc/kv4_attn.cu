@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (COLS == 16 ? 2 : 
         for (int jj = 0; jj < JT; jj++) {
             const int j = warp + jj * KA_WARPS;
             if (j >= NG) break;
-            kv4_query(x[jj], src + 32 * j, on, p.w.rotate ? turn + b * (HD / 2) + 16 * j + 4 * t : nullptr);
+            kv4_query<NG>(x[jj], src + 32 * j, on, p.w.rotate ? turn + b * (HD / 2) : nullptr, 32 * j + 8 * t);
 #pragma unroll
             for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(x[jj][i]) & 0x7FFFFFFFu);
         }
@@ -790,8 +790,8 @@ int kv4_attend(ibcu_ctx* ctx, const Kv4& c, float decay, const Kv4Place& at, con
     KaCall call;
     memset(&call, 0, sizeof call);
     call.rows = rows; call.decay = decay; call.cols = large ? 16 : columns > 4 ? 8 : 4;
-    // A prompt: tcgen05 (kv4_prompt.cu) takes a third of the time a row once its tiles of 128 columns have enough SMs, the tiles of 16 here fill the machine with fewer.
-    // 32 heads over 8 after 8000 rows, us here and there: of 128 values 152 and 166 with 32 tiles of 128, 245 and 166 with 40; of 64 values 126 and 145 with 48, 184 and 147 with 64.
+    // A prompt: tcgen05 (kv4_prompt.cu) takes half of the time a row and less once its tiles of 128 columns have enough SMs, the tiles of 16 here fill the machine with fewer.
+    // 32 heads over 8 after 8000 rows, us here and there: of 128 values 155 and 216 with 32 tiles of 128, 254 and 217 with 40; of 64 values 128 and 174 with 48, 186 and 174 with 56.
     if ((c.hd == 64 || c.hd == 128) && large && c.n_kv * (columns / 128) >= (c.hd == 64 ? ctx->sm_count * 3 / 8 : ctx->sm_count / 4)) {
         Kv4Columns tp = t;
         tp.ntiles = (int)((columns + 127) / 128) * 8;

@@ -5,12 +5,15 @@
 // K' = ks (n - 8) and V' = vs (n - 8) are held values, an 11-bit scale times a 4-bit code: 15 bits, which two fp16 pieces hold exactly. Q and P are
 // two pieces of 11 bits. Each product is three instructions a step, high.high + low.high + high.low; low.low is 2^-23 of the result.
 // (On mma.sync the scales stay FP32 factors outside the products, two instructions a step, but their rate is a third; 16
-// columns share an unpacked row there, 128 here. A prompt of 2048, 32 heads of 128 over 8: 370 us that way.)
+// columns share an unpacked row there, 128 here.)
 //
 // Warps: 8 softmax, two threads a column; 4 that turn key codes into the pieces of K', 4 for V' (transposed: the rows are the
 // contraction); 1 issues the products, 1 the copies. Everything is double buffered, and S of the next rows is computed while the softmax is at these.
 // The instruction cuts its sums off, towards zero, at every step: outputs after 16000 rows were 5.7e-5 off in one accumulator, 2.3e-6 after 2048. So after a run
 // of PK_RUN times 64 rows its outputs are added, rounded, to sums in shared memory.
+// What bounds it: 2048 positions of 32 heads of 128 values over 8 take 125 us, 160 with the preparing launch, of which the products would be 62 at the measured rate. Per 64 rows
+// the softmax's chain (load, maximum, exponentials, pieces, store: 1500 cycles without exponentials and dequantisers) and shared memory (values of K' and V' written and read,
+// sums of runs) are longer than the products' 1600 cycles: leaving two of three products out gained 1 %, leaving both dequantisers out 15 %.
 // A V' of a row with a NaN scale would reach columns that do not see the row (0 * NaN), so NaN goes into the row's K' instead, and with it
 // into every column that does see it.
 #include "kv4.cuh"
