@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(128) kv4_prep_kernel(const PrepParams p) {
             for (int jj = 0; jj < JT; jj++) {
                 const int j = warp + 4 * jj;
                 if (j >= NG) break;
-                uint4* qf = p.w.qf + unit * kv4_frags(NG, true) + lane;
+                uint4* qf = p.w.qf + unit * kv4_frags(NG) + lane;
 #pragma unroll
                 for (int s = 0; s < 2; s++) {
                     uint32_t hi[2][2], lo[2][2];

@@ -10,10 +10,9 @@ struct Kv4 {
 };
 
 // The columns of a KV head are its query heads at every position, column = position * group + head of the group. They go through the
-// kernels in tiles of 8 (all columns of a call, if they are no more than that) or of 16. A tile's queries are the A operand's fragments, two fp16 pieces of every
-// value: [unit = KV head * tiles + tile][part][group of 32][step][lane] uint4. Tiles of 16 have two parts, high and low pieces, with columns 0-7 in the
-// fragments' even registers and 8-15 in the odd ones; a tile of 8 has one, with high and low pieces there. Beside them
-// qc [unit][16]: the factor that turns a column's sums into exponents of 2.
+// kernels in one tile (up to 8 columns) or in tiles of 16. The queries of a tile of 16 are the A operand's fragments, two fp16 pieces of every
+// value: [unit = KV head * tiles + tile][part][group of 32][step][lane] uint4, a part for the high pieces and one for the low ones, with columns 0-7 in the
+// fragments' even registers and 8-15 in the odd ones. Beside them qc [unit][16]: the factor that turns a column's sums into exponents of 2.
 // Prompts (kv4_prompt.cu) go in tiles of 128 columns, eight of 16 side by side, as operand images instead: [KV head * tiles + tile][part][64 values][column]
 // rows of 128 bytes in the 128-byte swizzle, a row's 16-byte pieces in the order of a key row's words (piece t * (hd / 32) + j: values 32 j + 8 t..), the eight values of a
 // piece as 0, 4, 1, 5, 2, 6, 3, 7.
@@ -21,7 +20,7 @@ struct Kv4Columns {
     int n_heads, group, B, large, ntiles;                      // large: tiles of 16; 2: as images, ntiles a multiple of 8
     __host__ __device__ int cols() const { return large ? 16 : 8; }
 };
-__host__ __device__ constexpr size_t kv4_frags(int ng, bool large) { return (size_t)(large ? 2 : 1) * ng * 64; }     // uint4s of a unit
+__host__ __device__ constexpr size_t kv4_frags(int ng) { return (size_t)ng * 128; }            // uint4s of a unit
 
 // where rows and positions of a call are: arguments, or {row0, pos0} in device memory
 struct Kv4Place { int row0, pos0; const int* at; };

@@ -35,13 +35,17 @@ namespace {
 
 constexpr int KA_WARPS = 4, KA_ROWS = 32;            // warps of a block; rows of a ring stage
 constexpr int KA_CLUSTER = 8;                        // blocks of a cluster at most
+// Tiles up to which the scores are written down for the weights instead of computed again: 32 heads of 128 values over 8, two tiles after 1536 rows 18.5 us instead of 23.4, four
+// 27.6 instead of 31.3; eight after 8000 rows 76.8 against 70.3.
+constexpr int KA_FEW_TILES = 4;
 constexpr float KA_LOW = -3.0e38f;                   // where running maxima start (finite: nothing minus infinity)
 constexpr float KA_SLACK = 1.9f;                     // by how much a maximum may be outgrown before the sums are rescaled
 
 struct KaParams {
-    Kv4 c; Kv4Columns t; Kv4Place at; Kv4Prep w;     // w.qf, w.qc: fragments prepared (LARGE), or left for the weights (few, if stat)
+    Kv4 c; Kv4Columns t; Kv4Place at; Kv4Prep w;     // w.qf, w.qc: prepared fragments (LARGE)
     float* out; float2* stat;                        // stat [unit][16] or NULL: a column's softmax weight is 2^((score - x) - y)
     float* pacc; float2* pml;                        // results of clusters [unit][cluster][16][hd], [unit][cluster][16] (maximum, sum)
+    float* scores; int score_rows;                   // few tiles, for the weights, or NULL: [unit][score_rows][column]
     int want, grid_chunks, cluster;                  // chunks at most; blocks a tile, whole clusters of them
     int* err;
 };
@@ -339,8 +343,7 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (COLS == 16 ? 2 : 
 #pragma unroll
         for (int w = 0; w < KA_WARPS; w++) m = max(m, amax[w][column]);
         const Kv4Up up = kv4_up(m, HD);
-        const bool leave = p.stat && sp == 0;
-        if (warp == 0 && t == 0) { qc[column] = up.back; if (leave) p.w.qc[(size_t)unit * 16 + (FOUR && (g & 1) ? 4 : 0) + column] = up.back; }
+        if (warp == 0 && t == 0) qc[column] = up.back;
 #pragma unroll
         for (int jj = 0; jj < JT; jj++) {
             const int j = warp + jj * KA_WARPS;
@@ -351,21 +354,15 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (COLS == 16 ? 2 : 
             for (int s = 0; s < 2; s++) {
                 uint32_t hi[2], lo[2];
                 kv4_pieces(x[jj], s, hi, lo);
-                const uint4 v = make_uint4(hi[0], lo[0], hi[1], lo[1]);
                 if (FOUR) reinterpret_cast<uint2*>(qf)[(j * 2 + s) * 32 + lane] = g & 1 ? make_uint2(lo[0], lo[1]) : make_uint2(hi[0], hi[1]);
-                else qf[(j * 2 + s) * 32 + lane] = v;
-                if (leave) {                                                                       // columns of 8, the upper four of FOUR empty
-                    uint4* to = p.w.qf + unit * kv4_frags(NG, false) + (j * 2 + s) * 32;
-                    if (!FOUR) to[lane] = v;
-                    else to[((g & 1) * 4 + column) * 4 + t] = g & 1 ? make_uint4(0, 0, 0, 0) : v;
-                }
+                else qf[(j * 2 + s) * 32 + lane] = make_uint4(hi[0], lo[0], hi[1], lo[1]);
             }
         }
     } else {
         pdl_wait();
         pdl_launch_dependents();
         if (lane == 0) asm volatile("fence.proxy.async.global;" ::: "memory");                     // rows that the preparing launch wrote
-        const uint4* src = p.w.qf + unit * kv4_frags(NG, true);
+        const uint4* src = p.w.qf + unit * kv4_frags(NG);
         for (int e = tid; e < NG * 128; e += 32 * KA_WARPS) qf[e] = __ldcg(src + e);
         if (tid < 16) qc[tid] = __ldcg(p.w.qc + (size_t)unit * 16 + tid);
     }
@@ -428,6 +425,7 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (COLS == 16 ? 2 : 
 #pragma unroll
                     for (int h = 0; h < NH; h++) {
                         s[i][h][n] *= f[n];
+                        if (p.scores) p.scores[((size_t)unit * p.score_rows + r0 + 8 * i + (FOUR ? (g >> 1) + 4 * (g & 1) : 4 * h + t)) * COLS + (FOUR ? t : g + 8 * n)] = s[i][h][n];
                         if (seen(i, h, n)) top[n] = fmaxf(top[n], s[i][h][n] + L[i][h]);
                     }
                 grow = grow || top[n] > m[n] + KA_SLACK;
@@ -641,18 +639,47 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (COLS == 16 ? 2 : 
     cluster_arrive(); cluster_wait();                          // nobody reads this block's shared memory any more
 }
 
-// Attention that the rows draw. grid (128 rows, KV heads, parts of the tiles): a warp holds the unpacked keys of 32 rows and walks the columns that see them,
-// whose fragments come through a ring; the scores are computed again, which costs less than writing them down once there are several columns. The
-// parts of a row are added in order.
+// Attention that the rows draw, of few tiles: from the scores that the attention wrote down, a thread a row. (32 heads of 128 values over 8, one token after 4000
+// rows: 9.0 us without weights, 11.4 with them, 16.8 with the kernel below, which computes the scores again.)
+template <int COLS>
+__global__ void __launch_bounds__(256) kv4_weight_few_kernel(const KaParams p, float decay) {
+    pdl_launch_dependents();
+    pdl_wait();
+    int row0, pos0;
+    if (!kv4_place(p.at, p.t.B, p.c.max_rows, p.err, row0, pos0)) return;
+    const int r = blockIdx.x * 256 + threadIdx.x, kvh = blockIdx.y;
+    if (r >= row0 + p.t.B) return;
+    const size_t at = p.c.row(kvh, r);
+    const float old = decay == 0.0f ? 0.0f : decay * __ldcg(p.c.weight + at);
+    float sum = 0.0f;
+    for (int tile = max(0, r - row0) * p.t.group / COLS; tile < p.t.ntiles; tile++) {              // from the first that sees the row
+        const size_t unit = (size_t)kvh * p.t.ntiles + tile;
+        const float* s = p.scores + (unit * p.score_rows + r) * COLS;
+        float4 x[COLS / 4];
+#pragma unroll
+        for (int c = 0; c < COLS; c += 4) x[c / 4] = __ldcg(reinterpret_cast<const float4*>(s + c));
+#pragma unroll
+        for (int c = 0; c < COLS; c++) {
+            const int b = (tile * COLS + c) / p.t.group;
+            const float2 off = __ldcg(p.stat + unit * 16 + c);
+            const float v = c % 4 == 0 ? x[c / 4].x : c % 4 == 1 ? x[c / 4].y : c % 4 == 2 ? x[c / 4].z : x[c / 4].w;
+            if (b < p.t.B && r <= row0 + b) sum += ex2((v - off.x) - off.y);
+        }
+    }
+    p.c.weight[at] = old + sum;
+}
+
+// The same of many tiles. grid (128 rows, KV heads, parts of the tiles): a warp holds the unpacked keys of 32 rows and walks the columns that see them,
+// whose fragments come through a ring; the scores are computed again. The parts of a row are added in order.
 constexpr int KW_DEPTH = 3;
-template <int NG, bool LARGE> struct KwSmem {
-    static constexpr int FRAG_BYTES = (LARGE ? 2 : 1) * NG * 1024, QC = FRAG_BYTES, STAT = QC + 64, STAGE = STAT + 128 + 64;
+template <int NG> struct KwSmem {
+    static constexpr int FRAG_BYTES = 2 * NG * 1024, QC = FRAG_BYTES, STAT = QC + 64, STAGE = STAT + 128 + 64;
     static constexpr int SCALES = KW_DEPTH * STAGE, TOTAL = SCALES + KA_WARPS * NG * 128;
 };
-template <int NG, bool LARGE>
+template <int NG>
 __global__ void __launch_bounds__(32 * KA_WARPS) kv4_weight_kernel(const KaParams p, float decay, float* __restrict__ parts) {
-    using S = KwSmem<NG, LARGE>;
-    constexpr int NC = LARGE ? 2 : 1, COLS = 8 * NC;
+    using S = KwSmem<NG>;
+    constexpr int NC = 2, COLS = 16;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ unsigned long long full[KW_DEPTH];
     __shared__ int abort_flag;
@@ -675,7 +702,7 @@ __global__ void __launch_bounds__(32 * KA_WARPS) kv4_weight_kernel(const KaParam
         const int unit = kvh * p.t.ntiles + first + i * gridDim.z, d = i % KW_DEPTH;
         const uint32_t bar = smem_u32(&full[d]), to = smem_u32(smem + d * S::STAGE);
         mbar_expect_tx(bar, S::FRAG_BYTES + 64 + 128);
-        bulk_load(to, p.w.qf + unit * kv4_frags(NG, LARGE), S::FRAG_BYTES, bar);
+        bulk_load(to, p.w.qf + unit * kv4_frags(NG), S::FRAG_BYTES, bar);
         bulk_load(to + S::QC, p.w.qc + (size_t)unit * 16, 64, bar);
         bulk_load(to + S::STAT, p.stat + (size_t)unit * 16, 128, bar);
     };
@@ -705,7 +732,7 @@ __global__ void __launch_bounds__(32 * KA_WARPS) kv4_weight_kernel(const KaParam
         if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&full[d]), phase, &abort_flag, IBCU_KV4_WAIT_ERR))) { __syncthreads(); continue; }      // the barrier below is everyone's
         const unsigned char* stage = smem + d * S::STAGE;
         float s[4][2][NC];
-        score_rows<NG, LARGE>(s, [&](int k, int j, uint32_t* to) {
+        score_rows<NG, true>(s, [&](int k, int j, uint32_t* to) {
 #pragma unroll
             for (int u = 0; u < 4; u++) to[u] = kf[k][j][u];
         }, reinterpret_cast<const uint4*>(stage), sc, lane);
@@ -762,16 +789,20 @@ struct KaCall { int cols, chunks, rows, n_parts; float decay; float* parts; };
 
 template <int NG, int COLS>
 int launch_attention(ibcu_ctx* ctx, const KaParams& p, const KaCall& k) {
-    static SmemOptIn opt, opt_w;
+    static SmemOptIn opt;
     constexpr bool LARGE = COLS == 16;
     const size_t smem = KaSmem<NG, COLS>::TOTAL + (!LARGE && p.w.rotate ? (size_t)p.t.B * 16 * NG * sizeof(double2) : 0);
     if (int rc = ibcu_allow_smem(ctx, opt, kv4_attn_kernel<NG, COLS>, smem)) return rc;
     int rc = ibcu_launch(ctx, kv4_attn_kernel<NG, COLS>, dim3(p.c.n_kv * p.t.ntiles * k.chunks), dim3(32 * KA_WARPS), smem, p.cluster, true, p);
     if (!rc && k.chunks > p.cluster) rc = ibcu_launch(ctx, kv4_join_kernel, dim3(std::min(p.t.cols(), p.t.B * p.t.group), p.c.n_kv * p.t.ntiles), dim3(128), 0, 1, true, p);
     if (rc || !p.stat) return rc;
-    if ((rc = ibcu_allow_smem(ctx, opt_w, kv4_weight_kernel<NG, LARGE>, KwSmem<NG, LARGE>::TOTAL))) return rc;
-    rc = ibcu_launch(ctx, kv4_weight_kernel<NG, LARGE>, dim3((k.rows + 127) / 128, p.c.n_kv, k.n_parts), dim3(32 * KA_WARPS), KwSmem<NG, LARGE>::TOTAL, 1, true, p, k.decay, k.n_parts > 1 ? k.parts : (float*)nullptr);
-    if (!rc && k.n_parts > 1) rc = ibcu_launch(ctx, kv4_weight_join_kernel, dim3((k.rows + 255) / 256, p.c.n_kv), dim3(256), 0, 1, true, p, k.decay, (const float*)k.parts, k.n_parts);
+    if (p.scores) return ibcu_launch(ctx, kv4_weight_few_kernel<COLS>, dim3((k.rows + 255) / 256, p.c.n_kv), dim3(256), 0, 1, true, p, k.decay);
+    if constexpr (LARGE) {
+        static SmemOptIn opt_w;
+        if ((rc = ibcu_allow_smem(ctx, opt_w, kv4_weight_kernel<NG>, KwSmem<NG>::TOTAL))) return rc;
+        rc = ibcu_launch(ctx, kv4_weight_kernel<NG>, dim3((k.rows + 127) / 128, p.c.n_kv, k.n_parts), dim3(32 * KA_WARPS), KwSmem<NG>::TOTAL, 1, true, p, k.decay, k.n_parts > 1 ? k.parts : (float*)nullptr);
+        if (!rc && k.n_parts > 1) rc = ibcu_launch(ctx, kv4_weight_join_kernel, dim3((k.rows + 255) / 256, p.c.n_kv), dim3(256), 0, 1, true, p, k.decay, (const float*)k.parts, k.n_parts);
+    }
     return rc;
 }
 template <int NG>
@@ -826,11 +857,11 @@ int kv4_attend(ibcu_ctx* ctx, const Kv4& c, float decay, const Kv4Place& at, con
     const int row_blocks = (rows + 127) / 128;
     call.n_parts = c.weight && ntiles >= 16 ? std::min(std::min(ntiles, 16), std::max(1, 6 * ctx->sm_count / (row_blocks * c.n_kv))) : 1;
     auto round_up = [](size_t n) { return (n + 255) & ~(size_t)255; };
-    const bool frags = large || c.weight;
-    const size_t b_qf = frags ? round_up(units * kv4_frags(ng, large) * sizeof(uint4)) : 0, b_qc = frags ? round_up((size_t)units * 16 * sizeof(float)) : 0;
+    const size_t b_qf = large ? round_up(units * kv4_frags(ng) * sizeof(uint4)) : 0, b_qc = large ? round_up((size_t)units * 16 * sizeof(float)) : 0;
+    const size_t b_scores = c.weight && ntiles <= KA_FEW_TILES ? round_up((size_t)units * stages * KA_ROWS * call.cols * sizeof(float)) : 0;
     const size_t b_stat = c.weight ? round_up((size_t)units * 16 * sizeof(float2)) : 0, b_ml = joined > 1 ? round_up((size_t)units * joined * 16 * sizeof(float2)) : 0;
     const size_t b_acc = joined > 1 ? round_up((size_t)units * joined * 16 * c.hd * sizeof(float)) : 0, b_parts = call.n_parts > 1 ? round_up((size_t)call.n_parts * c.n_kv * c.max_rows * sizeof(float)) : 0;
-    if (int rc = ibcu_reserve(ctx, &ctx->scratch, &ctx->scratch_bytes, b_qf + b_qc + b_stat + b_ml + b_acc + b_parts)) return rc;
+    if (int rc = ibcu_reserve(ctx, &ctx->scratch, &ctx->scratch_bytes, b_qf + b_qc + b_scores + b_stat + b_ml + b_acc + b_parts)) return rc;
     char* s = (char*)ctx->scratch;
     auto take = [&](size_t n) { char* r = s; s += n; return r; };
     KaParams p;
@@ -838,6 +869,8 @@ int kv4_attend(ibcu_ctx* ctx, const Kv4& c, float decay, const Kv4Place& at, con
     p.c = c; p.t = t; p.at = at;
     uint4* qf = (uint4*)take(b_qf); float* qc = (float*)take(b_qc);
     p.w = Kv4Prep{ q, k, v, qf, qc, log2_theta, rotate };
+    p.scores = (float*)take(b_scores); if (!b_scores) p.scores = nullptr;
+    p.score_rows = stages * KA_ROWS;
     p.stat = (float2*)take(b_stat); if (!c.weight) p.stat = nullptr;
     p.pml = (float2*)take(b_ml); p.pacc = (float*)take(b_acc);
     call.parts = (float*)take(b_parts);
