@@ -168,7 +168,7 @@ int ibcu_linear_w4a8_fp32(ibcu_ctx* ctx, const ibcu_linear_t* tensor, const floa
 int ibcu_quantize_rows_int8(ibcu_ctx* ctx, const float* x, int8_t* q, float* scale, int N, int B);
 /* out[b*out_stride + m] = (sum_j w[m][j] * xq[b][j]) * (scale_w[m] * sx[b]), or added to out (IBCU_EPI_ADD), for n_tensors (1..4) INT8
  * tensors that share the activations. The sums are exact (int32): the same bits however the call is cut. The outputs of a
- * call do not overlap. N up to 131072, B up to 2^20. w and xq at any address; rows that do not start on 16 bytes (w or xq unaligned, or N no multiple
+ * call overlap neither one another nor its inputs. N up to 131072, B up to 2^20. w and xq at any address; rows that do not start on 16 bytes (w or xq unaligned, or N no multiple
  * of 16) are first copied so that they do. */
 int ibcu_linear_w8a8(ibcu_ctx* ctx, const ibcu_linear_t* tensors, int n_tensors, const int8_t* xq, const float* sx, int N, int B);
 /* Both steps for FP32 activations x[b*N + j]. Same bits as the two calls. */
@@ -282,8 +282,8 @@ int ibcu_kv4_write(ibcu_ctx* ctx, const ibcu_kv4_t* cache, const float* k, const
 /* The values that rows row0..row0+n-1 hold, as [n][n_kv_heads * head_dim]. */
 int ibcu_kv4_read(ibcu_ctx* ctx, const ibcu_kv4_t* cache, float* k, float* v, int row0, int n);
 /* GQA attention as ibcu_attention, over the cache: query position b (q [B][n_heads * head_dim], rotated already) sees rows 0..row0+b,
- * which includes its own. Any B that the cache has rows for. Products and sums keep FP32's accuracy (FP32 queries and
- * weights times the held codes; nothing is rounded to fewer bits). With cache->weight, row r of a KV head gets
+ * which includes its own. Any B that the cache has rows for; out overlaps no input. Queries and softmax weights enter the products as two
+ * pieces of 11 bits, sums are FP32: outputs are 3e-7 of their size off those in 64 bits, up to 1e-6 in prompts. With cache->weight, row r of a KV head gets
  * weight = decay * weight + the softmax weights that it had over all positions of the call and query heads of the group. */
 int ibcu_attention_kv4(ibcu_ctx* ctx, const ibcu_kv4_t* cache, const float* q, float* out, int n_heads, int row0, int B);
 /* The attention step of a decode layer, as ibcu_attention_decode: queries and keys rotated, the new rows row0..row0+B-1 written,

@@ -616,8 +616,9 @@ int launch_prompt(ibcu_ctx* ctx, const PkParams& p, int rows, float* parts, int 
 
 }  // namespace
 
+// Blocks of the weights an SM: 2048 positions of 32 heads over 8, attention and weights, us with two, three and four: of 128 values 211, 218 and 221, of 64 values 188, 167 and 160.
 int kv4_prompt_parts(ibcu_ctx* ctx, const Kv4& c, int tiles, int rows) {
-    return std::min(std::min(tiles, 16), std::max(1, (3 * ctx->sm_count) / (((rows + 127) / 128) * c.n_kv)));
+    return std::min(std::min(tiles, 16), std::max(1, ((c.hd == 64 ? 4 : 2) * ctx->sm_count) / (((rows + 127) / 128) * c.n_kv)));
 }
 int kv4_prompt(ibcu_ctx* ctx, const Kv4& c, const Kv4Columns& t, const Kv4Place& at, const unsigned char* image, const float* qc, float* out, float2* stat, int rows, float* parts, int n_parts) {
     PkParams p;
