@@ -44,7 +44,7 @@ __device__ __forceinline__ void kv4_angles(double2* turn, int positions, int pos
     const int half = hd / 2;
     for (int e = threadIdx.x; e < positions * half; e += blockDim.x) {
         double s, c;
-        sincos((double)(pos0 + e / half) * exp2((double)(e % half) * (-2.0 / hd * log2_theta)), &s, &c);
+        sincos(((double)pos0 + e / half) * exp2((double)(e % half) * (-2.0 / hd * log2_theta)), &s, &c);
         turn[e / half * half + (e & 3) * (half / 4) + e % half / 4] = make_double2(c, s);
     }
 }

@@ -303,3 +303,33 @@ def test_captured_at_a_device_place(backend, n_heads, n_kv, hd, B, max_rows):
                 assert np.array_equal(raw(a), raw(b))
     finally:
         be._check(be.lib.ibcu_graph_destroy(be.ctx, gid))
+
+
+@pytest.mark.parametrize("n_heads,n_kv,hd,row0,B", [(32, 8, 128, 6000, 1), (8, 1, 128, 9001, 1), (64, 8, 64, 5000, 1), (32, 32, 96, 4200, 1), (4, 2, 256, 8193, 2), (8, 1, 64, 7000, 6), (16, 2, 192, 4097, 3),
+                                                    (4, 4, 32, 20000, 1), (32, 8, 128, 4090, 6)])
+def test_contexts_of_many_chunks(backend, n_heads, n_kv, hd, row0, B):
+    """More chunks than a cluster has blocks, in tiles of 4, 8 and 16 columns."""
+    test_attention_and_weights(backend, n_heads, n_kv, hd, row0, B)
+
+
+@pytest.mark.parametrize("n_heads,n_kv,hd,row0,B", [(8, 1, 128, 8000, 640), (8, 1, 64, 8000, 900), (8, 2, 128, 12000, 60), (4, 1, 96, 12000, 100), (8, 1, 128, 30000, 1)])
+def test_sums_over_many_rows_stay_exact(backend, n_heads, n_kv, hd, row0, B):
+    """The tensor cores cut every addition off by up to 2^-23 of the sum, all in one direction. Within the 192 rows that a sum is theirs there are 36 additions, so that
+    the outputs are off by at most 36 * 2^-23 of their size, and by about as much again from scores of 24 additions (less than 2 log2 units in size) and
+    everything that is rounded. (All rows in one sum would be hundreds of additions: 5.7e-5 off.)"""
+    be, rng = backend, np.random.default_rng(row0)
+    R = row0 + B
+    max_rows = (R + 7) // 8 * 8
+    planes = _kv4.random_planes(rng, n_kv, hd, max_rows, R)
+    q = rng.standard_normal((B, n_heads * hd), dtype=np.float32)
+    dq, do = be.upload(q), be.alloc(q.nbytes)
+    be._check(be.lib.ibcu_attention_kv4(be.ctx, put(be, *planes), dq.ptr, do.ptr, n_heads, row0, B)); be.sync()
+    got = be.download(do, np.float32, q.size).reshape(B, n_heads, hd)
+    K, V = _kv4.plane_values(*(p[:, :R] for p in planes))
+    off = size = 0.0
+    for h in range(n_heads):
+        s = q.reshape(B, n_heads, hd)[:, h].astype(np.float64) @ K[h * n_kv // n_heads].T / np.sqrt(hd)
+        p = np.where(np.arange(R)[None] <= row0 + np.arange(B)[:, None], np.exp(s - s.max(1, keepdims=True)), 0.0)
+        want = p @ V[h * n_kv // n_heads] / p.sum(1, keepdims=True)
+        off, size = off + ((got[:, h] - want) ** 2).sum(), size + (want ** 2).sum()
+    assert np.sqrt(off / size) <= 2 * 36 * 2.0 ** -23, np.sqrt(off / size)
