@@ -198,15 +198,49 @@ __device__ __forceinline__ uint32_t weight_order(float w) {
 }
 
 // The choice: the `want` rows of [lo, hi) with the largest weights, equal ones from the lowest row, beside all rows outside it, in ascending
-// order into kept[]. A cluster of CS blocks per KV head, block r with the r-th part of the rows, a thread with `per` neighbouring ones (in registers up to CH_KEEP).
+// order into kept[]. A cluster of CS blocks per KV head, block r with the r-th part of the rows, a thread with `per` neighbouring ones, in registers up to KEYS (0: read again every time).
 // The bound is found eight bits at a time: every block counts its rows by those bits, and adds up the blocks' counts for itself; one barrier of
 // the cluster a round, since each round has counters of its own. MOVE: the block then copies its kept rows into another cache.
-// Bound by latency: four rounds of a meeting and a scan, 11 us for 4096 rows of 8 heads to 8, 14.5 for 65529, and 20 where 8192 stay (32 rounds of one bit by
-// one block a head, every weight read again each time: 330).
-constexpr int CH_THREADS = 1024, CH_KEEP = 8, CH_CLUSTER = 8;
-template <bool IN_REGISTERS, bool MOVE>
+// Bound by latency: a round is a meeting, the blocks' counts and a scan, 1.5 us, and there are three of them mostly (rows with equal bits that all stay end it):
+// 9.7 us for 4096 rows of 8 heads to 1024, 19 for 65529 to 8192. (32 rounds of one bit by one block a head, every weight read again each time: 330.) Keys in
+// registers: 131071 rows 23 us, 50 with the weights read every time; one a thread where that is enough: 4096 rows 9.7 us, 10.9 with room for eight.
+constexpr int CH_THREADS = 1024, CH_CLUSTER = 8;
+// Kept rows of a block times their values up to which the choosing launch copies them: 4096 rows of 8 heads of 128 values to 1024 take 9.7 us, 10.4 with a launch of its own; 65529 to
+// 40000 42.7 and 37.4; 65529 rows of one head to 20000 25.1 and 16.7.
+constexpr long CH_MOVE = 65536;
+// rows list[i0..i1-1] (list NULL: i0..i1-1) of a head to rows i0..i1-1 of another cache, by a block; two pieces a thread on their way at a time
+__device__ __forceinline__ void move_rows(const Kv4& src, const Kv4& dst, int h, const int32_t* list, long i0, long i1) {
+    const int ng = src.hd / 32, tid = threadIdx.x, piece = tid % ng, at_once = CH_THREADS / ng;
+    if (tid >= at_once * ng) return;
+    for (i0 += tid / ng; i0 < i1; i0 += 2 * at_once) {
+        uint4 vk[2], vv[2];
+        uint32_t vs[2];
+        float vw[2];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const long i = i0 + u * at_once;
+            if (i >= i1) break;
+            const size_t from = src.row(h, list ? __ldcg(list + i) : (int)i);
+            vk[u] = __ldcg(reinterpret_cast<const uint4*>(src.k) + from * ng + piece);
+            vv[u] = __ldcg(reinterpret_cast<const uint4*>(src.v) + from * ng + piece);
+            vs[u] = __ldcg(reinterpret_cast<const uint32_t*>(src.scale) + from * ng + piece);
+            vw[u] = piece == 0 ? __ldcg(src.weight + from) : 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const long i = i0 + u * at_once;
+            if (i >= i1) break;
+            const size_t to = dst.row(h, (int)i);
+            reinterpret_cast<uint4*>(dst.k)[to * ng + piece] = vk[u];
+            reinterpret_cast<uint4*>(dst.v)[to * ng + piece] = vv[u];
+            reinterpret_cast<uint32_t*>(dst.scale)[to * ng + piece] = vs[u];
+            if (piece == 0 && dst.weight) dst.weight[to] = vw[u];
+        }
+    }
+}
+template <int KEYS, bool MOVE>
 __global__ void __launch_bounds__(CH_THREADS) kv4_choose_kernel(Kv4 src, Kv4 dst, int32_t* __restrict__ kept, int rows, int keep, int lo, int hi, int want, int CS) {
-    __shared__ uint32_t hist[4][256], total[256], totals[2], found[2];
+    __shared__ uint32_t hist[4][256], total[256], totals[2], found[3];
     __shared__ uint32_t warp_gt[32], warp_eq[32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = blockIdx.x % CS, h = blockIdx.x / CS;
     for (int i = tid; i < 1024; i += CH_THREADS) (&hist[0][0])[i] = 0;
@@ -217,26 +251,32 @@ __global__ void __launch_bounds__(CH_THREADS) kv4_choose_kernel(Kv4 src, Kv4 dst
     const int slice = (rows + CS - 1) / CS, per = (slice + CH_THREADS - 1) / CH_THREADS;
     const int r0 = rank * slice + tid * per, n = max(0, min(min(per, slice - tid * per), rows - r0));
     const float* w = src.weight + src.row(h, 0);
-    uint32_t key[CH_KEEP];
-    if (IN_REGISTERS) {
+    uint32_t key[KEYS ? KEYS : 1];
+    if constexpr (KEYS > 0) {
 #pragma unroll
-        for (int i = 0; i < CH_KEEP; i += 4) {
-            if (i + 4 <= n && ((uintptr_t)(w + r0) & 15) == 0) {
+        for (int i = 0; i < KEYS; i += 4) {
+            if (KEYS >= 4 && i + 4 <= n && ((uintptr_t)(w + r0) & 15) == 0) {
                 const float4 x = __ldcg(reinterpret_cast<const float4*>(w + r0 + i));
                 key[i] = weight_order(x.x); key[i + 1] = weight_order(x.y); key[i + 2] = weight_order(x.z); key[i + 3] = weight_order(x.w);
             } else {
 #pragma unroll
-                for (int u = 0; u < 4; u++) key[i + u] = i + u < n ? weight_order(__ldcg(w + r0 + i + u)) : 0u;
+                for (int u = 0; u < 4; u++) if (i + u < KEYS) key[i + u] = i + u < n ? weight_order(__ldcg(w + r0 + i + u)) : 0u;
             }
         }
     }
     // f(row, order, whether the row is one of those chosen from) for this thread's rows in order
     auto each = [&](auto f) {
-        if (IN_REGISTERS) {
+        if constexpr (KEYS > 0) {
 #pragma unroll
-            for (int i = 0; i < CH_KEEP; i++) if (i < n) f(r0 + i, key[i], r0 + i >= lo && r0 + i < hi);
+            for (int i = 0; i < KEYS; i++) if (i < n) f(r0 + i, key[i], r0 + i >= lo && r0 + i < hi);
         } else {
-            for (int i = 0; i < n; i++) f(r0 + i, weight_order(__ldcg(w + r0 + i)), r0 + i >= lo && r0 + i < hi);
+            for (int i0 = 0; i0 < n; i0 += 8) {                // eight on their way at a time
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] = i0 + i < n ? __ldcg(w + r0 + i0 + i) : 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; i++) if (i0 + i < n) f(r0 + i0 + i, weight_order(x[i]), r0 + i0 + i >= lo && r0 + i0 + i < hi);
+            }
         }
     };
     uint32_t bound = 0, left = (uint32_t)want;                // rows still to be found among those that share the bound's bits so far
@@ -267,7 +307,7 @@ __global__ void __launch_bounds__(CH_THREADS) kv4_choose_kernel(Kv4 src, Kv4 dst
                 if (before < left && before + sum >= left) {
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
-                        if (before < left && before + c[i] >= left) { found[0] = 255 - 8 * lane - i; found[1] = before; }
+                        if (before < left && before + c[i] >= left) { found[0] = 255 - 8 * lane - i; found[1] = before; found[2] = c[i]; }
                         before += c[i];
                     }
                 }
@@ -275,6 +315,11 @@ __global__ void __launch_bounds__(CH_THREADS) kv4_choose_kernel(Kv4 src, Kv4 dst
             __syncthreads();
             bound |= found[0] << shift;
             left -= found[1];
+            if (found[2] == left && bound) {                  // all rows with these bits stay, whatever their other bits are: the same for every block
+                bound--;
+                left = 0;
+                break;
+            }
         }
     }
     // left: rows at the bound that stay, from the lowest. Who stays, and where it goes:
@@ -321,60 +366,15 @@ __global__ void __launch_bounds__(CH_THREADS) kv4_choose_kernel(Kv4 src, Kv4 dst
     });
     if (CS > 1) { cluster_arrive(); cluster_wait(); }         // nobody needs another block's shared memory any more, and the list is whole
     else __syncthreads();
-    if (MOVE) {
-        // Equal parts of the list (the last rows, which all stay, would otherwise fall to the last block).
-        const int ng = src.hd / 32, piece = tid % ng, at_once = CH_THREADS / ng;
-        const int i1 = (int)((long)keep * (rank + 1) / CS);
-        for (long i0 = (long)keep * rank / CS + tid / ng; tid < at_once * ng && i0 < i1; i0 += 2 * at_once) {
-            uint4 vk[2], vv[2];
-            uint32_t vs[2];
-            float vw[2];
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const long i = i0 + u * at_once;
-                if (i >= i1) break;
-                const size_t from = src.row(h, __ldcg(mine + i));
-                vk[u] = __ldcg(reinterpret_cast<const uint4*>(src.k) + from * ng + piece);
-                vv[u] = __ldcg(reinterpret_cast<const uint4*>(src.v) + from * ng + piece);
-                vs[u] = __ldcg(reinterpret_cast<const uint32_t*>(src.scale) + from * ng + piece);
-                vw[u] = piece == 0 ? __ldcg(src.weight + from) : 0.0f;
-            }
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const long i = i0 + u * at_once;
-                if (i >= i1) break;
-                const size_t to = dst.row(h, (int)i);
-                reinterpret_cast<uint4*>(dst.k)[to * ng + piece] = vk[u];
-                reinterpret_cast<uint4*>(dst.v)[to * ng + piece] = vv[u];
-                reinterpret_cast<uint32_t*>(dst.scale)[to * ng + piece] = vs[u];
-                if (piece == 0 && dst.weight) dst.weight[to] = vw[u];
-            }
-        }
-    }
+    if (MOVE) move_rows(src, dst, h, mine, (long)keep * rank / CS, (long)keep * (rank + 1) / CS);        // equal parts of the list (the last rows, which all stay, would otherwise fall to the last block)
 }
 
-// In place: grid (3, KV heads), a block moves the keys, the values or the scales and weights of all kept rows. Rows only move towards the
-// front, so a pass that has all its pieces in registers before it stores the first may write over the rows they came from.
-__global__ void __launch_bounds__(1024) kv4_move_kernel(Kv4 c, const int32_t* __restrict__ kept, int keep) {
+// The same copy by all SMs, where there is much of it. kept NULL: rows 0..keep-1. grid (parts, KV heads)
+__global__ void __launch_bounds__(CH_THREADS) kv4_move_kernel(Kv4 src, Kv4 dst, const int32_t* __restrict__ kept, int keep) {
     pdl_launch_dependents();
     pdl_wait();
-    const int h = blockIdx.y, ng = c.hd / 32, tid = threadIdx.x;
-    const int32_t* idx = kept + (size_t)h * keep;
-    auto shift = [&](auto* plane, int pieces) {
-        const int piece = tid % pieces, at_once = 1024 / pieces, mine = tid < at_once * pieces ? tid / pieces : keep;
-        for (int i0 = 0; i0 < keep; i0 += 4 * at_once) {
-            std::remove_reference_t<decltype(*plane)> v[4];
-#pragma unroll
-            for (int u = 0; u < 4; u++) { const long i = (long)mine + i0 + u * at_once; if (i < keep) v[u] = __ldcg(plane + c.row(h, __ldcg(idx + i)) * pieces + piece); }
-            __syncthreads();
-#pragma unroll
-            for (int u = 0; u < 4; u++) { const long i = (long)mine + i0 + u * at_once; if (i < keep) plane[c.row(h, (int)i) * pieces + piece] = v[u]; }
-            __syncthreads();
-        }
-    };
-    if (blockIdx.x == 0) shift(reinterpret_cast<uint4*>(c.k), ng);
-    else if (blockIdx.x == 1) shift(reinterpret_cast<uint4*>(c.v), ng);
-    else { shift(reinterpret_cast<uint32_t*>(c.scale), ng); shift(c.weight, 1); }
+    const int h = blockIdx.y;
+    move_rows(src, dst, h, kept ? kept + (size_t)h * keep : nullptr, (long)keep * blockIdx.x / gridDim.x, (long)keep * (blockIdx.x + 1) / gridDim.x);
 }
 
 Kv4 planes(const ibcu_kv4_t* t) { return Kv4{ t->k, t->v, (__half*)t->scale, t->weight, t->n_kv_heads, t->head_dim, t->max_rows }; }
@@ -475,18 +475,31 @@ extern "C" int ibcu_kv4_evict(ibcu_ctx* ctx, const ibcu_kv4_t* src, const ibcu_k
     const bool in_place = src->k == dst->k;
     IBCU_REQUIRE(ctx, in_place ? src->v == dst->v && src->scale == dst->scale && src->weight == dst->weight && src->max_rows == dst->max_rows
                                : src->v != dst->v && src->scale != dst->scale && src->weight != dst->weight, "ibcu_kv4_evict: two caches that share some planes");
-    if (!kept) {
-        int rc = ibcu_reserve(ctx, &ctx->scratch, &ctx->scratch_bytes, (size_t)nkv * keep * sizeof(int32_t));
-        if (rc) return rc;
-        kept = (int32_t*)ctx->scratch;
+    // In place the kept rows go by way of scratch.
+    Kv4 to = planes(dst);
+    const bool by_way = in_place && keep < rows;
+    auto round_up = [](size_t n) { return (n + 255) & ~(size_t)255; };
+    const size_t held = (size_t)nkv * keep, b_kept = kept ? 0 : round_up(held * sizeof(int32_t)), row_bytes = src->head_dim / 2, b_plane = round_up(held * row_bytes), b_scale = round_up(held * src->head_dim / 8);
+    if (int rc = ibcu_reserve(ctx, &ctx->scratch, &ctx->scratch_bytes, b_kept + (by_way ? 2 * b_plane + b_scale + held * sizeof(float) : 0))) return rc;
+    char* s = (char*)ctx->scratch;
+    if (!kept) kept = (int32_t*)s;
+    if (by_way) {
+        s += b_kept;
+        to.k = (uint8_t*)s; to.v = (uint8_t*)(s + b_plane); to.scale = (__half*)(s + 2 * b_plane); to.weight = (float*)(s + 2 * b_plane + b_scale);
+        to.max_rows = keep;
     }
     // A block a thousand rows, up to eight, as long as all clusters run at once: 12 of eight blocks, 33 of four, 74 of two find their places (8192 rows of 32 heads
     // by eight blocks each 38 us, by four 14).
     int CS = 1;
     while (CS < CH_CLUSTER && rows > 1024 * CS && nkv <= (CS == 4 ? ctx->sm_count / 12 : CS == 2 ? ctx->sm_count * 9 / 40 : ctx->sm_count / 2)) CS *= 2;
-    const bool regs = (rows + CS - 1) / CS <= CH_THREADS * CH_KEEP;
-    auto choose = regs ? (in_place ? kv4_choose_kernel<true, false> : kv4_choose_kernel<true, true>) : (in_place ? kv4_choose_kernel<false, false> : kv4_choose_kernel<false, true>);
-    int rc = ibcu_launch(ctx, choose, dim3(CS * nkv), dim3(CH_THREADS), 0, CS, true, planes(src), planes(dst), kept, rows, keep, sink, rows - recent, keep - sink - recent, CS);
-    if (!rc && in_place && keep < rows) rc = ibcu_launch(ctx, kv4_move_kernel, dim3(3, nkv), dim3(1024), 0, 1, true, planes(src), (const int32_t*)kept, keep);
+    const bool move = !in_place || by_way, here = move && (long)keep / CS * src->head_dim <= CH_MOVE;
+    const int per = ((rows + CS - 1) / CS + CH_THREADS - 1) / CH_THREADS;
+    auto pick = [&](auto with, auto without) { return here ? with : without; };
+    auto choose = per <= 1 ? pick(kv4_choose_kernel<1, true>, kv4_choose_kernel<1, false>) : per <= 8 ? pick(kv4_choose_kernel<8, true>, kv4_choose_kernel<8, false>)
+                : per <= 16 ? pick(kv4_choose_kernel<16, true>, kv4_choose_kernel<16, false>) : pick(kv4_choose_kernel<0, true>, kv4_choose_kernel<0, false>);
+    int rc = ibcu_launch(ctx, choose, dim3(CS * nkv), dim3(CH_THREADS), 0, CS, true, planes(src), to, kept, rows, keep, sink, rows - recent, keep - sink - recent, CS);
+    const dim3 grid((unsigned)std::max(1, std::min(2 * ctx->sm_count / nkv, (keep + 255) / 256)), nkv);
+    if (!rc && move && !here) rc = ibcu_launch(ctx, kv4_move_kernel, grid, dim3(CH_THREADS), 0, 1, true, planes(src), to, (const int32_t*)kept, keep);
+    if (!rc && by_way) rc = ibcu_launch(ctx, kv4_move_kernel, grid, dim3(CH_THREADS), 0, 1, true, to, planes(dst), (const int32_t*)nullptr, keep);
     return rc;
 }

@@ -333,3 +333,32 @@ def test_sums_over_many_rows_stay_exact(backend, n_heads, n_kv, hd, row0, B):
         want = p @ V[h * n_kv // n_heads] / p.sum(1, keepdims=True)
         off, size = off + ((got[:, h] - want) ** 2).sum(), size + (want ** 2).sum()
     assert np.sqrt(off / size) <= 2 * 36 * 2.0 ** -23, np.sqrt(off / size)
+
+
+@pytest.mark.parametrize("n_kv,hd,rows,keep,sink,recent", [(1, 32, 150001, 100000, 3, 7), (40, 64, 3000, 900, 4, 100), (14, 128, 9000, 5000, 0, 0), (1, 64, 131072, 1, 0, 0)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_eviction_by_size(backend, n_kv, hd, rows, keep, sink, recent, in_place):
+    """More rows than registers hold, more heads than clusters of eight or four have room, more kept rows than the choosing launch copies."""
+    test_eviction(backend, n_kv, hd, rows, keep, sink, recent, in_place)
+
+
+def test_eviction_by_weights_that_share_their_bits(backend):
+    """Bounds that are found after one round, two or three, and the smallest there is."""
+    be, rng = backend, np.random.default_rng(8)
+    n_kv, hd, rows = 6, 32, 4096
+    bits = np.empty((n_kv, rows), np.uint32)
+    bits[0] = np.where(np.arange(rows) % 4 == 0, 0x41000000, 0x3F000000)                   # the first eight bits decide for 1024 rows
+    bits[1] = 0x3F800000 + rng.permutation(rows).astype(np.uint32)                         # all but the last thirteen bits are equal
+    bits[2] = 0                                                                             # zeros: the lowest rows
+    bits[3] = 0x7FC00000                                                                    # NaN: the lowest rows
+    bits[4] = np.where(np.arange(rows) % 4 == 1, 0x3F900000, 0x3F800000)
+    bits[5] = np.where(np.arange(rows) < 1024, 0x80000000, 0xFF800000)                      # minus zero above minus infinity
+    w = bits.view(np.float32)
+    planes = _kv4.random_planes(rng, n_kv, hd, rows, rows)
+    for keep in (1024, 1023, 1025, 1):
+        src, dst = put(be, *planes, weight=w), be.make_kv4(n_kv, hd, rows, weights=True)
+        kept = be.alloc(n_kv * keep * 4)
+        be._check(be.lib.ibcu_kv4_evict(be.ctx, src, dst, rows, keep, 0, 0, kept.ptr)); be.sync()
+        got = be.download(kept, np.int32, n_kv * keep).reshape(n_kv, keep)
+        for h in range(n_kv):
+            assert np.array_equal(got[h], _kv4.choose(w[h], keep, 0, 0)), (keep, h)
