@@ -23,8 +23,13 @@ __device__ __forceinline__ float token_scale(uint32_t m, float& inv) {
     inv = __fdiv_rn(1.0f, s);
     return s;
 }
-__device__ __forceinline__ int code_of(float v, float inv) { return inv > 0.0f ? (int)rintf(__fmul_rn(v, inv)) & 255 : 0; }
-__device__ __forceinline__ uint32_t codes_of(const float4& v, float inv) { return (uint32_t)(code_of(v.x, inv) | code_of(v.y, inv) << 8 | code_of(v.z, inv) << 16 | code_of(v.w, inv) << 24); }
+// rint(v * inv) in the lowest byte: what is added lifts a value's integer part to the lowest bits, rounded to even
+__device__ __forceinline__ uint32_t code_bits(float v, float inv) { return __float_as_uint(__fadd_rn(__fmul_rn(v, inv), 12582912.0f)); }
+__device__ __forceinline__ int8_t code_of(float v, float inv) { return inv > 0.0f ? (int8_t)code_bits(v, inv) : (int8_t)0; }
+__device__ __forceinline__ uint32_t codes_of(const float4& v, float inv) {
+    const uint32_t lo = __byte_perm(code_bits(v.x, inv), code_bits(v.y, inv), 0x0040), hi = __byte_perm(code_bits(v.z, inv), code_bits(v.w, inv), 0x0040);
+    return inv > 0.0f ? __byte_perm(lo, hi, 0x5410) : 0u;
+}
 
 // Rows of `n` bytes that begin anywhere, `from` apart, into rows `to` apart (a multiple of 16): TMA wants rows that start on 16 bytes.
 struct AlignJob { const uint8_t* src; uint8_t* dst; long from, to, rows; int n; };
@@ -92,7 +97,7 @@ __global__ void __launch_bounds__(512) quantize_rows_kernel(const float* __restr
         for (int i = tid + QR_KEEP * nth; i < n4; i += nth) put(i, __ldcg(x4 + i));
         for (int i = N + tid; i < ldq; i += nth) qb[i] = 0;
     } else {
-        for (int i = tid; i < ldq; i += nth) qb[i] = i < N ? (int8_t)code_of(__ldcg(xb + i), inv) : (int8_t)0;
+        for (int i = tid; i < ldq; i += nth) qb[i] = i < N ? code_of(__ldcg(xb + i), inv) : (int8_t)0;
     }
     if (tid == 0) scale[b] = s;
 }
