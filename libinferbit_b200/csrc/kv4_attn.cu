@@ -843,15 +843,20 @@ int kv4_attend(ibcu_ctx* ctx, const Kv4& c, float decay, const Kv4Place& at, con
     const int stages = (rows + KA_ROWS - 1) / KA_ROWS;
     // Blocks an SM that chunks are cut for: what fits, but two where a stage is short beside a block's start (one token of 32 heads over 8 of 64 values after 32767
     // rows: 14.8 us, 17.3 with three; of 128 values 21.9 with two, 18.4 with three). One cluster of eight, and so no second launch, for contexts that leave each
-    // of its warps four stages at most (after 4000 rows 9.0 against 10.3 us, after 8000 12.4 against 11.9). Clusters of four beyond, since those of eight leave places of the
-    // machine empty (32767 rows: 28 against 20.7 us), unless there is an SM for each block (one KV head: 12.6 against 14.3).
-    int want = std::max(1, (large || (columns <= 4 && ng <= 2) || ng > 4 ? 2 : 3) * ctx->sm_count / units), chunk;
+    // of its warps four stages at most (after 4000 rows 9.0 against 10.3 us, after 8000 12.4 against 11.9). Beyond, clusters spare the second launch results to read, but find
+    // their places only while the machine is not full: of eight where there is an SM for each block (one KV head 12.6 us, 14.3 by four), of four up to four fifths of it (32 heads over 4 after
+    // 20000 rows 15.4 us, 17.5 without), of two for many chunks (32 over 8 after 131071 rows 43.5, 44.6 without and by four), none else (32 heads of their own after 32767
+    // rows 42.9, 46.6 by two).
+    const int fit = (large || ng > 4 ? 2 : 3) * ctx->sm_count;
+    int want = std::max(1, (columns <= 4 && ng <= 2 ? 2 * ctx->sm_count : fit) / units), chunk;
     if (stages <= KA_CLUSTER * KA_WARPS * 4) want = std::min(want, KA_CLUSTER);
-    if (want > KA_CLUSTER) want = want / 4 * 4;
+    if (want > 16) want &= ~1;
     ka_plan(rows, want, chunk, call.chunks);
     if (at.at) call.chunks = std::min(want, (stages + KA_WARPS - 1) / KA_WARPS);                   // shorter contexts may have more, shorter chunks
+    const long blocks = (long)units * call.chunks;
+    const int most = call.chunks <= KA_CLUSTER || blocks <= ctx->sm_count ? KA_CLUSTER : blocks * 5 / 4 <= fit ? 4 : call.chunks > 16 ? 2 : 1;
     int cluster = 1;
-    while (cluster < std::min(call.chunks, call.chunks > KA_CLUSTER && (long)units * call.chunks > ctx->sm_count ? 4 : KA_CLUSTER)) cluster *= 2;
+    while (cluster < std::min(call.chunks, most)) cluster *= 2;
     call.chunks = (call.chunks + cluster - 1) / cluster * cluster;
     const int joined = call.chunks / cluster;
     const int row_blocks = (rows + 127) / 128;
