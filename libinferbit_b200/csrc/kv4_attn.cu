@@ -35,8 +35,8 @@ namespace {
 
 constexpr int KA_WARPS = 4, KA_ROWS = 32;            // warps of a block; rows of a ring stage
 constexpr int KA_CLUSTER = 8;                        // blocks of a cluster at most
-// Tiles up to which the scores are written down for the weights instead of computed again: 32 heads of 128 values over 8, two tiles after 1536 rows 18.5 us instead of 23.4, four
-// 27.6 instead of 31.3; eight after 8000 rows 76.8 against 70.3.
+// Tiles up to which the scores are written down for the weights instead of computed again: 32 heads of 128 values over 8, two tiles after 1536 rows 15.8 us instead of 23.4, four
+// 21.6 instead of 31.3; eight after 8000 rows, a thread a row, 76.8 against 70.3.
 constexpr int KA_FEW_TILES = 4;
 constexpr float KA_LOW = -3.0e38f;                   // where running maxima start (finite: nothing minus infinity)
 constexpr float KA_SLACK = 1.9f;                     // by how much a maximum may be outgrown before the sums are rescaled
@@ -639,34 +639,43 @@ __global__ void __launch_bounds__(32 * KA_WARPS, NG > 4 ? 1 : (COLS == 16 ? 2 : 
     cluster_arrive(); cluster_wait();                          // nobody reads this block's shared memory any more
 }
 
-// Attention that the rows draw, of few tiles: from the scores that the attention wrote down, a thread a row. (32 heads of 128 values over 8, one token after 4000
-// rows: 9.0 us without weights, 11.4 with them, 16.8 with the kernel below, which computes the scores again.)
+// Attention that the rows draw, of few tiles: from the scores that the attention wrote down, a thread for a row's four columns of every tile, all loads on their way at once. (32
+// heads of 128 values over 8, one token after 4000 rows: 8.9 us without weights, 10.8 with them, 16.8 with the kernel below, which computes the scores again.)
 template <int COLS>
 __global__ void __launch_bounds__(256) kv4_weight_few_kernel(const KaParams p, float decay) {
+    constexpr int LANES = COLS / 4, TILES = COLS == 16 ? KA_FEW_TILES : 1;
     pdl_launch_dependents();
     pdl_wait();
     int row0, pos0;
     if (!kv4_place(p.at, p.t.B, p.c.max_rows, p.err, row0, pos0)) return;
-    const int r = blockIdx.x * 256 + threadIdx.x, kvh = blockIdx.y;
-    if (r >= row0 + p.t.B) return;
-    const size_t at = p.c.row(kvh, r);
-    const float old = decay == 0.0f ? 0.0f : decay * __ldcg(p.c.weight + at);
+    const long e = (long)blockIdx.x * 256 + threadIdx.x;
+    const int r = (int)min(e / LANES, (long)p.score_rows), c4 = (int)(e % LANES) * 4, kvh = blockIdx.y;
+    const bool on = r < row0 + p.t.B;
+    const size_t at = p.c.row(kvh, on ? r : 0);
+    float4 x[TILES], off[TILES][2];
+#pragma unroll
+    for (int i = 0; i < TILES; i++) {
+        const size_t unit = (size_t)kvh * p.t.ntiles + i;
+        if (!on || i >= p.t.ntiles) continue;
+        x[i] = __ldcg(reinterpret_cast<const float4*>(p.scores + (unit * p.score_rows + r) * COLS + c4));
+        off[i][0] = __ldcg(reinterpret_cast<const float4*>(p.stat + unit * 16 + c4));
+        off[i][1] = __ldcg(reinterpret_cast<const float4*>(p.stat + unit * 16 + c4) + 1);
+    }
+    const float old = !on || decay == 0.0f ? 0.0f : decay * __ldcg(p.c.weight + at);
     float sum = 0.0f;
-    for (int tile = max(0, r - row0) * p.t.group / COLS; tile < p.t.ntiles; tile++) {              // from the first that sees the row
-        const size_t unit = (size_t)kvh * p.t.ntiles + tile;
-        const float* s = p.scores + (unit * p.score_rows + r) * COLS;
-        float4 x[COLS / 4];
 #pragma unroll
-        for (int c = 0; c < COLS; c += 4) x[c / 4] = __ldcg(reinterpret_cast<const float4*>(s + c));
+    for (int i = 0; i < TILES; i++) {
+        if (!on || i >= p.t.ntiles) continue;
+        const float v[4] = { x[i].x, x[i].y, x[i].z, x[i].w }, m[4] = { off[i][0].x, off[i][0].z, off[i][1].x, off[i][1].z }, l[4] = { off[i][0].y, off[i][0].w, off[i][1].y, off[i][1].w };
 #pragma unroll
-        for (int c = 0; c < COLS; c++) {
-            const int b = (tile * COLS + c) / p.t.group;
-            const float2 off = __ldcg(p.stat + unit * 16 + c);
-            const float v = c % 4 == 0 ? x[c / 4].x : c % 4 == 1 ? x[c / 4].y : c % 4 == 2 ? x[c / 4].z : x[c / 4].w;
-            if (b < p.t.B && r <= row0 + b) sum += ex2((v - off.x) - off.y);
+        for (int c = 0; c < 4; c++) {
+            const int b = (i * COLS + c4 + c) / p.t.group;
+            if (b < p.t.B && r <= row0 + b) sum += ex2((v[c] - m[c]) - l[c]);
         }
     }
-    p.c.weight[at] = old + sum;
+#pragma unroll
+    for (int o = 1; o < LANES; o *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (on && c4 == 0) p.c.weight[at] = old + sum;
 }
 
 // The same of many tiles. grid (128 rows, KV heads, parts of the tiles): a warp holds the unpacked keys of 32 rows and walks the columns that see them,
@@ -796,7 +805,7 @@ int launch_attention(ibcu_ctx* ctx, const KaParams& p, const KaCall& k) {
     int rc = ibcu_launch(ctx, kv4_attn_kernel<NG, COLS>, dim3(p.c.n_kv * p.t.ntiles * k.chunks), dim3(32 * KA_WARPS), smem, p.cluster, true, p);
     if (!rc && k.chunks > p.cluster) rc = ibcu_launch(ctx, kv4_join_kernel, dim3(std::min(p.t.cols(), p.t.B * p.t.group), p.c.n_kv * p.t.ntiles), dim3(128), 0, 1, true, p);
     if (rc || !p.stat) return rc;
-    if (p.scores) return ibcu_launch(ctx, kv4_weight_few_kernel<COLS>, dim3((k.rows + 255) / 256, p.c.n_kv), dim3(256), 0, 1, true, p, k.decay);
+    if (p.scores) return ibcu_launch(ctx, kv4_weight_few_kernel<COLS>, dim3((unsigned)(((long)k.rows * (COLS / 4) + 255) / 256), p.c.n_kv), dim3(256), 0, 1, true, p, k.decay);
     if constexpr (LARGE) {
         static SmemOptIn opt_w;
         if ((rc = ibcu_allow_smem(ctx, opt_w, kv4_weight_kernel<NG>, KwSmem<NG>::TOTAL))) return rc;
