@@ -362,3 +362,56 @@ def test_eviction_by_weights_that_share_their_bits(backend):
         got = be.download(kept, np.int32, n_kv * keep).reshape(n_kv, keep)
         for h in range(n_kv):
             assert np.array_equal(got[h], _kv4.choose(w[h], keep, 0, 0)), (keep, h)
+
+
+@pytest.mark.parametrize("n_heads,n_kv,hd,row0,B", [(32, 8, 128, 40, 1), (8, 1, 64, 5000, 1), (16, 4, 96, 11, 9), (32, 8, 128, 3, 200), (12, 3, 256, 0, 2)])
+def test_activations_at_any_address(backend, n_heads, n_kv, hd, row0, B):
+    """Queries, keys, values and outputs four bytes off a 16-byte boundary, and rows written and read back so: the same bits as on one."""
+    be, rng = backend, np.random.default_rng(B)
+    max_rows = (row0 + B + 7) // 8 * 8
+    planes = _kv4.random_planes(rng, n_kv, hd, max_rows, row0 + B)
+    draw = lambda heads: rng.standard_normal((B, heads * hd), dtype=np.float32)
+    x = [draw(n_heads), draw(n_kv), draw(n_kv)]
+    results = []
+    for off in (0, 4):
+        t = put(be, *planes, weight=np.zeros((n_kv, max_rows), np.float32))
+        d = [be.alloc(a.nbytes + 16) for a in x]
+        for b, a in zip(d, x):
+            be.write(b, a, off)
+        o, kb, vb = be.alloc(x[0].nbytes + 16), be.alloc(x[1].nbytes + 16), be.alloc(x[1].nbytes + 16)
+        be._check(be.lib.ibcu_attention_decode_kv4(be.ctx, t, *(b.at(off) for b in d), o.at(off), n_heads, row0, row0 + 7, B, 10000.0))
+        be._check(be.lib.ibcu_kv4_read(be.ctx, t, kb.at(off), vb.at(off), row0, B)); be.sync()
+        raw_of = lambda b, n: be.download(b, np.float32, n + 4)[off // 4:off // 4 + n]
+        results.append([raw_of(o, x[0].size), raw_of(kb, x[1].size), raw_of(vb, x[1].size)] + [raw(a) for a in get(be, t)])
+    for a, b in zip(*results):
+        assert np.array_equal(a, b, equal_nan=a.dtype.kind == "f")
+
+
+def test_captured_eviction_in_place(backend):
+    """A captured step and cut of the same cache, replayed over fresh contents."""
+    import ctypes as C
+    be, rng = backend, np.random.default_rng(3)
+    n_kv, hd, rows, keep = 4, 64, 3000, 700
+    planes = _kv4.random_planes(rng, n_kv, hd, rows, rows)
+    t = put(be, *planes, weight=np.zeros((n_kv, rows), np.float32))
+    kept = be.alloc(n_kv * keep * 4)
+    call = lambda: be._check(be.lib.ibcu_kv4_evict(be.ctx, t, t, rows, keep, 4, 60, kept.ptr))
+    call(); be.sync()
+    gid = C.c_int()
+    be._check(be.lib.ibcu_graph_begin(be.ctx)); call(); be._check(be.lib.ibcu_graph_end(be.ctx, C.byref(gid)))
+    try:
+        for _ in range(3):
+            planes = _kv4.random_planes(rng, n_kv, hd, rows, rows)
+            w = rng.exponential(1.0, (n_kv, rows)).astype(np.float32)
+            for b, a in zip(t._keep, planes):
+                be.write(b, a.view(np.uint16) if a.dtype == np.float16 else a)
+            be.write(t._keep[3], w)
+            be._check(be.lib.ibcu_graph_launch(be.ctx, gid)); be.sync()
+            got, after = be.download(kept, np.int32, n_kv * keep).reshape(n_kv, keep), get(be, t)
+            for h in range(n_kv):
+                at = _kv4.choose(w[h], keep, 4, 60)
+                assert np.array_equal(got[h], at)
+                for a, b in zip(after, planes + (w,)):
+                    assert np.array_equal(raw(a[h, :keep]), raw(b[h, at])) and np.array_equal(raw(a[h, keep:]), raw(b[h, keep:]))
+    finally:
+        be._check(be.lib.ibcu_graph_destroy(be.ctx, gid))
