@@ -164,29 +164,36 @@ __global__ void __launch_bounds__(128) kv4_prep_kernel(const PrepParams p) {
     }
 }
 
-// The values that the cache holds: a thread has a word of eight codes of a key row and the word at the same place of the value row
+// The values that the cache holds: a thread has a word of eight codes of a key row and the word at the same place of the value row, a block as many whole positions as it
+// has threads for. 2048 rows of 8 heads of 128 values 5.4 us, of which the bytes are 2.9; 8192 rows 15.5 of 11.7.
+template <int NG>
 __global__ void __launch_bounds__(256) kv4_read_kernel(Kv4 c, float* __restrict__ k, float* __restrict__ v, int row0, int n) {
+    constexpr int WORDS = 4 * NG;
     pdl_launch_dependents();
     pdl_wait();
-    const int ng = c.hd / 32, words = 4 * ng, per_row = c.n_kv * words;
+    const int per_row = c.n_kv * WORDS, at_once = max(1, 256 / per_row), own = at_once > 1 ? threadIdx.x / per_row : 0;
     const bool vec = (((uintptr_t)k | (uintptr_t)v) & 15) == 0;
-    auto put = [&](float* to, uint32_t codes, float s) {      // the four lowest codes
-        const float x[4] = { (float)((int)(codes & 15) - 8) * s, (float)((int)(codes >> 4 & 15) - 8) * s, (float)((int)(codes >> 8 & 15) - 8) * s, (float)((int)(codes >> 12 & 15) - 8) * s };
+    if (own >= at_once) return;
+    auto put = [&](float* to, uint32_t codes, float s) {      // the four lowest codes: under the exponent of 2^23 a code n is the float 2^23 + n
+        float x[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) x[u] = (__uint_as_float((codes >> (4 * u) & 15u) | 0x4B000000u) - 8388616.0f) * s;
         if (vec) *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
         else { to[0] = x[0]; to[1] = x[1]; to[2] = x[2]; to[3] = x[3]; }
     };
-    for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < (long)n * per_row; e += (long)gridDim.x * 256) {
-        const int b = (int)(e / per_row), h = (int)(e % per_row) / words, w = (int)(e % per_row) % words;
-        const size_t row = c.row(h, row0 + b), out = ((size_t)b * c.n_kv + h) * c.hd;
-        const uint32_t kw = __ldcg(reinterpret_cast<const uint32_t*>(c.k) + row * words + w), vw = __ldcg(reinterpret_cast<const uint32_t*>(c.v) + row * words + w);
-        const __half* sc = c.scale + row * 2 * ng;
-        const int j = w % ng, t = w / ng, u0 = 2 * w, u1 = 2 * w + 1;                  // the key's group and piece; the value row's units of four codes
-        const float ks = scale_at(sc + j), v0 = scale_at(sc + ng + u0 % ng), v1 = scale_at(sc + ng + u1 % ng);
-        put(k + out + 32 * j + 8 * t, kw, ks);
-        put(k + out + 32 * j + 8 * t + 4, kw >> 16, ks);
-        put(v + out + 32 * (u0 % ng) + 4 * (u0 / ng), vw, v0);
-        put(v + out + 32 * (u1 % ng) + 4 * (u1 / ng), vw >> 16, v1);
-    }
+    for (long b = (long)blockIdx.x * at_once + own; b < n; b += (long)gridDim.x * at_once)
+        for (int i = threadIdx.x - own * per_row; i < per_row; i += 256) {
+            const int h = i / WORDS, w = i % WORDS;
+            const size_t row = c.row(h, row0 + (int)b), out = ((size_t)b * c.n_kv + h) * (32 * NG);
+            const uint32_t kw = __ldcg(reinterpret_cast<const uint32_t*>(c.k) + row * WORDS + w), vw = __ldcg(reinterpret_cast<const uint32_t*>(c.v) + row * WORDS + w);
+            const __half* sc = c.scale + row * 2 * NG;
+            const int j = w % NG, t = w / NG, u0 = 2 * w, u1 = 2 * w + 1;              // the key's group and piece; the value row's units of four codes
+            const float ks = scale_at(sc + j), v0 = scale_at(sc + NG + u0 % NG), v1 = scale_at(sc + NG + u1 % NG);
+            put(k + out + 32 * j + 8 * t, kw, ks);
+            put(k + out + 32 * j + 8 * t + 4, kw >> 16, ks);
+            put(v + out + 32 * (u0 % NG) + 4 * (u0 / NG), vw, v0);
+            put(v + out + 32 * (u1 % NG) + 4 * (u1 / NG), vw >> 16, v1);
+        }
 }
 
 // weights as whole numbers in the order of the choice: larger weight first, NaN last, the two zeros equal
@@ -423,8 +430,9 @@ extern "C" int ibcu_kv4_read(ibcu_ctx* ctx, const ibcu_kv4_t* cache, float* k, f
     if (int rc = check_cache(ctx, cache, "ibcu_kv4_read")) return rc;
     IBCU_REQUIRE(ctx, k && v, "ibcu_kv4_read: null pointer");
     if (int rc = check_rows(ctx, cache, row0, n, "ibcu_kv4_read")) return rc;
-    const long words = (long)n * cache->n_kv_heads * (cache->head_dim / 8);
-    return ibcu_launch(ctx, kv4_read_kernel, dim3((int)std::min((words + 255) / 256, 16L * ctx->sm_count)), dim3(256), 0, 1, true, planes(cache), k, v, row0, n);
+    const int per_row = cache->n_kv_heads * (cache->head_dim / 8), at_once = std::max(1, 256 / per_row), hd = cache->head_dim;
+    auto kern = hd == 32 ? kv4_read_kernel<1> : hd == 64 ? kv4_read_kernel<2> : hd == 96 ? kv4_read_kernel<3> : hd == 128 ? kv4_read_kernel<4> : hd == 192 ? kv4_read_kernel<6> : kv4_read_kernel<8>;
+    return ibcu_launch(ctx, kern, dim3((int)std::min(((long)n + at_once - 1) / at_once, 16L * ctx->sm_count)), dim3(256), 0, 1, true, planes(cache), k, v, row0, n);
 }
 
 static int check_heads(ibcu_ctx* ctx, const ibcu_kv4_t* cache, int n_heads, int B, const char* call) {
