@@ -37,7 +37,7 @@ template <int NG> struct PkSmem {
     static constexpr int KB = NG / 2, HD = 32 * NG;            // KB: blocks of 64 values, a swizzled row of 128 bytes each
     static constexpr int IMAGE = 2 * KB * 16384, KEYS = 2 * KB * 8192, VALUES = 2 * HD * 128, RAW_BYTES = PK_ROWS * 36 * NG;
     static constexpr int K = 0, V = K + 2 * KEYS, RAW = V + 2 * VALUES;
-    static constexpr int SUM = RAW + PK_RAW * RAW_BYTES, TOTAL = SUM + HD * PK_COLS * 4;         // SUM [TMEM column / 4][column] float4
+    static constexpr int SUM = RAW + PK_RAW * RAW_BYTES, TOTAL = SUM + HD * PK_COLS * 2;         // SUM [value / 4][column] float4, of the upper half of the values
 };
 struct PkShared {
     unsigned long long q_full, raw_full[PK_RAW], raw_empty[PK_RAW], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], s_empty[2], p_full[2], pv_done[2], drained;
@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem_o = sh->tmem_base, tmem_s = tmem_o + S::HD, tmem_p = tmem_s + 2 * PK_ROWS, tmem_q = tmem_p + 2 * PK_ROWS;          // 128 + 2 x 64 + 2 x 64 + 128 columns
+    const uint32_t tmem_o = sh->tmem_base, tmem_s = tmem_o + S::HD, tmem_p = tmem_s + 2 * PK_ROWS, tmem_sum = tmem_p + PK_ROWS, tmem_q = tmem_sum + 64;          // 128 + 2 x 64 + 64 + 64 + 128 columns
 
     if (warp == PK_TMA_WARP) {
         if (elect_one() && n) {
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
                 for (int m = 0; m < 3; m++)
 #pragma unroll
                     for (int st = 0; st < PK_ROWS / 16; st++)
-                        mma_f16_ts(tmem_o, tmem_p + b * PK_ROWS + (m == 0) * (PK_ROWS / 2) + st * 8, v + ((m == 1) * S::HD * 128 >> 4) + st * 2, idesc_o, m || st ? 1u : more);
+                        mma_f16_ts(tmem_o, tmem_p + (m == 0) * (PK_ROWS / 2) + st * 8, v + ((m == 1) * S::HD * 128 >> 4) + st * 2, idesc_o, m || st ? 1u : more);
                 mma_commit(smem_u32(&sh->v_empty[b]));
                 mma_commit(smem_u32(&sh->pv_done[b]));
             }
@@ -361,27 +361,34 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
                 high[u] = bits(x);
                 low[u] = bits(__floats2half2_rn(a - back.x, z - back.y));
             }
-            alive = i < 2 || __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->pv_done[b]), ph ^ 1u, abort_flag, 11));       // this half of P is free
-            if (begins && i) alive = alive && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->pv_done[b ^ 1]), ph_last, abort_flag, 14));
+            alive = !i || __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->pv_done[b ^ 1]), ph_last, abort_flag, 11));       // P has been read, and outputs are whole
             if (!alive) continue;
             if (begins && i) {                                 // a run has ended
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-                for (int d = half * (S::HD / 2); d < (half + 1) * (S::HD / 2); d += 16) {
+                for (int d = 0; d < S::HD / 2; d += 16) {
                     uint32_t o[16];
-                    tmem_ld16(tmem_o + lanes + d, o);
+                    tmem_ld16(tmem_o + lanes + half * (S::HD / 2) + d, o);
+                    if (half == 0) {
+                        uint32_t old[16];
+                        if (i > PK_RUN) tmem_ld16(tmem_sum + lanes + d, old);
 #pragma unroll
-                    for (int u = 0; u < 4; u++) {
-                        float4* at = sums + (d / 4 + u) * PK_COLS;
-                        const float4 old = i > PK_RUN ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
-                        *at = make_float4(fmaf(__uint_as_float(o[4 * u]), corr, old.x * aged), fmaf(__uint_as_float(o[4 * u + 1]), corr, old.y * aged),
-                                          fmaf(__uint_as_float(o[4 * u + 2]), corr, old.z * aged), fmaf(__uint_as_float(o[4 * u + 3]), corr, old.w * aged));
+                        for (int u = 0; u < 16; u++) old[u] = __float_as_uint(fmaf(__uint_as_float(o[u]), corr, i > PK_RUN ? __uint_as_float(old[u]) * aged : 0.0f));
+                        tmem_st16(tmem_sum + lanes + d, old);
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < 4; u++) {
+                            float4* at = sums + (d / 4 + u) * PK_COLS;
+                            const float4 old = i > PK_RUN ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
+                            *at = make_float4(fmaf(__uint_as_float(o[4 * u]), corr, old.x * aged), fmaf(__uint_as_float(o[4 * u + 1]), corr, old.y * aged),
+                                              fmaf(__uint_as_float(o[4 * u + 2]), corr, old.z * aged), fmaf(__uint_as_float(o[4 * u + 3]), corr, old.w * aged));
+                        }
                     }
                 }
                 aged = 1.0f;
             }
-            tmem_st16(tmem_p + lanes + b * PK_ROWS + 16 * half, high);
-            tmem_st16(tmem_p + lanes + b * PK_ROWS + PK_ROWS / 2 + 16 * half, low);
+            tmem_st16(tmem_p + lanes + 16 * half, high);
+            tmem_st16(tmem_p + lanes + PK_ROWS / 2 + 16 * half, low);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
@@ -403,13 +410,25 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
                 for (int h = 0; h < 2; h++) {
                     uint32_t x[16];
                     tmem_ld16(tmem_o + lanes + 32 * j + 16 * h, x);
+                    const int d = 32 * (j - half * (NG / 2)) + 16 * h;                             // of the thread's half
+                    float old[16];
+                    if (n <= PK_RUN) {
 #pragma unroll
-                    for (int u = 0; u < 4; u++) {
-                        const float4 old = n > PK_RUN ? sums[(8 * j + 4 * h + u) * PK_COLS] : make_float4(0.f, 0.f, 0.f, 0.f);
-                        float* to16 = o + 16 * h + 4 * u;
-                        to16[0] = fmaf(old.x, aged, __uint_as_float(x[4 * u])); to16[1] = fmaf(old.y, aged, __uint_as_float(x[4 * u + 1]));
-                        to16[2] = fmaf(old.z, aged, __uint_as_float(x[4 * u + 2])); to16[3] = fmaf(old.w, aged, __uint_as_float(x[4 * u + 3]));
+                        for (int u = 0; u < 16; u++) old[u] = 0.0f;
+                    } else if (half == 0) {
+                        uint32_t y[16];
+                        tmem_ld16(tmem_sum + lanes + d, y);
+#pragma unroll
+                        for (int u = 0; u < 16; u++) old[u] = __uint_as_float(y[u]);
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < 4; u++) {
+                            const float4 y = sums[(d / 4 + u) * PK_COLS];
+                            old[4 * u] = y.x; old[4 * u + 1] = y.y; old[4 * u + 2] = y.z; old[4 * u + 3] = y.w;
+                        }
                     }
+#pragma unroll
+                    for (int u = 0; u < 16; u++) o[16 * h + u] = fmaf(old[u], aged, __uint_as_float(x[u]));
                 }
                 if (!on) continue;
 #pragma unroll
