@@ -831,7 +831,7 @@ int kv4_attend(ibcu_ctx* ctx, const Kv4& c, float decay, const Kv4Place& at, con
     memset(&call, 0, sizeof call);
     call.rows = rows; call.decay = decay; call.cols = large ? 16 : columns > 4 ? 8 : 4;
     // A prompt: tcgen05 (kv4_prompt.cu) takes half of the time a row and less once its tiles of 128 columns have enough SMs, the tiles of 16 here fill the machine with fewer.
-    // 32 heads over 8 after 8000 rows, us here and there: of 128 values 155 and 216 with 32 tiles of 128, 254 and 217 with 40; of 64 values 128 and 174 with 48, 186 and 174 with 56.
+    // 32 heads over 8 after 8000 rows, us here and there: of 128 values 158 and 204 with 32 tiles of 128, 272 and 204 with 40; of 64 values 132 and 170 with 48, 193 and 168 with 56.
     if ((c.hd == 64 || c.hd == 128) && large && c.n_kv * (columns / 128) >= (c.hd == 64 ? ctx->sm_count * 3 / 8 : ctx->sm_count / 4)) {
         Kv4Columns tp = t;
         tp.ntiles = (int)((columns + 127) / 128) * 8;

@@ -8,10 +8,11 @@
 // columns share an unpacked row there, 128 here.)
 //
 // Warps: 8 softmax, two threads a column; 4 that turn key codes into the pieces of K', 4 for V' (transposed: the rows are the
-// contraction); 1 issues the products, 1 the copies. Everything is double buffered, and S of the next rows is computed while the softmax is at these.
+// contraction); 1 issues the products, 1 the copies. All but P is double buffered, and S of the next rows is computed while the softmax is at these.
 // The instruction cuts its sums off, towards zero, at every step: outputs after 16000 rows were 5.7e-5 off in one accumulator, 2.3e-6 after 2048. So after a run
-// of PK_RUN times 64 rows its outputs are added, rounded, to sums in shared memory.
-// What bounds it: 2048 positions of 32 heads of 128 values over 8 take 125 us, 160 with the preparing launch, of which the products would be 62 at the measured rate. Per 64 rows
+// of PK_RUN times 64 rows its outputs are added, rounded, to sums: half of them in tensor memory, beside one place for P, half in shared memory (all of them there, in steps
+// of 16: 160 us instead of 145).
+// What bounds it: 2048 positions of 32 heads of 128 values over 8 take 145 us with the preparing launch, of which the products would be 62 at the measured rate. Per 64 rows
 // the softmax's chain (load, maximum, exponentials, pieces, store: 1500 cycles without exponentials and dequantisers) and shared memory (values of K' and V' written and read,
 // sums of runs) are longer than the products' 1600 cycles: leaving two of three products out gained 1 %, leaving both dequantisers out 15 %.
 // A V' of a row with a NaN scale would reach columns that do not see the row (0 * NaN), so NaN goes into the row's K' instead, and with it
@@ -363,32 +364,35 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
             }
             alive = !i || __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->pv_done[b ^ 1]), ph_last, abort_flag, 11));       // P has been read, and outputs are whole
             if (!alive) continue;
+            tmem_st16(tmem_p + lanes + 16 * half, high);
+            tmem_st16(tmem_p + lanes + PK_ROWS / 2 + 16 * half, low);
             if (begins && i) {                                 // a run has ended
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-                for (int d = 0; d < S::HD / 2; d += 16) {
-                    uint32_t o[16];
-                    tmem_ld16(tmem_o + lanes + half * (S::HD / 2) + d, o);
+                for (int d = 0; d < S::HD / 2; d += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(tmem_o + lanes + half * (S::HD / 2) + d, o);
                     if (half == 0) {
-                        uint32_t old[16];
-                        if (i > PK_RUN) tmem_ld16(tmem_sum + lanes + d, old);
+                        uint32_t old[32];
+                        tmem_ld32(tmem_sum + lanes + d, old);
+                        tmem_wait_ld(o);
+                        tmem_wait_ld(old);
 #pragma unroll
-                        for (int u = 0; u < 16; u++) old[u] = __float_as_uint(fmaf(__uint_as_float(o[u]), corr, i > PK_RUN ? __uint_as_float(old[u]) * aged : 0.0f));
-                        tmem_st16(tmem_sum + lanes + d, old);
+                        for (int u = 0; u < 32; u++) old[u] = __float_as_uint(fmaf(__uint_as_float(o[u]), corr, i > PK_RUN ? __uint_as_float(old[u]) * aged : 0.0f));
+                        tmem_st32(tmem_sum + lanes + d, old);
                     } else {
+                        float4 old[8];
 #pragma unroll
-                        for (int u = 0; u < 4; u++) {
-                            float4* at = sums + (d / 4 + u) * PK_COLS;
-                            const float4 old = i > PK_RUN ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
-                            *at = make_float4(fmaf(__uint_as_float(o[4 * u]), corr, old.x * aged), fmaf(__uint_as_float(o[4 * u + 1]), corr, old.y * aged),
-                                              fmaf(__uint_as_float(o[4 * u + 2]), corr, old.z * aged), fmaf(__uint_as_float(o[4 * u + 3]), corr, old.w * aged));
-                        }
+                        for (int u = 0; u < 8; u++) old[u] = i > PK_RUN ? sums[(d / 4 + u) * PK_COLS] : make_float4(0.f, 0.f, 0.f, 0.f);
+                        tmem_wait_ld(o);
+#pragma unroll
+                        for (int u = 0; u < 8; u++)
+                            sums[(d / 4 + u) * PK_COLS] = make_float4(fmaf(__uint_as_float(o[4 * u]), corr, old[u].x * aged), fmaf(__uint_as_float(o[4 * u + 1]), corr, old[u].y * aged),
+                                                                      fmaf(__uint_as_float(o[4 * u + 2]), corr, old[u].z * aged), fmaf(__uint_as_float(o[4 * u + 3]), corr, old[u].w * aged));
                     }
                 }
                 aged = 1.0f;
             }
-            tmem_st16(tmem_p + lanes + 16 * half, high);
-            tmem_st16(tmem_p + lanes + PK_ROWS / 2 + 16 * half, low);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
