@@ -11,8 +11,8 @@
 // contraction); 1 issues the products, 1 the copies. All but P is double buffered, and S of the next rows is computed while the softmax is at these.
 // The instruction cuts its sums off, towards zero, at every step: outputs after 16000 rows were 5.7e-5 off in one accumulator, 2.3e-6 after 2048. So after a run
 // of PK_RUN times 64 rows its outputs are added, rounded, to sums: half of them in tensor memory, beside one place for P, half in shared memory (all of them there, in steps
-// of 16: 160 us instead of 145).
-// What bounds it: 2048 positions of 32 heads of 128 values over 8 take 145 us with the preparing launch, of which the products would be 62 at the measured rate. Per 64 rows
+// of 16: 160 us instead of 143).
+// What bounds it: 2048 positions of 32 heads of 128 values over 8 take 143 us with the preparing launch, of which the products would be 62 at the measured rate. Per 64 rows
 // the softmax's chain (load, maximum, exponentials, pieces, store: 1500 cycles without exponentials and dequantisers) and shared memory (values of K' and V' written and read,
 // sums of runs) are longer than the products' 1600 cycles: leaving two of three products out gained 1 %, leaving both dequantisers out 15 %.
 // A V' of a row with a NaN scale would reach columns that do not see the row (0 * NaN), so NaN goes into the row's K' instead, and with it
@@ -200,8 +200,8 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
         }
         __syncwarp();
     } else if (warp >= PK_KEY_WARP) {
-        // 96 registers a thread at the launch: 256 x 80 + 256 x 112 + 64 x 96 are the 576 x 96 there
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        // 96 registers a thread at the launch: 256 x 72 + 256 x 120 + 64 x 96 are the 576 x 96 there
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         const bool keys = warp < PK_VALUE_WARP;
         const int w = warp & 3;
         int s = 0; uint32_t ph = 0;
@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
         }
     } else {
         // A column has two threads, of warps w and w + 4: each has 32 of the rows, half of the queries' copy and of the outputs.
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
         const int quarter = warp & 3, half = warp >> 2, own = quarter * 32 + lane, c = c0 + own, b_col = c / p.t.group;
         const bool on = b_col < p.t.B;
         const int lim = row0 + b_col, lim0 = row0 + (c0 + quarter * 32) / p.t.group;             // last rows that this column, the warp's first column, see

@@ -415,3 +415,52 @@ def test_captured_eviction_in_place(backend):
                     assert np.array_equal(raw(a[h, :keep]), raw(b[h, at])) and np.array_equal(raw(a[h, keep:]), raw(b[h, keep:]))
     finally:
         be._check(be.lib.ibcu_graph_destroy(be.ctx, gid))
+
+
+@pytest.mark.parametrize("n_heads,n_kv,hd,row0,B", [(8, 2, 64, 700, 1), (16, 2, 128, 700, 1), (8, 2, 96, 500, 30), (8, 2, 128, 900, 70), (8, 2, 64, 300, 1000), (8, 2, 128, 300, 700)])
+def test_extreme_scores_in_every_form(backend, n_heads, n_kv, hd, row0, B):
+    """Queries times 1e30 give each softmax one row, whose weight is 1, zeros weigh all rows alike, NaN stays in its own position and head, and a key of NaN in the positions
+    that see it: for every kernel that a number of columns may reach."""
+    be, rng = backend, np.random.default_rng(hd + B)
+    R = row0 + B
+    max_rows = (R + 7) // 8 * 8
+    planes = _kv4.random_planes(rng, n_kv, hd, max_rows, R)
+    group = n_heads // n_kv
+    K, V = _kv4.plane_values(*(p[:, :R] for p in planes))
+    q = rng.standard_normal((B, n_heads, hd)).astype(np.float32)
+    q[:, 0] *= np.float32(1e30)
+    q[:, 1] = 0
+    q[B // 2, 2, 3] = np.nan
+    t = put(be, *planes, weight=np.zeros((n_kv, max_rows), np.float32))
+    dq, do = be.upload(q), be.alloc(q.nbytes)
+    be._check(be.lib.ibcu_attention_kv4(be.ctx, t, dq.ptr, do.ptr, n_heads, row0, B)); be.sync()
+    got = be.download(do, np.float32, q.size).reshape(q.shape)
+    bad = np.isnan(got).any(2)
+    assert bad[B // 2, 2] and bad.sum() == 1 and np.isnan(got[B // 2, 2]).all()
+    s = q[:, 0].astype(np.float64) @ K[0].T
+    s[np.arange(R)[None] > row0 + np.arange(B)[:, None]] = -np.inf
+    best = s.argmax(1)
+    assert np.allclose(got[:, 0], V[0, best], rtol=2.0 ** -18, atol=0)
+    mean = np.cumsum(V[0], 0)[row0:] / np.arange(row0 + 1, R + 1)[:, None]
+    size = np.cumsum(np.abs(V[0]), 0)[row0:] / np.arange(row0 + 1, R + 1)[:, None]
+    assert np.all(np.abs(got[:, 1] - mean) <= 1500 * 2.0 ** -24 * size)
+    w = get(be, t)[3]
+    assert np.isnan(w[0, : row0 + B // 2 + 1]).all() and np.isfinite(w[1:, :R]).all()                  # the NaN query's weights
+    assert np.allclose(w[1, :R].sum(), B * group, rtol=2.0 ** -12)
+    # the same without the NaN query: every row has what it drew as the best one, and its shares
+    q[B // 2, 2, 3] = 0
+    q[:, 2:group] = q[:, :1]
+    t = put(be, *planes, weight=np.zeros((n_kv, max_rows), np.float32))
+    dq = be.upload(q)
+    be._check(be.lib.ibcu_attention_kv4(be.ctx, t, dq.ptr, do.ptr, n_heads, row0, B)); be.sync()
+    w = get(be, t)[3][0, :R]
+    want = (group - 1) * np.bincount(best, minlength=R).astype(np.float64)
+    share = 1.0 / np.arange(row0 + 1, R + 1)
+    want += np.array([share[max(0, r - row0):].sum() for r in range(R)])
+    assert np.allclose(w, want, rtol=2.0 ** -12, atol=1e-7)
+    # a key that is not a number
+    planes[2][0, row0 // 2, 0] = np.nan
+    t = put(be, *planes, weight=np.zeros((n_kv, max_rows), np.float32))
+    be._check(be.lib.ibcu_attention_kv4(be.ctx, t, dq.ptr, do.ptr, n_heads, row0, B)); be.sync()
+    got = be.download(do, np.float32, q.size).reshape(q.shape)
+    assert np.isnan(got[:, [0, *range(2, group)]]).all() and np.isfinite(got[:, group:]).all()
