@@ -464,3 +464,9 @@ def test_extreme_scores_in_every_form(backend, n_heads, n_kv, hd, row0, B):
     be._check(be.lib.ibcu_attention_kv4(be.ctx, t, dq.ptr, do.ptr, n_heads, row0, B)); be.sync()
     got = be.download(do, np.float32, q.size).reshape(q.shape)
     assert np.isnan(got[:, [0, *range(2, group)]]).all() and np.isfinite(got[:, group:]).all()
+
+
+@pytest.mark.parametrize("n_heads,n_kv,hd,B,max_rows", [(8, 2, 128, 1, 40000), (64, 8, 64, 1, 20000), (8, 2, 96, 5, 30000), (4, 2, 64, 40, 20000), (32, 32, 32, 1, 9000)])
+def test_captured_at_a_device_place_of_a_long_cache(backend, n_heads, n_kv, hd, B, max_rows):
+    """Grids for a long cache and contexts that fill little of it, half and all."""
+    test_captured_at_a_device_place(backend, n_heads, n_kv, hd, B, max_rows)
