@@ -118,10 +118,10 @@ constexpr int IBCU_DECLINED = 1;
 // last graph is destroyed.
 int ibcu_reserve(ibcu_ctx* ctx, void** buf, size_t* have, size_t want);
 
-// Opt `kernel` in to `smem` bytes of dynamic shared memory; `opt` is that kernel's own, static at the place of the launch.
+// Opt `kernel` in to `smem` bytes of dynamic shared memory; `opt` is that kernel's own, static at the place of the launch. Every size asks: what a launch
+// may have unasked is 48 KB together with the kernel's static arrays, which only the compiler knows, so that 48 KB of dynamic memory alone may be too many.
 template <typename K>
 static inline int ibcu_allow_smem(ibcu_ctx* ctx, SmemOptIn& opt, K* kernel, size_t smem) {
-    if (smem <= 48 * 1024) return IBCU_OK;
     const int e = opt.raise(ctx->device, smem, [&](size_t n) { return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)n); });
     return e ? ibcu_fail(ctx, IBCU_ERR_CUDA, "%zu bytes of shared memory refused: %s", smem, cudaGetErrorString((cudaError_t)e)) : IBCU_OK;
 }
