@@ -257,7 +257,8 @@ int ibcu_pqkv_encode(ibcu_ctx* ctx, const float* vec, int dim, int n_vec, int G,
 /* Beside the FP32 cache of ibcu_attention*: 4.5 bits a value instead of 32. The reference keeps its cache in FP32
  * (src/forward.c:463-504); its compressed forms live in the session engine (see ibcu_pqkv_encode). A row of a KV head is head_dim
  * values in groups of 32, each with an fp16 scale s = max|x| * (1 / 7) and codes clamp(rint(x * (1 / s)), -7, 7) + 8 (products and
- * reciprocals in FP32): the value held is (code - 8) * s. A group that holds NaN or Inf has s = NaN, so that it shows wherever it is seen; one whose s rounds to zero
+ * reciprocals in FP32): the value held is (code - 8) * s. A group that holds NaN or Inf has s = NaN: at the positions that see its row a key's group spoils all outputs, and
+ * the weights of all rows that these see, a value's group its 32 outputs and no weight. One whose s rounds to zero
  * holds zeros; s is at most 8192 (values beyond 57344 saturate). Planes are per KV head, two codes a byte, first code in the low nibble:
  *   k, v   [n_kv_heads][max_rows][head_dim / 2] bytes, 16-byte aligned
  *   scale  [n_kv_heads][max_rows][2 * head_dim / 32] fp16: the key's groups, then the value's; 16-byte aligned

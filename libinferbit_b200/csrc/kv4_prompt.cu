@@ -15,8 +15,8 @@
 // What bounds it: 2048 positions of 32 heads of 128 values over 8 take 143 us with the preparing launch, of which the products would be 62 at the measured rate. Per 64 rows
 // the softmax's chain (load, maximum, exponentials, pieces, store: 1500 cycles without exponentials and dequantisers) and shared memory (values of K' and V' written and read,
 // sums of runs) are longer than the products' 1600 cycles: leaving two of three products out gained 1 %, leaving both dequantisers out 15 %.
-// A V' of a row with a NaN scale would reach columns that do not see the row (0 * NaN), so NaN goes into the row's K' instead, and with it
-// into every column that does see it.
+// A V' of a group with a NaN scale would reach columns that do not see the row (0 * NaN), so it is zeros, and the first row of a NaN in each of a row's groups is
+// remembered: columns see rows from the first on, so those that see that one give NaN in the group's outputs. (A NaN in K' reaches its own row's scores alone.)
 #include "kv4.cuh"
 #include "tc_common.cuh"
 #include <algorithm>
@@ -45,6 +45,7 @@ struct PkShared {
     uint32_t tmem_base;
     int abort_flag;
     float meet[2][PK_COLS];                                    // maxima, at last sums, of a column's two threads
+    int nan_from[4];                                           // first row whose value scale of this group is NaN
 };
 
 __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
@@ -81,15 +82,12 @@ __device__ __forceinline__ void held_pieces(const __half2 f, const __half2 scale
 __device__ __forceinline__ bool is_nan(uint32_t half_bits) { return (half_bits & 0x7FFFu) > 0x7C00u; }
 
 // Piece t of a key row (the values 8t..8t+7 of every group) into the operand image: rows of 128 bytes, 16-byte pieces swizzled, blocks of 64 values
-// `block` bytes apart, the low pieces `part` bytes behind the high ones. scales: the row's, keys' and values'.
+// `block` bytes apart, the low pieces `part` bytes behind the high ones. scales: the row's keys'.
 template <int NG>
-__device__ __forceinline__ void place_key(unsigned char* to, int block, int part, int r, int t, const uint32_t (&w)[NG], const uint32_t (&scales)[NG]) {
-    bool bad = false;
-#pragma unroll
-    for (int j = NG / 2; j < NG; j++) bad = bad || is_nan(scales[j]) || is_nan(scales[j] >> 16);
+__device__ __forceinline__ void place_key(unsigned char* to, int block, int part, int r, int t, const uint32_t (&w)[NG], const uint32_t (&scales)[NG / 2]) {
 #pragma unroll
     for (int j = 0; j < NG; j++) {
-        const uint32_t s = bad ? 0x7FFFu : (j & 1 ? scales[j / 2] >> 16 : scales[j / 2] & 0xFFFFu);
+        const uint32_t s = j & 1 ? scales[j / 2] >> 16 : scales[j / 2] & 0xFFFFu;
         const __half2 s2 = half2_of(s | s << 16);
         __half2 f[4];
         codes_of(w[j], f);
@@ -103,6 +101,7 @@ __device__ __forceinline__ void place_key(unsigned char* to, int block, int part
 }
 template <int N> __device__ __forceinline__ void load_words(uint32_t (&d)[N], const unsigned char* s) {
     if constexpr (N == 4) { const uint4 v = *reinterpret_cast<const uint4*>(s); d[0] = v.x; d[1] = v.y; d[2] = v.z; d[3] = v.w; }
+    else if constexpr (N == 1) d[0] = *reinterpret_cast<const uint32_t*>(s);
     else { const uint2 v = *reinterpret_cast<const uint2*>(s); d[0] = v.x; d[1] = v.y; }
 }
 
@@ -123,6 +122,7 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
             init(sh->s_full[i], 1); init(sh->s_empty[i], 8); init(sh->p_full[i], 8); init(sh->pv_done[i], 1);
         }
         sh->abort_flag = 0;
+        for (int j = 0; j < NG; j++) sh->nan_from[j] = 0x7FFFFFFF;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
@@ -216,9 +216,9 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
                     const int r = 8 * (w + 4 * u) + (lane & 7), t = lane >> 3;
-                    uint32_t k[NG], sc[NG];
+                    uint32_t k[NG], sc[NG / 2];
                     load_words<NG>(k, raw + r * 16 * NG + t * 4 * NG);
-                    load_words<NG>(sc, scales + r * 4 * NG);
+                    load_words<NG / 2>(sc, scales + r * 4 * NG);
                     place_key<NG>(smem + S::K + b * S::KEYS, 8192, S::KB * 8192, r, t, k, sc);
                 }
             } else {
@@ -236,13 +236,25 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
                     }
                     load_words<NG>(sa, scales + a * 4 * NG);
                     load_words<NG>(sb, scales + (a + 1) * 4 * NG);
-                    const bool in_a = i * PK_ROWS + a < rows, in_b = i * PK_ROWS + a + 1 < rows;
+                    uint32_t nan = 0;
+#pragma unroll
+                    for (int j = NG / 2; j < NG; j++) nan |= bits(__hisnan2(half2_of(sa[j]))) | bits(__hisnan2(half2_of(sb[j])));
+                    if (nan || (i + 1) * PK_ROWS > rows) {     // no rows behind the last one, no NaN
+                        auto keep = [&](uint32_t s, int r, int j) {                             // the scales of groups j and j + 1 of a row
+                            if (r >= rows) return 0u;
+                            if (is_nan(s)) { atomicMin(&sh->nan_from[j], r); s &= 0xFFFF0000u; }
+                            if (is_nan(s >> 16)) { atomicMin(&sh->nan_from[j + 1], r); s &= 0xFFFFu; }
+                            return s;
+                        };
+#pragma unroll
+                        for (int j = NG / 2; j < NG; j++) {
+                            sa[j] = keep(sa[j], i * PK_ROWS + a, 2 * j - NG);
+                            sb[j] = keep(sb[j], i * PK_ROWS + a + 1, 2 * j - NG);
+                        }
+                    }
 #pragma unroll
                     for (int j = 0; j < NG; j++) {
-                        uint32_t ha = j & 1 ? sa[(NG + j) / 2] >> 16 : sa[(NG + j) / 2] & 0xFFFFu, hb = j & 1 ? sb[(NG + j) / 2] >> 16 : sb[(NG + j) / 2] & 0xFFFFu;
-                        if (!in_a || is_nan(ha)) ha = 0;
-                        if (!in_b || is_nan(hb)) hb = 0;
-                        const __half2 s2 = half2_of(ha | hb << 16);
+                        const __half2 s2 = half2_of(__byte_perm(sa[(NG + j) / 2], sb[(NG + j) / 2], j & 1 ? 0x7632 : 0x5410));
                         __half2 f[4];
                         codes_of(__byte_perm(va[j / 2], vb[j / 2], j & 1 ? 0x7632 : 0x5410), f);
 #pragma unroll
@@ -402,7 +414,8 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
         sh->meet[half][own] = l;
         pair_sync(1 + quarter);
         l += sh->meet[half ^ 1][own];
-        if (n && alive && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->pv_done[(n - 1) & 1]), (uint32_t)((n - 1) >> 1) & 1u, abort_flag, 13))) {
+        if (n && alive && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->pv_done[(n - 1) & 1]), (uint32_t)((n - 1) >> 1) & 1u, abort_flag, 13)) &&
+            __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->v_full[(n - 1) & 1]), (uint32_t)((n - 1) >> 1) & 1u, abort_flag, 14))) {          // what was said of the values' NaN
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const float inv = 1.0f / l;
             float* to = p.out + ((size_t)b_col * p.t.n_heads + (size_t)kvh * p.t.group + c % p.t.group) * S::HD;
@@ -435,9 +448,10 @@ __global__ void __launch_bounds__(PK_THREADS, 1) kv4_prompt_kernel(const PkParam
                     for (int u = 0; u < 16; u++) o[16 * h + u] = fmaf(old[u], aged, __uint_as_float(x[u]));
                 }
                 if (!on) continue;
+                const float by = lim < sh->nan_from[j] ? inv : __uint_as_float(0x7FFFFFFFu);
 #pragma unroll
                 for (int g = 0; g < 8; g++) {
-                    const float4 x = make_float4(o[g] * inv, o[8 + g] * inv, o[16 + g] * inv, o[24 + g] * inv);
+                    const float4 x = make_float4(o[g] * by, o[8 + g] * by, o[16 + g] * by, o[24 + g] * by);
                     float* at = to + 32 * j + 4 * g;
                     if (vec) *reinterpret_cast<float4*>(at) = x;
                     else { at[0] = x.x; at[1] = x.y; at[2] = x.z; at[3] = x.w; }
@@ -546,19 +560,16 @@ __global__ void __launch_bounds__(PW_THREADS, 1) kv4_prompt_weight_kernel(const 
         if (n) {
             if (half == 0) {
                 const size_t row = p.c.row(kvh, min(r, R - 1));
-                uint32_t sc[NG];
+                uint32_t sc[NG / 2];
 #pragma unroll
-                for (int j = 0; j < NG; j++) sc[j] = __ldcg(reinterpret_cast<const uint32_t*>(p.c.scale + row * (2 * NG)) + j);
-                bool bad = false;
-#pragma unroll
-                for (int j = NG / 2; j < NG; j++) bad = bad || is_nan(sc[j]) || is_nan(sc[j] >> 16);
+                for (int j = 0; j < NG / 2; j++) sc[j] = __ldcg(reinterpret_cast<const uint32_t*>(p.c.scale + row * (2 * NG)) + j);
 #pragma unroll 1
                 for (int t = 0; t < 4; t += 2) {               // pieces of a key row, two at a time: 8 NG columns of tensor memory a part
                     uint32_t high[8 * NG], low[8 * NG];
 #pragma unroll
                     for (int e = 0; e < 2 * NG; e++) {
                         const int j = e % NG;
-                        const uint32_t w = __ldcg(reinterpret_cast<const uint32_t*>(p.c.k + row * (16 * NG)) + t * NG + e), k = bad ? 0x7FFFu : (j & 1 ? sc[j / 2] >> 16 : sc[j / 2] & 0xFFFFu);
+                        const uint32_t w = __ldcg(reinterpret_cast<const uint32_t*>(p.c.k + row * (16 * NG)) + t * NG + e), k = j & 1 ? sc[j / 2] >> 16 : sc[j / 2] & 0xFFFFu;
                         __half2 f[4];
                         codes_of(w, f);
 #pragma unroll
