@@ -120,6 +120,7 @@ struct W8Params {
     ibcu_linear_t t[4];
     int n_tensors, tile_start[5];                    // tiles of 128 rows of tensor i: [tile_start[i], tile_start[i + 1])
     int B, NT, token_tiles, nkb, S, stages, tmem_cols, early_weights;   // NT: tokens a tile; nkb: blocks of 128 columns; early_weights: no launch of this call writes them
+    int edge;                                        // 131072 columns: see w8_sum
     const float* sx;
     int* err;
 };
@@ -130,8 +131,12 @@ struct W8Shared {
     float sx[2][256];
 };
 
+// A sum as a float. 131072 products of -128 and -128 are 2^31, which wraps to -2^31; that no other codes come to (the lowest is -128 * 127 * 131072).
+__device__ __forceinline__ float w8_unwrap(float sum) { return sum == -2147483648.0f ? 2147483648.0f : sum; }
+__device__ __forceinline__ float w8_sum(uint32_t sum, bool edge) { const float f = (float)(int)sum; return edge ? w8_unwrap(f) : f; }
+
 // A tile's results from tensor memory, by eight warps: this thread's output row, 32 tokens at a time or the last 16. Each warp's store of a token is 128 bytes.
-__device__ __forceinline__ void write_tile(const ibcu_linear_t& W, uint32_t tmem, int row, int tok0, int tokens, int NT, float sw, const float* sx) {
+__device__ __forceinline__ void write_tile(const ibcu_linear_t& W, uint32_t tmem, int row, int tok0, int tokens, int NT, float sw, const float* sx, bool edge) {
     const int warp = threadIdx.x >> 5;
     const bool have = row < W.M;
     const size_t ld = (size_t)W.out_stride;
@@ -140,6 +145,13 @@ __device__ __forceinline__ void write_tile(const ibcu_linear_t& W, uint32_t tmem
         uint32_t acc[32];
         if (NT - c >= 32) { tmem_ld32(from + c, acc); tmem_wait_ld(acc); }
         else tmem_ld16(from + c, acc);
+        float sum[32];
+#pragma unroll
+        for (int u = 0; u < 32; u++) sum[u] = (float)(int)acc[u];
+        if (edge) {
+#pragma unroll
+            for (int u = 0; u < 32; u++) sum[u] = w8_unwrap(sum[u]);
+        }
         const int n = have ? min(32, tokens - c) : 0;
         float* o = W.out + (size_t)(tok0 + c) * ld + row;
         auto finish = [&](auto whole, auto add) {
@@ -152,7 +164,7 @@ __device__ __forceinline__ void write_tile(const ibcu_linear_t& W, uint32_t tmem
                 const float f[8] = { s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w };
 #pragma unroll
                 for (int u = 0; u < 8; u++) {
-                    const float y = (float)(int)acc[u0 + u] * (sw * f[u]);
+                    const float y = sum[u0 + u] * (sw * f[u]);
                     if (decltype(whole)::value || u0 + u < n) o[(size_t)u * ld] = decltype(add)::value ? old[u] + y : y;
                 }
                 o += 8 * ld;
@@ -293,7 +305,7 @@ __global__ void __launch_bounds__(W8_THREADS, 1) w8a8_tc_kernel(const __grid_con
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (S > 1) break;                        // one tile a cluster; its parts meet below
             if (!there) continue;                    // gave up: the barrier above is still everyone's
-            write_tile(W, tmem + (uint32_t)((j & 1) * p.NT), row, tok0, tokens, p.NT, sw, sx);
+            write_tile(W, tmem + (uint32_t)((j & 1) * p.NT), row, tok0, tokens, p.NT, sw, sx, p.edge);
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&sh->acc_empty[j & 1]));
@@ -322,18 +334,18 @@ __global__ void __launch_bounds__(W8_THREADS, 1) w8a8_tc_kernel(const __grid_con
             place(first, ti, row0, tok0);
             const ibcu_linear_t& W = p.t[ti];
             const int row = row0 + r, mine = min(TL, min(p.NT, p.B - tok0) - rank * TL);
-            const int4* got = reinterpret_cast<const int4*>(w8_smem);
+            const uint4* got = reinterpret_cast<const uint4*>(w8_smem);
             if (row < W.M) {
                 const float sw = W.scales_fp32 ? reinterpret_cast<const float*>(W.scales)[row] : __half2float(reinterpret_cast<const __half*>(W.scales)[row]);
                 for (int t = (tid >> 7) * 4; t < mine; t += 8) {
-                    int4 sum = got[(t / 4) * 128 + r];
-                    for (int k = 1; k < S; k++) { const int4 v = got[((k * TL + t) / 4) * 128 + r]; sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w; }
-                    const int four[4] = { sum.x, sum.y, sum.z, sum.w };
+                    uint4 sum = got[(t / 4) * 128 + r];
+                    for (int k = 1; k < S; k++) { const uint4 v = got[((k * TL + t) / 4) * 128 + r]; sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w; }
+                    const uint32_t four[4] = { sum.x, sum.y, sum.z, sum.w };
 #pragma unroll
                     for (int u = 0; u < 4; u++)
                         if (t + u < mine) {
                             float* to = W.out + (size_t)(tok0 + rank * TL + t + u) * W.out_stride + row;
-                            const float y = (float)four[u] * (sw * sh->sx[0][rank * TL + t + u]);
+                            const float y = w8_sum(four[u], p.edge) * (sw * sh->sx[0][rank * TL + t + u]);
                             *to = W.epilogue == IBCU_EPI_ADD ? __ldcg(to) + y : y;
                         }
                 }
@@ -470,7 +482,7 @@ __global__ void __launch_bounds__(W8_THREADS, 1) w8a8_pair_kernel(const __grid_c
             asm volatile("bar.sync 2, %0;" :: "n"(W8_OUT_WARPS * 32) : "memory");
             if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sh->acc_full[j & 1]), (uint32_t)((j >> 1) & 1), abort_flag, 5))) continue;          // gave up: the barrier above is still everyone's
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            write_tile(W, tmem + (uint32_t)((j & 1) * p.NT), row, tok0, tokens, p.NT, sw, sx);
+            write_tile(W, tmem + (uint32_t)((j & 1) * p.NT), row, tok0, tokens, p.NT, sw, sx, p.edge);
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive_peer(peer_address(smem_u32(&sh->acc_empty[j & 1]), 0));
@@ -682,7 +694,7 @@ int product(ibcu_ctx* ctx, const ibcu_linear_t* ts, int n, const float* x, int8_
         ok = ok && tensor_map_bytes(&maps.w[i], copy[i] ? (uint8_t*)ctx->scratch + at[i] : (const uint8_t*)ts[i].w, ts[i].M, N, copy[i] ? (long)pitch : N, 128);
     }
     for (int i = n; i < 4; i++) maps.w[i] = maps.w[0];
-    p.n_tensors = n; p.B = B; p.nkb = (N + 127) / 128; p.sx = sx; p.err = ctx->kern_err;
+    p.n_tensors = n; p.B = B; p.nkb = (N + 127) / 128; p.edge = N == 131072; p.sx = sx; p.err = ctx->kern_err;
     const long row_tiles = p.tile_start[n];
     long pair_tiles = 0;
     for (int i = 0; i < n; i++) pair_tiles += (ts[i].M + 255) / 256;

@@ -1,4 +1,4 @@
-"""INT8 x INT8 products: weights quantised on the device right ahead of the product that reads them."""
+"""INT8 x INT8 products at their edges: weights quantised on the device right ahead of the product that reads them, the largest sums."""
 import numpy as np
 import pytest
 
@@ -43,3 +43,23 @@ def test_weights_quantised_right_before_the_product(backend, M, N, B, form):
     assert not np.array_equal(want[0], want[1])
     for a, b in zip(want, run(False)):
         assert np.array_equal(a, b)
+
+
+@pytest.mark.parametrize("M,B", [(40, 1), (300, 9), (9700, 5), (9700, 300)])
+@pytest.mark.parametrize("add", [0, 1])
+def test_the_largest_sums_of_any_codes(backend, M, B, add):
+    """131072 columns of -128 by -128 are 2^31, one more than an int32 holds; beside it the largest and smallest sums of the other codes. Scales of 1: every sum is a float."""
+    be, N = backend, 131072
+    w, x = be.alloc(M * N), be.alloc(B * N)
+    sw, sx, o = be.upload(np.ones(M, np.float32)), be.upload(np.ones(B, np.float32)), be.alloc(B * M * 4)
+    t = (LinearT * 1)(LinearT(w.ptr, sw.ptr, o.ptr, M, M, 1, add))
+    for a, b in ((-128, -128), (-128, 127), (127, -128), (-127, -128), (-128, -127), (127, 127)):
+        be._check(be.lib.ibcu_memset(be.ctx, w.ptr, a & 255, M * N)); be._check(be.lib.ibcu_memset(be.ctx, x.ptr, b & 255, B * N)); be._check(be.lib.ibcu_memset(be.ctx, o.ptr, 0, B * M * 4))
+        be._check(be.lib.ibcu_linear_w8a8(be.ctx, t, 1, x.ptr, sx.ptr, N, B)); be.sync()
+        assert np.all(be.download(o, np.float32, B * M) == np.float32(a * b * N)), (a, b)
+    # one code less in the first token: 128 below 2^31, the float next to it
+    be.write(x, np.array([-127], np.int8)); be._check(be.lib.ibcu_memset(be.ctx, w.ptr, 128, M * N))
+    be._check(be.lib.ibcu_memset(be.ctx, x.at(1), 128, B * N - 1)); be._check(be.lib.ibcu_memset(be.ctx, o.ptr, 0, B * M * 4))
+    be._check(be.lib.ibcu_linear_w8a8(be.ctx, t, 1, x.ptr, sx.ptr, N, B)); be.sync()
+    got = be.download(o, np.float32, B * M).reshape(B, M)
+    assert np.all(got[0] == np.float32(2.0 ** 31 - 128)) and np.all(got[1:] == np.float32(2.0 ** 31))
