@@ -162,7 +162,8 @@ int  ib_b200_model_get_kv(ib_b200_model* m, int layer, float* k, float* v, int n
 int  ib_b200_model_kv4(ib_b200_model* m, int weights);
 /* Cuts the 4-bit cache, which holds positions up to n_pos - 1, to `keep` rows in every layer and KV head (ibcu_kv4_evict: the first
  * `sink` and last `recent` stay, of the others those that drew most attention). Steps go on at positions n_pos and up; max_ctx bounds the
- * rows, no longer the positions. Rows are then no positions any more: _set_kv and _get_kv count rows. */
+ * rows, no longer the positions. Rows are then no positions any more: _set_kv and _get_kv count rows. A step at position 0 begins a new
+ * sequence, and _fill_random fills one: rows are positions again. */
 int  ib_b200_model_evict(ib_b200_model* m, int n_pos, int keep, int sink, int recent);
 /* B consecutive positions pos0.. of one sequence (B == 1: forward_single_ex, src/forward.c:518-664;
  * B > 1: forward_batch, :682-846). tokens and logits are host arrays; logits [B*vocab] may be NULL.

@@ -216,6 +216,7 @@ int ib_b200_model_fill_random(ib_b200_model* m, uint64_t seed, int kv_fill) {
     const int H = c->hidden, kv = c->n_kv_heads * c->head_dim;
     int rc = 0;
     uint64_t s = seed * 1000003ull;
+    m->evicted = m->next_pos = 0;                             /* the cache holds positions 0..kv_fill-1 from here on */
     for (int l = 0; l <= c->n_layers && !rc; l++) {
         const int nt = l < c->n_layers ? 7 : 1;
         for (int i = 0; i < nt && !rc; i++) {
@@ -394,7 +395,9 @@ static int issue(ib_b200_model* m, int pos0, int B, int head_last) {
 }
 
 static int step_device(ib_b200_model* m, int pos0, int B, int head_last) {
-    if (!m || B < 1 || B > BMAX || pos0 < 0 || pos0 < m->next_pos || pos0 - m->evicted > m->c.max_ctx - B) return IBCU_ERR_PARAM;   /* src/forward.c:696-699, 857-862 */
+    if (!m || B < 1 || B > BMAX || B > m->c.max_ctx) return IBCU_ERR_PARAM;                             /* src/forward.c:696-699, 857-862 */
+    if (pos0 == 0) m->evicted = m->next_pos = 0;              /* a new sequence: rows are positions again */
+    if (pos0 < m->next_pos || pos0 - m->evicted > m->c.max_ctx - B) return IBCU_ERR_PARAM;
     int rc = ibcu_store_i32(m->ctx, m->pos_dev, pos0 - m->evicted);
     if (!rc && m->kv4) rc = ibcu_store_i32(m->ctx, m->pos_dev + 1, pos0);
     if (rc) return rc;
