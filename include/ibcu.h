@@ -164,7 +164,7 @@ int ibcu_linear_w4a8_fp32(ibcu_ctx* ctx, const ibcu_linear_t* tensor, const floa
  * row: the integer route for any number of tokens, where ibcu_linear takes up to 32 and W4A8 scales groups of 128 columns. No
  * counterpart in the reference.
  * ibcu_quantize_rows_int8: scale[b] = max|x[b]| * (1 / 127), q[b*N+j] = rint(x * (1 / scale)), ties to even, products and reciprocals in
- * FP32. A row whose maximum is below 2^-100 gives zeros and scale 0; one that holds NaN or Inf zeros and scale NaN. Codes and scales of weight rows are a
+ * FP32; N up to 2^30. A row whose maximum is below 2^-100 gives zeros and scale 0; one that holds NaN or Inf zeros and scale NaN. Codes and scales of weight rows are a
  * tensor as it is (scales_fp32 = 1): the calls behind this one may use them at once. */
 int ibcu_quantize_rows_int8(ibcu_ctx* ctx, const float* x, int8_t* q, float* scale, int N, int B);
 /* out[b*out_stride + m] = (sum_j w[m][j] * xq[b][j]) * (scale_w[m] * sx[b]), or added to out (IBCU_EPI_ADD), for n_tensors (1..4) INT8

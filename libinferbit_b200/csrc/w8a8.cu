@@ -728,7 +728,8 @@ int product(ibcu_ctx* ctx, const ibcu_linear_t* ts, int n, const float* x, int8_
 extern "C" int ibcu_quantize_rows_int8(ibcu_ctx* ctx, const float* x, int8_t* q, float* scale, int N, int B) {
     IBCU_CHECK_CTX(ctx);
     IBCU_REQUIRE(ctx, x && q && scale, "ibcu_quantize_rows_int8: null pointer");
-    IBCU_REQUIRE(ctx, N >= 1 && B >= 1, "ibcu_quantize_rows_int8: N=%d B=%d", N, B);
+    // a block's index into a row steps by 512 beyond its end
+    IBCU_REQUIRE(ctx, N >= 1 && N <= (1 << 30) && B >= 1, "ibcu_quantize_rows_int8: N=%d (up to 2^30) B=%d", N, B);
     AlignJobs none;
     memset(&none, 0, sizeof none);
     return quantize<false>(ctx, x, q, scale, N, N, B, none);

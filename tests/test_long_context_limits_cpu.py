@@ -1,0 +1,11 @@
+"""Sizes at the end of what an int holds, which the 4-bit cache and INT8 x INT8 calls refuse before anything is launched (see test_kv4_cpu.py for the zeroed context)."""
+import pytest
+
+from tests.test_w8a8_cpu import P, lib, refused
+
+pytestmark = pytest.mark.skipif(lib.ibcu_device_count() > 0, reason="with a GPU, a call that is not refused would launch")
+
+
+@pytest.mark.parametrize("N", [(1 << 30) + 1, 2**31 - 512, 2**31 - 1])
+def test_rows_whose_index_would_wrap(N):
+    assert refused(lib.ibcu_quantize_rows_int8, P, P, P, N, 1)
