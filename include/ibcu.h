@@ -169,7 +169,7 @@ int ibcu_linear_w4a8_fp32(ibcu_ctx* ctx, const ibcu_linear_t* tensor, const floa
 int ibcu_quantize_rows_int8(ibcu_ctx* ctx, const float* x, int8_t* q, float* scale, int N, int B);
 /* out[b*out_stride + m] = (sum_j w[m][j] * xq[b][j]) * (scale_w[m] * sx[b]), or added to out (IBCU_EPI_ADD), for n_tensors (1..4) INT8
  * tensors that share the activations. The sums are exact, for any codes: the same bits however the call is cut. The outputs of a
- * call overlap neither one another nor its inputs. N up to 131072, B up to 2^20. w and xq at any address; rows that do not start on 16 bytes (w or xq unaligned, or N no multiple
+ * call overlap neither one another nor its inputs. M up to 2^31 - 256, N up to 131072, B up to 2^20. w and xq at any address; rows that do not start on 16 bytes (w or xq unaligned, or N no multiple
  * of 16) are first copied so that they do. */
 int ibcu_linear_w8a8(ibcu_ctx* ctx, const ibcu_linear_t* tensors, int n_tensors, const int8_t* xq, const float* sx, int N, int B);
 /* Both steps for FP32 activations x[b*N + j]. Same bits as the two calls. */

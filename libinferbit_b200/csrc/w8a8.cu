@@ -595,7 +595,7 @@ int check_call(ibcu_ctx* ctx, const ibcu_linear_t* ts, int n, int N, int B, cons
     IBCU_REQUIRE(ctx, N >= 1 && N <= 131072 && B >= 1 && B <= (1 << 20), "%s: N=%d (up to 131072) B=%d (up to %d)", call, N, B, 1 << 20);
     for (int i = 0; i < n; i++) {
         IBCU_REQUIRE(ctx, ts[i].w && ts[i].scales && ts[i].out, "%s: null pointer", call);
-        IBCU_REQUIRE(ctx, ts[i].M >= 1 && ts[i].out_stride >= ts[i].M, "%s: M=%d out_stride=%d", call, ts[i].M, ts[i].out_stride);
+        IBCU_REQUIRE(ctx, ts[i].M >= 1 && ts[i].M <= 0x7FFFFF00 && ts[i].out_stride >= ts[i].M, "%s: M=%d (up to 2^31 - 256) out_stride=%d", call, ts[i].M, ts[i].out_stride);
         IBCU_REQUIRE(ctx, ts[i].epilogue == IBCU_EPI_STORE || ts[i].epilogue == IBCU_EPI_ADD, "%s: epilogue=%d", call, ts[i].epilogue);
     }
     return IBCU_OK;
