@@ -24,12 +24,12 @@ __host__ __device__ constexpr size_t kv4_frags(int ng) { return (size_t)ng * 128
 
 // where rows and positions of a call are: arguments, or {row0, pos0} in device memory
 struct Kv4Place { int row0, pos0; const int* at; };
-// Reads them where they are on the device. False, and the context's error word set, if the rows would not fit.
+// Reads them where they are on the device. False, and the context's error word set, if the rows would not fit or the positions pass 31 bits, as the calls with arguments refuse them.
 __device__ __forceinline__ bool kv4_place(const Kv4Place& p, int B, int max_rows, int* err, int& row0, int& pos0) {
     row0 = p.row0; pos0 = p.pos0;
     if (!p.at) return true;
     row0 = __ldcg(p.at); pos0 = __ldcg(p.at + 1);
-    if (row0 >= 0 && pos0 >= 0 && row0 <= max_rows - B) return true;
+    if (row0 >= 0 && pos0 >= 0 && row0 <= max_rows - B && pos0 <= 0x7FFFFFFF - B) return true;
     *err = IBCU_KV4_PLACE_ERR;
     return false;
 }

@@ -56,3 +56,35 @@ def test_a_key_group_with_nan_spoils_what_sees_it(backend, n_heads, n_kv, hd, ro
     assert np.array_equal(np.isnan(got), spoilt)
     assert np.all(np.abs(got - want)[~spoilt] <= tol[~spoilt])
     assert np.isnan(drawn[0]).all() and np.all(np.abs(drawn[1:] - weight[1:]) <= wtol[1:] + 2.0 ** -24 * weight[1:])
+
+
+@pytest.mark.parametrize("n_heads,n_kv,hd,B", [(8, 2, 64, 2), (8, 2, 64, 40), (8, 8, 128, 700)])
+def test_positions_at_the_end_of_31_bits(backend, n_heads, n_kv, hd, B):
+    """The last positions there are give what the call with arguments gives; further ones, read from the device, write nothing and are reported."""
+    be, rng = backend, np.random.default_rng(B)
+    max_rows, theta = (B + 8) // 8 * 8, 500000.0
+    planes = _kv4.random_planes(rng, n_kv, hd, max_rows, max_rows)
+    x = [rng.standard_normal((B, heads * hd), dtype=np.float32) for heads in (n_heads, n_kv, n_kv)]
+    d = [be.upload(a) for a in x]
+    last, at, outs = 2**31 - 1 - B, be.upload(np.zeros(2, np.int32)), []
+    for device in (False, True):
+        t, o = put(be, *planes), be.alloc(B * n_heads * hd * 4)
+        be.write(at, np.array([0, last], np.int32))
+        if device:
+            be._check(be.lib.ibcu_attention_decode_kv4_at(be.ctx, t, *(a.ptr for a in d), o.ptr, n_heads, at.ptr, B, theta))
+        else:
+            be._check(be.lib.ibcu_attention_decode_kv4(be.ctx, t, *(a.ptr for a in d), o.ptr, n_heads, 0, last, B, theta))
+        be.sync()
+        outs.append((be.download(o, np.float32, B * n_heads * hd).reshape(B, -1), *(a.tobytes() for a in get(be, t))))
+    assert outs[0][1:] == outs[1][1:]
+    tol = _kv4.attention(_kv4.rotate(x[0], n_heads, last, theta), _kv4.plane_values(*(a[:, :B] for a in get(be, t))), n_heads, 0)[2]
+    assert np.all(np.abs(outs[0][0] - outs[1][0]) <= 2 * tol)         # each is within it of the sums in 64 bits
+    assert be.lib.ibcu_attention_decode_kv4(be.ctx, t, *(a.ptr for a in d), o.ptr, n_heads, 0, last + 1, B, theta) == -1
+    be.lib.ibcu_clear_error(be.ctx)
+    for pos in (last + 1, 2**31 - 1):
+        before = [a.tobytes() for a in get(be, t)]
+        be.write(at, np.array([0, pos], np.int32))
+        be._check(be.lib.ibcu_attention_decode_kv4_at(be.ctx, t, *(a.ptr for a in d), o.ptr, n_heads, at.ptr, B, theta))
+        assert be.lib.ibcu_sync(be.ctx) == -1 and b"outside the cache" in be.lib.ibcu_last_error(be.ctx)
+        be.lib.ibcu_clear_error(be.ctx)
+        assert [a.tobytes() for a in get(be, t)] == before
