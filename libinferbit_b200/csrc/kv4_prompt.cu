@@ -12,7 +12,7 @@
 // The instruction cuts its sums off, towards zero, at every step: outputs after 16000 rows were 5.7e-5 off in one accumulator, 2.3e-6 after 2048. So after a run
 // of PK_RUN times 64 rows its outputs are added, rounded, to sums: half of them in tensor memory, beside one place for P, half in shared memory (all of them there, in steps
 // of 16: 160 us instead of 143).
-// What bounds it: 2048 positions of 32 heads of 128 values over 8 take 143 us with the preparing launch, of which the products would be 62 at the measured rate. Per 64 rows
+// What bounds it: 2048 positions of 32 heads of 128 values over 8 take 139 us with the preparing launch, replayed, of which the products would be 62 at the measured rate. Per 64 rows
 // the softmax's chain (load, maximum, exponentials, pieces, store: 1500 cycles without exponentials and dequantisers) and shared memory (values of K' and V' written and read,
 // sums of runs) are longer than the products' 1600 cycles: leaving two of three products out gained 1 %, leaving both dequantisers out 15 %.
 // A V' of a group with a NaN scale would reach columns that do not see the row (0 * NaN), so it is zeros, and the first row of a NaN in each of a row's groups is
